@@ -43,7 +43,11 @@ enum lcs_status {
     LCS_ERR_CAPACITY = -4     /* request exceeds the context's create-time limits */
 };
 
-enum lcs_dtype { LCS_F32 = 0, LCS_BF16 = 1 };
+enum lcs_dtype {
+    LCS_F32 = 0,
+    LCS_BF16 = 1,
+    LCS_E4M3 = 2              /* 8 bits (OCP e4m3, no infinities): lcs_add_rmsnorm, lcs_lmhead_ex */
+};
 
 enum lcs_flags {
     LCS_WANT_LOGPROBS = 1u,   /* write chosen_lp and the n_top alternatives */
@@ -210,6 +214,69 @@ typedef struct lcs_lmhead_out {
                                   these logits */
 } lcs_lmhead_out;
 
+/* The residual's addition and the root-mean-square norm ahead of the lm-head
+ * (norm(x) of matvec(out_w, norm(x)), src/locus/model/llama.cpp:512-513):
+ *   h = x + residual, y = h / sqrt(mean(h^2) + eps) * weight
+ * per row, sums in f32, y and sum rounded once from f32 values (y from the
+ * unrounded h). In e4m3, y holds y / y_scale with y_scale = max|y| / 448 of the
+ * row (1 for a row of zeros): the operand of lcs_lmhead_ex. A row that holds a
+ * NaN or an infinity has a NaN wherever the formula has one; in e4m3 its
+ * y_scale is 1 if its largest |y| is a NaN. Squares and their sum are f32: past
+ * 3e38 a row's y is 0. Rows and strides need the alignment of their elements only. */
+typedef struct lcs_norm_batch {
+    uint32_t rows;
+    uint32_t hidden;           /* 1..32768 */
+    uint32_t x_dtype;          /* LCS_F32 or LCS_BF16: x, residual, weight and sum */
+    uint32_t y_dtype;          /* LCS_F32, LCS_BF16 or LCS_E4M3 */
+    float eps;                 /* > 0 */
+    const void* x;             /* rows x x_stride */
+    const void* residual;      /* rows x residual_stride, or NULL */
+    const void* weight;        /* hidden */
+    uint64_t x_stride;         /* elements between rows (>= hidden), of each buffer */
+    uint64_t residual_stride;
+} lcs_norm_batch;
+
+typedef struct lcs_norm_out {
+    void* y;                   /* rows x y_stride */
+    float* y_scale;            /* rows (LCS_E4M3), else ignored */
+    void* sum;                 /* rows x sum_stride: h, or NULL; needs residual; it may be x or
+                                  residual itself (same stride), other overlaps may not be */
+    uint64_t y_stride;
+    uint64_t sum_stride;
+} lcs_norm_out;
+
+/* A pool of low-rank adapters beside the lm-head's weight: adapter i adds
+ * scale[i] (x a[i]^T) b[i]^T to the logits of the rows that name it. Only an
+ * adapter's first rank[i] ranks count, whatever the others hold. */
+typedef struct lcs_adapters {
+    uint32_t n;                /* 1..1024 */
+    uint32_t wide;             /* ranks a slot of the pool holds: a multiple of 8, up to 256 */
+    const void* a;             /* n x wide x hidden bf16, 16-byte aligned */
+    const void* b;             /* n x vocab x wide bf16, 16-byte aligned */
+    const int32_t* rank;       /* n (clamped to 0..wide), or NULL: wide */
+    const float* scale;        /* n, or NULL: 1 */
+} lcs_adapters;
+
+/* lcs_lmhead_batch with the operands' type, their scales and the rows' adapters:
+ * logits[i][v] = x_scale[i] w_scale[v] sum_k x[i][k] w[v][k], plus the product of
+ * the row's adapter on x_scale[i] x[i]. Low-rank states are kept to 16 bits of
+ * mantissa, everything else in f32. */
+typedef struct lcs_lmhead_ex_batch {
+    uint32_t rows;             /* hidden vectors, <= the context's max_rows */
+    uint32_t vocab;            /* <= the context's max_vocab */
+    uint32_t hidden;           /* multiple of 64, up to 65536 */
+    uint32_t rows_per_seq;     /* 1..64 rows per sequence (accept_len), or 0 */
+    uint32_t dtype;            /* LCS_BF16 or LCS_E4M3: x and w */
+    const void* x;             /* rows x hidden, 16-byte aligned */
+    const void* w;             /* vocab x hidden, 16-byte aligned */
+    const float* x_scale;      /* rows (LCS_E4M3), or NULL: 1 */
+    const float* w_scale;      /* vocab (LCS_E4M3), or NULL: 1 */
+    const int32_t* draft;      /* rows, or NULL: the token whose logprob each row reports */
+    const lcs_adapters* adapters;  /* host struct, or NULL: none */
+    const int32_t* slot;       /* rows (with adapters): the row's adapter; any id outside
+                                  [0, n): none */
+} lcs_lmhead_ex_batch;
+
 /* Number of usable gfx950 devices (0 when none). Replaces the runtime probe
  * that sets Backend::available (registry.cpp:148-223, cuda_stub.cpp:29). */
 int lcs_probe(int* n_devices);
@@ -279,6 +346,15 @@ int lcs_ngram_draft(lcs_ctx* ctx, const lcs_draft_batch* batch, const lcs_draft_
  * the reference, which computes the logits with matvec and reads them again
  * in argmax / logprobs_from. Allocates nothing. */
 int lcs_lmhead(lcs_ctx* ctx, const lcs_lmhead_batch* batch, const lcs_lmhead_out* out, void* stream);
+
+/* The fused lm-head product in bf16 or e4m3, with the rows' low-rank adapters (see
+ * lcs_lmhead_ex_batch); outputs as lcs_lmhead. No counterpart call in the
+ * reference. Allocates nothing. */
+int lcs_lmhead_ex(lcs_ctx* ctx, const lcs_lmhead_ex_batch* batch, const lcs_lmhead_out* out, void* stream);
+
+/* Residual addition and norm, optionally into 8 bits (see lcs_norm_batch). Allocates
+ * nothing and uses no context workspace: rows are not bounded by max_rows. */
+int lcs_add_rmsnorm(lcs_ctx* ctx, const lcs_norm_batch* batch, const lcs_norm_out* out, void* stream);
 
 /* Sticky device-side status bits of ctx (LCS_STATUS_*), set by kernels that
  * met an input they could not serve. Every bit comes with id -1 on each

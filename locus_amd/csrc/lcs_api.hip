@@ -13,6 +13,7 @@
 #include <string>
 #include <vector>
 
+#include "lcs_check.hpp"
 #include "lcs_internal.hpp"
 #include "locus_sampler.h"
 
@@ -27,6 +28,8 @@ hipError_t launch_logprobs(const LogprobArgs& a, uint32_t dtype, hipStream_t st)
 hipError_t launch_draft(const DraftArgs& a, hipStream_t st);
 hipError_t launch_lmhead(const LmArgs& a, uint32_t cus, hipStream_t st);
 uint32_t lmhead_max_blocks(uint32_t vocab, uint32_t cus);
+hipError_t launch_lmhead_ex(const LmArgs& a, bool f8, uint32_t cus, hipStream_t st);
+hipError_t launch_add_rmsnorm(const NormArgs& a, uint32_t x_dtype, uint32_t y_dtype, hipStream_t st);
 }  // namespace lcs
 
 struct lcs_ctx {
@@ -40,6 +43,10 @@ struct lcs_ctx {
     float* d_pen = nullptr;
     uint32_t* status = nullptr;
     lcs::LmRec* lmrecs = nullptr;   // lm-head epilogue records: max_rows x lmhead_max_blocks
+    // lcs_lmhead_ex with adapters: the rows' order and their low-rank states, max_rows each
+    uint32_t* ad_perm = nullptr;
+    int32_t* ad_slot = nullptr;
+    uint16_t* ad_low = nullptr;     // x 2 kAdWideMax
     uint32_t cus = 256;             // compute units of the device (the lm-head's tile shape)
     // nucleus path workspace (kNucRows rows at a time)
     lcs::NucRow* nrow = nullptr;
@@ -160,6 +167,9 @@ lcs_ctx* lcs_create(int device, uint32_t max_rows, uint32_t max_vocab, uint32_t 
         (e = hipMalloc(&c->nrow, nuc_rows * sizeof(lcs::NucRow))) != hipSuccess ||
         (e = hipMalloc(&c->nh_pk, nh_elems * 8)) != hipSuccess ||
         (e = hipMalloc(&c->nlist, nuc_rows * lcs::kNucList * 8)) != hipSuccess ||
+        (e = hipMalloc(&c->ad_perm, (size_t)max_rows * 4)) != hipSuccess ||
+        (e = hipMalloc(&c->ad_slot, (size_t)max_rows * 4)) != hipSuccess ||
+        (e = hipMalloc(&c->ad_low, (size_t)max_rows * 2 * lcs::kAdWideMax * 2)) != hipSuccess ||
         (e = hipMalloc(&c->lp_params, (size_t)max_rows * sizeof(lcs_params))) != hipSuccess ||
         (e = hipMalloc(&c->lp_ids, (size_t)max_rows * 4)) != hipSuccess ||
         (e = hipMemset(c->lp_params, 0, (size_t)max_rows * sizeof(lcs_params))) != hipSuccess ||
@@ -186,6 +196,9 @@ void lcs_destroy(lcs_ctx* c) {
     (void)hipFree(c->d_pen);
     (void)hipFree(c->status);
     (void)hipFree(c->lmrecs);
+    (void)hipFree(c->ad_perm);
+    (void)hipFree(c->ad_slot);
+    (void)hipFree(c->ad_low);
     (void)hipFree(c->lp_params);
     (void)hipFree(c->lp_ids);
     (void)hipFree(c->wh);
@@ -694,6 +707,72 @@ int lcs_lmhead(lcs_ctx* c, const lcs_lmhead_batch* b, const lcs_lmhead_out* o, v
     const hipError_t e = lcs::launch_lmhead(a, c->cus, static_cast<hipStream_t>(stream));
     if (e != hipSuccess) return hip_fail(c, e, "lm-head kernel launch");
     return LCS_OK;
+}
+
+int lcs_lmhead_ex(lcs_ctx* c, const lcs_lmhead_ex_batch* b, const lcs_lmhead_out* o, void* stream) {
+    if (!c) return LCS_ERR_INVALID_ARG;
+    const char* why = "";
+    const int rc = lcs::check_lmhead_ex(b, o, c->max_rows, c->max_vocab, &why);
+    if (rc != LCS_OK) return fail(c, rc, why);
+    if (b->rows == 0) return LCS_OK;
+    lcs::LmArgs a{};
+    a.x = static_cast<const uint16_t*>(b->x);
+    a.w = static_cast<const uint16_t*>(b->w);
+    a.rows = b->rows;
+    a.vocab = b->vocab;
+    a.hidden = b->hidden;
+    a.rows_per_seq = b->rows_per_seq;
+    a.ld_logits = o->ld_logits;
+    a.draft = b->draft;
+    a.logits = o->logits;
+    a.argmax_ids = o->argmax_ids;
+    a.log_z = o->log_z;
+    a.draft_lp = b->draft ? o->draft_lp : nullptr;
+    a.accept_len = o->accept_len;
+    a.recs = c->lmrecs;
+    a.stats = o->stats;
+    a.x_scale = b->x_scale;
+    a.w_scale = b->w_scale;
+    if (const lcs_adapters* d = b->adapters) {
+        a.ad_n = d->n;
+        a.ad_wide = d->wide;
+        a.ad_a = static_cast<const uint16_t*>(d->a);
+        a.ad_b = static_cast<const uint16_t*>(d->b);
+        a.ad_rank = d->rank;
+        a.ad_scale = d->scale;
+        a.slot = b->slot;
+        a.perm = c->ad_perm;
+        a.pslot = c->ad_slot;
+        a.low = c->ad_low;
+    }
+    DeviceGuard g(c->device);
+    const hipError_t e = lcs::launch_lmhead_ex(a, b->dtype == LCS_E4M3, c->cus, static_cast<hipStream_t>(stream));
+    return e == hipSuccess ? LCS_OK : hip_fail(c, e, "lm-head kernel launch");
+}
+
+int lcs_add_rmsnorm(lcs_ctx* c, const lcs_norm_batch* b, const lcs_norm_out* o, void* stream) {
+    if (!c) return LCS_ERR_INVALID_ARG;
+    const char* why = "";
+    const int rc = lcs::check_add_rmsnorm(b, o, lcs::kNormHiddenMax, &why);
+    if (rc != LCS_OK) return fail(c, rc, why);
+    if (b->rows == 0) return LCS_OK;
+    lcs::NormArgs a{};
+    a.x = b->x;
+    a.residual = b->residual;
+    a.weight = b->weight;
+    a.y = o->y;
+    a.y_scale = o->y_scale;
+    a.sum = o->sum;
+    a.x_stride = b->x_stride;
+    a.residual_stride = b->residual_stride;
+    a.y_stride = o->y_stride;
+    a.sum_stride = o->sum_stride;
+    a.rows = b->rows;
+    a.hidden = b->hidden;
+    a.eps = b->eps;
+    DeviceGuard g(c->device);
+    const hipError_t e = lcs::launch_add_rmsnorm(a, b->x_dtype, b->y_dtype, static_cast<hipStream_t>(stream));
+    return e == hipSuccess ? LCS_OK : hip_fail(c, e, "norm kernel launch");
 }
 
 int lcs_get_status(lcs_ctx* c, uint32_t* status_out, int reset) {

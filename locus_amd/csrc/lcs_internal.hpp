@@ -261,6 +261,38 @@ struct LmArgs {
     uint32_t* accept_len;
     LmRec* recs;                    // rows x nblocks
     lcs_row_stats* stats;           // rows, or NULL
+    // 8-bit operands (x and w then hold e4m3 bytes)
+    const float* x_scale;           // rows, or NULL: 1
+    const float* w_scale;           // vocab, or NULL: 1
+    // adapters (ad_n 0: none)
+    uint32_t ad_n, ad_wide;
+    const uint16_t* ad_a;           // ad_n x ad_wide x hidden bf16
+    const uint16_t* ad_b;           // ad_n x vocab x ad_wide bf16
+    const int32_t* ad_rank;         // ad_n, or NULL: ad_wide
+    const float* ad_scale;          // ad_n, or NULL: 1
+    const int32_t* slot;            // rows: the row's adapter, or -1
+    // ... as lm_low leaves them: the rows in the order of their adapters
+    uint32_t* perm;                 // rows: the row at a position
+    int32_t* pslot;                 // rows: its adapter, or -1 (also for a rank of 0)
+    uint16_t* low;                  // rows x 2 x ad_wide: its low-rank state, upper and lower bf16 part
+};
+constexpr uint32_t kAdMax = 1024;       // adapters of a pool
+constexpr uint32_t kAdWideMax = 256;    // their widest rank
+constexpr uint32_t kExHiddenMax = 65536;
+
+// residual addition and norm (lcs_norm.hip)
+constexpr uint32_t kNormHiddenMax = 32768;
+struct NormArgs {
+    const void* x;
+    const void* residual;           // or NULL
+    const void* weight;
+    void* y;
+    float* y_scale;                 // rows (e4m3)
+    void* sum;                      // or NULL
+    uint64_t x_stride, residual_stride, y_stride, sum_stride;
+    uint64_t rows;
+    uint32_t hidden;
+    float eps;
 };
 
 // status bits

@@ -1,0 +1,493 @@
+// The lm-head's tiled product with the sampler's first statistics in its epilogue
+// (gfx950): one kernel template for bf16 and 8-bit operands, with and without
+// the rows' low-rank adapters. lcs_lmhead.hip and lcs_lmhead_ex.hip launch it.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include <type_traits>
+
+#include "lcs_device.hpp"
+#include "lcs_internal.hpp"
+
+namespace lcs {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4_a __attribute__((ext_vector_type(4), may_alias));
+constexpr float kL2E = 1.4426950408889634f;
+
+// Waits until at most N vector memory operations are outstanding (and every
+// LDS operation is done); the compiler moves no memory access across it.
+template <int N>
+__device__ __forceinline__ void wait_vm() {
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+template <int N>
+__device__ __forceinline__ void wait_vm_lgkm() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
+}
+
+// 16 bytes per lane from a buffer (offsets vo per lane + so) to LDS at
+// dst + 16 lane (dst is wave-uniform).
+__device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t rs, unsigned char* dst, uint32_t vo, uint32_t so) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)dst, 16, (int)vo, (int)so, 0, 0);
+}
+// The same from a per-lane address.
+__device__ __forceinline__ void dma16_at(const void* src, unsigned char* dst) {
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
+                                     (__attribute__((address_space(3))) void*)dst, 16, 0, 0);
+}
+// NaN, by its bits: the build's float comparisons and selects assume that there
+// are none (the empty asm keeps the compiler from concluding the same here).
+__device__ __forceinline__ bool nan_bits(float v) {
+    uint32_t u = __float_as_uint(v);
+    asm("" : "+v"(u));
+    return (u & 0x7fffffffu) > 0x7f800000u;
+}
+// A workgroup barrier that waits for no memory operation.
+__device__ __forceinline__ void block_sync() {
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
+
+// A workgroup computes 64 VT columns of BR rows, transposed (columns on the
+// MFMA's row side, so that a lane holds many columns of one row and the
+// epilogue reduces in registers): NW waves, two over the rows, in
+// v_mfma_f32_32x32x16_bf16 tiles (lane l carries 8 consecutive k of row l % 32
+// of either operand, k chunk l / 32, and returns rows 8 (e / 4) + 4 (l / 32) +
+// e % 4 of column l % 32). The 256 x 256 tile takes eight waves, so that two
+// share a SIMD and one's loads, barriers and epilogue leave the matrix cores to
+// the other (1024 rows: 990 us with four, 963 with eight).
+//
+// Both operands go straight from memory into a ring of ST LDS stages of 16 KS k
+// with 16-byte DMA loads, so that no register holds data in flight. The loads
+// are what holds the matrix cores up (1024 rows: busy 1.03 M of 1.52 M cycles): a
+// stage of 64 k reads whole 128-byte lines, half the requests of 32 k, and two
+// such stages serve as well as four (1024 rows 963 -> 921 us, 64 rows 209 ->
+// 199); narrow and 128-row tiles have too few bytes in flight then (8 x 32000
+// 52 -> 69 us, 128 rows 218 -> 229) and keep 32 k. A row's 16-byte chunks are
+// permuted by its bits from kSw up: a fragment read's 16 lanes of a phase then
+// cover the 64 banks once (0 conflict cycles of 101 M). One barrier per stage, ahead of its last products: each wave has then
+// read the stage and its loads of the next one have landed.
+//
+// The workgroups of a column block are placed on one XCD in consecutive
+// dispatch slots (workgroups are dealt to the 8 XCDs in turn): they run
+// together, so the block's weight rows come from HBM once and from that XCD's
+// L2 for the other row tiles. With one row tile each workgroup starts at its
+// own k-step and wraps round, so that those in flight do not all read the same
+// offset of their rows (72 rows x 128256 x 4096: 245 -> 225 us); with more the
+// row tiles share x through the L2 by running in step (1024 rows: 1013 against
+// 1057 us with a start of its own).
+//
+// F8: e4m3 operands, 128 bytes of k a stage row (KS 4), two of them per product
+// (v_mfma_f32_32x32x64_f8f6f4: lane l carries two of the 16-byte chunks of a row,
+// the same ones of either operand, so which k they hold does not matter), and a
+// last half stage of 64 k straight from memory. Sums are f32 and unscaled; the row's and the
+// column's scale multiply them once, ahead of the adapters.
+// AD: the rows are taken in the order of their adapters (lm_low, which also
+// has left each row's low-rank state in two bf16 parts): see the adapters' part
+// below.
+template <int VT, int BR, int ST, int NW = 4, int KS = 2, bool BIG = false, bool F8 = false, bool AD = false>
+__global__ __launch_bounds__(NW * kWave, 2) void lmhead_tile(LmArgs a) {
+    constexpr uint32_t kTV = 64u * VT;        // columns per workgroup
+    constexpr uint32_t EB = F8 ? 1u : 2u;     // bytes of an element
+    constexpr uint32_t kTRowB = 32u * KS;     // bytes of a row in a stage
+    constexpr int kTK = (int)(kTRowB / EB);   // k per LDS stage
+    constexpr int SPS = F8 ? KS / 2 : KS;     // products of a tile per stage
+    constexpr uint32_t kStage = (kTV + BR) * kTRowB;
+    constexpr int WM = NW / 2;                // waves side by side over the columns, two over the rows
+    constexpr int CT = 2 * VT / WM, RT = BR / 64;   // 32-column and 32-row tiles per wave
+    constexpr uint32_t kCh = 2 * KS, kLog = KS == 4 ? 3 : 2;   // 16-byte chunks of a row
+    constexpr uint32_t kSw = KS == 4 ? 1 : 2;   // the row bits that permute them start here
+    constexpr int kLR = 64 / (int)kCh * NW;   // rows that one DMA load of every wave covers
+    constexpr int LA = kTV / kLR, LB = BR / kLR;   // DMA loads per wave and stage
+    constexpr bool SPLIT = KS == 4 && ST == 2;   // half of a stage's loads ahead of the barrier
+    static_assert(KS == 2 || SPLIT || F8, "the schedule of the k-loop");
+    static_assert(SPS % 2 == 0 && !(BIG && (F8 || AD)), "the schedule of the k-loop");
+    static_assert(LA * kLR == (int)kTV && LB * kLR == BR && CT * WM == 2 * VT, "tile shape");
+    constexpr int LPS = LA + LB;
+    __shared__ __attribute__((aligned(128))) unsigned char lds[ST * kStage];
+    const uint32_t tid = tid_x();
+    const int lane = lane_id(), wv = __builtin_amdgcn_readfirstlane((int)(tid / kWave));
+    uint32_t nb = wg_x();
+    const uint32_t slot = nb >> 3;
+    const uint32_t r0 = (slot % a.nchunks) * BR;
+    nb = 8u * (slot / a.nchunks) + (nb & 7u);
+    if (nb >= a.nblocks) return;   // (the grid is a multiple of 8 blocks)
+    const uint32_t K = a.hidden, V = a.vocab;
+    const uint32_t n0 = nb * kTV;
+    const uint32_t vrows = min((uint32_t)BR, a.rows - r0), vcols = min(kTV, V - n0);
+    const uint32_t wm = (uint32_t)wv % WM, wn = (uint32_t)wv / WM;   // the wave's columns and rows
+    const unsigned char* wbase = reinterpret_cast<const unsigned char*>(a.w) + (uint64_t)n0 * K * EB;
+    // (AD: rows from anywhere in x, which is under 4 GiB then)
+    const unsigned char* xbase = reinterpret_cast<const unsigned char*>(a.x) + (AD ? 0ull : (uint64_t)r0 * K * EB);
+    const __amdgpu_buffer_rsrc_t wrs =
+        __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(wbase), 0, (int)(vcols * K * EB), 0x00020000);
+    const __amdgpu_buffer_rsrc_t xrs =
+        __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(xbase), 0, (int)((AD ? a.rows : vrows) * K * EB), 0x00020000);
+    auto row_of = [&](uint32_t r) -> uint32_t { return AD ? a.perm[r0 + r] : r0 + r; };   // (r < vrows)
+    // DMA load i of a wave covers rows kLR i + 16 wv + lane / 4, a 16-byte
+    // chunk per lane; rows past the tile read row 0 (masked in the epilogue)
+    const uint32_t rr = kWave / kCh * (uint32_t)wv + ((uint32_t)lane >> kLog);
+    const uint32_t ch = (((uint32_t)lane & (kCh - 1u)) ^ ((rr >> kSw) & (kCh - 1u))) * 16u;
+    uint32_t wo[LA], xo[LB];
+#pragma unroll
+    for (int i = 0; i < LA; ++i) wo[i] = (kLR * i + rr < vcols ? kLR * i + rr : 0u) * K * EB + ch;
+#pragma unroll
+    for (int i = 0; i < LB; ++i) {
+        const uint32_t r = kLR * i + rr < vrows ? kLR * i + rr : 0u;
+        xo[i] = (AD ? row_of(r) : r) * K * EB + ch;
+    }
+    const uint32_t nsteps = K / kTK;
+    const uint32_t rot = a.nchunks == 1u ? nb % nsteps : 0u;
+    // (the byte offset of stage t in a row; stages past the end re-read the last)
+    auto koff = [&](uint32_t t) -> uint32_t {
+        uint32_t q = (t < nsteps ? t : nsteps - 1u) + rot;
+        return (q >= nsteps ? q - nsteps : q) * kTRowB;
+    };
+    auto issue1 = [&](int i, uint32_t ko, uint32_t sl) {   // DMA load i of a stage
+        unsigned char* b = lds + sl * kStage + (uint32_t)wv * 1024u + i * (kLR * kTRowB);
+        if (BIG) {   // (the row offsets need 64 bits)
+            const uint32_t r = kLR * (uint32_t)(i < LA ? i : i - LA) + rr;
+            const unsigned char* p = i < LA ? wbase + (uint64_t)(r < vcols ? r : 0u) * K * EB : xbase + (uint64_t)(r < vrows ? r : 0u) * K * EB;
+            dma16_at(p + ko + ch, b);
+        } else if (i < LA) {
+            dma16(wrs, b, wo[i < LA ? i : 0], ko);
+        } else {
+            dma16(xrs, b, xo[i >= LA ? i - LA : 0], ko);
+        }
+    };
+    auto issue = [&](uint32_t t, uint32_t sl) {
+#pragma unroll
+        for (int i = 0; i < LPS; ++i) issue1(i, koff(t), sl);
+    };
+    f32x16 acc[CT][RT];
+#pragma unroll
+    for (int i = 0; i < CT; ++i)
+#pragma unroll
+        for (int j = 0; j < RT; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
+    // fragment s (16 k) of row r: chunk 2 s + lane / 32
+    const uint32_t lr = (uint32_t)lane & 31u, lh = (uint32_t)lane >> 5;
+    uint32_t fo[KS];
+#pragma unroll
+    for (uint32_t s = 0; s < KS; ++s) fo[s] = lr * kTRowB + (((2u * s + lh) ^ ((lr >> kSw) & (kCh - 1u))) * 16u);
+    struct Frag { std::conditional_t<F8, i32x8, bf16x8> w[CT], x[RT]; };
+    // read i of a fragment set: x first (every product needs all of it), then w
+    constexpr int NR = CT + RT, NP = CT * RT;
+    auto frag_at = [&](const unsigned char* p, int s) {
+        if constexpr (F8) {
+            union { u32x4 q[2]; i32x8 v; } u;
+            u.q[0] = *reinterpret_cast<const u32x4_a*>(p + fo[2 * s]);
+            u.q[1] = *reinterpret_cast<const u32x4_a*>(p + fo[2 * s + 1]);
+            return u.v;
+        } else {
+            return *reinterpret_cast<const bf16x8*>(p + fo[s]);
+        }
+    };
+    auto read1 = [&](Frag& f, int i, uint32_t sl, int s) {
+        const unsigned char* pw = lds + sl * kStage + wm * (kTV / WM * kTRowB);
+        const unsigned char* px = lds + sl * kStage + kTV * kTRowB + wn * (BR / 2 * kTRowB);
+        if (i < RT) f.x[i < RT ? i : 0] = frag_at(px + i * 32 * kTRowB, s);
+        else f.w[i >= RT ? i - RT : 0] = frag_at(pw + (i - RT) * 32 * kTRowB, s);
+    };
+    auto mul = [&](const auto& w, const auto& x, const f32x16& c) {
+        if constexpr (F8) return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w, x, c, 0, 0, 0, 0, 0, 0);
+        else return __builtin_amdgcn_mfma_f32_32x32x16_bf16(w, x, c, 0, 0, 0);
+    };
+    auto mul1 = [&](const Frag& f, int k) {   // product k of NP
+        const int i = k / RT, j = k % RT;
+        acc[i][j] = mul(f.w[i], f.x[j], acc[i][j]);
+    };
+    if (!F8 || nsteps != 0u) {
+    Frag f0, f1;
+#pragma unroll
+    for (int t = 0; t < ST; ++t) issue((uint32_t)t, (uint32_t)t);
+    wait_vm<(ST - 1) * LPS>();
+    block_sync();
+#pragma unroll
+    for (int i = 0; i < NR; ++i) read1(f0, i, 0u, 0);
+    uint32_t sl = 0u;
+    // Every LDS read and DMA load is issued behind a product: a wave issues
+    // in order, and eight DMA loads in a row hold it for longer than the
+    // products queued ahead of them last (1024 rows, four waves: 1022 -> 980 us).
+    // (SPLIT: half of a stage's loads go out behind the last products
+    // of the stage whose place it takes, half behind the next stage's first)
+    uint32_t kn = 0u;   // the offset of the stage whose second half is to be issued
+    for (uint32_t t = 0; t < nsteps; ++t) {
+        const uint32_t ns = sl + 1u == (uint32_t)ST ? 0u : sl + 1u;
+        constexpr int H = LPS / 2;
+#pragma unroll
+        for (int s = 0; s < SPS - 1; ++s) {
+            const bool more = SPLIT && s == 0;
+#pragma unroll
+            for (int k = 0; k < NP; ++k) {
+                mul1(s % 2 == 0 ? f0 : f1, k);
+#pragma unroll
+                for (int i = k * (NR + (more ? LPS - H : 0)) / NP; i < (k + 1) * (NR + (more ? LPS - H : 0)) / NP; ++i) {
+                    if (i < NR) read1(s % 2 == 0 ? f1 : f0, i, sl, s + 1);
+                    else if (t != 0u) issue1(H + i - NR, kn, ns);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+        // stage t is read, stage t + 1 has landed, in every wave
+        wait_vm_lgkm<SPLIT ? 0 : (ST - 2) * LPS>();
+        block_sync();
+        kn = koff(t + ST);
+        constexpr int L = SPLIT ? H : LPS;
+#pragma unroll
+        for (int k = 0; k < NP; ++k) {
+            mul1(f1, k);
+#pragma unroll
+            for (int i = k * (NR + L) / NP; i < (k + 1) * (NR + L) / NP; ++i) {
+                if (i < NR) read1(f0, i, ns, 0);
+                else issue1(i - NR, kn, sl);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        sl = ns;
+    }
+    }
+    wait_vm_lgkm<0>();
+    __syncthreads();   // (the last loads have landed: the ring is free)
+
+    const uint32_t cw = kTV / WM * wm;   // the wave's first column in the tile
+    if constexpr (F8) {
+        if (K % (uint32_t)kTK != 0u) {   // the last 64 k
+            auto rest = [&](const unsigned char* row) {
+                const unsigned char* p = row + (K - 64u) + lh * 16u;
+                union { u32x4 q[2]; i32x8 v; } u;
+                u.q[0] = *reinterpret_cast<const u32x4_a*>(p);
+                u.q[1] = *reinterpret_cast<const u32x4_a*>(p + 32);
+                return u.v;
+            };
+            Frag f;
+#pragma unroll
+            for (int j = 0; j < RT; ++j) {
+                const uint32_t r = wn * (BR / 2) + 32u * j + lr;
+                const uint32_t rs = r < vrows ? r : 0u;
+                f.x[j] = rest(xbase + (uint64_t)(AD ? row_of(rs) : rs) * K);
+            }
+#pragma unroll
+            for (int i = 0; i < CT; ++i) {
+                const uint32_t c = cw + 32u * i + lr;
+                f.w[i] = rest(wbase + (uint64_t)(c < vcols ? c : 0u) * K);
+            }
+#pragma unroll
+            for (int k = 0; k < NP; ++k) mul1(f, k);
+        }
+        float xs[RT];
+#pragma unroll
+        for (int j = 0; j < RT; ++j) {
+            const uint32_t r = wn * (BR / 2) + 32u * j + lr;
+            xs[j] = a.x_scale && r < vrows ? a.x_scale[row_of(r)] : 1.0f;
+        }
+#pragma unroll
+        for (int i = 0; i < CT; ++i)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const uint32_t c = cw + 32u * i + 8u * q + 4u * lh;
+                float ws[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) ws[e] = a.w_scale && c + e < vcols ? a.w_scale[n0 + c + e] : 1.0f;
+#pragma unroll
+                for (int j = 0; j < RT; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[i][j][4 * q + e] *= xs[j] * ws[e];
+            }
+    }
+    // ---- the adapters: acc += low b^T for the rows of each adapter that the wave's
+    // 32-row tiles hold. The rows are in the order of their adapters, so
+    // an adapter's columns are read by one wave of two, as a rule, straight into the
+    // fragments (each lane 8 consecutive k of its column, which is how the factor
+    // lies in memory; nothing would be shared through LDS). A row's state is the
+    // sum of two bf16 parts (16 bits of mantissa: an error of 2^-17 a term, below
+    // that of the product's f32 sums). Each adapter has an accumulator of its
+    // own, added to its rows only: a product with zeros instead would carry an
+    // inf or NaN of one request's adapter into the others' logits.
+    if constexpr (AD) {
+        const uint32_t wide = a.ad_wide;
+#pragma unroll
+        for (int j = 0; j < RT; ++j) {
+            const uint32_t r = wn * (BR / 2) + 32u * j + lr;
+            const uint32_t pos = r0 + (r < vrows ? r : 0u);
+            const int32_t s = r < vrows ? a.pslot[pos] : -1;
+            const uint16_t* low = a.low + (uint64_t)pos * 2u * wide;
+            uint64_t todo = ballot(s >= 0);
+            while (todo != 0u) {
+                const int32_t ad = __builtin_amdgcn_readlane(s, __builtin_ctzll(todo));
+                const bool mine = s == ad;
+                todo &= ~ballot(mine);
+                const uint32_t rank = a.ad_rank ? min((uint32_t)a.ad_rank[ad], wide) : wide;
+                const uint16_t* b = a.ad_b + ((uint64_t)(uint32_t)ad * V + n0) * wide;
+                f32x16 t[CT];
+#pragma unroll
+                for (int i = 0; i < CT; ++i)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) t[i][e] = 0.0f;
+                for (uint32_t k0 = 0u; k0 < rank; k0 += 16u) {
+                    const uint32_t k = k0 + 8u * lh;
+                    const uint32_t left = k < rank ? rank - k : 0u, kk = k < rank ? k : 0u;
+                    // (what lies past the rank counts as zero, whatever it holds)
+                    u32x4 live;
+#pragma unroll
+                    for (uint32_t e = 0; e < 4u; ++e) live[e] = left > 2u * e + 1u ? 0xffffffffu : left == 2u * e + 1u ? 0xffffu : 0u;
+                    const u32x4 hi = *reinterpret_cast<const u32x4_a*>(low + kk) & live;
+                    const u32x4 lo = *reinterpret_cast<const u32x4_a*>(low + wide + kk) & live;
+#pragma unroll
+                    for (int i = 0; i < CT; ++i) {
+                        const uint32_t c = cw + 32u * i + lr;
+                        const u32x4 f = *reinterpret_cast<const u32x4_a*>(b + (c < vcols ? c : 0u) * wide + kk) & live;
+                        t[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, f), __builtin_bit_cast(bf16x8, lo), t[i], 0, 0, 0);
+                        t[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, f), __builtin_bit_cast(bf16x8, hi), t[i], 0, 0, 0);
+                    }
+                }
+                if (mine) {
+#pragma unroll
+                    for (int i = 0; i < CT; ++i)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) acc[i][j][e] += t[i][e];
+                }
+            }
+        }
+    }
+
+    // ---- epilogue: acc[i][j][e] is column n0 + kTV / WM wm + 32 i + 8 (e / 4) +
+    // 4 lh + e % 4 of row r0 + BR / 2 wn + 32 j + lr ----
+    struct Part { float max, sum, draft; uint32_t idx; };
+    Part* part = reinterpret_cast<Part*>(lds);   // [WM][BR]: by the wave's columns
+    const bool full = vcols == kTV;
+    const bool vec = a.logits && (a.ld_logits & 3u) == 0u && (reinterpret_cast<uintptr_t>(a.logits) & 15u) == 0u;
+#pragma unroll
+    for (int j = 0; j < RT; ++j) {
+        const uint32_t rl = wn * (BR / 2) + 32u * j + lr;   // the lane's row in the tile
+        const bool rin = rl < vrows;
+        const uint32_t cb = kTV / WM * wm + 4u * lh;            // columns cb + 32 i + 8 (e / 4) + e % 4
+        if (a.logits && rin) {
+            float* out = a.logits + (uint64_t)row_of(rl) * a.ld_logits + n0;
+#pragma unroll
+            for (int i = 0; i < CT; ++i)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const uint32_t c = cb + 32u * i + 8u * q;
+                    if (vec && c + 4u <= vcols) {
+                        *reinterpret_cast<float4*>(out + c) =
+                            make_float4(acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (c + e < vcols) out[c + e] = acc[i][j][4 * q + e];
+                    }
+                }
+        }
+        const float NEG = -__builtin_huge_valf();
+        if (!full) {
+#pragma unroll
+            for (int i = 0; i < CT; ++i)
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    if (cb + 32u * i + 8u * (e / 4) + e % 4 >= vcols) acc[i][j][e] = NEG;
+        }
+        // the lane's max, its first column, the draft's logit
+        float m = acc[0][j][0];
+#pragma unroll
+        for (int i = 0; i < CT; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) m = fmaxf(m, acc[i][j][e]);
+        const int32_t dr = a.draft && rin ? a.draft[row_of(rl)] : -1;
+        const uint32_t dc = (uint32_t)dr < V ? (uint32_t)dr - n0 - cb : 0xffffffffu;   // the draft's column, from cb
+        uint32_t ci = kTV;
+        float dl = 0.0f;
+#pragma unroll
+        for (int i = CT - 1; i >= 0; --i)
+#pragma unroll
+            for (int e = 15; e >= 0; --e) {
+                const uint32_t c = 32u * i + 8u * (e / 4) + e % 4;
+                ci = acc[i][j][e] == m ? c : ci;
+            }
+        uint32_t found = 0u;
+        if (ballot(dc < kTV / WM && (dc & 4u) == 0u) != 0u) {
+#pragma unroll
+            for (int i = 0; i < CT; ++i)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const uint32_t c = 32u * i + 8u * (e / 4) + e % 4;
+                    if (dc == c) { dl = acc[i][j][e]; found = kLmDraftBit; }
+                }
+        }
+        float s = 0.0f;
+#pragma unroll
+        for (int i = 0; i < CT; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+                float t[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) t[k] = __builtin_amdgcn_exp2f((acc[i][j][e + k] - m) * kL2E);
+                s += (t[0] + t[1]) + (t[2] + t[3]);
+            }
+        if (nan_bits(s)) {
+            // a NaN or +inf, or nothing but -inf (columns past the vocabulary
+            // too): the max and its first column again, NaNs left out, which
+            // keep the sum a NaN; columns of -inf have no term
+            bool nan = false;
+            m = NEG;
+            ci = kTV;
+#pragma unroll
+            for (int i = 0; i < CT; ++i)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const float v = acc[i][j][e];
+                    const bool n = nan_bits(v), up = !n && (ci == kTV || v > m);
+                    nan = nan || n;
+                    m = up ? v : m;
+                    ci = up ? 32u * i + 8u * (e / 4) + e % 4 : ci;
+                }
+            s = m == NEG && !nan ? 0.0f : s;
+        }
+        ci += cb;
+        // lanes l and l + 32 share a row
+        const float m2 = __shfl_xor(m, 32), s2 = __shfl_xor(s, 32), d2 = __shfl_xor(dl, 32);
+        const uint32_t c2 = (uint32_t)__shfl_xor((int)ci, 32), f2 = (uint32_t)__shfl_xor((int)found, 32);
+        const float M = fmaxf(m, m2);
+        s = (m == NEG ? s : s * __builtin_amdgcn_exp2f((m - M) * kL2E)) +
+            (m2 == NEG ? s2 : s2 * __builtin_amdgcn_exp2f((m2 - M) * kL2E));
+        ci = m > m2 ? ci : m2 > m ? c2 : min(ci, c2);
+        if (lh == 0u) part[wm * BR + rl] = Part{M, s, found ? dl : d2, ci | found | f2};
+    }
+    __syncthreads();
+    if (tid < vrows) {
+        const float NEG = -__builtin_huge_valf();
+        Part p = part[tid];
+#pragma unroll
+        for (int w = 1; w < WM; ++w) {
+            // (a side of -inf: its sum is 0, or NaN where it holds one)
+            const Part q = part[w * BR + tid];
+            const float M = fmaxf(p.max, q.max);
+            p.sum = (p.max == NEG ? p.sum : p.sum * __builtin_amdgcn_exp2f((p.max - M) * kL2E)) +
+                    (q.max == NEG ? q.sum : q.sum * __builtin_amdgcn_exp2f((q.max - M) * kL2E));
+            p.draft = (p.idx & kLmDraftBit) ? p.draft : q.draft;
+            const uint32_t pc = p.idx & ~kLmDraftBit, qc = q.idx & ~kLmDraftBit;
+            p.idx = (p.max > q.max ? pc : q.max > p.max ? qc : min(pc, qc)) | ((p.idx | q.idx) & kLmDraftBit);
+            p.max = M;
+        }
+        LmRec rec;
+        rec.max = p.max;
+        // (a block of NaNs has no column that equals its max: its first one)
+        const uint32_t col = p.idx & ~kLmDraftBit;
+        rec.idx = (n0 + (col < vcols ? col : 0u)) | (p.idx & kLmDraftBit);
+        rec.sum = p.sum;
+        rec.draft = p.draft;
+        a.recs[(uint64_t)row_of(tid) * a.nblocks + nb] = rec;
+    }
+}
+
+}  // namespace lcs

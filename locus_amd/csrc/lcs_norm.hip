@@ -1,0 +1,310 @@
+// The residual's addition and the root-mean-square norm ahead of the lm-head, for
+// MI355X (gfx950): h = x + residual, y = h / sqrt(mean(h^2) + eps) * weight, per
+// row, with y in bf16, f32 or in 8 bits (e4m3) with a scale per row, the operand
+// that lcs_lmhead_ex takes.
+//
+// Reference: the output norm ahead of matvec(out_w, norm(x))
+// (src/locus/model/llama.cpp:512-513, 754-761).
+//
+// Memory bounds it: a row is read once, held in registers, and written once.
+// The sum of squares and the largest |h w| come from the same pass, so one
+// exchange between the row's waves gives both. In 8 bits the norm's factor r
+// cancels (y / scale = h w r / (max|h w| r / 448)), so an element costs one
+// product after it. Squares, sums and h are f32 (h unrounded: the norm reads it
+// from the registers and not from the rounded sum); y is rounded once.
+//
+// Rows, strides and widths are any: the vector loads and stores ask for the
+// element's alignment only, which the hardware's unaligned access mode serves,
+// and the lane that holds a row's end takes its elements one by one.
+//
+// (This file is compiled with NaNs honoured: a NaN in a row has to stay one.)
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "lcs_device.hpp"
+#include "lcs_internal.hpp"
+
+namespace lcs {
+
+namespace {
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+// (vectors at the alignment of their elements)
+typedef u32x4 u32x4_2 __attribute__((aligned(2), may_alias));
+typedef u32x4 u32x4_4 __attribute__((aligned(4), may_alias));
+typedef u32x2 u32x2_1 __attribute__((aligned(1), may_alias));
+
+constexpr float kE4m3Max = 448.0f;
+
+__device__ __forceinline__ float bf16_to_f(uint32_t u) { return __uint_as_float(u << 16); }
+// (round to nearest even; a NaN keeps its upper bits with the quiet one set)
+__device__ __forceinline__ uint32_t f_to_bf16(float f) {
+    const uint32_t u = __float_as_uint(f);
+    if ((u & 0x7fffffffu) > 0x7f800000u) return (u >> 16) | 0x40u;
+    return (u + 0x7fffu + ((u >> 16) & 1u)) >> 16;
+}
+
+// 8 elements from p; in a row's last lane only the first n exist.
+template <typename T> struct Io;
+template <> struct Io<uint16_t> {   // bf16
+    static __device__ __forceinline__ void load(const uint16_t* p, uint32_t n, float (&v)[8]) {
+        if (n >= 8u) {
+            const u32x4 q = *reinterpret_cast<const u32x4_2*>(p);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                v[2 * i] = bf16_to_f(q[i] & 0xffffu);
+                v[2 * i + 1] = __uint_as_float(q[i] & 0xffff0000u);
+            }
+        } else {
+#pragma unroll
+            for (uint32_t i = 0; i < 8u; ++i) v[i] = i < n ? bf16_to_f(p[i]) : 0.0f;
+        }
+    }
+    static __device__ __forceinline__ void store(uint16_t* p, uint32_t n, const float (&v)[8]) {
+        uint32_t b[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) b[i] = f_to_bf16(v[i]);
+        if (n >= 8u) {
+            *reinterpret_cast<u32x4_2*>(p) = u32x4{b[0] | b[1] << 16, b[2] | b[3] << 16, b[4] | b[5] << 16, b[6] | b[7] << 16};
+        } else {
+#pragma unroll
+            for (uint32_t i = 0; i < 8u; ++i)
+                if (i < n) p[i] = (uint16_t)b[i];
+        }
+    }
+};
+template <> struct Io<float> {
+    static __device__ __forceinline__ void load(const float* p, uint32_t n, float (&v)[8]) {
+        if (n >= 8u) {
+            const u32x4 q = *reinterpret_cast<const u32x4_4*>(p), r = *reinterpret_cast<const u32x4_4*>(p + 4);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                v[i] = __uint_as_float(q[i]);
+                v[4 + i] = __uint_as_float(r[i]);
+            }
+        } else {
+#pragma unroll
+            for (uint32_t i = 0; i < 8u; ++i) v[i] = i < n ? p[i] : 0.0f;
+        }
+    }
+    static __device__ __forceinline__ void store(float* p, uint32_t n, const float (&v)[8]) {
+        if (n >= 8u) {
+            u32x4 q, r;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                q[i] = __float_as_uint(v[i]);
+                r[i] = __float_as_uint(v[4 + i]);
+            }
+            *reinterpret_cast<u32x4_4*>(p) = q;
+            *reinterpret_cast<u32x4_4*>(p + 4) = r;
+        } else {
+#pragma unroll
+            for (uint32_t i = 0; i < 8u; ++i)
+                if (i < n) p[i] = v[i];
+        }
+    }
+};
+template <> struct Io<uint8_t> {   // e4m3; finite values are inside +-448 already
+    static __device__ __forceinline__ void store(uint8_t* p, uint32_t n, const float (&v)[8]) {
+        uint32_t q[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            int w = 0;
+            w = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * i], v[4 * i + 1], w, false);
+            w = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * i + 2], v[4 * i + 3], w, true);
+            q[i] = (uint32_t)w;
+        }
+        if (n >= 8u) {
+            *reinterpret_cast<u32x2_1*>(p) = u32x2{q[0], q[1]};
+        } else {
+#pragma unroll
+            for (uint32_t i = 0; i < 8u; ++i)
+                if (i < n) p[i] = (uint8_t)(q[i / 4u] >> (8u * (i % 4u)));
+        }
+    }
+};
+
+__device__ __forceinline__ uint32_t wave_max_u(uint32_t v) {
+    auto u_max = [](uint32_t a, uint32_t b) { return a > b ? a : b; };
+    LCS_WAVE_REDUCE_32(uint32_t, v, 0u, u_max);
+    return v;
+}
+__device__ __forceinline__ float clamp448(float v) {   // (a NaN stays one)
+    return v > kE4m3Max ? kE4m3Max : v < -kE4m3Max ? -kE4m3Max : v;
+}
+
+}  // namespace
+
+// WPR waves per row, each lane NV groups of 8 elements; a workgroup of up to
+// four waves takes 4 / WPR rows.
+template <typename XT, typename YT, bool RES, int WPR, int NV>
+__global__ __launch_bounds__((WPR < 4 ? 4 : WPR) * kWave) void add_rmsnorm(NormArgs a) {
+    constexpr bool Q8 = sizeof(YT) == 1;
+    constexpr int NW = WPR < 4 ? 4 : WPR;
+    struct Part { float ss; uint32_t top; };
+    __shared__ Part part[NW];
+    __shared__ uint32_t part2[NW];
+    const uint32_t tid = tid_x(), wv = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid / kWave));
+    const uint32_t first = wv / WPR * WPR;                     // the row's first wave
+    const uint64_t row0 = (uint64_t)wg_x() * (NW / WPR) + wv / WPR;
+    const bool live = row0 < a.rows;                           // (no early end: the waves meet at a barrier)
+    const uint64_t row = live ? row0 : a.rows - 1u;
+    const uint32_t H = a.hidden, t = (wv - first) * kWave + (uint32_t)lane_id();
+    const XT* x = static_cast<const XT*>(a.x) + row * a.x_stride;
+    const XT* res = static_cast<const XT*>(a.residual) + row * a.residual_stride;
+    const XT* w = static_cast<const XT*>(a.weight);
+    float v[NV][8], g[NV][8];
+    uint32_t c[NV], n[NV];
+    float ss = 0.0f;
+    uint32_t top = 0u;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        c[i] = ((uint32_t)i * WPR * kWave + t) * 8u;
+        n[i] = c[i] < H ? H - c[i] : 0u;
+        if (n[i] == 0u) c[i] = 0u;
+        Io<XT>::load(x + c[i], n[i], v[i]);
+    }
+    if (RES) {
+        float r[NV][8];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) Io<XT>::load(res + c[i], n[i], r[i]);
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[i][e] = v[i][e] + r[i][e];
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) Io<XT>::load(w + c[i], n[i], g[i]);
+    if (RES && live && a.sum) {
+        XT* sum = static_cast<XT*>(a.sum) + row * a.sum_stride;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) Io<XT>::store(sum + c[i], n[i], v[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            ss = __builtin_fmaf(v[i][e], v[i][e], ss);
+            if (Q8) {
+                // (as integers the bits of non-negative floats order as the floats do, NaNs above all)
+                v[i][e] = v[i][e] * g[i][e];
+                const uint32_t b = __float_as_uint(v[i][e]) & 0x7fffffffu;
+                top = b > top ? b : top;
+            }
+        }
+    ss = wave_sum_f(ss);
+    if (Q8) top = wave_max_u(top);
+    if (WPR > 1) {
+        if (lane_id() == 0) part[wv] = Part{ss, top};
+        __syncthreads();
+        ss = 0.0f;
+        top = 0u;
+#pragma unroll
+        for (int i = 0; i < WPR; ++i) {
+            const Part p = part[first + i];
+            ss = ss + p.ss;
+            top = p.top > top ? p.top : top;
+        }
+    }
+    const float r = 1.0f / __builtin_sqrtf(ss / (float)H + a.eps);
+    YT* y = static_cast<YT*>(a.y) + row * a.y_stride;
+    if constexpr (!Q8) {
+        if (!live) return;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[i][e] = v[i][e] * r * g[i][e];
+            Io<YT>::store(y + c[i], n[i], v[i]);
+        }
+    } else {
+        // The factor out of [1e-30, 1e30], or a row with an inf, a NaN or a sum of squares
+        // past f32: the formula itself, element by element. A row whose largest
+        // |y| is 0 or a NaN has scale 1.
+        const float m = __uint_as_float(top);
+        const bool plain = top == 0u || (m > 1e-30f && m < 1e30f && ss < 3e38f);
+        float scale, inv;
+        if (plain) {
+            scale = top == 0u ? 1.0f : m * r / kE4m3Max;
+            inv = top == 0u ? 0.0f : kE4m3Max / m;
+        } else {
+            uint32_t t2 = 0u;
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    v[i][e] = v[i][e] * r;
+                    const uint32_t b = (uint32_t)e < n[i] ? __float_as_uint(v[i][e]) & 0x7fffffffu : 0u;
+                    t2 = b > t2 ? b : t2;
+                }
+            top = wave_max_u(t2);
+            scale = inv = 1.0f;
+        }
+        if (WPR > 1) {
+            // (every wave of a row goes the same way; rows of one workgroup may not: the barrier is outside the branch)
+            if (!plain && lane_id() == 0) part2[wv] = top;
+            __syncthreads();
+        }
+        if (!plain) {
+            if (WPR > 1) {
+                top = 0u;
+#pragma unroll
+                for (int i = 0; i < WPR; ++i) top = part2[first + i] > top ? part2[first + i] : top;
+            }
+            const bool nan = top > 0x7f800000u;
+            // (a scale below the smallest normal number would lose its bits)
+            if (!nan && top != 0u) {
+                scale = __uint_as_float(top) / kE4m3Max;
+                scale = scale < 1.17549435e-38f ? 1.17549435e-38f : scale;
+            }
+        }
+        if (!live) return;
+        if (t == 0u) a.y_scale[row] = scale;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[i][e] = clamp448(plain ? v[i][e] * inv : v[i][e] / scale);
+            Io<YT>::store(y + c[i], n[i], v[i]);
+        }
+    }
+}
+
+namespace {
+
+template <typename XT, typename YT, bool RES, int WPR, int NV>
+void go(const NormArgs& a, hipStream_t st) {
+    constexpr uint32_t per = WPR < 4 ? 4 / WPR : 1;
+    hipLaunchKernelGGL((add_rmsnorm<XT, YT, RES, WPR, NV>), dim3((uint32_t)((a.rows + per - 1u) / per)),
+                       dim3((WPR < 4 ? 4 : WPR) * kWave), 0, st, a);
+}
+template <typename XT, typename YT, bool RES>
+void pick(const NormArgs& a, hipStream_t st) {
+    const uint32_t groups = (a.hidden + 7u) / 8u;
+    if (groups <= 64u) go<XT, YT, RES, 1, 1>(a, st);
+    else if (groups <= 256u) go<XT, YT, RES, 4, 1>(a, st);
+    else if (groups <= 512u) go<XT, YT, RES, 4, 2>(a, st);
+    else if (groups <= 1024u) go<XT, YT, RES, 4, 4>(a, st);
+    else if (groups <= 2048u) go<XT, YT, RES, 8, 4>(a, st);
+    else go<XT, YT, RES, 16, 4>(a, st);
+}
+template <typename XT, typename YT>
+void pick_res(const NormArgs& a, hipStream_t st) {
+    if (a.residual) pick<XT, YT, true>(a, st);
+    else pick<XT, YT, false>(a, st);
+}
+template <typename XT>
+void pick_out(const NormArgs& a, uint32_t y_dtype, hipStream_t st) {
+    if (y_dtype == LCS_E4M3) pick_res<XT, uint8_t>(a, st);
+    else if (y_dtype == LCS_BF16) pick_res<XT, uint16_t>(a, st);
+    else pick_res<XT, float>(a, st);
+}
+
+}  // namespace
+
+hipError_t launch_add_rmsnorm(const NormArgs& a, uint32_t x_dtype, uint32_t y_dtype, hipStream_t st) {
+    if (x_dtype == LCS_BF16) pick_out<uint16_t>(a, y_dtype, st);
+    else pick_out<float>(a, y_dtype, st);
+    return hipGetLastError();
+}
+
+}  // namespace lcs

@@ -17,7 +17,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "liblocus_sampler.so")
 
 LCS_OK, LCS_ERR_INVALID_ARG, LCS_ERR_NO_DEVICE, LCS_ERR_HIP, LCS_ERR_CAPACITY = 0, -1, -2, -3, -4
-LCS_F32, LCS_BF16 = 0, 1
+LCS_F32, LCS_BF16, LCS_E4M3 = 0, 1, 2
 LCS_WANT_LOGPROBS, LCS_WRITE_PENALIZED = 1, 2
 PATH_GREEDY, PATH_WINDOW, PATH_WINDOW_EXACT, PATH_GENERAL = 1, 2, 3, 4
 
@@ -27,6 +27,7 @@ DIAG_DTYPE = np.dtype([
 ])
 
 _P = C.c_void_p
+_DTYPES = {"torch.float32": LCS_F32, "torch.bfloat16": LCS_BF16, "torch.float8_e4m3fn": LCS_E4M3}
 
 
 class _Batch(C.Structure):
@@ -70,8 +71,59 @@ class _LOut(C.Structure):
                 ("draft_lp", _P), ("accept_len", _P), ("stats", _P)]
 
 
+class _Adapters(C.Structure):
+    _fields_ = [("n", C.c_uint32), ("wide", C.c_uint32), ("a", _P), ("b", _P), ("rank", _P), ("scale", _P)]
+
+
+class _LExBatch(C.Structure):
+    _fields_ = [("rows", C.c_uint32), ("vocab", C.c_uint32), ("hidden", C.c_uint32),
+                ("rows_per_seq", C.c_uint32), ("dtype", C.c_uint32), ("x", _P), ("w", _P), ("x_scale", _P),
+                ("w_scale", _P), ("draft", _P), ("adapters", C.POINTER(_Adapters)), ("slot", _P)]
+
+
+class _NBatch(C.Structure):
+    _fields_ = [("rows", C.c_uint32), ("hidden", C.c_uint32), ("x_dtype", C.c_uint32), ("y_dtype", C.c_uint32),
+                ("eps", C.c_float), ("x", _P), ("residual", _P), ("weight", _P), ("x_stride", C.c_uint64),
+                ("residual_stride", C.c_uint64)]
+
+
+class _NOut(C.Structure):
+    _fields_ = [("y", _P), ("y_scale", _P), ("sum", _P), ("y_stride", C.c_uint64), ("sum_stride", C.c_uint64)]
+
+
 class SamplerError(RuntimeError):
     pass
+
+
+def _addr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _need(ok: bool, what: str):
+    if not ok:
+        raise SamplerError(what)
+
+
+class Adapters:
+    """A pool of n low-rank adapters for lmhead_ex_dev: `a` (n, wide, hidden)
+    and `b` (n, vocab, wide) bf16, contiguous, wide a multiple of 8; `rank`
+    (n,) int32 and `scale` (n,) f32, or None (wide, and 1). Device tensors;
+    nothing is copied."""
+
+    def __init__(self, a, b, rank=None, scale=None):
+        import torch
+        _need(a.dtype == torch.bfloat16 and b.dtype == torch.bfloat16, "adapters: a and b must be bfloat16")
+        _need(a.dim() == 3 and b.dim() == 3 and a.shape[0] == b.shape[0] and a.shape[1] == b.shape[2],
+              "adapters: a must be (n, wide, hidden) and b (n, vocab, wide)")
+        _need(a.is_contiguous() and b.is_contiguous(), "adapters: a and b must be contiguous")
+        n, self.wide, self.hidden = a.shape
+        self.n, self.vocab, self.device = n, b.shape[1], a.device
+        _need(b.device == a.device, "adapters: tensors on different devices")
+        for t, dtype, name in ((rank, torch.int32, "rank"), (scale, torch.float32, "scale")):
+            _need(t is None or (t.dtype == dtype and t.shape == (n,) and t.is_contiguous() and t.device == a.device),
+                  f"adapters: {name} must be (n,) {dtype}, contiguous, on the adapters' device")
+        self._keep = (a, b, rank, scale)
+        self._c = _Adapters(n, self.wide, a.data_ptr(), b.data_ptr(), _addr(rank), _addr(scale))
 
 
 _lib = None
@@ -100,6 +152,10 @@ def lib():
         L.lcs_ngram_draft.argtypes = [_P, C.POINTER(_DBatch), C.POINTER(_DOut), _P]
         L.lcs_lmhead.restype = C.c_int
         L.lcs_lmhead.argtypes = [_P, C.POINTER(_LBatch), C.POINTER(_LOut), _P]
+        L.lcs_lmhead_ex.restype = C.c_int
+        L.lcs_lmhead_ex.argtypes = [_P, C.POINTER(_LExBatch), C.POINTER(_LOut), _P]
+        L.lcs_add_rmsnorm.restype = C.c_int
+        L.lcs_add_rmsnorm.argtypes = [_P, C.POINTER(_NBatch), C.POINTER(_NOut), _P]
         L.lcs_last_error.restype = C.c_char_p
         L.lcs_last_error.argtypes = [_P]
         L.lcs_logprobs.restype = C.c_int
@@ -137,6 +193,7 @@ class Sampler:
         import torch  # plumbing: device memory and streams
         self.torch = torch
         self.device = device
+        self._dev = torch.device("cuda", device)
         L = lib()
         self.ctx = L.lcs_create(device, max_rows, max_vocab, max_hist, max_top)
         if not self.ctx:
@@ -471,6 +528,84 @@ class Sampler:
         if stats:   # lcs_row_stats: (f64 log_z, f32 max, i32 argmax) per row
             out["stats"] = torch.full((rows, 2), -7.0, dtype=torch.float64, device=dev)
         return out
+
+    def _vec(self, t, n: int, dtype, name: str):
+        """The address of an optional (n,) device vector."""
+        if t is None:
+            return None
+        _need(t.dtype == dtype and t.shape == (n,) and t.is_contiguous() and t.device == self._dev,
+              f"{name} must be ({n},) {dtype}, contiguous, on the sampler's device")
+        return t.data_ptr()
+
+    def lmhead_ex_dev(self, x, w, out, x_scale=None, w_scale=None, adapters: Adapters | None = None, slot=None,
+                      draft=None, rows_per_seq: int = 0, stream=None):
+        """The fused lm-head product in bf16 or 8 bits, with the rows' adapters
+        (lcs_lmhead_ex): x (rows, hidden) and w (vocab, hidden), contiguous,
+        both bf16 or both float8_e4m3fn (then `x_scale` (rows,) and `w_scale`
+        (vocab,) f32, or None for 1); `adapters` with `slot` (rows,) int32, the
+        row's adapter or -1. `out` as for lmhead_dev."""
+        torch = self.torch
+        dtype = _DTYPES.get(str(x.dtype))
+        _need(dtype in (LCS_BF16, LCS_E4M3) and w.dtype == x.dtype, "x and w must both be bfloat16 or both float8_e4m3fn")
+        _need(x.dim() == 2 and w.dim() == 2 and x.is_contiguous() and w.is_contiguous(),
+              "x and w must be 2-d and contiguous")
+        _need(x.device == self._dev and w.device == self._dev, "x and w must be on the sampler's device")
+        (rows, hidden), vocab = x.shape, w.shape[0]
+        _need(w.shape[1] == hidden, "x and w disagree on hidden")
+        ad = None
+        if adapters is not None:
+            _need(adapters.hidden == hidden and adapters.vocab == vocab and adapters.device == self._dev,
+                  "the adapters' hidden, vocab or device are not those of x and w")
+            _need(slot is not None, "adapters need slot")
+            ad = C.pointer(adapters._c)
+        i32, f32, vec = torch.int32, torch.float32, self._vec
+        b = _LExBatch(rows, vocab, hidden, rows_per_seq, dtype, x.data_ptr(), w.data_ptr(),
+                      vec(x_scale, rows, f32, "x_scale"), vec(w_scale, vocab, f32, "w_scale"),
+                      vec(draft, rows, i32, "draft"), ad, vec(slot, rows, i32, "slot"))
+        lg, ld = out.get("logits"), 0
+        if lg is not None:
+            _need(lg.dtype == f32 and lg.dim() == 2 and lg.shape[0] == rows and lg.shape[1] >= vocab and
+                  lg.stride(1) == 1 and lg.device == self._dev,
+                  "logits must be (rows, >= vocab) f32 with unit column stride, on the sampler's device")
+            ld = lg.stride(0) if rows > 1 else max(lg.stride(0), vocab)
+        acc, st = out.get("accept_len"), out.get("stats")
+        _need(acc is None or (rows_per_seq > 0 and acc.dtype == i32 and acc.numel() * rows_per_seq >= rows and
+                              acc.is_contiguous() and acc.device == self._dev),
+              "accept_len must be (rows / rows_per_seq,) int32")
+        _need(st is None or (st.is_contiguous() and st.numel() * st.element_size() >= 16 * rows and st.device == self._dev),
+              "stats must hold 16 contiguous bytes a row")
+        o = _LOut(_addr(lg), ld, vec(out.get("argmax_ids"), rows, i32, "argmax_ids"), vec(out.get("log_z"), rows, f32, "log_z"),
+                  vec(out.get("draft_lp"), rows, f32, "draft_lp"), _addr(acc), _addr(st))
+        self._check(lib().lcs_lmhead_ex(self.ctx, b, o, _stream_handle(torch, stream)))
+
+    def add_rmsnorm_dev(self, x, weight, out, residual=None, eps: float = 1e-6, stream=None):
+        """Residual addition and root-mean-square norm (lcs_add_rmsnorm): x and
+        `residual` (rows, hidden), bf16 or f32, any row stride; `weight`
+        (hidden,) of their type. `out` holds "y" (rows, hidden) in bf16, f32 or
+        float8_e4m3fn (then "y_scale" (rows,) f32 too) and, with a residual,
+        optionally "sum" of x's type; missing keys are not written (y is
+        required)."""
+        torch, dev = self.torch, self._dev
+        y, total = out["y"], out.get("sum")
+        xt, yt = _DTYPES.get(str(x.dtype)), _DTYPES.get(str(y.dtype))
+        _need(xt in (LCS_F32, LCS_BF16), "x must be float32 or bfloat16")
+        _need(yt is not None, "y must be float32, bfloat16 or float8_e4m3fn")
+        _need(x.dim() == 2, "x must be (rows, hidden)")
+        rows, hidden = x.shape
+        _need(weight.dtype == x.dtype, "weight must have x's type")
+
+        def mat(t, dtype, name):
+            _need(t.dtype == dtype and t.shape == (rows, hidden) and (t.stride(1) == 1 or hidden == 1) and t.device == dev,
+                  f"{name} must be ({rows}, {hidden}) {dtype} with unit column stride, on the sampler's device")
+            return t.data_ptr(), t.stride(0) if rows > 1 else hidden
+
+        xp, xs = mat(x, x.dtype, "x")
+        rp, rs = (None, 0) if residual is None else mat(residual, x.dtype, "residual")
+        yp, ys = mat(y, y.dtype, "y")
+        sp, ss = (None, 0) if total is None else mat(total, x.dtype, "sum")
+        b = _NBatch(rows, hidden, xt, yt, eps, xp, rp, self._vec(weight, hidden, x.dtype, "weight"), xs, rs)
+        o = _NOut(yp, self._vec(out.get("y_scale"), rows, torch.float32, "y_scale"), sp, ys, ss)
+        self._check(lib().lcs_add_rmsnorm(self.ctx, b, o, _stream_handle(torch, stream)))
 
     def verify(self, w):
         d = self.upload(w)
