@@ -259,8 +259,7 @@ typedef struct lcs_adapters {
 
 /* lcs_lmhead_batch with the operands' type, their scales and the rows' adapters:
  * logits[i][v] = x_scale[i] w_scale[v] sum_k x[i][k] w[v][k], plus the product of
- * the row's adapter on x_scale[i] x[i]. Low-rank states are kept to 16 bits of
- * mantissa, everything else in f32. */
+ * the row's adapter on x_scale[i] x[i]. All sums are f32 sums of exact products. */
 typedef struct lcs_lmhead_ex_batch {
     uint32_t rows;             /* hidden vectors, <= the context's max_rows */
     uint32_t vocab;            /* <= the context's max_vocab */

@@ -273,8 +273,8 @@ struct LmArgs {
     const int32_t* slot;            // rows: the row's adapter, or -1
     // ... as lm_low leaves them: the rows in the order of their adapters
     uint32_t* perm;                 // rows: the row at a position
-    int32_t* pslot;                 // rows: its adapter, or -1 (also for a rank of 0)
-    uint16_t* low;                  // rows x 2 x ad_wide: its low-rank state, upper and lower bf16 part
+    int32_t* pslot;                 // rows: its adapter's rank << 16 | its adapter, or -1 (also for a rank of 0)
+    uint16_t* low;                  // rows x 3 x ad_wide: its low-rank state, as the sum of three bf16 parts
 };
 constexpr uint32_t kAdMax = 1024;       // adapters of a pool
 constexpr uint32_t kAdWideMax = 256;    // their widest rank

@@ -27,7 +27,6 @@ DIAG_DTYPE = np.dtype([
 ])
 
 _P = C.c_void_p
-_DTYPES = {"torch.float32": LCS_F32, "torch.bfloat16": LCS_BF16, "torch.float8_e4m3fn": LCS_E4M3}
 
 
 class _Batch(C.Structure):
@@ -99,11 +98,6 @@ def _addr(t):
     return None if t is None else t.data_ptr()
 
 
-def _need(ok: bool, what: str):
-    if not ok:
-        raise SamplerError(what)
-
-
 class Adapters:
     """A pool of n low-rank adapters for lmhead_ex_dev: `a` (n, wide, hidden)
     and `b` (n, vocab, wide) bf16, contiguous, wide a multiple of 8; `rank`
@@ -112,16 +106,20 @@ class Adapters:
 
     def __init__(self, a, b, rank=None, scale=None):
         import torch
-        _need(a.dtype == torch.bfloat16 and b.dtype == torch.bfloat16, "adapters: a and b must be bfloat16")
-        _need(a.dim() == 3 and b.dim() == 3 and a.shape[0] == b.shape[0] and a.shape[1] == b.shape[2],
-              "adapters: a must be (n, wide, hidden) and b (n, vocab, wide)")
-        _need(a.is_contiguous() and b.is_contiguous(), "adapters: a and b must be contiguous")
+        if a.dtype != torch.bfloat16 or b.dtype != torch.bfloat16:
+            raise SamplerError("adapters: a and b must be bfloat16")
+        if a.dim() != 3 or b.dim() != 3 or a.shape[0] != b.shape[0] or a.shape[1] != b.shape[2]:
+            raise SamplerError("adapters: a must be (n, wide, hidden) and b (n, vocab, wide)")
+        if not (a.is_contiguous() and b.is_contiguous()):
+            raise SamplerError("adapters: a and b must be contiguous")
         n, self.wide, self.hidden = a.shape
-        self.n, self.vocab, self.device = n, b.shape[1], a.device
-        _need(b.device == a.device, "adapters: tensors on different devices")
+        self.n, self.vocab, self.device = n, b.shape[1], a.get_device()
+        if b.get_device() != self.device:
+            raise SamplerError("adapters: tensors on different devices")
         for t, dtype, name in ((rank, torch.int32, "rank"), (scale, torch.float32, "scale")):
-            _need(t is None or (t.dtype == dtype and t.shape == (n,) and t.is_contiguous() and t.device == a.device),
-                  f"adapters: {name} must be (n,) {dtype}, contiguous, on the adapters' device")
+            if t is not None and (t.dtype != dtype or t.dim() != 1 or t.numel() != n or not t.is_contiguous() or
+                                  t.get_device() != self.device):
+                raise SamplerError(f"adapters: {name} must be ({n},) {dtype}, contiguous, on the adapters' device")
         self._keep = (a, b, rank, scale)
         self._c = _Adapters(n, self.wide, a.data_ptr(), b.data_ptr(), _addr(rank), _addr(scale))
 
@@ -193,7 +191,7 @@ class Sampler:
         import torch  # plumbing: device memory and streams
         self.torch = torch
         self.device = device
-        self._dev = torch.device("cuda", device)
+        self._types = {torch.float32: LCS_F32, torch.bfloat16: LCS_BF16, torch.float8_e4m3fn: LCS_E4M3}
         L = lib()
         self.ctx = L.lcs_create(device, max_rows, max_vocab, max_hist, max_top)
         if not self.ctx:
@@ -529,13 +527,20 @@ class Sampler:
             out["stats"] = torch.full((rows, 2), -7.0, dtype=torch.float64, device=dev)
         return out
 
+    # (a serving step makes these two calls once a token: their checks read each
+    # tensor's attributes once, and messages are put together where one is raised)
     def _vec(self, t, n: int, dtype, name: str):
         """The address of an optional (n,) device vector."""
         if t is None:
             return None
-        _need(t.dtype == dtype and t.shape == (n,) and t.is_contiguous() and t.device == self._dev,
-              f"{name} must be ({n},) {dtype}, contiguous, on the sampler's device")
+        if t.dtype != dtype or t.dim() != 1 or t.numel() != n or not t.is_contiguous() or t.get_device() != self.device:
+            raise SamplerError(f"{name} must be ({n},) {dtype}, contiguous, on the sampler's device")
         return t.data_ptr()
+
+    def _raw_stream(self, stream):
+        if stream is not None:
+            return stream.cuda_stream
+        return self.torch.cuda.current_stream(self.device).cuda_stream
 
     def lmhead_ex_dev(self, x, w, out, x_scale=None, w_scale=None, adapters: Adapters | None = None, slot=None,
                       draft=None, rows_per_seq: int = 0, stream=None):
@@ -545,38 +550,47 @@ class Sampler:
         (vocab,) f32, or None for 1); `adapters` with `slot` (rows,) int32, the
         row's adapter or -1. `out` as for lmhead_dev."""
         torch = self.torch
-        dtype = _DTYPES.get(str(x.dtype))
-        _need(dtype in (LCS_BF16, LCS_E4M3) and w.dtype == x.dtype, "x and w must both be bfloat16 or both float8_e4m3fn")
-        _need(x.dim() == 2 and w.dim() == 2 and x.is_contiguous() and w.is_contiguous(),
-              "x and w must be 2-d and contiguous")
-        _need(x.device == self._dev and w.device == self._dev, "x and w must be on the sampler's device")
-        (rows, hidden), vocab = x.shape, w.shape[0]
-        _need(w.shape[1] == hidden, "x and w disagree on hidden")
+        dtype = self._types.get(x.dtype)
+        if dtype not in (LCS_BF16, LCS_E4M3) or w.dtype != x.dtype:
+            raise SamplerError("x and w must both be bfloat16 or both float8_e4m3fn")
+        if x.dim() != 2 or w.dim() != 2 or not (x.is_contiguous() and w.is_contiguous()):
+            raise SamplerError("x and w must be 2-d and contiguous")
+        if x.get_device() != self.device or w.get_device() != self.device:
+            raise SamplerError("x and w must be on the sampler's device")
+        (rows, hidden), (vocab, wh) = x.shape, w.shape
+        if wh != hidden:
+            raise SamplerError("x and w disagree on hidden")
         ad = None
         if adapters is not None:
-            _need(adapters.hidden == hidden and adapters.vocab == vocab and adapters.device == self._dev,
-                  "the adapters' hidden, vocab or device are not those of x and w")
-            _need(slot is not None, "adapters need slot")
+            if adapters.hidden != hidden or adapters.vocab != vocab or adapters.device != self.device:
+                raise SamplerError("the adapters' hidden, vocab or device are not those of x and w")
+            if slot is None:
+                raise SamplerError("adapters need slot")
             ad = C.pointer(adapters._c)
         i32, f32, vec = torch.int32, torch.float32, self._vec
         b = _LExBatch(rows, vocab, hidden, rows_per_seq, dtype, x.data_ptr(), w.data_ptr(),
                       vec(x_scale, rows, f32, "x_scale"), vec(w_scale, vocab, f32, "w_scale"),
                       vec(draft, rows, i32, "draft"), ad, vec(slot, rows, i32, "slot"))
-        lg, ld = out.get("logits"), 0
+        lg, lp, ld = out.get("logits"), None, 0
         if lg is not None:
-            _need(lg.dtype == f32 and lg.dim() == 2 and lg.shape[0] == rows and lg.shape[1] >= vocab and
-                  lg.stride(1) == 1 and lg.device == self._dev,
-                  "logits must be (rows, >= vocab) f32 with unit column stride, on the sampler's device")
-            ld = lg.stride(0) if rows > 1 else max(lg.stride(0), vocab)
+            if (lg.dtype != f32 or lg.dim() != 2 or lg.shape[0] != rows or lg.shape[1] < vocab or
+                    (lg.stride(1) != 1 and vocab > 1) or lg.get_device() != self.device):
+                raise SamplerError("logits must be (rows, >= vocab) f32 with unit column stride, on the sampler's device")
+            lp, ld = lg.data_ptr(), lg.stride(0) if rows > 1 else vocab
         acc, st = out.get("accept_len"), out.get("stats")
-        _need(acc is None or (rows_per_seq > 0 and acc.dtype == i32 and acc.numel() * rows_per_seq >= rows and
-                              acc.is_contiguous() and acc.device == self._dev),
-              "accept_len must be (rows / rows_per_seq,) int32")
-        _need(st is None or (st.is_contiguous() and st.numel() * st.element_size() >= 16 * rows and st.device == self._dev),
-              "stats must hold 16 contiguous bytes a row")
-        o = _LOut(_addr(lg), ld, vec(out.get("argmax_ids"), rows, i32, "argmax_ids"), vec(out.get("log_z"), rows, f32, "log_z"),
-                  vec(out.get("draft_lp"), rows, f32, "draft_lp"), _addr(acc), _addr(st))
-        self._check(lib().lcs_lmhead_ex(self.ctx, b, o, _stream_handle(torch, stream)))
+        if acc is not None and rows_per_seq > 0:
+            acc = vec(acc, rows // rows_per_seq, i32, "accept_len")
+        elif acc is not None:
+            raise SamplerError("accept_len needs rows_per_seq")
+        if st is not None:
+            if not st.is_contiguous() or st.numel() * st.element_size() < 16 * rows or st.get_device() != self.device:
+                raise SamplerError("stats must hold 16 contiguous bytes a row, on the sampler's device")
+            st = st.data_ptr()
+        o = _LOut(lp, ld, vec(out.get("argmax_ids"), rows, i32, "argmax_ids"), vec(out.get("log_z"), rows, f32, "log_z"),
+                  vec(out.get("draft_lp"), rows, f32, "draft_lp"), acc, st)
+        rc = _lib.lcs_lmhead_ex(self.ctx, b, o, self._raw_stream(stream))
+        if rc != LCS_OK:
+            self._check(rc)
 
     def add_rmsnorm_dev(self, x, weight, out, residual=None, eps: float = 1e-6, stream=None):
         """Residual addition and root-mean-square norm (lcs_add_rmsnorm): x and
@@ -585,27 +599,35 @@ class Sampler:
         float8_e4m3fn (then "y_scale" (rows,) f32 too) and, with a residual,
         optionally "sum" of x's type; missing keys are not written (y is
         required)."""
-        torch, dev = self.torch, self._dev
-        y, total = out["y"], out.get("sum")
-        xt, yt = _DTYPES.get(str(x.dtype)), _DTYPES.get(str(y.dtype))
-        _need(xt in (LCS_F32, LCS_BF16), "x must be float32 or bfloat16")
-        _need(yt is not None, "y must be float32, bfloat16 or float8_e4m3fn")
-        _need(x.dim() == 2, "x must be (rows, hidden)")
-        rows, hidden = x.shape
-        _need(weight.dtype == x.dtype, "weight must have x's type")
-
-        def mat(t, dtype, name):
-            _need(t.dtype == dtype and t.shape == (rows, hidden) and (t.stride(1) == 1 or hidden == 1) and t.device == dev,
-                  f"{name} must be ({rows}, {hidden}) {dtype} with unit column stride, on the sampler's device")
-            return t.data_ptr(), t.stride(0) if rows > 1 else hidden
-
-        xp, xs = mat(x, x.dtype, "x")
-        rp, rs = (None, 0) if residual is None else mat(residual, x.dtype, "residual")
-        yp, ys = mat(y, y.dtype, "y")
-        sp, ss = (None, 0) if total is None else mat(total, x.dtype, "sum")
-        b = _NBatch(rows, hidden, xt, yt, eps, xp, rp, self._vec(weight, hidden, x.dtype, "weight"), xs, rs)
-        o = _NOut(yp, self._vec(out.get("y_scale"), rows, torch.float32, "y_scale"), sp, ys, ss)
-        self._check(lib().lcs_add_rmsnorm(self.ctx, b, o, _stream_handle(torch, stream)))
+        y, total, dtype, dev = out["y"], out.get("sum"), x.dtype, self.device
+        ytype = y.dtype
+        xt, yt = self._types.get(dtype), self._types.get(ytype)
+        if xt not in (LCS_F32, LCS_BF16):
+            raise SamplerError("x must be float32 or bfloat16")
+        if yt is None:
+            raise SamplerError("y must be float32, bfloat16 or float8_e4m3fn")
+        shape = x.shape
+        if len(shape) != 2:
+            raise SamplerError("x must be (rows, hidden)")
+        rows, hidden = shape
+        at = []   # address and row stride of each
+        for t, want in ((x, dtype), (residual, dtype), (y, ytype), (total, dtype)):
+            if t is None:
+                at += (None, 0)
+                continue
+            if t.dtype != want or t.shape != shape or t.get_device() != dev:
+                name = "x" if t is x else "residual" if t is residual else "y" if t is y else "sum"
+                raise SamplerError(f"{name} must be ({rows}, {hidden}) {want} on the sampler's device")
+            per, one = t.stride()
+            if one != 1 and hidden > 1:
+                raise SamplerError("rows must have unit column stride")
+            at += (t.data_ptr(), per if rows > 1 else hidden)
+        xp, xs, rp, rs, yp, ys, sp, ss = at
+        b = _NBatch(rows, hidden, xt, yt, eps, xp, rp, self._vec(weight, hidden, dtype, "weight"), xs, rs)
+        o = _NOut(yp, self._vec(out.get("y_scale"), rows, self.torch.float32, "y_scale"), sp, ys, ss)
+        rc = _lib.lcs_add_rmsnorm(self.ctx, b, o, self._raw_stream(stream))
+        if rc != LCS_OK:
+            self._check(rc)
 
     def verify(self, w):
         d = self.upload(w)
