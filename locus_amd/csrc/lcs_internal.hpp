@@ -293,6 +293,7 @@ struct NormArgs {
     uint64_t rows;
     uint32_t hidden;
     float eps;
+    uint32_t waves, per;            // waves a row, rows a workgroup (launch_add_rmsnorm)
 };
 
 // status bits

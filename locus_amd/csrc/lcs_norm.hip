@@ -38,11 +38,10 @@ typedef u32x2 u32x2_1 __attribute__((aligned(1), may_alias));
 constexpr float kE4m3Max = 448.0f;
 
 __device__ __forceinline__ float bf16_to_f(uint32_t u) { return __uint_as_float(u << 16); }
-// (round to nearest even; a NaN keeps its upper bits with the quiet one set)
-__device__ __forceinline__ uint32_t f_to_bf16(float f) {
-    const uint32_t u = __float_as_uint(f);
-    if ((u & 0x7fffffffu) > 0x7f800000u) return (u >> 16) | 0x40u;
-    return (u + 0x7fffu + ((u >> 16) & 1u)) >> 16;
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t f_to_bf16x2(float a, float b) {   // to nearest even
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){a, b}, bf16x2));
 }
 
 // 8 elements from p; in a row's last lane only the first n exist.
@@ -62,15 +61,15 @@ template <> struct Io<uint16_t> {   // bf16
         }
     }
     static __device__ __forceinline__ void store(uint16_t* p, uint32_t n, const float (&v)[8]) {
-        uint32_t b[8];
+        u32x4 q;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) b[i] = f_to_bf16(v[i]);
+        for (int i = 0; i < 4; ++i) q[i] = f_to_bf16x2(v[2 * i], v[2 * i + 1]);
         if (n >= 8u) {
-            *reinterpret_cast<u32x4_2*>(p) = u32x4{b[0] | b[1] << 16, b[2] | b[3] << 16, b[4] | b[5] << 16, b[6] | b[7] << 16};
+            __builtin_nontemporal_store(q, reinterpret_cast<u32x4_2*>(p));
         } else {
 #pragma unroll
             for (uint32_t i = 0; i < 8u; ++i)
-                if (i < n) p[i] = (uint16_t)b[i];
+                if (i < n) p[i] = (uint16_t)(q[i / 2u] >> (16u * (i % 2u)));
         }
     }
 };
@@ -96,8 +95,8 @@ template <> struct Io<float> {
                 q[i] = __float_as_uint(v[i]);
                 r[i] = __float_as_uint(v[4 + i]);
             }
-            *reinterpret_cast<u32x4_4*>(p) = q;
-            *reinterpret_cast<u32x4_4*>(p + 4) = r;
+            __builtin_nontemporal_store(q, reinterpret_cast<u32x4_4*>(p));
+            __builtin_nontemporal_store(r, reinterpret_cast<u32x4_4*>(p + 4));
         } else {
 #pragma unroll
             for (uint32_t i = 0; i < 8u; ++i)
@@ -116,7 +115,7 @@ template <> struct Io<uint8_t> {   // e4m3; finite values are inside +-448 alrea
             q[i] = (uint32_t)w;
         }
         if (n >= 8u) {
-            *reinterpret_cast<u32x2_1*>(p) = u32x2{q[0], q[1]};
+            __builtin_nontemporal_store(u32x2{q[0], q[1]}, reinterpret_cast<u32x2_1*>(p));
         } else {
 #pragma unroll
             for (uint32_t i = 0; i < 8u; ++i)
@@ -136,18 +135,24 @@ __device__ __forceinline__ float clamp448(float v) {   // (a NaN stays one)
 
 }  // namespace
 
-// WPR waves per row, each lane NV groups of 8 elements; a workgroup of up to
-// four waves takes 4 / WPR rows.
-template <typename XT, typename YT, bool RES, int WPR, int NV>
-__global__ __launch_bounds__((WPR < 4 ? 4 : WPR) * kWave) void add_rmsnorm(NormArgs a) {
+// a.waves waves per row, each lane NV groups of 8 elements, a.per rows per workgroup.
+// One group a lane up to 8192 columns, as many waves as that takes: the row's
+// chain of loads, exchange and stores is then shortest, and most rows are in
+// flight (bf16 into e4m3 with a residual, us by 4 / 2 / 1 groups: 8192 x 8192
+// 117 / 96 / 93, 1 x 4096 6.7 / 4.3 / 3.2, 512 x 4096 10.0 / 7.1 / 6.1). Above,
+// four (4096 x 16384: 115, with two 120). What is written is not read here
+// again: stores past the caches' usual order (8192 x 8192 93 -> 90, 4096 x 16384
+// 115 -> 106; loads like that cost 3 to 15 %).
+template <typename XT, typename YT, bool RES, int NV>
+__global__ __launch_bounds__(1024) void add_rmsnorm(NormArgs a) {
     constexpr bool Q8 = sizeof(YT) == 1;
-    constexpr int NW = WPR < 4 ? 4 : WPR;
     struct Part { float ss; uint32_t top; };
-    __shared__ Part part[NW];
-    __shared__ uint32_t part2[NW];
+    __shared__ Part part[16];
+    __shared__ uint32_t part2[16];
+    const uint32_t WPR = a.waves;
     const uint32_t tid = tid_x(), wv = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid / kWave));
-    const uint32_t first = wv / WPR * WPR;                     // the row's first wave
-    const uint64_t row0 = (uint64_t)wg_x() * (NW / WPR) + wv / WPR;
+    const uint32_t rw = wv / WPR, first = rw * WPR;            // the row in the workgroup, its first wave
+    const uint64_t row0 = (uint64_t)wg_x() * a.per + rw;
     const bool live = row0 < a.rows;                           // (no early end: the waves meet at a barrier)
     const uint64_t row = live ? row0 : a.rows - 1u;
     const uint32_t H = a.hidden, t = (wv - first) * kWave + (uint32_t)lane_id();
@@ -195,17 +200,13 @@ __global__ __launch_bounds__((WPR < 4 ? 4 : WPR) * kWave) void add_rmsnorm(NormA
         }
     ss = wave_sum_f(ss);
     if (Q8) top = wave_max_u(top);
-    if (WPR > 1) {
+    if (WPR > 1u) {
         if (lane_id() == 0) part[wv] = Part{ss, top};
         __syncthreads();
-        ss = 0.0f;
-        top = 0u;
-#pragma unroll
-        for (int i = 0; i < WPR; ++i) {
-            const Part p = part[first + i];
-            ss = ss + p.ss;
-            top = p.top > top ? p.top : top;
-        }
+        const bool in = (uint32_t)lane_id() < WPR;
+        const Part p = part[in ? first + (uint32_t)lane_id() : first];
+        ss = wave_sum_f(in ? p.ss : 0.0f);
+        if (Q8) top = wave_max_u(p.top);
     }
     const float r = 1.0f / __builtin_sqrtf(ss / (float)H + a.eps);
     YT* y = static_cast<YT*>(a.y) + row * a.y_stride;
@@ -240,16 +241,14 @@ __global__ __launch_bounds__((WPR < 4 ? 4 : WPR) * kWave) void add_rmsnorm(NormA
             top = wave_max_u(t2);
             scale = inv = 1.0f;
         }
-        if (WPR > 1) {
+        if (WPR > 1u) {
             // (every wave of a row goes the same way; rows of one workgroup may not: the barrier is outside the branch)
             if (!plain && lane_id() == 0) part2[wv] = top;
             __syncthreads();
         }
         if (!plain) {
-            if (WPR > 1) {
-                top = 0u;
-#pragma unroll
-                for (int i = 0; i < WPR; ++i) top = part2[first + i] > top ? part2[first + i] : top;
+            if (WPR > 1u) {
+                top = wave_max_u(part2[(uint32_t)lane_id() < WPR ? first + (uint32_t)lane_id() : first]);
             }
             const bool nan = top > 0x7f800000u;
             // (a scale below the smallest normal number would lose its bits)
@@ -271,21 +270,18 @@ __global__ __launch_bounds__((WPR < 4 ? 4 : WPR) * kWave) void add_rmsnorm(NormA
 
 namespace {
 
-template <typename XT, typename YT, bool RES, int WPR, int NV>
-void go(const NormArgs& a, hipStream_t st) {
-    constexpr uint32_t per = WPR < 4 ? 4 / WPR : 1;
-    hipLaunchKernelGGL((add_rmsnorm<XT, YT, RES, WPR, NV>), dim3((uint32_t)((a.rows + per - 1u) / per)),
-                       dim3((WPR < 4 ? 4 : WPR) * kWave), 0, st, a);
+template <typename XT, typename YT, bool RES, int NV>
+void go(const NormArgs& a0, hipStream_t st) {
+    NormArgs a = a0;
+    a.waves = (a.hidden + 512u * NV - 1u) / (512u * NV);
+    a.per = a.waves < 4u ? 4u / a.waves : 1u;
+    hipLaunchKernelGGL((add_rmsnorm<XT, YT, RES, NV>), dim3((uint32_t)((a.rows + a.per - 1u) / a.per)), dim3(a.waves * a.per * kWave), 0,
+                       st, a);
 }
 template <typename XT, typename YT, bool RES>
 void pick(const NormArgs& a, hipStream_t st) {
-    const uint32_t groups = (a.hidden + 7u) / 8u;
-    if (groups <= 64u) go<XT, YT, RES, 1, 1>(a, st);
-    else if (groups <= 256u) go<XT, YT, RES, 4, 1>(a, st);
-    else if (groups <= 512u) go<XT, YT, RES, 4, 2>(a, st);
-    else if (groups <= 1024u) go<XT, YT, RES, 4, 4>(a, st);
-    else if (groups <= 2048u) go<XT, YT, RES, 8, 4>(a, st);
-    else go<XT, YT, RES, 16, 4>(a, st);
+    if (a.hidden <= 8192u) go<XT, YT, RES, 1>(a, st);
+    else go<XT, YT, RES, 4>(a, st);
 }
 template <typename XT, typename YT>
 void pick_res(const NormArgs& a, hipStream_t st) {
