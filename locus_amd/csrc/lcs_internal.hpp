@@ -266,6 +266,7 @@ struct LmArgs {
     const float* w_scale;           // vocab, or NULL: 1
     // adapters (ad_n 0: none)
     uint32_t ad_n, ad_wide;
+    uint32_t low_z;                 // lm_low's gridDim.z
     const uint16_t* ad_a;           // ad_n x ad_wide x hidden bf16
     const uint16_t* ad_b;           // ad_n x vocab x ad_wide bf16
     const int32_t* ad_rank;         // ad_n, or NULL: ad_wide

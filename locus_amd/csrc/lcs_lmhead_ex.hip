@@ -56,142 +56,139 @@ __device__ __forceinline__ uint32_t to_bf16(float f) {   // finite: to nearest e
 }
 }  // namespace
 
-// Workgroup (i, q): up to 16 rows of one adapter (the i-th such group in the order of
-// the adapters), ranks 16 q to 16 q + 15, over all of k: the waves take 64 k in
-// turn in v_mfma_f32_16x16x32_bf16 tiles (ranks on its row side; lane l carries
-// 8 consecutive k of row l % 16, k chunk l / 16, and returns rows 4 (l / 16) + e of
-// column l % 16), and their sums meet in LDS in a fixed order. Latency bounds it:
-// small tiles make many workgroups, and up to 256 k a wave are loaded at once.
-// Every workgroup finds its group from the rows' slots by itself (a histogram over
-// the adapters and its prefix sums), which costs less than a launch for it would.
-// The groups' first workgroups also write the order, and workgroup 0 that of
-// the rows without an adapter.
+// Workgroup (i, q, z): adapter i, ranks 16 q to 16 q + 15, every gridDim.z-th group of
+// 16 of its rows, from the z-th; where there are fewer rows than adapters i is a row,
+// and the workgroup of an adapter's first row takes it. The rows' slots give the
+// adapter's rows and, by the slots below its own, its place in the order, with one
+// exchange between the waves; the workgroups without work end there. A group goes
+// over all of k, the waves taking 64 k in turn in v_mfma_f32_16x16x32_bf16 tiles (ranks
+// on its row side; lane l carries 8 consecutive k of row l % 16, k chunk l / 16,
+// and returns rows 4 (l / 16) + e of column l % 16), up to 256 k a wave loaded at
+// once, and their sums meet in LDS in a fixed order. Latency bounds it (a launch, the
+// slots, the factor from HBM): small tiles make many workgroups.
 template <bool F8>
 __global__ __launch_bounds__(kLowThreads) void lm_low(LmArgs a) {
-    __shared__ uint32_t hist[kAdMax];
-    __shared__ uint2 wsum[kLowWaves];
-    __shared__ uint32_t wcnt[kLowWaves];
+    struct Count { uint32_t below, mine, none, ahead; };
+    __shared__ Count part[kLowWaves];
     __shared__ uint32_t rid[kLowRows];
-    __shared__ uint32_t my[4];   // the adapter, its first position, its rows, the group's number in it
     __shared__ float red[kLowWaves][16 * 17];
     const uint32_t tid = tid_x();
     const int lane = lane_id(), wv = __builtin_amdgcn_readfirstlane((int)(tid / kWave));
-    const uint32_t item = wg_x(), rt = __builtin_amdgcn_workgroup_id_y();
+    const uint32_t item = wg_x(), rt = __builtin_amdgcn_workgroup_id_y(), z0 = __builtin_amdgcn_workgroup_id_z(), zs = a.low_z;
     const uint32_t K = a.hidden, wide = a.ad_wide;
-    // (kAdMax: none; the first kLowThreads rows' slots stay in a register)
-    auto slot_at = [&](uint32_t row) -> uint32_t {
+    auto slot_at = [&](uint32_t row) -> uint32_t {   // (kAdMax: none)
         const uint32_t s = row < a.rows ? (uint32_t)a.slot[row] : kAdMax;
         return s < a.ad_n ? s : kAdMax;
     };
-    const uint32_t s0 = slot_at(tid);
-    hist[tid] = 0u;   // (as many threads as adapters at most)
-    if (tid == 0u) my[0] = kAdMax;
-    __syncthreads();
-    for (uint32_t i = tid; i < a.rows; i += kLowThreads) {
-        const uint32_t s = i < kLowThreads ? s0 : slot_at(i);
-        if (s < kAdMax) atomicAdd(&hist[s], 1u);
-    }
-    __syncthreads();
-    const uint32_t cnt = hist[tid], its = (cnt + kLowRows - 1u) / kLowRows;
-    uint2 inc = make_uint2(cnt, its);   // inclusive sums over the adapters
+    // wave w holds the rows from w span, 64 at a time
+    const uint32_t span = (a.rows + kLowThreads - 1u) / kLowThreads * kWave;
+    const uint32_t i0 = (uint32_t)wv * span, i1 = min(i0 + span, a.rows);
+    const uint32_t s0 = slot_at(i0 + (uint32_t)lane);
+    const uint32_t ad = a.rows < a.ad_n ? slot_at(item) : item;
+    const int32_t rk = ad == kAdMax ? 0 : a.ad_rank ? a.ad_rank[ad] : (int32_t)wide;
+    const float scale = ad != kAdMax && a.ad_scale ? a.ad_scale[ad] : 1.0f;
+    const uint32_t rank = rk <= 0 ? 0u : min((uint32_t)rk, wide);
+    // the factor's first 256 k of each wave: on their way while the rows are counted (of
+    // a hidden size up to 4096 they serve every group)
+    const uint32_t lr = (uint32_t)lane & 15u, lh = (uint32_t)lane >> 4;
+    const uint32_t kf = (uint32_t)wv * 64u, q = rt * 16u + lr;
+    const uint16_t* af = a.ad_a + ((uint64_t)(ad == kAdMax ? 0u : ad) * wide + (q < rank ? q : 0u)) * K;
+    bf16x8 fa[8];
+    auto at = [&](uint32_t k0, uint32_t s) -> uint32_t {   // the lane's k of product s of 8
+        const uint32_t k = k0 + (s / 2u) * (kLowWaves * 64u) + 32u * (s % 2u) + 8u * lh;
+        return k < K ? k : 8u * lh;
+    };
+    auto load_a = [&](uint32_t k0) {
 #pragma unroll
-    for (int d = 1; d < kWave; d <<= 1) {
-        const uint32_t u = (uint32_t)__shfl_up((int)inc.x, d), v = (uint32_t)__shfl_up((int)inc.y, d);
-        if (lane >= d) { inc.x += u; inc.y += v; }
+        for (uint32_t s = 0; s < 8u; ++s) fa[s] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4_a*>(af + at(k0, s)));
+    };
+    bool first = z0 == 0u && rt * 16u < rank;   // fa holds the first ones
+    if (first) load_a(kf);
+    Count c = {0u, 0u, 0u, 0u};
+    for (uint32_t i = i0; i < i1; i += kWave) {
+        const uint32_t row = i + (uint32_t)lane, s = i == i0 ? s0 : slot_at(row);
+        auto n = [](bool p) { return (uint32_t)__builtin_popcountll(ballot(p)); };
+        c.below += n(row < a.rows && s < ad);
+        c.mine += n(row < a.rows && s == ad);
+        c.none += n(row < a.rows && s == kAdMax);
+        c.ahead += n(row < item && s == ad);
     }
-    if (lane == kWave - 1) wsum[wv] = inc;
+    if (lane == 0) part[wv] = c;
     __syncthreads();
-    uint32_t total = 0u;
+    uint32_t pos = 0u, total = 0u, none = 0u, ahead = 0u, nmine = 0u, nnone = 0u;   // (nmine, nnone: in the waves ahead)
 #pragma unroll
     for (int w = 0; w < kLowWaves; ++w) {
-        const uint2 p = wsum[w];
-        if (w < wv) { inc.x += p.x; inc.y += p.y; }
-        total += p.x;
+        const Count p = part[w];
+        if (w < wv) { nmine += p.mine; nnone += p.none; }
+        pos += p.below;
+        total += p.mine;
+        none += p.none;
+        ahead += p.ahead;
     }
-    if (item >= inc.y - its && item < inc.y) {
-        my[0] = tid;
-        my[1] = inc.x - cnt;
-        my[2] = cnt;
-        my[3] = item - (inc.y - its);
-    }
-    __syncthreads();
-    // the rows of adapter s (kAdMax: of none) in their order: fn(number, row)
-    auto each = [&](uint32_t s, auto fn) {
-        uint32_t seen = 0u;
-        for (uint32_t i0 = 0u; i0 < a.rows; i0 += kLowThreads) {
-            const uint32_t i = i0 + tid;
-            const bool hit = i < a.rows && (i0 == 0u ? s0 : slot_at(i)) == s;
+    // this wave's rows of slot s in their order, from number n: fn(number, row)
+    auto each = [&](uint32_t s, uint32_t n, auto fn) {
+        for (uint32_t i = i0; i < i1; i += kWave) {
+            const uint32_t row = i + (uint32_t)lane;
+            const bool hit = row < a.rows && (i == i0 ? s0 : slot_at(row)) == s;
             const uint64_t b = ballot(hit);
-            if (lane == 0) wcnt[wv] = (uint32_t)__builtin_popcountll(b);
-            __syncthreads();
-            uint32_t before = seen, all = 0u;
-#pragma unroll
-            for (int w = 0; w < kLowWaves; ++w) {
-                const uint32_t n = wcnt[w];
-                before += w < wv ? n : 0u;
-                all += n;
-            }
-            if (hit) fn(before + (uint32_t)__builtin_popcountll(b & ((1ull << lane) - 1ull)), i);
-            seen += all;
-            __syncthreads();
+            if (hit) fn(n + (uint32_t)__builtin_popcountll(b & ((1ull << lane) - 1ull)), row);
+            n += (uint32_t)__builtin_popcountll(b);
         }
     };
-    if (item == 0u && rt == 0u && total < a.rows) {
-        each(kAdMax, [&](uint32_t n, uint32_t row) {
-            a.perm[total + n] = row;
-            a.pslot[total + n] = -1;
+    if (item == 0u && rt == 0u && z0 == 0u && none != 0u) {
+        each(kAdMax, nnone, [&](uint32_t n, uint32_t row) {
+            a.perm[a.rows - none + n] = row;
+            a.pslot[a.rows - none + n] = -1;
         });
     }
-    const uint32_t ad = my[0];
-    if (ad == kAdMax) return;
-    const int32_t rk = a.ad_rank ? a.ad_rank[ad] : (int32_t)wide;
-    const uint32_t rank = rk <= 0 ? 0u : min((uint32_t)rk, wide);
-    if (rt != 0u && rt * 16u >= rank) return;
-    const uint32_t g0 = my[3] * kLowRows, pos0 = my[1] + g0, rows = min(kLowRows, my[2] - g0);
-    each(ad, [&](uint32_t n, uint32_t row) {
-        if (n - g0 < kLowRows) {
-            rid[n - g0] = row;
-            if (rt == 0u) {
-                a.perm[my[1] + n] = row;
-                a.pslot[my[1] + n] = rank ? (int32_t)(rank << 16 | ad) : -1;
+    if (ad == kAdMax || total <= z0 * kLowRows || (a.rows < a.ad_n && ahead != 0u)) return;
+    if (rt == 0u && z0 == 0u) {
+        each(ad, nmine, [&](uint32_t n, uint32_t row) {
+            a.perm[pos + n] = row;
+            a.pslot[pos + n] = rank ? (int32_t)(rank << 16 | ad) : -1;
+        });
+    }
+    if (rt * 16u >= rank) return;
+    for (uint32_t g0 = z0 * kLowRows; g0 < total; g0 += zs * kLowRows) {
+        const uint32_t rows = min(kLowRows, total - g0);
+        each(ad, nmine, [&](uint32_t n, uint32_t row) {
+            if (n - g0 < kLowRows) rid[n - g0] = row;
+        });
+        __syncthreads();
+        const unsigned char* x = reinterpret_cast<const unsigned char*>(a.x) + (uint64_t)rid[lr < rows ? lr : 0u] * K * (F8 ? 1u : 2u);
+        const uint32_t row = tid / 16u, co = tid % 16u, qo = rt * 16u + co;   // the state that the thread writes
+        const float xs = F8 && a.x_scale && row < rows ? a.x_scale[rid[row]] : 1.0f;
+        f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (uint32_t k0 = kf; k0 < K; k0 += 4u * kLowWaves * 64u) {
+            bf16x8 fx[8];
+#pragma unroll
+            for (uint32_t s = 0; s < 8u; ++s) fx[s] = x_frag<F8>(x, at(k0, s));
+            if (!first || k0 != kf) {
+                load_a(k0);
+                first = k0 == kf;
+            }
+#pragma unroll
+            for (uint32_t s = 0; s < 8u; ++s)
+                if (k0 + (s / 2u) * (kLowWaves * 64u) < K) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[s], fx[s], acc, 0, 0, 0);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) red[wv][(4 * (int)lh + e) * 17 + (int)lr] = acc[e];
+        __syncthreads();
+        if (row < rows && qo < wide) {
+            float p = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kLowWaves; ++w) p += red[w][co * 17u + row];
+            // (ranks past the adapter's read rank 0's factor: nothing of theirs is kept)
+            p = qo < rank ? p * scale * xs : 0.0f;
+            uint16_t* low = a.low + (uint64_t)(pos + g0 + row) * 3u * wide + qo;
+#pragma unroll
+            for (uint32_t i = 0; i < 3u; ++i) {
+                const uint32_t u = to_bf16(p);
+                low[i * wide] = (uint16_t)u;
+                p = (u & 0x7f80u) == 0x7f80u ? 0.0f : p - __uint_as_float(u << 16);   // (an inf or NaN is whole in the first part)
             }
         }
-    });
-    if (rank == 0u) return;   // (each ends with a barrier)
-    const uint32_t lr = (uint32_t)lane & 15u, lh = (uint32_t)lane >> 4;
-    const unsigned char* x = reinterpret_cast<const unsigned char*>(a.x) + (uint64_t)rid[lr < rows ? lr : 0u] * K * (F8 ? 1u : 2u);
-    const uint32_t q = rt * 16u + lr;
-    const uint16_t* af = a.ad_a + ((uint64_t)ad * wide + (q < rank ? q : 0u)) * K;
-    f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (uint32_t k0 = (uint32_t)wv * 64u; k0 < K; k0 += 4u * kLowWaves * 64u) {
-        bf16x8 fa[8], fx[8];
-#pragma unroll
-        for (uint32_t s = 0; s < 8u; ++s) {
-            const uint32_t k = k0 + (s / 2u) * (kLowWaves * 64u) + 32u * (s % 2u) + 8u * lh;
-            fa[s] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4_a*>(af + (k < K ? k : 8u * lh)));
-            fx[s] = x_frag<F8>(x, k < K ? k : 8u * lh);
-        }
-#pragma unroll
-        for (uint32_t s = 0; s < 8u; ++s)
-            if (k0 + (s / 2u) * (kLowWaves * 64u) < K) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[s], fx[s], acc, 0, 0, 0);
-    }
-#pragma unroll
-    for (int e = 0; e < 4; ++e) red[wv][(4 * (int)lh + e) * 17 + (int)lr] = acc[e];
-    __syncthreads();
-    const uint32_t row = tid / 16u, c = tid % 16u, qo = rt * 16u + c;
-    if (row < rows && qo < wide) {
-        float p = 0.0f;
-#pragma unroll
-        for (int w = 0; w < kLowWaves; ++w) p += red[w][c * 17u + row];
-        // (ranks past the adapter's read rank 0's factor: nothing of theirs is kept)
-        p = qo < rank ? p * (a.ad_scale ? a.ad_scale[ad] : 1.0f) * (F8 && a.x_scale ? a.x_scale[rid[row]] : 1.0f) : 0.0f;
-        uint16_t* low = a.low + (uint64_t)(pos0 + row) * 3u * wide + qo;
-#pragma unroll
-        for (uint32_t i = 0; i < 3u; ++i) {
-            const uint32_t u = to_bf16(p);
-            low[i * wide] = (uint16_t)u;
-            p = (u & 0x7f80u) == 0x7f80u ? 0.0f : p - __uint_as_float(u << 16);   // (an inf or NaN is whole in the first part)
-        }
+        __syncthreads();   // (rid and red are free for the next group)
     }
 }
 
@@ -203,28 +200,48 @@ void tile(const LmArgs& a, hipStream_t st) {
                        dim3(NW * kWave), 0, st, a);
 }
 
-// (the stages: as for bf16 operands, lcs_lmhead.hip)
-template <bool AD>
-void tiles_f8(const LmArgs& a, uint32_t vt, uint32_t br, hipStream_t st) {
-    if (br == 256u && vt == 4u) tile<4, 256, 2, 8, 4, true, AD>(a, st);
-    else if (br == 256u) tile<2, 256, 3, 4, 2, true, AD>(a, st);
-    else if (br == 128u && vt == 4u) tile<4, 128, 3, 4, 2, true, AD>(a, st);
-    else if (br == 128u) tile<2, 128, 2, 4, 4, true, AD>(a, st);
-    else if (vt == 5u) tile<5, 64, 3, 4, 2, true, AD>(a, st);
-    else if (vt == 4u) tile<4, 64, 2, 4, 4, true, AD>(a, st);
-    else if (vt == 2u) tile<2, 64, 2, 4, 4, true, AD>(a, st);
-    else tile<1, 64, 2, 4, 4, true, AD>(a, st);
+// The tiles: up to 64 rows lmhead_shape's columns, above by the same measure (rounds of
+// workgroups over the CUs times what one takes). Rings of 64-k stages (128 k of
+// e4m3), three where they fit, and eight waves on the tiles from 256 columns up:
+// us by 64 VT columns x rows, ST stages, NW waves,
+//   64 rows, one block of 256 columns a CU: 50257 x 1600 bf16 with adapters, ST 3
+//     NW 8 41.0, NW 4 45.3, two stages 50; 151936 x 3584 e4m3 (594 blocks) 132,
+//     144, 142; 128256 x 4096 e4m3 (501) 116.5, 126, 116
+//   320 columns, ST 3 NW 4: 151936 x 3584 e4m3 116 (32-k stages 124), bf16 with adapters
+//     225 (235), but e4m3 with 64 adapters 197 (180: their reads want the two
+//     workgroups a CU that the smaller stages leave room for)
+//   128 columns, ST 3 NW 4: 32000 x 2048 e4m3 15.5 (NW 8 16.1)
+//   64 columns: 16000 x 4096 e4m3 18.0 with ST 4, 19.2 with six 32-k stages, bf16 27.0, 26.6
+//   128 rows, 256 columns: 128256 x 4096 e4m3 ST 3 NW 8 138, NW 4 153, 32-k stages
+//     163; bf16 with adapters 230, -, 266
+//   1024 rows, 256 x 256, ST 2 NW 8: 128256 x 4096 e4m3 683 (1576 TFLOP/s)
+struct LmExShape { uint32_t vt, br; };
+LmExShape lmhead_ex_shape(uint32_t rows, uint32_t vocab, bool f8, uint32_t cus) {
+    // (us a round, 4096 k of e4m3; bf16 takes 1.4 times as long, 128 rows a little more:
+    // 384 x 128256 256 rows 481 us, 128 rows 507, e4m3 342, 308)
+    struct { uint32_t vt, br, weight; } const shapes[] = {{4, 256, 86}, {4, 128, f8 ? 56u : 58u}, {2, 128, 42}};
+    LmExShape best{4u, 256u};
+    uint64_t least = ~0ull;
+    for (const auto& s : shapes) {
+        const uint64_t n = ((uint64_t)vocab + 64u * s.vt - 1u) / (64u * s.vt), chunks = (rows + s.br - 1u) / s.br;
+        if (n > kLmMaxBlocks || (s.vt == 2u && n > 4u * cus)) continue;   // (lmhead_max_blocks)
+        const uint64_t cost = (n * chunks + cus - 1u) / cus * s.weight;
+        if (cost < least) {
+            least = cost;
+            best = LmExShape{s.vt, s.br};
+        }
+    }
+    return best;
 }
-void tiles_ad(const LmArgs& a, uint32_t vt, uint32_t br, uint32_t cus, hipStream_t st) {
-    if (br == 256u && vt == 4u) tile<4, 256, 2, 8, 4, false, true>(a, st);
-    else if (br == 256u) tile<2, 256, 3, 4, 2, false, true>(a, st);
-    else if (br == 128u && vt == 4u) tile<4, 128, 3, 4, 2, false, true>(a, st);
-    else if (br == 128u) tile<2, 128, 4, 4, 2, false, true>(a, st);
-    else if (vt == 5u) tile<5, 64, 3, 4, 2, false, true>(a, st);
-    else if (vt == 4u && a.nblocks > cus && a.nblocks <= 2u * cus) tile<4, 64, 2, 4, 4, false, true>(a, st);
-    else if (vt == 4u) tile<4, 64, 4, 4, 2, false, true>(a, st);
-    else if (vt == 2u) tile<2, 64, 4, 4, 2, false, true>(a, st);
-    else tile<1, 64, 6, 4, 2, false, true>(a, st);
+template <bool F8, bool AD>
+void tiles(const LmArgs& a, uint32_t vt, uint32_t br, hipStream_t st) {
+    if (br == 256u) tile<4, 256, 2, 8, 4, F8, AD>(a, st);
+    else if (br == 128u && vt == 4u) tile<4, 128, 3, 8, 4, F8, AD>(a, st);
+    else if (br == 128u) tile<2, 128, F8 ? 2 : 3, F8 ? 4 : 8, 4, F8, AD>(a, st);
+    else if (vt == 5u) tile<5, 64, 3, 4, F8 && AD ? 2 : 4, F8, AD>(a, st);
+    else if (vt == 4u) tile<4, 64, 3, 8, 4, F8, AD>(a, st);
+    else if (vt == 2u) tile<2, 64, 3, 4, 4, F8, AD>(a, st);
+    else tile<1, 64, F8 ? 4 : 6, 4, F8 ? 4 : 2, F8, AD>(a, st);
 }
 
 }  // namespace
@@ -233,18 +250,27 @@ hipError_t launch_lmhead_ex(const LmArgs& a0, bool f8, uint32_t cus, hipStream_t
     if (!f8 && a0.ad_n == 0u) return launch_lmhead(a0, cus, st);
     LmArgs a = a0;
     uint32_t vt, br;
-    lmhead_shape_of(a.rows, a.vocab, a.hidden, cus, &vt, &br);
+    if (a.rows <= 64u) {
+        lmhead_shape_of(a.rows, a.vocab, a.hidden, cus, &vt, &br);
+    } else {
+        const LmExShape s = lmhead_ex_shape(a.rows, a.vocab, f8, cus);
+        vt = s.vt;
+        br = s.br;
+    }
     a.nblocks = (a.vocab + 64u * vt - 1u) / (64u * vt);
     a.nchunks = (a.rows + br - 1u) / br;
     if (a.ad_n != 0u) {
-        // (groups: at most one that is not full per adapter in use)
-        const dim3 grid((a.ad_n < a.rows ? a.ad_n : a.rows) + a.rows / kLowRows, (a.ad_wide + 15u) / 16u);
+        // (the rows' groups side by side as long as that makes no more than 2048 workgroups)
+        const uint32_t nx = a.ad_n < a.rows ? a.ad_n : a.rows, ny = (a.ad_wide + 15u) / 16u, groups = (a.rows + kLowRows - 1u) / kLowRows;
+        const uint32_t nz = 2048u / (nx * ny);
+        a.low_z = nz == 0u ? 1u : nz < groups ? nz : groups;
+        const dim3 grid(nx, ny, a.low_z);
         if (f8) hipLaunchKernelGGL((lm_low<true>), grid, dim3(kLowThreads), 0, st, a);
         else hipLaunchKernelGGL((lm_low<false>), grid, dim3(kLowThreads), 0, st, a);
-        if (f8) tiles_f8<true>(a, vt, br, st);
-        else tiles_ad(a, vt, br, cus, st);
+        if (f8) tiles<true, true>(a, vt, br, st);
+        else tiles<false, true>(a, vt, br, st);
     } else {
-        tiles_f8<false>(a, vt, br, st);
+        tiles<true, false>(a, vt, br, st);
     }
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? launch_lmhead_fin(a, st) : e;

@@ -109,7 +109,7 @@ __global__ __launch_bounds__(NW * kWave, 2) void lmhead_tile(LmArgs a) {
     constexpr int kLR = 64 / (int)kCh * NW;   // rows that one DMA load of every wave covers
     constexpr int LA = kTV / kLR, LB = BR / kLR;   // DMA loads per wave and stage
     constexpr bool SPLIT = KS == 4 && ST == 2;   // half of a stage's loads ahead of the barrier
-    static_assert(KS == 2 || SPLIT, "the schedule of the k-loop");
+    static_assert(KS == 2 || KS == 4, "the schedule of the k-loop");
     static_assert(!(BIG && (F8 || AD)), "row offsets");
     static_assert(LA * kLR == (int)kTV && LB * kLR == BR && CT * WM == 2 * VT, "tile shape");
     constexpr int LPS = LA + LB;
@@ -342,7 +342,7 @@ __global__ __launch_bounds__(NW * kWave, 2) void lmhead_tile(LmArgs a) {
     // product with zeros instead would carry an inf or NaN of one request's
     // adapter into the others' logits.
     if constexpr (AD) {
-        constexpr int DP = CT == 4 && RT == 2 ? 1 : CT == 5 ? 2 : 3;   // (what the registers hold)
+        constexpr int DP = CT == 5 || (F8 && RT == 4) ? 2 : 3;   // (what the registers hold)
         struct Step { u32x4 b[CT], p[3]; int32_t who; uint32_t k; };
         const uint32_t wide = a.ad_wide;
 #pragma unroll

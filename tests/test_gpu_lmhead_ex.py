@@ -8,10 +8,19 @@ product. The statistics are held against the written logits."""
 import numpy as np
 import pytest
 
-from tests.test_gpu_lmhead import STEADY, check_epilogue
+from tests.test_gpu_lmhead import check_epilogue
 
 pytestmark = pytest.mark.gpu
 U = 2.0 ** -24
+
+
+# cases of each tile of lcs_lmhead_ex (rows, vocab, the tile's 64-column and row
+# counts), full ones and with a row, a column and a row tile more or less;
+# tests/test_lmhead_ex_shape.py holds the choice of the tile to this list (256 CUs)
+TILES = [
+    (3, 300, 1, 64), (64, 16384, 1, 64), (64, 20001, 2, 64), (33, 32768, 2, 64), (64, 33001, 4, 64), (17, 100001, 4, 64),
+    (2, 80001, 5, 64), (65, 140, 2, 128), (128, 20001, 2, 128), (300, 1001, 2, 128), (128, 50257, 4, 128),
+    (300, 20001, 4, 128), (256, 60000, 4, 256), (200, 50257, 4, 256), (511, 30000, 4, 256)]
 
 
 @pytest.fixture(scope="module")
@@ -109,15 +118,15 @@ def check_lse(g, logits, draft):
 
 # every tile, with fewer and more stages than its ring and a half stage at the end
 @pytest.mark.parametrize("hidden", [64, 128, 192, 704, 1152])
-@pytest.mark.parametrize("rows,vocab", [c[:2] for c in STEADY])
+@pytest.mark.parametrize("rows,vocab", [c[:2] for c in TILES])
 def test_8_bits_exact(sampler, rows, vocab, hidden):
     exact_case(sampler, rows, vocab, hidden, True, (), rows + vocab + hidden)
 
 
 @pytest.mark.parametrize("f8", [False, True])
-@pytest.mark.parametrize("rows,vocab", [c[:2] for c in STEADY])
+@pytest.mark.parametrize("rows,vocab", [c[:2] for c in TILES])
 def test_adapters_exact_on_every_tile(sampler, rows, vocab, f8):
-    exact_case(sampler, rows, vocab, 320, f8, (8, 3, 16, 24), rows * 3 + vocab)
+    exact_case(sampler, rows, vocab, 448, f8, (8, 3, 16, 24, 70), rows * 3 + vocab)
 
 
 @pytest.mark.parametrize("f8", [False, True])
