@@ -88,22 +88,14 @@ __global__ __launch_bounds__(kLowThreads) void lm_low(LmArgs a) {
     const int32_t rk = ad == kAdMax ? 0 : a.ad_rank ? a.ad_rank[ad] : (int32_t)wide;
     const float scale = ad != kAdMax && a.ad_scale ? a.ad_scale[ad] : 1.0f;
     const uint32_t rank = rk <= 0 ? 0u : min((uint32_t)rk, wide);
-    // the factor's first 256 k of each wave: on their way while the rows are counted (of
-    // a hidden size up to 4096 they serve every group)
     const uint32_t lr = (uint32_t)lane & 15u, lh = (uint32_t)lane >> 4;
     const uint32_t kf = (uint32_t)wv * 64u, q = rt * 16u + lr;
     const uint16_t* af = a.ad_a + ((uint64_t)(ad == kAdMax ? 0u : ad) * wide + (q < rank ? q : 0u)) * K;
-    bf16x8 fa[8];
     auto at = [&](uint32_t k0, uint32_t s) -> uint32_t {   // the lane's k of product s of 8
         const uint32_t k = k0 + (s / 2u) * (kLowWaves * 64u) + 32u * (s % 2u) + 8u * lh;
         return k < K ? k : 8u * lh;
     };
-    auto load_a = [&](uint32_t k0) {
-#pragma unroll
-        for (uint32_t s = 0; s < 8u; ++s) fa[s] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4_a*>(af + at(k0, s)));
-    };
-    bool first = z0 == 0u && rt * 16u < rank;   // fa holds the first ones
-    if (first) load_a(kf);
+    auto a_frag = [&](uint32_t k0, uint32_t s) { return __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4_a*>(af + at(k0, s))); };
     Count c = {0u, 0u, 0u, 0u};
     for (uint32_t i = i0; i < i1; i += kWave) {
         const uint32_t row = i + (uint32_t)lane, s = i == i0 ? s0 : slot_at(row);
@@ -142,6 +134,11 @@ __global__ __launch_bounds__(kLowThreads) void lm_low(LmArgs a) {
         });
     }
     if (ad == kAdMax || total <= z0 * kLowRows || (a.rows < a.ad_n && ahead != 0u)) return;
+    // the factor's first 256 k of each wave serve every group; they are on their way
+    // while the first group's rows are found
+    bf16x8 fa[8];
+#pragma unroll
+    for (uint32_t s = 0; s < 8u; ++s) fa[s] = a_frag(kf, s);
     if (rt == 0u && z0 == 0u) {
         each(ad, nmine, [&](uint32_t n, uint32_t row) {
             a.perm[pos + n] = row;
@@ -159,17 +156,23 @@ __global__ __launch_bounds__(kLowThreads) void lm_low(LmArgs a) {
         const uint32_t row = tid / 16u, co = tid % 16u, qo = rt * 16u + co;   // the state that the thread writes
         const float xs = F8 && a.x_scale && row < rows ? a.x_scale[rid[row]] : 1.0f;
         f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-        for (uint32_t k0 = kf; k0 < K; k0 += 4u * kLowWaves * 64u) {
-            bf16x8 fx[8];
+        bf16x8 fx[8];
 #pragma unroll
-            for (uint32_t s = 0; s < 8u; ++s) fx[s] = x_frag<F8>(x, at(k0, s));
-            if (!first || k0 != kf) {
-                load_a(k0);
-                first = k0 == kf;
+        for (uint32_t s = 0; s < 8u; ++s) fx[s] = x_frag<F8>(x, at(kf, s));
+#pragma unroll
+        for (uint32_t s = 0; s < 8u; ++s)
+            if (kf + (s / 2u) * (kLowWaves * 64u) < K) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[s], fx[s], acc, 0, 0, 0);
+#pragma unroll 1
+        for (uint32_t k0 = kf + 4u * kLowWaves * 64u; k0 < K; k0 += 2u * kLowWaves * 64u) {
+            bf16x8 fb[4];
+#pragma unroll
+            for (uint32_t s = 0; s < 4u; ++s) {
+                fb[s] = a_frag(k0, s);
+                fx[s] = x_frag<F8>(x, at(k0, s));
             }
 #pragma unroll
-            for (uint32_t s = 0; s < 8u; ++s)
-                if (k0 + (s / 2u) * (kLowWaves * 64u) < K) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[s], fx[s], acc, 0, 0, 0);
+            for (uint32_t s = 0; s < 4u; ++s)
+                if (k0 + (s / 2u) * (kLowWaves * 64u) < K) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[s], fx[s], acc, 0, 0, 0);
         }
 #pragma unroll
         for (int e = 0; e < 4; ++e) red[wv][(4 * (int)lh + e) * 17 + (int)lr] = acc[e];
@@ -238,7 +241,7 @@ void tiles(const LmArgs& a, uint32_t vt, uint32_t br, hipStream_t st) {
     if (br == 256u) tile<4, 256, 2, 8, 4, F8, AD>(a, st);
     else if (br == 128u && vt == 4u) tile<4, 128, 3, 8, 4, F8, AD>(a, st);
     else if (br == 128u) tile<2, 128, F8 ? 2 : 3, F8 ? 4 : 8, 4, F8, AD>(a, st);
-    else if (vt == 5u) tile<5, 64, 3, 4, F8 && AD ? 2 : 4, F8, AD>(a, st);
+    else if (vt == 5u) tile<5, 64, 3, 4, 4, F8, AD>(a, st);
     else if (vt == 4u) tile<4, 64, 3, 8, 4, F8, AD>(a, st);
     else if (vt == 2u) tile<2, 64, 3, 4, 4, F8, AD>(a, st);
     else tile<1, 64, F8 ? 4 : 6, 4, F8 ? 4 : 2, F8, AD>(a, st);
@@ -260,9 +263,9 @@ hipError_t launch_lmhead_ex(const LmArgs& a0, bool f8, uint32_t cus, hipStream_t
     a.nblocks = (a.vocab + 64u * vt - 1u) / (64u * vt);
     a.nchunks = (a.rows + br - 1u) / br;
     if (a.ad_n != 0u) {
-        // (the rows' groups side by side as long as that makes no more than 2048 workgroups)
+        // (the rows' groups side by side as long as all the workgroups can run at once)
         const uint32_t nx = a.ad_n < a.rows ? a.ad_n : a.rows, ny = (a.ad_wide + 15u) / 16u, groups = (a.rows + kLowRows - 1u) / kLowRows;
-        const uint32_t nz = 2048u / (nx * ny);
+        const uint32_t nz = 2u * cus / (nx * ny);
         a.low_z = nz == 0u ? 1u : nz < groups ? nz : groups;
         const dim3 grid(nx, ny, a.low_z);
         if (f8) hipLaunchKernelGGL((lm_low<true>), grid, dim3(kLowThreads), 0, st, a);

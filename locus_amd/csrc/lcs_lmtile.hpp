@@ -315,117 +315,144 @@ __global__ __launch_bounds__(NW * kWave, 2) void lmhead_tile(LmArgs a) {
         for (uint32_t i = 0; i < NSC; ++i)
             if (NW * kWave * i + tid < kTV + BR) sc[NW * kWave * i + tid] = scales[i];
         __syncthreads();
+        float xs[RT];
 #pragma unroll
-        for (int j = 0; j < RT; ++j) {
-            const float xs = sc[kTV + wn * (BR / 2) + 32u * j + lr];
+        for (int j = 0; j < RT; ++j) xs[j] = sc[kTV + wn * (BR / 2) + 32u * j + lr];
 #pragma unroll
-            for (int i = 0; i < CT; ++i)
+        for (int i = 0; i < CT; ++i)
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const float4 ws = *reinterpret_cast<const float4*>(sc + cw + 32u * i + 8u * q + 4u * lh);
-                    acc[i][j][4 * q] *= xs * ws.x;
-                    acc[i][j][4 * q + 1] *= xs * ws.y;
-                    acc[i][j][4 * q + 2] *= xs * ws.z;
-                    acc[i][j][4 * q + 3] *= xs * ws.w;
+            for (int q = 0; q < 4; ++q) {
+                const float4 ws = *reinterpret_cast<const float4*>(sc + cw + 32u * i + 8u * q + 4u * lh);
+#pragma unroll
+                for (int j = 0; j < RT; ++j) {
+                    acc[i][j][4 * q] *= xs[j] * ws.x;
+                    acc[i][j][4 * q + 1] *= xs[j] * ws.y;
+                    acc[i][j][4 * q + 2] *= xs[j] * ws.z;
+                    acc[i][j][4 * q + 3] *= xs[j] * ws.w;
                 }
-            __builtin_amdgcn_sched_barrier(0);
-        }
+                __builtin_amdgcn_sched_barrier(0);
+            }
     }
     // ---- the adapters: acc += low b^T for the rows of each adapter that the wave's
     // 32-row tiles hold. The rows are in the order of their adapters, so
-    // an adapter's columns are read by one wave of two, as a rule, straight into the
-    // fragments (each lane 8 consecutive k of its column, which is how the factor
-    // lies in memory; nothing would be shared through LDS), DP steps of 16 ranks
-    // ahead. A row's state is the sum of three bf16 parts (24 bits of mantissa, as f32:
+    // an adapter's columns are read by one wave of two, as a rule, each lane 8
+    // consecutive k of its column, which is how the factor lies in memory, by DMA into
+    // the wave's own part of the free ring (no register holds them in flight), DP steps
+    // of 16 ranks ahead. A row's state is the sum of three bf16 parts (24 bits of mantissa, as f32:
     // two leave an error of 1e-6 of the logits, ten times that of the product's
     // sums). Each adapter has an accumulator of its own, added to its rows only: a
     // product with zeros instead would carry an inf or NaN of one request's
     // adapter into the others' logits.
     if constexpr (AD) {
-        constexpr int DP = CT == 5 || (F8 && RT == 4) ? 2 : 3;   // (what the registers hold)
-        struct Step { u32x4 b[CT], p[3]; int32_t who; uint32_t k; };
+        constexpr int DP = CT == 5 || RT == 4 ? 2 : 3;   // steps ahead (what the registers hold)
+        struct Step { u32x4 b[CT], p[3]; int32_t who; uint32_t k, j; };
         const uint32_t wide = a.ad_wide;
+        const uint32_t rw = wn * (BR / 2) + lr;   // the lane's row in the wave's first 32-row tile
+        int32_t sj[RT];                            // rank << 16 | adapter of its rows, or -1
 #pragma unroll
-        for (int j = 0; j < RT; ++j) {
-            const uint32_t r = wn * (BR / 2) + 32u * j + lr;
-            const uint32_t pos = r0 + (r < vrows ? r : 0u);
-            const int32_t s = r < vrows ? a.pslot[pos] : -1;   // rank << 16 | adapter, or -1
-            uint64_t todo = ballot(s >= 0);
-            int32_t who = 0;
-            uint32_t kn = 0u;
-            const uint16_t *bp = nullptr, *lp = nullptr;
-            // the loads of the next step; false: none is left
-            auto fetch = [&](Step& st) {
-                if (kn >= (uint32_t)who >> 16) {
-                    if (todo == 0u) return false;
-                    const int l = __builtin_ctzll(todo);
-                    who = __builtin_amdgcn_readlane(s, l);
-                    todo &= ~ballot(s == who);
-                    kn = 0u;
-                    bp = a.ad_b + ((uint64_t)((uint32_t)who & 0xffffu) * V + n0) * wide;
-                    // (the other rows' states are not used: all theirs from one place)
-                    const uint32_t p0 = (uint32_t)__builtin_amdgcn_readlane((int)pos, l);
-                    lp = a.low + (uint64_t)(s == who ? pos : p0) * 3u * wide;
-                }
-                const uint32_t k = kn + 8u * lh, kk = k < (uint32_t)who >> 16 ? k : 0u;
+        for (int j = 0; j < RT; ++j) sj[j] = rw + 32u * j < vrows ? a.pslot[r0 + rw + 32u * j] : -1;
+        // (the tile at hand changes as the steps go: its rows' adapters by way of the wave's
+        // own part of LDS, past the epilogue's partial results and the scales)
+        constexpr uint32_t kPast = 16u * WM * BR + (F8 ? 4u * (kTV + BR) : 0u);
+        int32_t* ps = reinterpret_cast<int32_t*>(lds + kPast) + (uint32_t)wv * (BR / 2) + lr;
+        if (RT > 1) {
 #pragma unroll
-                for (int i = 0; i < CT; ++i) {
-                    const uint32_t c = cw + 32u * i + lr;
-                    st.b[i] = *reinterpret_cast<const u32x4_a*>(bp + (c < vcols ? c : 0u) * wide + kk);
-                }
+            for (int j = 0; j < RT; ++j) ps[32 * j] = sj[j];   // (lanes l and l + 32 write the same)
+        }
+        auto of = [&](uint32_t j) -> int32_t { return RT > 1 ? ps[32u * j] : sj[0]; };
+        uint64_t todo = ballot(sj[0] >= 0);
+        uint32_t jn = 0u, kn = 0u;
+        int32_t who = 0;
+        const uint16_t *bp = a.ad_b, *lp = a.low;
+        bool more = true;
+        // The loads of the next step, tile by tile and adapter by adapter. Past the last
+        // one (who -1) they are made all the same, from where the last one's were: the
+        // count of loads in flight is then known where a step is used, and the ones
+        // after it stay in flight.
+        auto fetch = [&](Step& st) {
+            if (more && kn >= (uint32_t)who >> 16) {
+                while (todo == 0u && jn + 1u < (uint32_t)RT) todo = ballot(of(++jn) >= 0);
+                more = todo != 0u;
+            }
+            if (more && kn >= (uint32_t)who >> 16) {
+                const int l = __builtin_ctzll(todo);
+                const int32_t s = of(jn);
+                who = __builtin_amdgcn_readlane(s, l);
+                todo &= ~ballot(s == who);
+                kn = 0u;
+                bp = a.ad_b + ((uint64_t)((uint32_t)who & 0xffffu) * V + n0) * wide;
+                // (the other rows' states are not used: all theirs from one place)
+                const uint32_t p = r0 + wn * (BR / 2) + 32u * jn;
+                lp = a.low + (uint64_t)(p + (s == who ? lr : (uint32_t)l & 31u)) * 3u * wide;
+            }
+            const uint32_t k = kn + 8u * lh, kk = k < (uint32_t)who >> 16 ? k : 0u;
 #pragma unroll
-                for (int i = 0; i < 3; ++i) st.p[i] = *reinterpret_cast<const u32x4_a*>(lp + i * wide + kk);
-                st.who = who;
-                st.k = kn;
-                kn += 16u;
-                return true;
-            };
-            f32x16 t[CT];
+            for (int i = 0; i < CT; ++i) {
+                const uint32_t c = cw + 32u * i + lr;
+                st.b[i] = *reinterpret_cast<const u32x4_a*>(bp + (c < vcols ? c : 0u) * wide + kk);
+            }
 #pragma unroll
-            for (int i = 0; i < CT; ++i)
+            for (int i = 0; i < 3; ++i) st.p[i] = *reinterpret_cast<const u32x4_a*>(lp + i * wide + kk);
+            st.who = more ? who : -1;
+            st.k = kn;
+            st.j = jn;
+            kn += more ? 16u : 0u;
+        };
+        f32x16 t[CT];
 #pragma unroll
-                for (int e = 0; e < 16; ++e) t[i][e] = 0.0f;
-            auto use = [&](Step& st) {
-                const uint32_t rank = (uint32_t)st.who >> 16;
-                if (st.k + 16u > rank) {   // what lies past the rank counts as zero, whatever it holds
-                    const uint32_t k = st.k + 8u * lh, left = k < rank ? rank - k : 0u;
-                    u32x4 live;
+        for (int i = 0; i < CT; ++i)
 #pragma unroll
-                    for (uint32_t e = 0; e < 4u; ++e) live[e] = left > 2u * e + 1u ? 0xffffffffu : left == 2u * e + 1u ? 0xffffu : 0u;
+            for (int e = 0; e < 16; ++e) t[i][e] = 0.0f;
+        auto use = [&](Step& st) {
+            const uint32_t rank = (uint32_t)st.who >> 16;
+            auto& b = st.b;
+            if (st.k + 16u > rank) {   // what lies past the rank counts as zero, whatever it holds
+                const uint32_t k = st.k + 8u * lh, left = k < rank ? rank - k : 0u;
+                u32x4 live;
 #pragma unroll
-                    for (int i = 0; i < CT; ++i) st.b[i] &= live;
+                for (uint32_t e = 0; e < 4u; ++e) live[e] = left > 2u * e + 1u ? 0xffffffffu : left == 2u * e + 1u ? 0xffffu : 0u;
 #pragma unroll
-                    for (int i = 0; i < 3; ++i) st.p[i] &= live;
-                }
+                for (int i = 0; i < CT; ++i) b[i] &= live;
 #pragma unroll
-                for (int p = 2; p >= 0; --p)
+                for (int i = 0; i < 3; ++i) st.p[i] &= live;
+            }
+            const f32x16 zero = {};
+            if (st.k == 0u) {
 #pragma unroll
-                    for (int i = 0; i < CT; ++i)
-                        t[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, st.b[i]), __builtin_bit_cast(bf16x8, st.p[p]), t[i], 0, 0, 0);
-                if (st.k + 16u >= rank) {
-                    if (s == st.who) {
+                for (int i = 0; i < CT; ++i)
+                    t[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, b[i]), __builtin_bit_cast(bf16x8, st.p[2]), zero, 0, 0, 0);
+            } else {
+#pragma unroll
+                for (int i = 0; i < CT; ++i)
+                    t[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, b[i]), __builtin_bit_cast(bf16x8, st.p[2]), t[i], 0, 0, 0);
+            }
+#pragma unroll
+            for (int p = 1; p >= 0; --p)
+#pragma unroll
+                for (int i = 0; i < CT; ++i)
+                    t[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, b[i]), __builtin_bit_cast(bf16x8, st.p[p]), t[i], 0, 0, 0);
+            if (st.k + 16u >= rank) {
+#pragma unroll
+                for (int j = 0; j < RT; ++j) {
+                    if ((RT == 1 || st.j == (uint32_t)j) && sj[j] == st.who) {
 #pragma unroll
                         for (int i = 0; i < CT; ++i)
 #pragma unroll
                             for (int e = 0; e < 16; ++e) acc[i][j][e] += t[i][e];
                     }
-#pragma unroll
-                    for (int i = 0; i < CT; ++i)
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) t[i][e] = 0.0f;
                 }
-            };
-            Step st[DP];
-            bool have[DP];
+            }
+        };
+        Step st[DP];
 #pragma unroll
-            for (int d = 0; d < DP; ++d) have[d] = fetch(st[d]);
-            while (have[0]) {
+        for (int d = 0; d < DP; ++d) fetch(st[d]);
+        // (one way out of the loop, so that the count of loads in flight is the same on every
+        // way in: a step past the last one adds to t, which nothing takes any more)
+        while (st[0].who >= 0) {
 #pragma unroll
-                for (int d = 0; d < DP; ++d) {
-                    if (!have[d]) break;
-                    use(st[d]);
-                    have[d] = fetch(st[d]);
-                }
+            for (int d = 0; d < DP; ++d) {
+                use(st[d]);
+                fetch(st[d]);
             }
         }
     }
