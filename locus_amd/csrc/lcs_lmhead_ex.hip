@@ -107,16 +107,12 @@ __global__ __launch_bounds__(kLowThreads) void lm_low(LmArgs a) {
     }
     if (lane == 0) part[wv] = c;
     __syncthreads();
-    uint32_t pos = 0u, total = 0u, none = 0u, ahead = 0u, nmine = 0u, nnone = 0u;   // (nmine, nnone: in the waves ahead)
-#pragma unroll
-    for (int w = 0; w < kLowWaves; ++w) {
-        const Count p = part[w];
-        if (w < wv) { nmine += p.mine; nnone += p.none; }
-        pos += p.below;
-        total += p.mine;
-        none += p.none;
-        ahead += p.ahead;
-    }
+    // (lane w takes wave w's counts; nmine, nnone: those of the waves ahead)
+    c = part[lane < kLowWaves ? lane : 0];
+    const bool in = lane < kLowWaves, before = lane < wv;
+    const uint32_t pos = wave_sum_u(in ? c.below : 0u), total = wave_sum_u(in ? c.mine : 0u), none = wave_sum_u(in ? c.none : 0u);
+    const uint32_t ahead = wave_sum_u(in ? c.ahead : 0u);
+    const uint32_t nmine = wave_sum_u(before ? c.mine : 0u), nnone = wave_sum_u(before ? c.none : 0u);
     // this wave's rows of slot s in their order, from number n: fn(number, row)
     auto each = [&](uint32_t s, uint32_t n, auto fn) {
         for (uint32_t i = i0; i < i1; i += kWave) {

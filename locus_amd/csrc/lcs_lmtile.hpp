@@ -335,124 +335,142 @@ __global__ __launch_bounds__(NW * kWave, 2) void lmhead_tile(LmArgs a) {
     }
     // ---- the adapters: acc += low b^T for the rows of each adapter that the wave's
     // 32-row tiles hold. The rows are in the order of their adapters, so
-    // an adapter's columns are read by one wave of two, as a rule, each lane 8
-    // consecutive k of its column, which is how the factor lies in memory, by DMA into
-    // the wave's own part of the free ring (no register holds them in flight), DP steps
-    // of 16 ranks ahead. A row's state is the sum of three bf16 parts (24 bits of mantissa, as f32:
+    // an adapter's columns are read by one wave of two, as a rule, straight into the
+    // fragments (each lane 8 consecutive k of its column, which is how the factor
+    // lies in memory), DP steps of 16 ranks ahead; the rows' states, which every wave
+    // over the columns needs, go by way of LDS, as many ranks at a time as the free ring
+    // holds. A row's state is the sum of three bf16 parts (24 bits of mantissa, as f32:
     // two leave an error of 1e-6 of the logits, ten times that of the product's
     // sums). Each adapter has an accumulator of its own, added to its rows only: a
     // product with zeros instead would carry an inf or NaN of one request's
     // adapter into the others' logits.
     if constexpr (AD) {
-        constexpr int DP = CT == 5 || RT == 4 ? 2 : 3;   // steps ahead (what the registers hold)
-        struct Step { u32x4 b[CT], p[3]; int32_t who; uint32_t k, j; };
+        constexpr int DP = CT == 5 || RT == 4 ? 3 : 4;   // (what the registers hold)
+        struct Step { u32x4 b[CT]; int32_t who; uint32_t k, j; };
+        // (past the epilogue's partial results, the scales and the waves' rows' adapters)
+        constexpr uint32_t kPast = 16u * WM * BR + (F8 ? 4u * (kTV + BR) : 0u);
+        constexpr uint32_t kLow = (kPast + (RT > 1 ? 4u * WM * BR : 0u) + 127u) / 128u * 128u;
+        constexpr uint32_t kFits = ((sizeof(lds) - kLow) / BR - 16u) / 96u * 16u;   // ranks at a time
+        static_assert(kFits >= 16u, "the adapters' place");
         const uint32_t wide = a.ad_wide;
+        const uint32_t ww = min(wide, kFits), rowb = 6u * ww + 16u;   // (16 bytes more: the rows' banks differ)
         const uint32_t rw = wn * (BR / 2) + lr;   // the lane's row in the wave's first 32-row tile
         int32_t sj[RT];                            // rank << 16 | adapter of its rows, or -1
 #pragma unroll
         for (int j = 0; j < RT; ++j) sj[j] = rw + 32u * j < vrows ? a.pslot[r0 + rw + 32u * j] : -1;
         // (the tile at hand changes as the steps go: its rows' adapters by way of the wave's
-        // own part of LDS, past the epilogue's partial results and the scales)
-        constexpr uint32_t kPast = 16u * WM * BR + (F8 ? 4u * (kTV + BR) : 0u);
+        // own part of LDS)
         int32_t* ps = reinterpret_cast<int32_t*>(lds + kPast) + (uint32_t)wv * (BR / 2) + lr;
         if (RT > 1) {
 #pragma unroll
             for (int j = 0; j < RT; ++j) ps[32 * j] = sj[j];   // (lanes l and l + 32 write the same)
         }
         auto of = [&](uint32_t j) -> int32_t { return RT > 1 ? ps[32u * j] : sj[0]; };
-        uint64_t todo = ballot(sj[0] >= 0);
-        uint32_t jn = 0u, kn = 0u;
-        int32_t who = 0;
-        const uint16_t *bp = a.ad_b, *lp = a.low;
-        bool more = true;
-        // The loads of the next step, tile by tile and adapter by adapter. Past the last
-        // one (who -1) they are made all the same, from where the last one's were: the
-        // count of loads in flight is then known where a step is used, and the ones
-        // after it stay in flight.
-        auto fetch = [&](Step& st) {
-            if (more && kn >= (uint32_t)who >> 16) {
-                while (todo == 0u && jn + 1u < (uint32_t)RT) todo = ballot(of(++jn) >= 0);
-                more = todo != 0u;
-            }
-            if (more && kn >= (uint32_t)who >> 16) {
-                const int l = __builtin_ctzll(todo);
-                const int32_t s = of(jn);
-                who = __builtin_amdgcn_readlane(s, l);
-                todo &= ~ballot(s == who);
-                kn = 0u;
-                bp = a.ad_b + ((uint64_t)((uint32_t)who & 0xffffu) * V + n0) * wide;
-                // (the other rows' states are not used: all theirs from one place)
-                const uint32_t p = r0 + wn * (BR / 2) + 32u * jn;
-                lp = a.low + (uint64_t)(p + (s == who ? lr : (uint32_t)l & 31u)) * 3u * wide;
-            }
-            const uint32_t k = kn + 8u * lh, kk = k < (uint32_t)who >> 16 ? k : 0u;
-#pragma unroll
-            for (int i = 0; i < CT; ++i) {
-                const uint32_t c = cw + 32u * i + lr;
-                st.b[i] = *reinterpret_cast<const u32x4_a*>(bp + (c < vcols ? c : 0u) * wide + kk);
-            }
-#pragma unroll
-            for (int i = 0; i < 3; ++i) st.p[i] = *reinterpret_cast<const u32x4_a*>(lp + i * wide + kk);
-            st.who = more ? who : -1;
-            st.k = kn;
-            st.j = jn;
-            kn += more ? 16u : 0u;
-        };
-        f32x16 t[CT];
-#pragma unroll
-        for (int i = 0; i < CT; ++i)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) t[i][e] = 0.0f;
-        auto use = [&](Step& st) {
-            const uint32_t rank = (uint32_t)st.who >> 16;
-            auto& b = st.b;
-            if (st.k + 16u > rank) {   // what lies past the rank counts as zero, whatever it holds
-                const uint32_t k = st.k + 8u * lh, left = k < rank ? rank - k : 0u;
-                u32x4 live;
-#pragma unroll
-                for (uint32_t e = 0; e < 4u; ++e) live[e] = left > 2u * e + 1u ? 0xffffffffu : left == 2u * e + 1u ? 0xffffu : 0u;
-#pragma unroll
-                for (int i = 0; i < CT; ++i) b[i] &= live;
-#pragma unroll
-                for (int i = 0; i < 3; ++i) st.p[i] &= live;
-            }
-            const f32x16 zero = {};
-            if (st.k == 0u) {
-#pragma unroll
-                for (int i = 0; i < CT; ++i)
-                    t[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, b[i]), __builtin_bit_cast(bf16x8, st.p[2]), zero, 0, 0, 0);
-            } else {
-#pragma unroll
-                for (int i = 0; i < CT; ++i)
-                    t[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, b[i]), __builtin_bit_cast(bf16x8, st.p[2]), t[i], 0, 0, 0);
-            }
-#pragma unroll
-            for (int p = 1; p >= 0; --p)
-#pragma unroll
-                for (int i = 0; i < CT; ++i)
-                    t[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, b[i]), __builtin_bit_cast(bf16x8, st.p[p]), t[i], 0, 0, 0);
-            if (st.k + 16u >= rank) {
-#pragma unroll
-                for (int j = 0; j < RT; ++j) {
-                    if ((RT == 1 || st.j == (uint32_t)j) && sj[j] == st.who) {
-#pragma unroll
-                        for (int i = 0; i < CT; ++i)
-#pragma unroll
-                            for (int e = 0; e < 16; ++e) acc[i][j][e] += t[i][e];
-                    }
+#pragma unroll 1
+        for (uint32_t kw = 0u; kw < wide; kw += kFits) {
+            const uint32_t kend = kw + kFits;
+            if (kw != 0u) __syncthreads();
+            {   // ranks kw to kw + ww - 1 of the rows' states: per row three parts of ww
+                const uint32_t per = ww / 8u, all = vrows * 3u * per;
+                for (uint32_t c = tid; c < all; c += NW * kWave) {
+                    const uint32_t rp = c / per, ch8 = c % per, row = rp / 3u, part = rp % 3u;
+                    const uint32_t kk = min(kw + 8u * ch8, wide - 8u);
+                    const u32x4 v = *reinterpret_cast<const u32x4_a*>(a.low + ((uint64_t)(r0 + row) * 3u + part) * wide + kk);
+                    *reinterpret_cast<u32x4_a*>(lds + kLow + row * rowb + part * 2u * ww + 16u * ch8) = v;
                 }
             }
-        };
-        Step st[DP];
+            __syncthreads();
+            uint64_t todo = ballot(sj[0] >= 0);
+            uint32_t jn = 0u, kn = kw, end = kw;
+            int32_t who = 0;
+            const uint16_t* bp = a.ad_b;
+            bool more = true;
+            // The loads of the next step, tile by tile and adapter by adapter. Past the last
+            // one (who -1) they are made all the same, from where the last one's were: the
+            // count of loads in flight is then known where a step is used, and the ones
+            // after it stay in flight.
+            auto fetch = [&](Step& st) {
+                while (more && kn >= end) {
+                    while (todo == 0u && jn + 1u < (uint32_t)RT) todo = ballot(of(++jn) >= 0);
+                    more = todo != 0u;
+                    if (!more) break;
+                    const int32_t s = of(jn);
+                    who = __builtin_amdgcn_readlane(s, __builtin_ctzll(todo));
+                    todo &= ~ballot(s == who);
+                    kn = kw;
+                    end = min((uint32_t)who >> 16, kend);   // (below kw: nothing of it is left)
+                    bp = a.ad_b + ((uint64_t)((uint32_t)who & 0xffffu) * V + n0) * wide;
+                }
+                const uint32_t k = kn + 8u * lh, kk = k < end ? k : 0u;
 #pragma unroll
-        for (int d = 0; d < DP; ++d) fetch(st[d]);
-        // (one way out of the loop, so that the count of loads in flight is the same on every
-        // way in: a step past the last one adds to t, which nothing takes any more)
-        while (st[0].who >= 0) {
+                for (int i = 0; i < CT; ++i) {
+                    const uint32_t c = cw + 32u * i + lr;
+                    st.b[i] = *reinterpret_cast<const u32x4_a*>(bp + (c < vcols ? c : 0u) * wide + kk);
+                }
+                st.who = more ? who : -1;
+                st.k = more ? kn : kw;
+                st.j = jn;
+                kn += more ? 16u : 0u;
+            };
+            f32x16 t[CT];
 #pragma unroll
-            for (int d = 0; d < DP; ++d) {
-                use(st[d]);
-                fetch(st[d]);
+            for (int i = 0; i < CT; ++i)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) t[i][e] = 0.0f;
+            auto use = [&](Step& st) {
+                const uint32_t rank = (uint32_t)st.who >> 16;
+                const unsigned char* lp = lds + kLow + (rw + 32u * st.j) * rowb + 2u * (st.k - kw) + 16u * lh;
+                u32x4 p[3];
+#pragma unroll
+                for (int i = 0; i < 3; ++i) p[i] = *reinterpret_cast<const u32x4_a*>(lp + 2u * i * ww);
+                if (st.k + 16u > rank) {   // what lies past the rank counts as zero, whatever it holds
+                    const uint32_t k = st.k + 8u * lh, left = k < rank ? rank - k : 0u;
+                    u32x4 live;
+#pragma unroll
+                    for (uint32_t e = 0; e < 4u; ++e) live[e] = left > 2u * e + 1u ? 0xffffffffu : left == 2u * e + 1u ? 0xffffu : 0u;
+#pragma unroll
+                    for (int i = 0; i < CT; ++i) st.b[i] &= live;
+#pragma unroll
+                    for (int i = 0; i < 3; ++i) p[i] &= live;
+                }
+                const f32x16 zero = {};
+                if (st.k == kw) {
+#pragma unroll
+                    for (int i = 0; i < CT; ++i)
+                        t[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, st.b[i]), __builtin_bit_cast(bf16x8, p[2]), zero, 0, 0, 0);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < CT; ++i)
+                        t[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, st.b[i]), __builtin_bit_cast(bf16x8, p[2]), t[i], 0, 0, 0);
+                }
+#pragma unroll
+                for (int q = 1; q >= 0; --q)
+#pragma unroll
+                    for (int i = 0; i < CT; ++i)
+                        t[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, st.b[i]), __builtin_bit_cast(bf16x8, p[q]), t[i], 0, 0, 0);
+                if (st.k + 16u >= min(rank, kend)) {
+#pragma unroll
+                    for (int j = 0; j < RT; ++j) {
+                        if ((RT == 1 || st.j == (uint32_t)j) && sj[j] == st.who) {
+#pragma unroll
+                            for (int i = 0; i < CT; ++i)
+#pragma unroll
+                                for (int e = 0; e < 16; ++e) acc[i][j][e] += t[i][e];
+                        }
+                    }
+                }
+            };
+            Step st[DP];
+#pragma unroll
+            for (int d = 0; d < DP; ++d) fetch(st[d]);
+            // (one way out of the loop, so that the count of loads in flight is the same on every
+            // way in: a step past the last one adds to t, which nothing takes any more)
+            while (st[0].who >= 0) {
+#pragma unroll
+                for (int d = 0; d < DP; ++d) {
+                    use(st[d]);
+                    fetch(st[d]);
+                }
             }
         }
     }
