@@ -146,7 +146,7 @@ __global__ __launch_bounds__(NW * kWave, 2) void lmhead_tile(LmArgs a) {
         xo[i] = (AD ? row_of(r) : r) * K * EB + ch;
     }
     const uint32_t nsteps = K / kTK;
-    const uint32_t rot = a.nchunks == 1u ? nb % nsteps : 0u;
+    const uint32_t rot = a.nchunks == 1u && (!F8 || nsteps != 0u) ? nb % nsteps : 0u;
     // (the byte offset of stage t in a row; stages past the end re-read the last)
     auto koff = [&](uint32_t t) -> uint32_t {
         uint32_t q = (t < nsteps ? t : nsteps - 1u) + rot;
