@@ -134,7 +134,11 @@ def test_adapters_exact_on_every_tile(sampler, rows, vocab, f8):
     (1, 1, 64, (1,), 1), (1, 300, 64, (16,), 1), (2, 65, 128, (0, 5), 1), (5, 700, 192, (256,), 1),
     (33, 1000, 256, (128, 40), 1), (64, 513, 128, tuple(range(1, 65)), 1), (64, 200, 64, (8,) * 200, 1),
     (130, 257, 64, (20, 33, 7), 5), (1024, 300, 64, (16,) * 1024, 1), (1100, 500, 128, (12, 4, 30, 64, 100), 3),
-    (1027, 40, 1024, (32,), 1), (640, 333, 64, (-3, 9, 50), 64), (7, 90, 4096, (17, 32), 1)])
+    (1027, 40, 1024, (32,), 1), (640, 333, 64, (-3, 9, 50), 64), (7, 90, 4096, (17, 32), 1),
+    # more ranks than a tile's LDS holds at a time, on each tile; hidden sizes past one and two rounds of lm_low
+    (511, 30000, 128, (128, 40, 201), 1), (300, 20001, 64, (256, 30), 1), (128, 20001, 64, (256, 8), 1), (64, 80001, 64, (250,), 1),
+    (64, 33001, 64, (256, 7), 1), (64, 20001, 64, (200, 16), 1), (64, 300, 64, (256, 100), 1),
+    (5, 70, 4160, (16, 9), 1), (17, 100, 8256, (24,), 1)])
 def test_adapters_exact(sampler, rows, vocab, hidden, ranks, per, f8):
     exact_case(sampler, rows, vocab, hidden, f8, ranks, rows + vocab + len(ranks), per)
 
@@ -315,6 +319,39 @@ def test_captured_into_a_graph(sampler):
         for a, b in ((n1, n2), (o1, o2)):
             for k in a:
                 assert torch.equal(a[k].view(torch.uint8), b[k].view(torch.uint8)), (i, k)
+
+
+@pytest.mark.parametrize("f8", [False, True])
+def test_on_a_side_stream_after_its_inputs(sampler, f8):
+    torch = sampler.torch
+    gen = torch.Generator(device="cuda").manual_seed(16)
+    x, w, kw, ad, ref = whole(torch, gen, 50, 3000, 256, f8, (16, 5, 40))
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    out = sampler.alloc_lmhead_out(50, 3000)
+    st.wait_stream(torch.cuda.current_stream())
+    from locus_amd.sampler import Adapters
+    sampler.lmhead_ex_dev(x, w, out, adapters=Adapters(ad["a"], ad["b"], rank=ad["rank"], scale=ad["scale"]), slot=ad["slot"],
+                          stream=st, **kw)
+    st.synchronize()
+    assert torch.equal(out["logits"], ref.float())
+
+
+@pytest.mark.parametrize("f8", [False, True])
+def test_pools_without_rank_and_scale(sampler, f8):
+    torch = sampler.torch
+    gen = torch.Generator(device="cuda").manual_seed(17)
+    x, w, kw, ad, _ = whole(torch, gen, 20, 600, 128, f8, (24, 24))
+    base = call(sampler, x, w, sampler.alloc_lmhead_out(20, 600), dict(ad, scale=torch.ones(2, device="cuda")), **kw)
+    g = call(sampler, x, w, sampler.alloc_lmhead_out(20, 600), {"a": ad["a"], "b": ad["b"], "slot": ad["slot"]}, **kw)
+    for k in base:
+        assert np.array_equal(g[k], base[k]), k
+
+
+def test_no_rows(sampler):
+    torch = sampler.torch
+    w = torch.zeros(100, 64, device="cuda", dtype=torch.bfloat16)
+    sampler.lmhead_ex_dev(w[:0], w, {"argmax_ids": torch.zeros(0, device="cuda", dtype=torch.int32)})
 
 
 def test_refusals_of_the_binding(sampler):
