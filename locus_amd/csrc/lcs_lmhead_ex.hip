@@ -193,29 +193,37 @@ __global__ __launch_bounds__(kLowThreads) void lm_low(LmArgs a) {
 
 namespace {
 
-template <int VT, int BR, int ST, int NW, int KS, bool F8, bool AD>
+template <int VT, int BR, int ST, int NW, int KS, bool F8, bool AD, int WN = 2>
 void tile(const LmArgs& a, hipStream_t st) {
-    hipLaunchKernelGGL((lmhead_tile<VT, BR, ST, NW, KS, false, F8, AD>), dim3(8u * ((a.nblocks + 7u) / 8u) * a.nchunks),
+    hipLaunchKernelGGL((lmhead_tile<VT, BR, ST, NW, KS, false, F8, AD, WN>), dim3(8u * ((a.nblocks + 7u) / 8u) * a.nchunks),
                        dim3(NW * kWave), 0, st, a);
 }
 
 // The tiles: up to 64 rows lmhead_shape's columns, above by the same measure (rounds of
 // workgroups over the CUs times what one takes). Rings of 64-k stages (128 k of
-// e4m3), three where they fit, and eight waves on the tiles from 256 columns up:
-// us by 64 VT columns x rows, ST stages, NW waves,
-//   64 rows, one block of 256 columns a CU: 50257 x 1600 bf16 with adapters, ST 3
-//     NW 8 41.0, NW 4 45.3, two stages 50; 151936 x 3584 e4m3 (594 blocks) 132,
-//     144, 142; 128256 x 4096 e4m3 (501) 116.5, 126, 116
-//   320 columns, ST 3 NW 4: 151936 x 3584 e4m3 116 (32-k stages 124), bf16 with adapters
-//     225 (235), but e4m3 with 64 adapters 197 (180: their reads want the two
-//     workgroups a CU that the smaller stages leave room for)
-//   128 columns, ST 3 NW 4: 32000 x 2048 e4m3 15.5 (NW 8 16.1)
-//   64 columns: 16000 x 4096 e4m3 18.0 with ST 4, 19.2 with six 32-k stages, bf16 27.0, 26.6
-//   128 rows, 256 columns: 128256 x 4096 e4m3 ST 3 NW 8 138, NW 4 153, 32-k stages
+// e4m3), three where they fit, and eight waves on the tiles from 256 columns up.
+// Us by columns x rows, ST stages, NW waves (rings of four to eight stages are no
+// faster):
+//   256 x 64: 50257 x 1600 bf16 with adapters, ST 3 NW 8 41.0, NW 4 45.3, ST 2 50;
+//     151936 x 3584 e4m3 (594 blocks) 132, 144, 142; 128256 x 4096 e4m3 (501) 116, 126, 116
+//   320 x 64, ST 3 NW 4: 151936 x 3584 e4m3 116 (32-k stages 124), bf16 with adapters
+//     225 (235), e4m3 with 64 adapters 176 (186)
+//   128 x 64, ST 3 NW 4: 32000 x 2048 e4m3 15.5 (NW 8 16.1)
+//   64 x 64: 16000 x 4096 e4m3 18.0 with ST 4, 19.2 with six 32-k stages, bf16 27.0, 26.6
+//   256 x 128: 128 x 128256 x 4096 e4m3 ST 3 NW 8 138, NW 4 153, 32-k stages
 //     163; bf16 with adapters 230, -, 266
-//   1024 rows, 256 x 256, ST 2 NW 8: 128256 x 4096 e4m3 683 (1576 TFLOP/s)
+//   256 x 256, ST 2 NW 8: 1024 x 128256 x 4096 e4m3 683 (1576 TFLOP/s; power bounds it:
+//     751 where the operands' bits vary more)
 struct LmExShape { uint32_t vt, br; };
-LmExShape lmhead_ex_shape(uint32_t rows, uint32_t vocab, bool f8, uint32_t cus) {
+LmExShape lmhead_ex_shape(uint32_t rows, uint32_t vocab, uint32_t hidden, bool f8, uint32_t cus) {
+    if (rows <= 64u) {
+        // 32-row tiles read half as much of x: 5 x 32000 x 2048 e4m3 17.4 -> 15.0, 16 x 128256 x
+        // 4096 102.6 -> 98.6; of 64 columns 16000 x 4096 18.0 against 19.5
+        LmExShape s{};
+        lmhead_shape_of(rows, vocab, hidden, cus, &s.vt, &s.br);
+        if (rows <= 32u && (s.vt == 2u || s.vt == 4u)) s.br = 32u;
+        return s;
+    }
     // (us a round, 4096 k of e4m3; bf16 takes 1.4 times as long, 128 rows a little more:
     // 384 x 128256 256 rows 481 us, 128 rows 507, e4m3 342, 308)
     struct { uint32_t vt, br, weight; } const shapes[] = {{4, 256, 86}, {4, 128, f8 ? 56u : 58u}, {2, 128, 42}};
@@ -238,6 +246,8 @@ void tiles(const LmArgs& a, uint32_t vt, uint32_t br, hipStream_t st) {
     else if (br == 128u && vt == 4u) tile<4, 128, 3, 8, 4, F8, AD>(a, st);
     else if (br == 128u) tile<2, 128, F8 ? 2 : 3, F8 ? 4 : 8, 4, F8, AD>(a, st);
     else if (vt == 5u) tile<5, 64, 3, 4, 4, F8, AD>(a, st);
+    else if (br == 32u && vt == 4u) tile<4, 32, 3, 4, 4, F8, AD, 1>(a, st);
+    else if (br == 32u) tile<2, 32, 3, 4, 4, F8, AD, 1>(a, st);
     else if (vt == 4u) tile<4, 64, 3, 8, 4, F8, AD>(a, st);
     else if (vt == 2u) tile<2, 64, 3, 4, 4, F8, AD>(a, st);
     else tile<1, 64, F8 ? 4 : 6, 4, F8 ? 4 : 2, F8, AD>(a, st);
@@ -248,14 +258,8 @@ void tiles(const LmArgs& a, uint32_t vt, uint32_t br, hipStream_t st) {
 hipError_t launch_lmhead_ex(const LmArgs& a0, bool f8, uint32_t cus, hipStream_t st) {
     if (!f8 && a0.ad_n == 0u) return launch_lmhead(a0, cus, st);
     LmArgs a = a0;
-    uint32_t vt, br;
-    if (a.rows <= 64u) {
-        lmhead_shape_of(a.rows, a.vocab, a.hidden, cus, &vt, &br);
-    } else {
-        const LmExShape s = lmhead_ex_shape(a.rows, a.vocab, f8, cus);
-        vt = s.vt;
-        br = s.br;
-    }
+    const LmExShape shape = lmhead_ex_shape(a.rows, a.vocab, a.hidden, f8, cus);
+    const uint32_t vt = shape.vt, br = shape.br;
     a.nblocks = (a.vocab + 64u * vt - 1u) / (64u * vt);
     a.nchunks = (a.rows + br - 1u) / br;
     if (a.ad_n != 0u) {

@@ -95,15 +95,15 @@ __device__ __forceinline__ void block_sync() {
 // AD: the rows are taken in the order of their adapters (lm_low, which also
 // has left each row's low-rank state in three bf16 parts): see the adapters' part
 // below.
-template <int VT, int BR, int ST, int NW = 4, int KS = 2, bool BIG = false, bool F8 = false, bool AD = false>
+template <int VT, int BR, int ST, int NW = 4, int KS = 2, bool BIG = false, bool F8 = false, bool AD = false, int WN = 2>
 __global__ __launch_bounds__(NW * kWave, 2) void lmhead_tile(LmArgs a) {
     constexpr uint32_t kTV = 64u * VT;        // columns per workgroup
     constexpr uint32_t EB = F8 ? 1u : 2u;     // bytes of an element
     constexpr uint32_t kTRowB = 32u * KS;     // bytes of a row in a stage
     constexpr int kTK = (int)(kTRowB / EB);   // k per LDS stage
     constexpr uint32_t kStage = (kTV + BR) * kTRowB;
-    constexpr int WM = NW / 2;                // waves side by side over the columns, two over the rows
-    constexpr int CT = 2 * VT / WM, RT = BR / 64;   // 32-column and 32-row tiles per wave
+    constexpr int WM = NW / WN;               // waves side by side over the columns, WN over the rows
+    constexpr int CT = 2 * VT / WM, RT = BR / (32 * WN);   // 32-column and 32-row tiles per wave
     constexpr uint32_t kCh = 2 * KS, kLog = KS == 4 ? 3 : 2;   // 16-byte chunks of a row
     constexpr uint32_t kSw = KS == 4 ? 1 : 2;   // the row bits that permute them start here
     constexpr int kLR = 64 / (int)kCh * NW;   // rows that one DMA load of every wave covers
@@ -201,7 +201,7 @@ __global__ __launch_bounds__(NW * kWave, 2) void lmhead_tile(LmArgs a) {
     constexpr int NR = CT + RT, NP = CT * RT;
     auto read1 = [&](Frag& f, int i, uint32_t sl, int s) {
         const unsigned char* pw = lds + sl * kStage + wm * (kTV / WM * kTRowB) + fo[s];
-        const unsigned char* px = lds + sl * kStage + kTV * kTRowB + wn * (BR / 2 * kTRowB) + fo[s];
+        const unsigned char* px = lds + sl * kStage + kTV * kTRowB + wn * (BR / WN * kTRowB) + fo[s];
         using At = std::conditional_t<F8, u32x4_a, bf16x8>;
         if (i < RT) f.x[i < RT ? i : 0] = *reinterpret_cast<const At*>(px + i * 32 * kTRowB);
         else f.w[i >= RT ? i - RT : 0] = *reinterpret_cast<const At*>(pw + (i - RT) * 32 * kTRowB);
@@ -294,7 +294,7 @@ __global__ __launch_bounds__(NW * kWave, 2) void lmhead_tile(LmArgs a) {
                 Frag f;
 #pragma unroll
                 for (int j = 0; j < RT; ++j) {
-                    const uint32_t r = wn * (BR / 2) + 32u * j + lr, rs = r < vrows ? r : 0u;
+                    const uint32_t r = wn * (BR / WN) + 32u * j + lr, rs = r < vrows ? r : 0u;
                     f.x[j] = *reinterpret_cast<const u32x4_a*>(xbase + (uint64_t)(AD ? row_of(rs) : rs) * K + ko);
                 }
 #pragma unroll
@@ -317,7 +317,7 @@ __global__ __launch_bounds__(NW * kWave, 2) void lmhead_tile(LmArgs a) {
         __syncthreads();
         float xs[RT];
 #pragma unroll
-        for (int j = 0; j < RT; ++j) xs[j] = sc[kTV + wn * (BR / 2) + 32u * j + lr];
+        for (int j = 0; j < RT; ++j) xs[j] = sc[kTV + wn * (BR / WN) + 32u * j + lr];
 #pragma unroll
         for (int i = 0; i < CT; ++i)
 #pragma unroll
@@ -354,13 +354,13 @@ __global__ __launch_bounds__(NW * kWave, 2) void lmhead_tile(LmArgs a) {
         static_assert(kFits >= 16u, "the adapters' place");
         const uint32_t wide = a.ad_wide;
         const uint32_t ww = min(wide, kFits), rowb = 6u * ww + 16u;   // (16 bytes more: the rows' banks differ)
-        const uint32_t rw = wn * (BR / 2) + lr;   // the lane's row in the wave's first 32-row tile
+        const uint32_t rw = wn * (BR / WN) + lr;   // the lane's row in the wave's first 32-row tile
         int32_t sj[RT];                            // rank << 16 | adapter of its rows, or -1
 #pragma unroll
         for (int j = 0; j < RT; ++j) sj[j] = rw + 32u * j < vrows ? a.pslot[r0 + rw + 32u * j] : -1;
         // (the tile at hand changes as the steps go: its rows' adapters by way of the wave's
         // own part of LDS)
-        int32_t* ps = reinterpret_cast<int32_t*>(lds + kPast) + (uint32_t)wv * (BR / 2) + lr;
+        int32_t* ps = reinterpret_cast<int32_t*>(lds + kPast) + (uint32_t)wv * (BR / WN) + lr;
         if (RT > 1) {
 #pragma unroll
             for (int j = 0; j < RT; ++j) ps[32 * j] = sj[j];   // (lanes l and l + 32 write the same)
@@ -476,14 +476,14 @@ __global__ __launch_bounds__(NW * kWave, 2) void lmhead_tile(LmArgs a) {
     }
 
     // ---- epilogue: acc[i][j][e] is column n0 + kTV / WM wm + 32 i + 8 (e / 4) +
-    // 4 lh + e % 4 of row r0 + BR / 2 wn + 32 j + lr ----
+    // 4 lh + e % 4 of row r0 + BR / WN wn + 32 j + lr ----
     struct Part { float max, sum, draft; uint32_t idx; };
     Part* part = reinterpret_cast<Part*>(lds);   // [WM][BR]: by the wave's columns
     const bool full = vcols == kTV;
     const bool vec = a.logits && (a.ld_logits & 3u) == 0u && (reinterpret_cast<uintptr_t>(a.logits) & 15u) == 0u;
 #pragma unroll
     for (int j = 0; j < RT; ++j) {
-        const uint32_t rl = wn * (BR / 2) + 32u * j + lr;   // the lane's row in the tile
+        const uint32_t rl = wn * (BR / WN) + 32u * j + lr;   // the lane's row in the tile
         const bool rin = rl < vrows;
         const uint32_t cb = kTV / WM * wm + 4u * lh;            // columns cb + 32 i + 8 (e / 4) + e % 4
         if (a.logits && rin) {

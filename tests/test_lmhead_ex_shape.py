@@ -1,6 +1,6 @@
-"""lcs_lmhead_ex's choice of a tile above 64 rows (lmhead_ex_shape), compiled for the
-CPU from the kernel's source, and lmhead_shape's below: the GPU tests' list names
-the tile that each case runs on, and every tile has one."""
+"""lcs_lmhead_ex's choice of a tile (lmhead_ex_shape, and lmhead_shape's under it),
+compiled for the CPU from the kernels' sources: the GPU tests' list names the tile
+that each case runs on, and every tile has one."""
 import ctypes
 import os
 import re
@@ -24,10 +24,14 @@ def test_cases_cover_every_tile(tmp_path):
     consts = re.findall(r"^constexpr uint32_t (?:kMaxVocab|kLmMaxBlocks) = .*$", source("lcs_internal.hpp"), re.M)
     big = re.search(r"^constexpr uint32_t kBigHidden = .*$", plain, re.M).group(0)
     (tmp_path / "shape.cpp").write_text(
-        "#include <cstdint>\n" + "\n".join(consts) + "\n" + big + "\n" + below + above +
-        """extern "C" void shape(uint32_t rows, uint32_t vocab, int f8, uint32_t cus, uint32_t* o) {
-    if (rows <= 64) { const LmShape s = lmhead_shape(rows, vocab, 448, cus); o[0] = s.vt, o[1] = s.br; }
-    else { const LmExShape s = lmhead_ex_shape(rows, vocab, f8 != 0, cus); o[0] = s.vt, o[1] = s.br; }
+        "#include <cstdint>\n" + "\n".join(consts) + "\n" + big + "\n" + below +
+        """static void lmhead_shape_of(uint32_t rows, uint32_t vocab, uint32_t hidden, uint32_t cus, uint32_t* vt, uint32_t* br) {
+    const LmShape s = lmhead_shape(rows, vocab, hidden, cus);
+    *vt = s.vt, *br = s.br;
+}
+""" + above + """extern "C" void shape(uint32_t rows, uint32_t vocab, int f8, uint32_t cus, uint32_t* o) {
+    const LmExShape s = lmhead_ex_shape(rows, vocab, 448, f8 != 0, cus);
+    o[0] = s.vt, o[1] = s.br;
 }
 """)
     so = str(tmp_path / "shape.so")
@@ -38,15 +42,15 @@ def test_cases_cover_every_tile(tmp_path):
         for f8 in (0, 1):
             fn(rows, vocab, f8, CUS, out)
             assert tuple(out) == (vt, br), (rows, vocab, f8, tuple(out))
-    launched = {(int(v), int(b)) for v, b in re.findall(r"tile<(\d+), (\d+), [^>]*F8, AD>\(", ex)}
-    assert launched == {(4, 256), (4, 128), (2, 128), (5, 64), (4, 64), (2, 64), (1, 64)} == {c[2:] for c in TILES}
+    launched = {(int(v), int(b)) for v, b in re.findall(r"tile<(\d+), (\d+), [^>]*F8, AD(?:, 1)?>\(", ex)}
+    assert launched == {(4, 256), (4, 128), (2, 128), (5, 64), (4, 64), (2, 64), (1, 64), (4, 32), (2, 32)} == {c[2:] for c in TILES}
     # with several row tiles too
     assert {c[2:] for c in TILES if c[0] > c[3]} == {(4, 256), (4, 128), (2, 128)}
     # every shape fits the context's records (lmhead_max_blocks, by the vocabulary alone)
     for vocab in list(range(1, 262145, 997)) + [262144]:
         most = max(min(-(-vocab // 64), 2 * CUS), min(-(-vocab // 128), 4 * CUS))
         most = max(min(most, 1024), -(-vocab // 256))
-        for rows in (1, 64, 65, 128, 200, 300, 1024):
+        for rows in (1, 33, 64, 65, 128, 200, 300, 1024):
             for f8 in (0, 1):
                 fn(rows, vocab, f8, CUS, out)
                 assert -(-vocab // (64 * out[0])) <= most, (rows, vocab, tuple(out))
