@@ -279,7 +279,6 @@ struct LmArgs {
 };
 constexpr uint32_t kAdMax = 1024;       // adapters of a pool
 constexpr uint32_t kAdWideMax = 256;    // their widest rank
-constexpr uint32_t kExHiddenMax = 65536;
 
 // residual addition and norm (lcs_norm.hip)
 constexpr uint32_t kNormHiddenMax = 32768;

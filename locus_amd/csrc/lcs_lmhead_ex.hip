@@ -224,15 +224,18 @@ LmExShape lmhead_ex_shape(uint32_t rows, uint32_t vocab, uint32_t hidden, bool f
         if (rows <= 32u && (s.vt == 2u || s.vt == 4u)) s.br = 32u;
         return s;
     }
-    // (us a round, 4096 k of e4m3; bf16 takes 1.4 times as long, 128 rows a little more:
-    // 384 x 128256 256 rows 481 us, 128 rows 507, e4m3 342, 308)
-    struct { uint32_t vt, br, weight; } const shapes[] = {{4, 256, 86}, {4, 128, f8 ? 56u : 58u}, {2, 128, 42}};
+    // us a round, 4096 k of e4m3 (bf16: / 1.36), from 128 to 1024 rows x 32000 to 128256. Two
+    // 128 x 128 tiles of e4m3 share a CU: one takes 42, two 54. 384 x 128256 e4m3 291 in rows
+    // of 192, 308 in 128, 353 in 256; bf16 with adapters 437, 411, 466; 176 x 42468 x 7552 bf16 205, 233,
+    // 213; 128 x 32000 e4m3 43 in 128 columns, 48 in 256, bf16 66, 81
+    struct { uint32_t vt, br, weight, on; } const shapes[] = {   // on: tiles a CU holds
+        {4, 256, 86, 1}, {4, 192, f8 ? 72u : 80u, 1}, {4, 128, 52, 1}, {2, 128, f8 ? 54u : 46u, f8 ? 2u : 1u}};
     LmExShape best{4u, 256u};
     uint64_t least = ~0ull;
     for (const auto& s : shapes) {
-        const uint64_t n = ((uint64_t)vocab + 64u * s.vt - 1u) / (64u * s.vt), chunks = (rows + s.br - 1u) / s.br;
+        const uint64_t n = ((uint64_t)vocab + 64u * s.vt - 1u) / (64u * s.vt), all = n * ((rows + s.br - 1u) / s.br);
         if (n > kLmMaxBlocks || (s.vt == 2u && n > 4u * cus)) continue;   // (lmhead_max_blocks)
-        const uint64_t cost = (n * chunks + cus - 1u) / cus * s.weight;
+        const uint64_t cost = s.on == 2u && all <= cus ? 42u : (all + s.on * cus - 1u) / (s.on * cus) * s.weight;
         if (cost < least) {
             least = cost;
             best = LmExShape{s.vt, s.br};
@@ -243,6 +246,7 @@ LmExShape lmhead_ex_shape(uint32_t rows, uint32_t vocab, uint32_t hidden, bool f
 template <bool F8, bool AD>
 void tiles(const LmArgs& a, uint32_t vt, uint32_t br, hipStream_t st) {
     if (br == 256u) tile<4, 256, 2, 8, 4, F8, AD>(a, st);
+    else if (br == 192u) tile<4, 192, 2, 8, 4, F8, AD>(a, st);
     else if (br == 128u && vt == 4u) tile<4, 128, 3, 8, 4, F8, AD>(a, st);
     else if (br == 128u) tile<2, 128, F8 ? 2 : 3, F8 ? 4 : 8, 4, F8, AD>(a, st);
     else if (vt == 5u) tile<5, 64, 3, 4, 4, F8, AD>(a, st);

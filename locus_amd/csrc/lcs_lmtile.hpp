@@ -59,7 +59,7 @@ __device__ __forceinline__ void block_sync() {
 
 // A workgroup computes 64 VT columns of BR rows, transposed (columns on the
 // MFMA's row side, so that a lane holds many columns of one row and the
-// epilogue reduces in registers): NW waves, two over the rows, in
+// epilogue reduces in registers): NW waves, WN of them over the rows, in
 // v_mfma_f32_32x32x16_bf16 tiles (lane l carries 8 consecutive k of row l % 32
 // of either operand, k chunk l / 32, and returns rows 8 (e / 4) + 4 (l / 32) +
 // e % 4 of column l % 32). The 256 x 256 tile takes eight waves, so that two
