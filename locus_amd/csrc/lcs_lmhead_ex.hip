@@ -224,18 +224,21 @@ LmExShape lmhead_ex_shape(uint32_t rows, uint32_t vocab, uint32_t hidden, bool f
         if (rows <= 32u && (s.vt == 2u || s.vt == 4u)) s.br = 32u;
         return s;
     }
-    // us a round, 4096 k of e4m3 (bf16: / 1.36), from 128 to 1024 rows x 32000 to 128256. Two
-    // 128 x 128 tiles of e4m3 share a CU: one takes 42, two 54. 384 x 128256 e4m3 291 in rows
-    // of 192, 308 in 128, 353 in 256; bf16 with adapters 437, 411, 466; 176 x 42468 x 7552 bf16 205, 233,
-    // 213; 128 x 32000 e4m3 43 in 128 columns, 48 in 256, bf16 66, 81
-    struct { uint32_t vt, br, weight, on; } const shapes[] = {   // on: tiles a CU holds
-        {4, 256, 86, 1}, {4, 192, f8 ? 72u : 80u, 1}, {4, 128, 52, 1}, {2, 128, f8 ? 54u : 46u, f8 ? 2u : 1u}};
+    // us a round, 4096 k of e4m3 (bf16: / 1.36), from 128 to 1024 rows x 2000 to 128256; one: where
+    // no CU gets a second tile. 384 x 128256 e4m3 291 in rows of 192, 308 in 128, 353 in
+    // 256; bf16 with adapters 437, 411, 466; 176 x 42468 x 7552 bf16 205, 233, 213; 128 x 32000
+    // e4m3 43 in 128 columns, 48 in 256, bf16 66, 81; small vocabularies in 64 x 64, 128 x 64,
+    // 128 x 128: 128 x 8000 e4m3 19.5, 23.0, 37.8, bf16 32, 37, 45; 128 x 16000 28.2, 25.9, 39.0 and
+    // 59, 43, 49; 512 x 4000 bf16 52, 36, 43; 850 x 6861 x 6144 e4m3 135, 114, 100
+    struct { uint32_t vt, br, weight, one, on; } const shapes[] = {   // on: tiles a CU holds
+        {4, 256, 86, 86, 1}, {4, 192, f8 ? 72u : 80u, f8 ? 72u : 80u, 1}, {4, 128, 52, 52, 1},
+        {2, 128, f8 ? 54u : 46u, f8 ? 42u : 38u, f8 ? 2u : 1u}, {2, 64, 47, f8 ? 24u : 28u, 2}, {1, 64, f8 ? 28u : 40u, f8 ? 20u : 23u, 2}};
     LmExShape best{4u, 256u};
     uint64_t least = ~0ull;
     for (const auto& s : shapes) {
         const uint64_t n = ((uint64_t)vocab + 64u * s.vt - 1u) / (64u * s.vt), all = n * ((rows + s.br - 1u) / s.br);
-        if (n > kLmMaxBlocks || (s.vt == 2u && n > 4u * cus)) continue;   // (lmhead_max_blocks)
-        const uint64_t cost = s.on == 2u && all <= cus ? 42u : (all + s.on * cus - 1u) / (s.on * cus) * s.weight;
+        if (n > kLmMaxBlocks || (s.vt <= 2u && n > 2u * s.vt * cus)) continue;   // (lmhead_max_blocks)
+        const uint64_t cost = all <= cus ? s.one : (all + s.on * cus - 1u) / (s.on * cus) * s.weight;
         if (cost < least) {
             least = cost;
             best = LmExShape{s.vt, s.br};

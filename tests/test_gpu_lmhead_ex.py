@@ -20,8 +20,8 @@ U = 2.0 ** -24
 TILES = [
     (3, 300, 1, 64), (64, 16384, 1, 64), (1, 20001, 2, 32), (32, 32768, 2, 32), (31, 33001, 4, 32), (17, 100001, 4, 32),
     (64, 20001, 2, 64), (33, 32768, 2, 64), (64, 33001, 4, 64), (47, 100001, 4, 64), (2, 80001, 5, 64), (64, 80001, 5, 64),
-    (65, 140, 2, 128), (128, 20001, 2, 128), (300, 1001, 2, 128), (128, 50257, 4, 128), (300, 20001, 4, 128),
-    (192, 50257, 4, 192),
+    (65, 140, 1, 64), (300, 1001, 1, 64), (128, 16001, 2, 64), (128, 20001, 2, 128), (300, 8001, 2, 128),
+    (128, 50257, 4, 128), (300, 20001, 4, 128), (192, 50257, 4, 192),
     (150, 60000, 4, 192), (570, 21000, 4, 192), (256, 60000, 4, 256), (200, 50257, 4, 256), (511, 30000, 4, 256)]
 
 
@@ -140,6 +140,7 @@ def test_adapters_exact_on_every_tile(sampler, rows, vocab, f8):
     # more ranks than a tile's LDS holds at a time, on each tile; hidden sizes past one and two rounds of lm_low
     (511, 30000, 128, (128, 40, 201), 1), (190, 50257, 64, (128, 40, 201), 1), (300, 20001, 64, (256, 30), 1), (128, 20001, 64, (256, 8), 1), (64, 80001, 64, (250,), 1),
     (64, 33001, 64, (256, 7), 1), (64, 20001, 64, (200, 16), 1), (32, 33001, 64, (256, 7), 1), (9, 20001, 64, (200, 16), 1), (64, 300, 64, (256, 100), 1),
+    (300, 1001, 64, (256, 30), 1), (128, 16001, 64, (200, 16), 1),
     (5, 70, 4160, (16, 9), 1), (17, 100, 8256, (24,), 1)])
 def test_adapters_exact(sampler, rows, vocab, hidden, ranks, per, f8):
     exact_case(sampler, rows, vocab, hidden, f8, ranks, rows + vocab + len(ranks), per)

@@ -45,7 +45,7 @@ def test_cases_cover_every_tile(tmp_path):
     launched = {(int(v), int(b)) for v, b in re.findall(r"tile<(\d+), (\d+), [^>]*F8, AD(?:, 1)?>\(", ex)}
     assert launched == {(4, 256), (4, 192), (4, 128), (2, 128), (5, 64), (4, 64), (2, 64), (1, 64), (4, 32), (2, 32)} == {c[2:] for c in TILES}
     # with several row tiles too
-    assert {c[2:] for c in TILES if c[0] > c[3]} == {(4, 256), (4, 192), (4, 128), (2, 128)}
+    assert {c[2:] for c in TILES if c[0] > c[3]} == {(4, 256), (4, 192), (4, 128), (2, 128), (2, 64), (1, 64)}
     # every shape fits the context's records (lmhead_max_blocks, by the vocabulary alone)
     for vocab in list(range(1, 262145, 997)) + [262144]:
         most = max(min(-(-vocab // 64), 2 * CUS), min(-(-vocab // 128), 4 * CUS))
