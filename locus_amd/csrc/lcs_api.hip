@@ -46,7 +46,7 @@ struct lcs_ctx {
     // lcs_lmhead_ex with adapters: the rows' order and their low-rank states, max_rows each
     uint32_t* ad_perm = nullptr;
     int32_t* ad_slot = nullptr;
-    uint16_t* ad_low = nullptr;     // x 3 kAdWideMax
+    float* ad_low = nullptr;        // x kAdParts kAdWideMax
     uint32_t cus = 256;             // compute units of the device (the lm-head's tile shape)
     // nucleus path workspace (kNucRows rows at a time)
     lcs::NucRow* nrow = nullptr;
@@ -169,7 +169,7 @@ lcs_ctx* lcs_create(int device, uint32_t max_rows, uint32_t max_vocab, uint32_t 
         (e = hipMalloc(&c->nlist, nuc_rows * lcs::kNucList * 8)) != hipSuccess ||
         (e = hipMalloc(&c->ad_perm, (size_t)max_rows * 4)) != hipSuccess ||
         (e = hipMalloc(&c->ad_slot, (size_t)max_rows * 4)) != hipSuccess ||
-        (e = hipMalloc(&c->ad_low, (size_t)max_rows * 3 * lcs::kAdWideMax * 2)) != hipSuccess ||
+        (e = hipMalloc(&c->ad_low, (size_t)max_rows * lcs::kAdParts * lcs::kAdWideMax * 4)) != hipSuccess ||
         (e = hipMalloc(&c->lp_params, (size_t)max_rows * sizeof(lcs_params))) != hipSuccess ||
         (e = hipMalloc(&c->lp_ids, (size_t)max_rows * 4)) != hipSuccess ||
         (e = hipMemset(c->lp_params, 0, (size_t)max_rows * sizeof(lcs_params))) != hipSuccess ||

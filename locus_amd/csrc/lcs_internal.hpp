@@ -266,7 +266,7 @@ struct LmArgs {
     const float* w_scale;           // vocab, or NULL: 1
     // adapters (ad_n 0: none)
     uint32_t ad_n, ad_wide;
-    uint32_t low_z;                 // lm_low's gridDim.z
+    uint32_t low_z, low_s;          // lm_low: groups of rows side by side; k in 1 << low_s parts, up to kAdParts
     const uint16_t* ad_a;           // ad_n x ad_wide x hidden bf16
     const uint16_t* ad_b;           // ad_n x vocab x ad_wide bf16
     const int32_t* ad_rank;         // ad_n, or NULL: ad_wide
@@ -275,10 +275,11 @@ struct LmArgs {
     // ... as lm_low leaves them: the rows in the order of their adapters
     uint32_t* perm;                 // rows: the row at a position
     int32_t* pslot;                 // rows: its adapter's rank << 16 | its adapter, or -1 (also for a rank of 0)
-    uint16_t* low;                  // rows x 3 x ad_wide: its low-rank state, as the sum of three bf16 parts
+    float* low;                     // rows x (1 << low_s) x ad_wide: its low-rank state, summands by part of k
 };
 constexpr uint32_t kAdMax = 1024;       // adapters of a pool
 constexpr uint32_t kAdWideMax = 256;    // their widest rank
+constexpr uint32_t kAdParts = 4;
 
 // residual addition and norm (lcs_norm.hip)
 constexpr uint32_t kNormHiddenMax = 32768;

@@ -49,32 +49,32 @@ __device__ __forceinline__ bf16x8 x_frag(const unsigned char* row, uint32_t k) {
         return __builtin_bit_cast(bf16x8, r);
     }
 }
-__device__ __forceinline__ uint32_t to_bf16(float f) {   // finite: to nearest even
-    const uint32_t u = __float_as_uint(f);
-    if ((u & 0x7f800000u) == 0x7f800000u) return (u >> 16) | ((u & 0x7fffffu) ? 0x40u : 0u);
-    return (u + 0x7fffu + ((u >> 16) & 1u)) >> 16;
-}
 }  // namespace
 
-// Workgroup (i, q, z): adapter i, ranks 16 q to 16 q + 15, every gridDim.z-th group of
-// 16 of its rows, from the z-th; where there are fewer rows than adapters i is a row,
-// and the workgroup of an adapter's first row takes it. The rows' slots give the
+// Workgroup (i, q, z): adapter i, ranks 16 q to 16 q + 15, one of the parts of k (z's low
+// bits) and, from the one that z's other bits name, every low_z-th group of 16 of its
+// rows; where there are fewer rows than adapters i is a row, and the workgroup of an
+// adapter's first row takes it. The rows' slots give the
 // adapter's rows and, by the slots below its own, its place in the order, with one
 // exchange between the waves; the workgroups without work end there. A group goes
-// over all of k, the waves taking 64 k in turn in v_mfma_f32_16x16x32_bf16 tiles (ranks
+// over the part of k, the waves taking 64 k in turn in v_mfma_f32_16x16x32_bf16 tiles (ranks
 // on its row side; lane l carries 8 consecutive k of row l % 16, k chunk l / 16,
-// and returns rows 4 (l / 16) + e of column l % 16), up to 256 k a wave loaded at
-// once, and their sums meet in LDS in a fixed order. Latency bounds it (a launch, the
-// slots, the factor from HBM): small tiles make many workgroups.
-template <bool F8>
+// and returns rows 4 (l / 16) + e of column l % 16), up to 32 N k a wave loaded at
+// once, and their sums meet in LDS in a fixed order; lmhead_tile adds up the parts of k.
+// Latency bounds it (a launch, the slots, the factor from HBM), and past 128 KB of the
+// factor what one CU can have in flight: hence the parts. Us with one part and as it
+// is: 1 x 4096 k 8.2 and 5.6, 64 rows with 32 adapters 8.3 and 6.7; the whole call for 33 x
+// 67281 x 7808 214 and 203, for 163 x 50257 x 7936 e4m3 181 and 168.
+template <bool F8, uint32_t N>
 __global__ __launch_bounds__(kLowThreads) void lm_low(LmArgs a) {
     struct Count { uint32_t below, mine, none, ahead; };
-    __shared__ Count part[kLowWaves];
+    __shared__ Count counts[kLowWaves];
     __shared__ uint32_t rid[kLowRows];
     __shared__ float red[kLowWaves][16 * 17];
     const uint32_t tid = tid_x();
     const int lane = lane_id(), wv = __builtin_amdgcn_readfirstlane((int)(tid / kWave));
-    const uint32_t item = wg_x(), rt = __builtin_amdgcn_workgroup_id_y(), z0 = __builtin_amdgcn_workgroup_id_z(), zs = a.low_z;
+    const uint32_t item = wg_x(), rt = __builtin_amdgcn_workgroup_id_y(), z = __builtin_amdgcn_workgroup_id_z(), zs = a.low_z;
+    const uint32_t parts = 1u << a.low_s, part = z & (parts - 1u), z0 = z >> a.low_s, kstep = parts * (kLowWaves * 64u);
     const uint32_t K = a.hidden, wide = a.ad_wide;
     auto slot_at = [&](uint32_t row) -> uint32_t {   // (kAdMax: none)
         const uint32_t s = row < a.rows ? (uint32_t)a.slot[row] : kAdMax;
@@ -89,10 +89,10 @@ __global__ __launch_bounds__(kLowThreads) void lm_low(LmArgs a) {
     const float scale = ad != kAdMax && a.ad_scale ? a.ad_scale[ad] : 1.0f;
     const uint32_t rank = rk <= 0 ? 0u : min((uint32_t)rk, wide);
     const uint32_t lr = (uint32_t)lane & 15u, lh = (uint32_t)lane >> 4;
-    const uint32_t kf = (uint32_t)wv * 64u, q = rt * 16u + lr;
+    const uint32_t kf = (part * kLowWaves + (uint32_t)wv) * 64u, q = rt * 16u + lr;
     const uint16_t* af = a.ad_a + ((uint64_t)(ad == kAdMax ? 0u : ad) * wide + (q < rank ? q : 0u)) * K;
-    auto at = [&](uint32_t k0, uint32_t s) -> uint32_t {   // the lane's k of product s of 8
-        const uint32_t k = k0 + (s / 2u) * (kLowWaves * 64u) + 32u * (s % 2u) + 8u * lh;
+    auto at = [&](uint32_t k0, uint32_t s) -> uint32_t {   // the lane's k of product s
+        const uint32_t k = k0 + (s / 2u) * kstep + 32u * (s % 2u) + 8u * lh;
         return k < K ? k : 8u * lh;
     };
     auto a_frag = [&](uint32_t k0, uint32_t s) { return __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4_a*>(af + at(k0, s))); };
@@ -105,10 +105,10 @@ __global__ __launch_bounds__(kLowThreads) void lm_low(LmArgs a) {
         c.none += n(row < a.rows && s == kAdMax);
         c.ahead += n(row < item && s == ad);
     }
-    if (lane == 0) part[wv] = c;
+    if (lane == 0) counts[wv] = c;
     __syncthreads();
     // (lane w takes wave w's counts; nmine, nnone: those of the waves ahead)
-    c = part[lane < kLowWaves ? lane : 0];
+    c = counts[lane < kLowWaves ? lane : 0];
     const bool in = lane < kLowWaves, before = lane < wv;
     const uint32_t pos = wave_sum_u(in ? c.below : 0u), total = wave_sum_u(in ? c.mine : 0u), none = wave_sum_u(in ? c.none : 0u);
     const uint32_t ahead = wave_sum_u(in ? c.ahead : 0u);
@@ -123,19 +123,19 @@ __global__ __launch_bounds__(kLowThreads) void lm_low(LmArgs a) {
             n += (uint32_t)__builtin_popcountll(b);
         }
     };
-    if (item == 0u && rt == 0u && z0 == 0u && none != 0u) {
+    if (item == 0u && rt == 0u && z == 0u && none != 0u) {
         each(kAdMax, nnone, [&](uint32_t n, uint32_t row) {
             a.perm[a.rows - none + n] = row;
             a.pslot[a.rows - none + n] = -1;
         });
     }
     if (ad == kAdMax || total <= z0 * kLowRows || (a.rows < a.ad_n && ahead != 0u)) return;
-    // the factor's first 256 k of each wave serve every group; they are on their way
+    // the factor's first 32 N k of each wave serve every group; they are on their way
     // while the first group's rows are found
-    bf16x8 fa[8];
+    bf16x8 fa[N];
 #pragma unroll
-    for (uint32_t s = 0; s < 8u; ++s) fa[s] = a_frag(kf, s);
-    if (rt == 0u && z0 == 0u) {
+    for (uint32_t s = 0; s < N; ++s) fa[s] = a_frag(kf, s);
+    if (rt == 0u && z == 0u) {
         each(ad, nmine, [&](uint32_t n, uint32_t row) {
             a.perm[pos + n] = row;
             a.pslot[pos + n] = rank ? (int32_t)(rank << 16 | ad) : -1;
@@ -152,14 +152,14 @@ __global__ __launch_bounds__(kLowThreads) void lm_low(LmArgs a) {
         const uint32_t row = tid / 16u, co = tid % 16u, qo = rt * 16u + co;   // the state that the thread writes
         const float xs = F8 && a.x_scale && row < rows ? a.x_scale[rid[row]] : 1.0f;
         f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-        bf16x8 fx[8];
+        bf16x8 fx[N];
 #pragma unroll
-        for (uint32_t s = 0; s < 8u; ++s) fx[s] = x_frag<F8>(x, at(kf, s));
+        for (uint32_t s = 0; s < N; ++s) fx[s] = x_frag<F8>(x, at(kf, s));
 #pragma unroll
-        for (uint32_t s = 0; s < 8u; ++s)
-            if (kf + (s / 2u) * (kLowWaves * 64u) < K) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[s], fx[s], acc, 0, 0, 0);
+        for (uint32_t s = 0; s < N; ++s)
+            if (kf + (s / 2u) * kstep < K) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[s], fx[s], acc, 0, 0, 0);
 #pragma unroll 1
-        for (uint32_t k0 = kf + 4u * kLowWaves * 64u; k0 < K; k0 += 2u * kLowWaves * 64u) {
+        for (uint32_t k0 = kf + N / 2u * kstep; k0 < K; k0 += 2u * kstep) {
             bf16x8 fb[4];
 #pragma unroll
             for (uint32_t s = 0; s < 4u; ++s) {
@@ -168,7 +168,7 @@ __global__ __launch_bounds__(kLowThreads) void lm_low(LmArgs a) {
             }
 #pragma unroll
             for (uint32_t s = 0; s < 4u; ++s)
-                if (k0 + (s / 2u) * (kLowWaves * 64u) < K) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[s], fx[s], acc, 0, 0, 0);
+                if (k0 + (s / 2u) * kstep < K) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[s], fx[s], acc, 0, 0, 0);
         }
 #pragma unroll
         for (int e = 0; e < 4; ++e) red[wv][(4 * (int)lh + e) * 17 + (int)lr] = acc[e];
@@ -178,14 +178,7 @@ __global__ __launch_bounds__(kLowThreads) void lm_low(LmArgs a) {
 #pragma unroll
             for (int w = 0; w < kLowWaves; ++w) p += red[w][co * 17u + row];
             // (ranks past the adapter's read rank 0's factor: nothing of theirs is kept)
-            p = qo < rank ? p * scale * xs : 0.0f;
-            uint16_t* low = a.low + (uint64_t)(pos + g0 + row) * 3u * wide + qo;
-#pragma unroll
-            for (uint32_t i = 0; i < 3u; ++i) {
-                const uint32_t u = to_bf16(p);
-                low[i * wide] = (uint16_t)u;
-                p = (u & 0x7f80u) == 0x7f80u ? 0.0f : p - __uint_as_float(u << 16);   // (an inf or NaN is whole in the first part)
-            }
+            a.low[((uint64_t)(pos + g0 + row) * parts + part) * wide + qo] = qo < rank ? p * scale * xs : 0.0f;
         }
         __syncthreads();   // (rid and red are free for the next group)
     }
@@ -270,13 +263,19 @@ hipError_t launch_lmhead_ex(const LmArgs& a0, bool f8, uint32_t cus, hipStream_t
     a.nblocks = (a.vocab + 64u * vt - 1u) / (64u * vt);
     a.nchunks = (a.rows + br - 1u) / br;
     if (a.ad_n != 0u) {
-        // (the rows' groups side by side as long as all the workgroups can run at once)
+        // Parts of k, then the rows' groups, side by side as long as all the workgroups can
+        // run at once. A part costs every tile another read of its rows' states: 425 x 32000
+        // x 2688 with two parts 107, four 112; with up to 64 rows they pay from 1024 k up (37 x
+        // 50257 x 1600 with one 57.3, two 55.3).
         const uint32_t nx = a.ad_n < a.rows ? a.ad_n : a.rows, ny = (a.ad_wide + 15u) / 16u, groups = (a.rows + kLowRows - 1u) / kLowRows;
-        const uint32_t nz = 2u * cus / (nx * ny);
+        const uint32_t most = 2u * cus / (nx * ny), least = kLowWaves * (a.rows <= 64u ? 64u : 128u);
+        a.low_s = 0u;
+        while ((2u << a.low_s) <= kAdParts && (4u << a.low_s) <= most && least << a.low_s < a.hidden) ++a.low_s;
+        const uint32_t nz = most >> a.low_s;
         a.low_z = nz == 0u ? 1u : nz < groups ? nz : groups;
-        const dim3 grid(nx, ny, a.low_z);
-        if (f8) hipLaunchKernelGGL((lm_low<true>), grid, dim3(kLowThreads), 0, st, a);
-        else hipLaunchKernelGGL((lm_low<false>), grid, dim3(kLowThreads), 0, st, a);
+        const bool few = a.hidden <= (uint32_t)(kLowWaves * 128) << a.low_s;
+        auto low = f8 ? (few ? lm_low<true, 4> : lm_low<true, 8>) : (few ? lm_low<false, 4> : lm_low<false, 8>);
+        hipLaunchKernelGGL(low, dim3(nx, ny, a.low_z << a.low_s), dim3(kLowThreads), 0, st, a);
         if (f8) tiles<true, true>(a, vt, br, st);
         else tiles<false, true>(a, vt, br, st);
     } else {

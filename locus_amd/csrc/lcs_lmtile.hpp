@@ -49,6 +49,13 @@ __device__ __forceinline__ bool nan_bits(float v) {
     asm("" : "+v"(u));
     return (u & 0x7fffffffu) > 0x7f800000u;
 }
+// To bf16, to nearest even; NaN stays NaN (by its bits, as above).
+__device__ __forceinline__ uint32_t bf16_bits(float v) {
+    uint32_t u = __float_as_uint(v);
+    asm("" : "+v"(u));
+    if ((u & 0x7f800000u) == 0x7f800000u) return (u >> 16) | ((u & 0x7fffffu) ? 0x40u : 0u);
+    return (u + 0x7fffu + ((u >> 16) & 1u)) >> 16;
+}
 // A workgroup barrier that waits for no memory operation.
 __device__ __forceinline__ void block_sync() {
     __builtin_amdgcn_sched_barrier(0);
@@ -56,6 +63,9 @@ __device__ __forceinline__ void block_sync() {
     asm volatile("" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
 }
+
+template <uint32_t P>
+struct Parts { static constexpr uint32_t value = P; };
 
 // A workgroup computes 64 VT columns of BR rows, transposed (columns on the
 // MFMA's row side, so that a lane holds many columns of one row and the
@@ -93,7 +103,7 @@ __device__ __forceinline__ void block_sync() {
 // of the logits' norm against 9e-8 here (4096 random k), and sums are to be f32.
 // The row's and the column's scale multiply the sums once, ahead of the adapters.
 // AD: the rows are taken in the order of their adapters (lm_low, which also
-// has left each row's low-rank state in three bf16 parts): see the adapters' part
+// has left each row's low-rank state): see the adapters' part
 // below.
 template <int VT, int BR, int ST, int NW = 4, int KS = 2, bool BIG = false, bool F8 = false, bool AD = false, int WN = 2>
 __global__ __launch_bounds__(NW * kWave, 2) void lmhead_tile(LmArgs a) {
@@ -370,15 +380,46 @@ __global__ __launch_bounds__(NW * kWave, 2) void lmhead_tile(LmArgs a) {
         for (uint32_t kw = 0u; kw < wide; kw += kFits) {
             const uint32_t kend = kw + kFits;
             if (kw != 0u) __syncthreads();
-            {   // ranks kw to kw + ww - 1 of the rows' states: per row three parts of ww
-                const uint32_t per = ww / 8u, all = vrows * 3u * per;
-                for (uint32_t c = tid; c < all; c += NW * kWave) {
-                    const uint32_t rp = c / per, ch8 = c % per, row = rp / 3u, part = rp % 3u;
-                    const uint32_t kk = min(kw + 8u * ch8, wide - 8u);
-                    const u32x4 v = *reinterpret_cast<const u32x4_a*>(a.low + ((uint64_t)(r0 + row) * 3u + part) * wide + kk);
-                    *reinterpret_cast<u32x4_a*>(lds + kLow + row * rowb + part * 2u * ww + 16u * ch8) = v;
+            // ranks kw to kw + ww - 1 of the rows' states: per row three bf16 parts of ww. What a
+            // thread reads at a time is asked for together: the states come from another XCD.
+            auto stage = [&](auto np) {
+                constexpr uint32_t P = decltype(np)::value, U = P == 4u ? 1u : 2u;
+                const uint32_t per = ww / 4u, all = vrows * per;
+                for (uint32_t c0 = tid; c0 < all; c0 += U * NW * kWave) {
+                    float4 v[U][P];
+                    uint32_t row[U], ch[U];
+#pragma unroll
+                    for (uint32_t u = 0; u < U; ++u) {
+                        const uint32_t c = c0 + u * NW * kWave, cc = c < all ? c : c0;
+                        row[u] = cc / per, ch[u] = cc - row[u] * per;
+                        const float* s = a.low + (uint64_t)(r0 + row[u]) * P * wide + min(kw + 4u * ch[u], wide - 4u);
+#pragma unroll
+                        for (uint32_t i = 0; i < P; ++i) v[u][i] = *reinterpret_cast<const float4*>(s + i * wide);
+                    }
+#pragma unroll
+                    for (uint32_t u = 0; u < U; ++u) {
+                        if (c0 + u * NW * kWave >= all) break;
+                        float f[4] = {v[u][0].x, v[u][0].y, v[u][0].z, v[u][0].w};
+#pragma unroll
+                        for (uint32_t i = 1; i < P; ++i) f[0] += v[u][i].x, f[1] += v[u][i].y, f[2] += v[u][i].z, f[3] += v[u][i].w;
+#pragma unroll
+                        for (uint32_t i = 0; i < 3u; ++i) {
+                            uint32_t h[4];
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                h[e] = bf16_bits(f[e]);
+                                // (an inf or NaN is whole in the first part)
+                                f[e] = (h[e] & 0x7f80u) == 0x7f80u ? 0.0f : f[e] - __uint_as_float(h[e] << 16);
+                            }
+                            *reinterpret_cast<uint2*>(lds + kLow + row[u] * rowb + i * 2u * ww + 8u * ch[u]) =
+                                make_uint2(h[0] | h[1] << 16, h[2] | h[3] << 16);
+                        }
+                    }
                 }
-            }
+            };
+            if (a.low_s == 0u) stage(Parts<1>{});
+            else if (a.low_s == 1u) stage(Parts<2>{});
+            else stage(Parts<4>{});
             __syncthreads();
             uint64_t todo = ballot(sj[0] >= 0);
             uint32_t jn = 0u, kn = kw, end = kw;

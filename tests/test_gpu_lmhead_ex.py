@@ -141,7 +141,9 @@ def test_adapters_exact_on_every_tile(sampler, rows, vocab, f8):
     (511, 30000, 128, (128, 40, 201), 1), (190, 50257, 64, (128, 40, 201), 1), (300, 20001, 64, (256, 30), 1), (128, 20001, 64, (256, 8), 1), (64, 80001, 64, (250,), 1),
     (64, 33001, 64, (256, 7), 1), (64, 20001, 64, (200, 16), 1), (32, 33001, 64, (256, 7), 1), (9, 20001, 64, (200, 16), 1), (64, 300, 64, (256, 100), 1),
     (300, 1001, 64, (256, 30), 1), (128, 16001, 64, (200, 16), 1),
-    (5, 70, 4160, (16, 9), 1), (17, 100, 8256, (24,), 1)])
+    (5, 70, 4160, (16, 9), 1), (17, 100, 8256, (24,), 1),
+    # the states' sums in one, two and four parts of the hidden size, a part in one round and in several
+    (9, 70, 1600, (16, 9), 1), (70, 90, 2112, (20, 5), 1), (70, 90, 16448, (33,), 1), (150, 40, 4224, (64, 7) * 20, 1)])
 def test_adapters_exact(sampler, rows, vocab, hidden, ranks, per, f8):
     exact_case(sampler, rows, vocab, hidden, f8, ranks, rows + vocab + len(ranks), per)
 
