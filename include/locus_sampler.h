@@ -247,7 +247,9 @@ typedef struct lcs_norm_out {
 
 /* A pool of low-rank adapters beside the lm-head's weight: adapter i adds
  * scale[i] (x a[i]^T) b[i]^T to the logits of the rows that name it. Only an
- * adapter's first rank[i] ranks count, whatever the others hold. */
+ * adapter's first rank[i] ranks count, whatever the others hold. Infinities and
+ * NaNs come out where the formula has them, in the rows of their adapter: a b of
+ * -inf times a state above zero takes that column out. */
 typedef struct lcs_adapters {
     uint32_t n;                /* 1..1024 */
     uint32_t wide;             /* ranks a slot of the pool holds: a multiple of 8, up to 256 */
