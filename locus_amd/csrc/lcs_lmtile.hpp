@@ -72,6 +72,12 @@ __device__ __forceinline__ void block_sync() {
     __builtin_amdgcn_sched_barrier(0);
 }
 
+// Whether the step of 16 ranks from k is the last one below `end` of an adapter
+// (who: its rank << 16 | its id; below 0 there is no step, and nothing ends).
+constexpr bool last_step(int32_t who, uint32_t k, uint32_t end) {
+    return who >= 0 && k + 16u >= ((uint32_t)who >> 16 < end ? (uint32_t)who >> 16 : end);
+}
+
 template <uint32_t P>
 struct Parts { static constexpr uint32_t value = P; };
 
@@ -506,7 +512,7 @@ __global__ __launch_bounds__(NW * kWave, 2) void lmhead_tile(LmArgs a) {
                 for (int q = 1; q <= 2; ++q)
 #pragma unroll
                     for (int i = 0; i < CT; ++i) mul(i, p[q], false);
-                if (st.k + 16u >= min(rank, kend)) {
+                if (last_step(st.who, st.k, kend)) {
 #pragma unroll
                     for (int j = 0; j < RT; ++j) {
                         if ((RT == 1 || st.j == (uint32_t)j) && sj[j] == st.who) {
