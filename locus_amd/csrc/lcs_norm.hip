@@ -275,8 +275,19 @@ void go(const NormArgs& a0, hipStream_t st) {
     NormArgs a = a0;
     a.waves = (a.hidden + 512u * NV - 1u) / (512u * NV);
     a.per = a.waves < 4u ? 4u / a.waves : 1u;
-    hipLaunchKernelGGL((add_rmsnorm<XT, YT, RES, NV>), dim3((uint32_t)((a.rows + a.per - 1u) / a.per)), dim3(a.waves * a.per * kWave), 0,
-                       st, a);
+    // (a launch's threads are counted in 32 bits, and past them go missing without an
+    // error: 2^31 at a time, 2 M rows of 8192 columns)
+    const uint32_t threads = a.waves * a.per * kWave;
+    const uint64_t most = (uint64_t)((1u << 31) / threads) * a.per;
+    for (uint64_t r0 = 0; r0 < a0.rows; r0 += most) {
+        a.rows = a0.rows - r0 < most ? a0.rows - r0 : most;
+        a.x = static_cast<const XT*>(a0.x) + r0 * a.x_stride;
+        if (RES) a.residual = static_cast<const XT*>(a0.residual) + r0 * a.residual_stride;
+        if (a0.sum) a.sum = static_cast<XT*>(a0.sum) + r0 * a.sum_stride;
+        a.y = static_cast<YT*>(a0.y) + r0 * a.y_stride;
+        if (a0.y_scale) a.y_scale = a0.y_scale + r0;
+        hipLaunchKernelGGL((add_rmsnorm<XT, YT, RES, NV>), dim3((uint32_t)((a.rows + a.per - 1u) / a.per)), dim3(threads), 0, st, a);
+    }
 }
 template <typename XT, typename YT, bool RES>
 void pick(const NormArgs& a, hipStream_t st) {

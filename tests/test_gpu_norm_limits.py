@@ -1,0 +1,47 @@
+"""lcs_add_rmsnorm at the ends of its range. Tolerances as in test_gpu_norm.py: 64 2^-24 of |y| for the f32 arithmetic,
+half a step for the rounding to y's type."""
+import pytest
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+
+
+@pytest.fixture(scope="module")
+def sampler():
+    from locus_amd.sampler import Sampler
+    s = Sampler(device=0, max_rows=16, max_vocab=4096, max_hist=64, max_top=4)
+    yield s
+    s.close()
+
+
+@pytest.mark.parametrize("out", ["bf16", "e4m3"])
+def test_more_rows_than_one_launch_has_threads(sampler, out):
+    """2^26 + 5 rows of a wave each: past 2^32 threads."""
+    torch = sampler.torch
+    rows, hidden = (1 << 26) + 5, 2
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.randn(rows, hidden, generator=gen, device="cuda").to(torch.bfloat16)
+    r = torch.randn(rows, hidden, generator=gen, device="cuda").to(torch.bfloat16)
+    w = torch.tensor([1.0, -0.5], device="cuda").to(torch.bfloat16)
+    o = {"y": torch.full((rows, hidden), 3.0, device="cuda").to(torch.bfloat16 if out == "bf16" else torch.float8_e4m3fn),
+         "sum": torch.full_like(x, 3.0)}
+    if out == "e4m3":
+        o["y_scale"] = torch.full((rows,), -7.0, device="cuda")
+    sampler.add_rmsnorm_dev(x, w, o, residual=r)
+    torch.cuda.synchronize()
+    for a in range(0, rows, 1 << 23):
+        s = slice(a, min(rows, a + (1 << 23)))
+        h = x[s].float() + r[s].float()
+        assert torch.equal(o["sum"][s], h.to(torch.bfloat16))
+        h = h.double()
+        ref = h / (h.square().mean(1, keepdim=True) + 1e-6).sqrt() * w.double()
+        got, tol = o["y"][s].to(torch.float64), 64 * U * ref.abs()
+        if out == "bf16":
+            tol = tol + ref.abs() * 2.0 ** -8
+        else:
+            top = ref.abs().amax(1)
+            step = torch.where(top > 0, top / 448.0, torch.ones_like(top))
+            assert ((o["y_scale"][s].double() - step).abs() <= 70 * U * step).all()
+            got = got * o["y_scale"][s].double()[:, None]
+            tol = tol + torch.maximum(ref.abs() * 2.0 ** -4, step[:, None] * 2.0 ** -10) * (1 + 70 * U)
+        assert ((got - ref).abs() <= tol).all(), a
