@@ -9,8 +9,8 @@
 // Memory bounds it: a row is read once, held in registers, and written once.
 // The sum of squares and the largest |h w| come from the same pass, so one
 // exchange between the row's waves gives both. In 8 bits the norm's factor r
-// cancels (y / scale = h w r / (max|h w| r / 448)), so an element costs one
-// product after it. Squares, sums and h are f32 (h unrounded: the norm reads it
+// cancels (y / scale = h w r / (max|h w| r / 448)), so an element costs two
+// products after it. Squares, sums and h are f32 (h unrounded: the norm reads it
 // from the registers and not from the rounded sum); y is rounded once.
 //
 // Rows, strides and widths are any: the vector loads and stores ask for the
@@ -193,8 +193,7 @@ __global__ __launch_bounds__(1024) void add_rmsnorm(NormArgs a) {
             ss = __builtin_fmaf(v[i][e], v[i][e], ss);
             if (Q8) {
                 // (as integers the bits of non-negative floats order as the floats do, NaNs above all)
-                v[i][e] = v[i][e] * g[i][e];
-                const uint32_t b = __float_as_uint(v[i][e]) & 0x7fffffffu;
+                const uint32_t b = __float_as_uint(v[i][e] * g[i][e]) & 0x7fffffffu;
                 top = b > top ? b : top;
             }
         }
@@ -219,22 +218,22 @@ __global__ __launch_bounds__(1024) void add_rmsnorm(NormArgs a) {
             Io<YT>::store(y + c[i], n[i], v[i]);
         }
     } else {
-        // The factor out of [1e-30, 1e30], or a row with an inf, a NaN or a sum of squares
-        // past f32: the formula itself, element by element. A row whose largest
-        // |y| is 0 or a NaN has scale 1.
+        // The largest |h w| out of (1e-30, 1e30), which products may have left f32 to reach, a
+        // row with an inf or a NaN, or a sum of squares past f32: the formula itself, element by
+        // element. A row whose largest |y| is 0 or a NaN has scale 1.
         const float m = __uint_as_float(top);
-        const bool plain = top == 0u || (m > 1e-30f && m < 1e30f && ss < 3e38f);
+        const bool plain = m > 1e-30f && m < 1e30f && ss < 3e38f;
         float scale, inv;
         if (plain) {
-            scale = top == 0u ? 1.0f : m * r / kE4m3Max;
-            inv = top == 0u ? 0.0f : kE4m3Max / m;
+            scale = m * r / kE4m3Max;
+            inv = kE4m3Max / m;
         } else {
             uint32_t t2 = 0u;
 #pragma unroll
             for (int i = 0; i < NV; ++i)
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    v[i][e] = v[i][e] * r;
+                    v[i][e] = v[i][e] * r * g[i][e];
                     const uint32_t b = (uint32_t)e < n[i] ? __float_as_uint(v[i][e]) & 0x7fffffffu : 0u;
                     t2 = b > t2 ? b : t2;
                 }
@@ -262,7 +261,7 @@ __global__ __launch_bounds__(1024) void add_rmsnorm(NormArgs a) {
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[i][e] = clamp448(plain ? v[i][e] * inv : v[i][e] / scale);
+            for (int e = 0; e < 8; ++e) v[i][e] = clamp448(plain ? v[i][e] * g[i][e] * inv : v[i][e] / scale);
             Io<YT>::store(y + c[i], n[i], v[i]);
         }
     }

@@ -45,3 +45,34 @@ def test_more_rows_than_one_launch_has_threads(sampler, out):
             got = got * o["y_scale"][s].double()[:, None]
             tol = tol + torch.maximum(ref.abs() * 2.0 ** -4, step[:, None] * 2.0 ** -10) * (1 + 70 * U)
         assert ((got - ref).abs() <= tol).all(), a
+
+
+def against_float64(torch, sampler, x, w, eps, out):
+    rows, hidden = x.shape
+    o = {"y": torch.empty(rows, hidden, device="cuda", dtype=out), "y_scale": torch.empty(rows, device="cuda")}
+    sampler.add_rmsnorm_dev(x, w, o, eps=eps)
+    torch.cuda.synchronize()
+    h = x.double()
+    ref = h / (h.square().mean(1, keepdim=True) + eps).sqrt() * w.double()
+    got, tol = o["y"].to(torch.float64), 64 * U * ref.abs()
+    if out == torch.float8_e4m3fn:
+        s = ref.abs().amax(1) / 448.0
+        assert ((o["y_scale"].double() - s).abs() <= 70 * U * s).all(), (o["y_scale"], s)
+        got = got * o["y_scale"].double()[:, None]
+        tol = tol + torch.maximum(ref.abs() * 2.0 ** -4, s[:, None] * 2.0 ** -10) * (1 + 70 * U)
+    elif out == torch.bfloat16:
+        tol = tol + ref.abs() * 2.0 ** -8
+    assert ((got - ref).abs() <= tol).all(), (got[0, :4], ref[0, :4])
+
+
+@pytest.mark.parametrize("out", ["f32", "bf16", "e4m3"])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("hidden", [40, 2049, 9000])
+def test_products_with_the_weight_that_leave_f32(sampler, hidden, dtype, out):
+    """h w past 3e38 or below 1e-38, while y is well inside: y = (h / sqrt(...)) w."""
+    torch = sampler.torch
+    types = {"f32": torch.float32, "bf16": torch.bfloat16, "e4m3": torch.float8_e4m3fn}
+    gen = torch.Generator(device="cuda").manual_seed(hidden)
+    v, g = (torch.randn(*n, generator=gen, device="cuda") for n in ((4, hidden), (hidden,)))
+    for size, weight, eps in ((1e16, 1e25, 1e-6), (1e-25, 1e-20, 1e-36), (1e-12, 1e-30, 1e-20)):
+        against_float64(torch, sampler, (v * size).to(types[dtype]), (g * weight).to(types[dtype]), eps, types[out])
