@@ -219,10 +219,11 @@ typedef struct lcs_lmhead_out {
  *   h = x + residual, y = h / sqrt(mean(h^2) + eps) * weight
  * per row, sums in f32, y and sum rounded once from f32 values (y from the
  * unrounded h). In e4m3, y holds y / y_scale with y_scale = max|y| / 448 of the
- * row (1 for a row of zeros): the operand of lcs_lmhead_ex. A row that holds a
- * NaN or an infinity has a NaN wherever the formula has one; in e4m3 its
- * y_scale is 1 if its largest |y| is a NaN. Squares and their sum are f32: past
- * 3e38 a row's y is 0. Rows and strides need the alignment of their elements only. */
+ * row (1 for a row of zeros, else 2^-126 at least): the operand of lcs_lmhead_ex.
+ * A row that holds a NaN or an infinity has a NaN wherever the formula has one; in
+ * e4m3 its y_scale is 1 if its largest |y| is a NaN. Squares and their sum are f32:
+ * past 3e38 a row's y is 0. Rows and strides need the alignment of their elements
+ * only. */
 typedef struct lcs_norm_batch {
     uint32_t rows;
     uint32_t hidden;           /* 1..32768 */

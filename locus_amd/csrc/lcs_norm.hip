@@ -36,6 +36,7 @@ typedef u32x4 u32x4_4 __attribute__((aligned(4), may_alias));
 typedef u32x2 u32x2_1 __attribute__((aligned(1), may_alias));
 
 constexpr float kE4m3Max = 448.0f;
+constexpr float kLeastScale = 1.17549435e-38f;   // 2^-126: a scale below the normal numbers would lose its bits
 
 __device__ __forceinline__ float bf16_to_f(uint32_t u) { return __uint_as_float(u << 16); }
 typedef float f32x2 __attribute__((ext_vector_type(2)));
@@ -219,10 +220,10 @@ __global__ __launch_bounds__(1024) void add_rmsnorm(NormArgs a) {
         }
     } else {
         // The largest |h w| out of (1e-30, 1e30), which products may have left f32 to reach, a
-        // row with an inf or a NaN, or a sum of squares past f32: the formula itself, element by
-        // element. A row whose largest |y| is 0 or a NaN has scale 1.
+        // row with an inf or a NaN, a sum of squares past f32, or a scale below the normal numbers:
+        // the formula itself, element by element. A row whose largest |y| is 0 or a NaN has scale 1.
         const float m = __uint_as_float(top);
-        const bool plain = m > 1e-30f && m < 1e30f && ss < 3e38f;
+        const bool plain = m > 1e-30f && m < 1e30f && ss < 3e38f && m * r >= kE4m3Max * kLeastScale;
         float scale, inv;
         if (plain) {
             scale = m * r / kE4m3Max;
@@ -250,10 +251,9 @@ __global__ __launch_bounds__(1024) void add_rmsnorm(NormArgs a) {
                 top = wave_max_u(part2[(uint32_t)lane_id() < WPR ? first + (uint32_t)lane_id() : first]);
             }
             const bool nan = top > 0x7f800000u;
-            // (a scale below the smallest normal number would lose its bits)
             if (!nan && top != 0u) {
                 scale = __uint_as_float(top) / kE4m3Max;
-                scale = scale < 1.17549435e-38f ? 1.17549435e-38f : scale;
+                scale = scale < kLeastScale ? kLeastScale : scale;
             }
         }
         if (!live) return;

@@ -76,3 +76,27 @@ def test_products_with_the_weight_that_leave_f32(sampler, hidden, dtype, out):
     v, g = (torch.randn(*n, generator=gen, device="cuda") for n in ((4, hidden), (hidden,)))
     for size, weight, eps in ((1e16, 1e25, 1e-6), (1e-25, 1e-20, 1e-36), (1e-12, 1e-30, 1e-20)):
         against_float64(torch, sampler, (v * size).to(types[dtype]), (g * weight).to(types[dtype]), eps, types[out])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("hidden", [40, 2049, 9000])
+def test_scales_stay_normal_numbers(sampler, hidden, dtype):
+    """Rows whose largest |y| / 448 is below 2^-126, by the weight and by eps, beside one
+    that is above: y_scale is 2^-126, and y within half a step of it."""
+    torch = sampler.torch
+    t = {"f32": torch.float32, "bf16": torch.bfloat16}[dtype]
+    least = 2.0 ** -126
+    gen = torch.Generator(device="cuda").manual_seed(hidden)
+    v, g = (torch.randn(*n, generator=gen, device="cuda") for n in ((4, hidden), (hidden,)))
+    for size, weight, eps in ((1e12, 2e-38, 1e-6), (1e-5, 1e-10, 1e37), (1e-2, 1.0, 1e37)):
+        x, w = (v * size).to(t), (g * weight).to(t)
+        o = {"y": torch.empty(4, hidden, device="cuda", dtype=torch.float8_e4m3fn), "y_scale": torch.empty(4, device="cuda")}
+        sampler.add_rmsnorm_dev(x, w, o, eps=eps)
+        torch.cuda.synchronize()
+        h = x.double()
+        ref = h / (h.square().mean(1, keepdim=True) + eps).sqrt() * w.double()
+        s = (ref.abs().amax(1) / 448.0).clamp(min=least)
+        assert ((o["y_scale"].double() - s).abs() <= 70 * U * s).all() and (o["y_scale"].double() >= least).all(), (o["y_scale"], s)
+        got = o["y"].to(torch.float64) * o["y_scale"].double()[:, None]
+        tol = 64 * U * ref.abs() + torch.maximum(ref.abs() * 2.0 ** -4, s[:, None] * 2.0 ** -10) * (1 + 70 * U)
+        assert ((got - ref).abs() <= tol).all()
