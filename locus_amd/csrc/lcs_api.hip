@@ -46,7 +46,7 @@ struct lcs_ctx {
     // lcs_lmhead_ex with adapters: the rows' order and their low-rank states, max_rows each
     uint32_t* ad_perm = nullptr;
     int32_t* ad_slot = nullptr;
-    float* ad_low = nullptr;        // x kAdParts kAdWideMax
+    float* ad_low = nullptr;        // ad_low_floats(max_rows) in all
     uint32_t cus = 256;             // compute units of the device (the lm-head's tile shape)
     // nucleus path workspace (kNucRows rows at a time)
     lcs::NucRow* nrow = nullptr;
@@ -169,7 +169,7 @@ lcs_ctx* lcs_create(int device, uint32_t max_rows, uint32_t max_vocab, uint32_t 
         (e = hipMalloc(&c->nlist, nuc_rows * lcs::kNucList * 8)) != hipSuccess ||
         (e = hipMalloc(&c->ad_perm, (size_t)max_rows * 4)) != hipSuccess ||
         (e = hipMalloc(&c->ad_slot, (size_t)max_rows * 4)) != hipSuccess ||
-        (e = hipMalloc(&c->ad_low, (size_t)max_rows * lcs::kAdParts * lcs::kAdWideMax * 4)) != hipSuccess ||
+        (e = hipMalloc(&c->ad_low, (size_t)lcs::ad_low_floats(max_rows) * 4)) != hipSuccess ||
         (e = hipMalloc(&c->lp_params, (size_t)max_rows * sizeof(lcs_params))) != hipSuccess ||
         (e = hipMalloc(&c->lp_ids, (size_t)max_rows * 4)) != hipSuccess ||
         (e = hipMemset(c->lp_params, 0, (size_t)max_rows * sizeof(lcs_params))) != hipSuccess ||
@@ -744,6 +744,7 @@ int lcs_lmhead_ex(lcs_ctx* c, const lcs_lmhead_ex_batch* b, const lcs_lmhead_out
         a.perm = c->ad_perm;
         a.pslot = c->ad_slot;
         a.low = c->ad_low;
+        a.low_floats = lcs::ad_low_floats(c->max_rows);
     }
     DeviceGuard g(c->device);
     const hipError_t e = lcs::launch_lmhead_ex(a, b->dtype == LCS_E4M3, c->cus, static_cast<hipStream_t>(stream));

@@ -276,10 +276,18 @@ struct LmArgs {
     uint32_t* perm;                 // rows: the row at a position
     int32_t* pslot;                 // rows: its adapter's rank << 16 | its adapter, or -1 (also for a rank of 0)
     float* low;                     // rows x (1 << low_s) x ad_wide: its low-rank state, summands by part of k
+    uint64_t low_floats;            // what low holds
 };
 constexpr uint32_t kAdMax = 1024;       // adapters of a pool
 constexpr uint32_t kAdWideMax = 256;    // their widest rank
 constexpr uint32_t kAdParts = 4;
+// The states' scratch of a context, in floats: one part of the widest ranks for every
+// row, all the parts for up to 256 (more rows fill the CUs with fewer, and have them
+// where their ranks leave the room): 1 KB a row of every context, used or not.
+constexpr uint64_t ad_low_floats(uint32_t max_rows) {
+    const uint64_t all = (uint64_t)max_rows * kAdWideMax, some = (uint64_t)(max_rows < 256u ? max_rows : 256u) * kAdParts * kAdWideMax;
+    return all > some ? all : some;
+}
 
 // residual addition and norm (lcs_norm.hip)
 constexpr uint32_t kNormHiddenMax = 32768;

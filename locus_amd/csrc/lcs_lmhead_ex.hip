@@ -192,6 +192,22 @@ void tile(const LmArgs& a, hipStream_t st) {
                        dim3(NW * kWave), 0, st, a);
 }
 
+// lm_low's workgroups: adapters or rows, 16 ranks each, z groups of rows side by side by
+// 1 << s parts of k. Parts of k, then the rows' groups, side by side as long as all the
+// workgroups can run at once and the states' scratch holds the parts. A part costs
+// every tile another read of its rows' states: 425 x 32000 x 2688 with two parts 107, four
+// 112; with up to 64 rows they pay from 1024 k up (37 x 50257 x 1600 with one 57.3, two 55.3).
+struct LowGrid { uint32_t x, y, z, s; };
+LowGrid low_grid(uint32_t rows, uint32_t n, uint32_t wide, uint32_t hidden, uint64_t floats, uint32_t cus) {
+    LowGrid g{n < rows ? n : rows, (wide + 15u) / 16u, 1u, 0u};
+    const uint32_t groups = (rows + kLowRows - 1u) / kLowRows;
+    const uint32_t most = 2u * cus / (g.x * g.y), least = kLowWaves * (rows <= 64u ? 64u : 128u);
+    while ((2u << g.s) <= kAdParts && (4u << g.s) <= most && least << g.s < hidden && ((uint64_t)rows * wide << g.s) * 2u <= floats) ++g.s;
+    const uint32_t nz = most >> g.s;
+    g.z = nz == 0u ? 1u : nz < groups ? nz : groups;
+    return g;
+}
+
 // The tiles: up to 64 rows lmhead_shape's columns, above by the same measure (rounds of
 // workgroups over the CUs times what one takes). Rings of 64-k stages (128 k of
 // e4m3), three where they fit, and eight waves on the tiles from 256 columns up.
@@ -263,19 +279,12 @@ hipError_t launch_lmhead_ex(const LmArgs& a0, bool f8, uint32_t cus, hipStream_t
     a.nblocks = (a.vocab + 64u * vt - 1u) / (64u * vt);
     a.nchunks = (a.rows + br - 1u) / br;
     if (a.ad_n != 0u) {
-        // Parts of k, then the rows' groups, side by side as long as all the workgroups can
-        // run at once. A part costs every tile another read of its rows' states: 425 x 32000
-        // x 2688 with two parts 107, four 112; with up to 64 rows they pay from 1024 k up (37 x
-        // 50257 x 1600 with one 57.3, two 55.3).
-        const uint32_t nx = a.ad_n < a.rows ? a.ad_n : a.rows, ny = (a.ad_wide + 15u) / 16u, groups = (a.rows + kLowRows - 1u) / kLowRows;
-        const uint32_t most = 2u * cus / (nx * ny), least = kLowWaves * (a.rows <= 64u ? 64u : 128u);
-        a.low_s = 0u;
-        while ((2u << a.low_s) <= kAdParts && (4u << a.low_s) <= most && least << a.low_s < a.hidden) ++a.low_s;
-        const uint32_t nz = most >> a.low_s;
-        a.low_z = nz == 0u ? 1u : nz < groups ? nz : groups;
+        const LowGrid g = low_grid(a.rows, a.ad_n, a.ad_wide, a.hidden, a.low_floats, cus);
+        a.low_s = g.s;
+        a.low_z = g.z;
         const bool few = a.hidden <= (uint32_t)(kLowWaves * 128) << a.low_s;
         auto low = f8 ? (few ? lm_low<true, 4> : lm_low<true, 8>) : (few ? lm_low<false, 4> : lm_low<false, 8>);
-        hipLaunchKernelGGL(low, dim3(nx, ny, a.low_z << a.low_s), dim3(kLowThreads), 0, st, a);
+        hipLaunchKernelGGL(low, dim3(g.x, g.y, a.low_z << a.low_s), dim3(kLowThreads), 0, st, a);
         if (f8) tiles<true, true>(a, vt, br, st);
         else tiles<false, true>(a, vt, br, st);
     } else {

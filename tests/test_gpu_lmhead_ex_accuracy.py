@@ -150,6 +150,25 @@ def test_states_of_20_bits(sampler, rows, vocab, f8):
     assert torch.equal(out["logits"].double(), ref)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("max_rows,rows,wide,hidden", [(1, 1, 256, 8256), (5, 5, 256, 4224), (300, 300, 256, 8256), (520, 520, 200, 4224)])
+def test_contexts_of_the_calls_own_rows(max_rows, rows, wide, hidden):
+    """The states in as many parts of the hidden size as the context's scratch holds, up to its end."""
+    from locus_amd.sampler import Adapters, Sampler
+    s = Sampler(device=0, max_rows=max_rows, max_vocab=300, max_hist=1, max_top=1)
+    torch = s.torch
+    gen = torch.Generator(device="cuda").manual_seed(rows)
+    x, w = ints(torch, gen, -4, 4, rows, hidden), ints(torch, gen, -3, 3, 300, hidden)
+    a, b = ints(torch, gen, -1, 1, 1, wide, hidden), ints(torch, gen, -2, 2, 1, 300, wide)
+    out = s.alloc_lmhead_out(rows, 300)
+    slot = torch.zeros(rows, device="cuda", dtype=torch.int32)
+    for _ in range(2):
+        s.lmhead_ex_dev(x.to(torch.bfloat16), w.to(torch.bfloat16), out,
+                        adapters=Adapters(a.to(torch.bfloat16), b.to(torch.bfloat16)), slot=slot)
+        assert torch.equal(out["logits"].double(), x.double() @ w.double().t() + (x.double() @ a[0].double().t()) @ b[0].double().t())
+    s.close()
+
+
 # ---------------------------------------------- what the bounds have to see --
 def test_the_product_bound_sees_sums_of_14_bits():
     """8 neighbouring products cut 13 bits below the largest of them, the groups added in 64 bits."""
