@@ -216,13 +216,14 @@ LowGrid low_grid(uint32_t rows, uint32_t n, uint32_t wide, uint32_t hidden, uint
 //   256 x 64: 50257 x 1600 bf16 with adapters, ST 3 NW 8 41.0, NW 4 45.3, ST 2 50;
 //     151936 x 3584 e4m3 (594 blocks) 132, 144, 142; 128256 x 4096 e4m3 (501) 116, 126, 116
 //   320 x 64, ST 3 NW 4: 151936 x 3584 e4m3 116 (32-k stages 124), bf16 with adapters
-//     225 (235), e4m3 with 64 adapters 176 (186)
+//     225 (235), e4m3 with 64 adapters 176 (186; 180 to 183 since the factor's clamps)
 //   128 x 64, ST 3 NW 4: 32000 x 2048 e4m3 15.5 (NW 8 16.1)
 //   64 x 64: 16000 x 4096 e4m3 18.0 with ST 4, 19.2 with six 32-k stages, bf16 27.0, 26.6
 //   256 x 128: 128 x 128256 x 4096 e4m3 ST 3 NW 8 138, NW 4 153, 32-k stages
 //     163; bf16 with adapters 230, -, 266
-//   256 x 256, ST 2 NW 8: 1024 x 128256 x 4096 e4m3 683 (1576 TFLOP/s; power bounds it:
-//     751 where the operands' bits vary more)
+//   256 x 256, ST 2 NW 8: 1024 x 128256 x 4096 e4m3 751 (1433 TFLOP/s); power bounds it: the
+//     tile's 1.31 M cycles, of which the matrix cores are busy for 1.03 M, take 745 us on random
+//     operands (1.76 GHz); on zeros 1.32 M take 562 (2.36 GHz)
 struct LmExShape { uint32_t vt, br; };
 LmExShape lmhead_ex_shape(uint32_t rows, uint32_t vocab, uint32_t hidden, bool f8, uint32_t cus) {
     if (rows <= 64u) {
@@ -233,6 +234,8 @@ LmExShape lmhead_ex_shape(uint32_t rows, uint32_t vocab, uint32_t hidden, bool f
         if (rows <= 32u && (s.vt == 2u || s.vt == 4u)) s.br = 32u;
         return s;
     }
+    // (the weights are of 4096 k without adapters; what a tile takes beside its k, which tells at
+    // short hidden sizes, and idle CUs at long ones, are not in them)
     // us a round, 4096 k of e4m3 (bf16: / 1.36), from 128 to 1024 rows x 2000 to 128256; one: where
     // no CU gets a second tile. 384 x 128256 e4m3 291 in rows of 192, 308 in 128, 353 in
     // 256; bf16 with adapters 437, 411, 466; 176 x 42468 x 7552 bf16 205, 233, 213; 128 x 32000
