@@ -5,9 +5,19 @@
 
 #include <stdint.h>
 
+#include <cstring>
+
 #include "locus_sampler.h"
 
 namespace lcs {
+
+// Neither an infinity nor a NaN, by its bits: the library's build assumes that there
+// are no NaNs and would take a comparison for one away.
+inline bool finite_bits(float v) {
+    uint32_t u;
+    std::memcpy(&u, &v, 4);
+    return (u & 0x7f800000u) != 0x7f800000u;
+}
 
 inline bool misaligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1u)) != 0u; }
 
@@ -18,7 +28,7 @@ inline int check_add_rmsnorm(const lcs_norm_batch* b, const lcs_norm_out* o, uin
     if (b->x_dtype != LCS_F32 && b->x_dtype != LCS_BF16) return no("x_dtype must be f32 or bf16");
     if (b->y_dtype != LCS_F32 && b->y_dtype != LCS_BF16 && b->y_dtype != LCS_E4M3) return no("y_dtype must be f32, bf16 or e4m3");
     if (b->hidden == 0 || b->hidden > max_hidden) return no("hidden must be 1..32768");
-    if (!(b->eps > 0.0f && b->eps <= 3.0e38f)) return no("eps must be positive and finite");
+    if (!finite_bits(b->eps) || !(b->eps > 0.0f && b->eps <= 3.0e38f)) return no("eps must be positive and finite");
     if (!b->x || !b->weight || !o->y) return no("null x / weight / y");
     if (b->y_dtype == LCS_E4M3 && !o->y_scale) return no("y in e4m3 needs y_scale");
     if (o->sum && !b->residual) return no("sum given without residual");
