@@ -279,6 +279,119 @@ typedef struct lcs_lmhead_ex_batch {
                                   [0, n): none */
 } lcs_lmhead_ex_batch;
 
+/* A paged cache of keys and values for all layers. A sequence is a slot of `table`:
+ * token t of sequence s lies in page table[s * max_pages + t / page_tokens], row t %
+ * page_tokens. A page holds every layer's and head's rows of its tokens, and
+ * refs[page] counts the sequences that hold it (0: free); pages may be shared
+ * (lcs_kv_fork) and are then replaced by copies ahead of writes (lcs_kv_grow). The
+ * reference's counterpart: its ref-counted copy-on-write cache on the host
+ * (src/locus/kv/block_allocator.hpp:25-55, paged_cache.hpp:24-120). All buffers
+ * are the caller's; a new cache's table is all -1, its refs all 0. */
+typedef struct lcs_kv_cache {
+    uint32_t layers, pages;
+    uint32_t page_tokens;      /* a power of two, 16..1024 */
+    uint32_t kv_heads;
+    uint32_t head_dim;         /* a multiple of 16, up to 256 */
+    uint32_t dtype;            /* LCS_BF16, or LCS_E4M3 with a scale per row */
+    uint32_t seqs, max_pages;  /* slots of the table, pages a slot can hold */
+    void* k;                   /* element d of a row: base + layer * layer_stride + page * page_stride + */
+    void* v;                   /*   head * head_stride + row * token_stride + d, for both */
+    float* k_scale;            /* layers x pages x kv_heads x page_tokens (LCS_E4M3): a row holds */
+    float* v_scale;            /*   its values / its scale; else NULL */
+    uint64_t layer_stride;     /* elements. Bases and strides are multiples of 16 bytes, rows do */
+    uint64_t page_stride;      /*   not overlap (a size of 1 leaves its stride free), and a page's */
+    uint64_t head_stride;      /*   rows of one head span less than 2 GiB */
+    uint64_t token_stride;
+    int32_t* table;            /* seqs x max_pages, -1: none */
+    int32_t* refs;             /* pages */
+} lcs_kv_cache;
+
+/* Attention of a step's new tokens, R = rows_per_seq for each of n_seq sequences (one
+ * token, a chain, or a tree of drafts), over their cached context and over each
+ * other:
+ *   o[r] = sum_j p_j v_j,  p = softmax_j(scale q[r] . k_j),  lse[r] = log sum_j exp(scale q[r] . k_j)
+ * where j runs over the sequence's first length[i] cached tokens and over those of
+ * its new tokens that row r's mask names. The new tokens' keys and values come from
+ * k and v, not from the cache: what becomes of them is known after lcs_tree_verify
+ * only (lcs_kv_append puts the accepted ones there). Query head h reads kv head
+ * h / (heads / kv_heads). Scores, statistics and sums are f32; a weight is rounded
+ * to bf16 for the product with the values, o once at the end. A row that sees
+ * nothing has o = 0 and lse = -inf. What a row does not see is no part of its
+ * result, whatever it holds. */
+typedef struct lcs_tree_attn_batch {
+    uint32_t n_seq;            /* up to 1024 */
+    uint32_t rows_per_seq;     /* 1..256 */
+    uint32_t heads;            /* a multiple of the cache's kv_heads */
+    uint32_t layer;
+    float scale;               /* finite */
+    uint32_t mask_words;       /* >= ceil(rows_per_seq / 32) when mask != NULL */
+    const lcs_kv_cache* cache; /* host struct */
+    const void* q;             /* row r = i * rows_per_seq + j, head h: q + r * q_stride + h * head_dim; bf16 */
+    const void* k;             /* likewise, kv_heads a row */
+    const void* v;
+    uint64_t q_stride;         /* elements; bases and strides are multiples of 16 bytes */
+    uint64_t k_stride;
+    uint64_t v_stride;
+    const int32_t* seq;        /* n_seq: the sequence's slot of the cache, -1: no context; NULL: i */
+    const int32_t* length;     /* n_seq: cached tokens (below 0: none) */
+    const uint32_t* mask;      /* rows x mask_words, bit j & 31 of word j >> 5: the row sees its sequence's new
+                                  token j; NULL: new tokens 0 .. its own */
+} lcs_tree_attn_batch;
+
+typedef struct lcs_tree_attn_out {
+    void* o;                   /* as q, bf16 */
+    uint64_t o_stride;         /* elements, a multiple of 16 bytes */
+    float* lse;                /* rows x heads, or NULL */
+} lcs_tree_attn_out;
+
+/* The greedy verdict on a tree of drafts: lcs_verify for trees. Node j of sequence i
+ * is row i * rows_per_seq + j. Node 0 is the root, the last token that is certain;
+ * node j > 0 drafts tokens[j] as a continuation of node parent[j] < j (a node with
+ * another parent is never accepted). Row j of the logits predicts what follows node
+ * j: from the root on, the lowest child whose token is its parent's argmax is
+ * accepted (engine.cpp:357-396 along a chain). */
+typedef struct lcs_tree_verify_batch {
+    uint32_t n_seq;
+    uint32_t rows_per_seq;     /* 1..256 */
+    uint32_t vocab;
+    uint32_t dtype;            /* LCS_F32 or LCS_BF16 */
+    uint64_t row_stride;       /* elements; multiple of 4 (f32) / 8 (bf16) */
+    const void* logits;        /* rows x row_stride, 16-byte aligned; NULL: out->argmax_ids holds the rows'
+                                  argmax (lcs_lmhead), vocab, dtype and row_stride are not read */
+    const int32_t* tokens;     /* rows */
+    const int32_t* parent;     /* rows (the root's is not read) */
+    const int32_t* length;     /* n_seq: cached tokens, for out->length; or NULL */
+} lcs_tree_verify_batch;
+
+typedef struct lcs_tree_verify_out {
+    int32_t* argmax_ids;       /* rows: argmax (llama.cpp:1237-1245); read where logits is NULL */
+    float* node_lp;            /* rows: log-probability of the node's token under its parent's row (0 for the
+                                  root, other parents and ids outside [0, vocab)), or NULL; needs logits */
+    int32_t* path;             /* rows: each sequence's accepted nodes, the root first, then -1 */
+    int32_t* n_path;           /* n_seq: their number, 1 .. rows_per_seq */
+    int32_t* next_id;          /* n_seq: the argmax at the path's end */
+    int32_t* length;           /* n_seq: length + n_path, or NULL; needs length; it may be the same buffer */
+} lcs_tree_verify_out;
+
+/* New rows of a cache: token j < count[i] of sequence i goes to position pos[i] + j,
+ * from row i * rows_per_seq + (index ? index[i * rows_per_seq + j] : j) of each of
+ * n_layers layers. Into e4m3 as lcs_add_rmsnorm's y: a scale of max|x| / 448 per row
+ * (1 for a row of zeros, or whose largest |x| is a NaN; 2^-126 at least), x / scale
+ * rounded to nearest even. */
+typedef struct lcs_kv_append_batch {
+    uint32_t n_seq;
+    uint32_t rows_per_seq;
+    uint32_t layer, n_layers;  /* the first one, and how many */
+    const void* k;             /* layer l (from 0), row r, head h: k + l * layer_stride + r * k_stride + h * head_dim; bf16 */
+    const void* v;
+    uint64_t layer_stride;     /* elements, of both; bases and strides are multiples of 16 bytes */
+    uint64_t k_stride, v_stride;
+    const int32_t* seq;        /* n_seq: slots, -1: nothing to do; NULL: i */
+    const int32_t* pos;        /* n_seq */
+    const int32_t* count;      /* n_seq (clamped to 0..rows_per_seq), or NULL: rows_per_seq */
+    const int32_t* index;      /* n_seq x rows_per_seq, or NULL */
+} lcs_kv_append_batch;
+
 /* Number of usable gfx950 devices (0 when none). Replaces the runtime probe
  * that sets Backend::available (registry.cpp:148-223, cuda_stub.cpp:29). */
 int lcs_probe(int* n_devices);
@@ -358,9 +471,62 @@ int lcs_lmhead_ex(lcs_ctx* ctx, const lcs_lmhead_ex_batch* batch, const lcs_lmhe
  * nothing and uses no context workspace: rows are not bounded by max_rows. */
 int lcs_add_rmsnorm(lcs_ctx* ctx, const lcs_norm_batch* batch, const lcs_norm_out* out, void* stream);
 
+/* The workspace of the calls below: room for `new_pages` pages that one lcs_kv_grow
+ * call may allocate, and for the partial results of lcs_tree_attn (about 17 MB).
+ * Allocates once, ahead of the hot loop (a call with a larger limit reallocates). */
+int lcs_kv_reserve(lcs_ctx* ctx, uint32_t new_pages);
+
+/* The bookkeeping of a paged cache, on the device, for n <= 1024 requests per call. Slots
+ * are in device memory, so bad ones are refused there: result[i] is 0, or -1 for a
+ * request that changed nothing, with LCS_STATUS_PAGES set. A slot of -1 asks for
+ * nothing (result 0). A slot outside [0, seqs) is refused, and one that an earlier
+ * request of the call has named. No counterpart call in the reference, which does this on
+ * the host (paged_cache.hpp:24-120).
+ *
+ * lcs_kv_grow: slot seq[i] gets a page of its own wherever one is missing or shared at
+ * its tokens [start[i], end[i]): a missing one a free page, a shared one a copy (all
+ * layers) that takes its place, also if all its holders ask in this call. Free pages
+ * go to the requests in order, the lowest first; from the first request that there
+ * are not enough for, none is served. start > end and ends past the table are
+ * refused.
+ * lcs_kv_fork: slot dst[i], which holds no page, shares slot src[i]'s first tokens[i]
+ * tokens. Refused where a page of them is missing, dst holds any, or src is itself
+ * some request's dst.
+ * lcs_kv_free: slot seq[i] gives up its pages past its first keep[i] tokens (keep NULL
+ * or below 0: all). A page that nobody else holds is free again. */
+int lcs_kv_grow(lcs_ctx* ctx, const lcs_kv_cache* cache, uint32_t n, const int32_t* seq, const int32_t* start,
+                const int32_t* end, int32_t* result, void* stream);
+int lcs_kv_fork(lcs_ctx* ctx, const lcs_kv_cache* cache, uint32_t n, const int32_t* src, const int32_t* dst,
+                const int32_t* tokens, int32_t* result, void* stream);
+int lcs_kv_free(lcs_ctx* ctx, const lcs_kv_cache* cache, uint32_t n, const int32_t* seq, const int32_t* keep,
+                int32_t* result, void* stream);
+
+/* Keeps count[i] (clamped to 0..max_keep) of slot seq[i]'s tokens, in all layers: row
+ * keep[i * max_keep + j] moves to position j, in place. keep is ascending. Refused
+ * (result -1, nothing moved) where it is not, where a page is missing, or where a page
+ * that would be written is shared (lcs_kv_grow gives copies). What lies past the
+ * last one is left as it was; lcs_kv_free gives its pages back. Slots as above. */
+int lcs_kv_compact(lcs_ctx* ctx, const lcs_kv_cache* cache, uint32_t n, uint32_t max_keep, const int32_t* seq,
+                   const int32_t* count, const int32_t* keep, int32_t* result, void* stream);
+
+/* New rows of a cache (see lcs_kv_append_batch). A row whose page is missing or shared,
+ * or whose index or position is out of range, is not written and sets
+ * LCS_STATUS_PAGES. Rows that go to one place (a slot named twice) are a race.
+ * Allocates nothing and uses no context workspace. */
+int lcs_kv_append(lcs_ctx* ctx, const lcs_kv_cache* cache, const lcs_kv_append_batch* batch, void* stream);
+
+/* Attention over the cache and the new tokens (see lcs_tree_attn_batch). Allocates nothing.
+ * A page that is missing below length[i] counts as not seen and sets LCS_STATUS_PAGES, as
+ * does a slot outside [-1, seqs) or a length past the table. */
+int lcs_tree_attn(lcs_ctx* ctx, const lcs_tree_attn_batch* batch, const lcs_tree_attn_out* out, void* stream);
+
+/* Verdict on a tree of drafts (see lcs_tree_verify_batch). Allocates nothing and uses no
+ * context workspace. */
+int lcs_tree_verify(lcs_ctx* ctx, const lcs_tree_verify_batch* batch, const lcs_tree_verify_out* out, void* stream);
+
 /* Sticky device-side status bits of ctx (LCS_STATUS_*), set by kernels that
- * met an input they could not serve. Every bit comes with id -1 on each
- * affected row (also from lcs_sample_noalloc, whose status is not readable),
+ * met an input they could not serve. Every bit of the sampling calls comes with id
+ * -1 on each affected row (also from lcs_sample_noalloc, whose status is not readable),
  * so a caller that sees no -1 id needs no status read. Blocking:
  * reads device memory; call after the work's stream has been synchronised.
  * No counterpart in the reference (its sampler cannot fail). */
@@ -369,8 +535,9 @@ int lcs_get_status(lcs_ctx* ctx, uint32_t* status_out, int reset);
 enum lcs_status_bits {
     LCS_STATUS_HIST_CAPACITY = 1u,  /* a penalty window exceeded max_hist */
     LCS_STATUS_SELECT = 2u,         /* a selection bin exceeded its capacity */
-    LCS_STATUS_WINDOW = 4u          /* a row's window slot did not match it (win_len, window,
+    LCS_STATUS_WINDOW = 4u,         /* a row's window slot did not match it (win_len, window,
                                        vocabulary) */
+    LCS_STATUS_PAGES = 8u           /* a cache request was refused, or a page was missing */
 };
 
 /* Message of the last failure on ctx (or, when NULL, of the last lcs_create

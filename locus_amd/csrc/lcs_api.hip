@@ -15,6 +15,7 @@
 
 #include "lcs_check.hpp"
 #include "lcs_internal.hpp"
+#include "lcs_kv_check.hpp"
 #include "locus_sampler.h"
 
 namespace lcs {
@@ -30,6 +31,13 @@ hipError_t launch_lmhead(const LmArgs& a, uint32_t cus, hipStream_t st);
 uint32_t lmhead_max_blocks(uint32_t vocab, uint32_t cus);
 hipError_t launch_lmhead_ex(const LmArgs& a, bool f8, uint32_t cus, hipStream_t st);
 hipError_t launch_add_rmsnorm(const NormArgs& a, uint32_t x_dtype, uint32_t y_dtype, hipStream_t st);
+hipError_t launch_kv_free(const KvArgs& a, hipStream_t st);
+hipError_t launch_kv_fork(const KvArgs& a, hipStream_t st);
+hipError_t launch_kv_grow(const KvArgs& a, hipStream_t st);
+hipError_t launch_kv_compact(const KvArgs& a, hipStream_t st);
+hipError_t launch_kv_append(const KvAppendArgs& a, hipStream_t st);
+hipError_t launch_tree_attn(const TreeArgs& a, hipStream_t st);
+hipError_t launch_tree_verify(const TreeVerifyArgs& a, hipStream_t st);
 }  // namespace lcs
 
 struct lcs_ctx {
@@ -58,6 +66,10 @@ struct lcs_ctx {
     lcs::WinStage* wstage = nullptr;   // max_rows
     int32_t* wring = nullptr;
     uint64_t* wbkt = nullptr;
+    // paged cache (lcs_kv_reserve): the pages that one lcs_kv_grow call gives out, what
+    // each copies, and their number
+    uint32_t kv_cap = 0;
+    int32_t* kv_fresh = nullptr;   // kv_cap, then kv_cap for what they copy, then the number
     // lcs_logprobs: greedy parameters (all fields zero) for max_rows rows, on
     // the device and on the host, and its argmax ids when the caller wants none
     lcs_params* lp_params = nullptr;
@@ -205,6 +217,7 @@ void lcs_destroy(lcs_ctx* c) {
     (void)hipFree(c->wring);
     (void)hipFree(c->wbkt);
     (void)hipFree(c->wstage);
+    (void)hipFree(c->kv_fresh);
     delete c;
 }
 
@@ -774,6 +787,202 @@ int lcs_add_rmsnorm(lcs_ctx* c, const lcs_norm_batch* b, const lcs_norm_out* o, 
     DeviceGuard g(c->device);
     const hipError_t e = lcs::launch_add_rmsnorm(a, b->x_dtype, b->y_dtype, static_cast<hipStream_t>(stream));
     return e == hipSuccess ? LCS_OK : hip_fail(c, e, "norm kernel launch");
+}
+
+int lcs_kv_reserve(lcs_ctx* c, uint32_t new_pages) {
+    if (!c) return LCS_ERR_INVALID_ARG;
+    if (new_pages == 0 || new_pages > 0x3fffffffu) return fail(c, LCS_ERR_INVALID_ARG, "lcs_kv_reserve: new_pages must be 1..2^30 - 1");
+    if (c->kv_fresh && new_pages <= c->kv_cap) return LCS_OK;
+    DeviceGuard g(c->device);
+    (void)hipDeviceSynchronize();
+    (void)hipFree(c->kv_fresh);
+    c->kv_fresh = nullptr;
+    c->kv_cap = 0;
+    const hipError_t e = hipMalloc(&c->kv_fresh, ((size_t)new_pages * 2 + 1) * 4);
+    if (e != hipSuccess) {
+        c->kv_fresh = nullptr;
+        return hip_fail(c, e, "lcs_kv_reserve");
+    }
+    c->kv_cap = new_pages;
+    return LCS_OK;
+}
+
+static lcs::KvArgs kv_args(const lcs_ctx* c, const lcs_kv_cache* k, uint32_t n, const int32_t* seq, int32_t* result) {
+    lcs::KvArgs a{};
+    a.layers = k->layers;
+    a.pages = k->pages;
+    a.page_tokens = k->page_tokens;
+    a.page_shift = (uint32_t)__builtin_ctz(k->page_tokens);
+    a.kv_heads = k->kv_heads;
+    a.head_dim = k->head_dim;
+    a.seqs = k->seqs;
+    a.max_pages = k->max_pages;
+    a.f8 = k->dtype == LCS_E4M3 ? 1u : 0u;
+    a.n = n;
+    a.k = k->k;
+    a.v = k->v;
+    a.k_scale = k->k_scale;
+    a.v_scale = k->v_scale;
+    // (the stride of a size of 1 is anything: none is added up)
+    a.layer_stride = k->layers > 1 ? k->layer_stride : 0u;
+    a.page_stride = k->pages > 1 ? k->page_stride : 0u;
+    a.head_stride = k->kv_heads > 1 ? k->head_stride : 0u;
+    a.token_stride = k->token_stride;
+    a.table = k->table;
+    a.refs = k->refs;
+    a.seq = seq;
+    a.result = result;
+    a.status = c->status;
+    a.cap = c->kv_cap;
+    if (c->kv_fresh) {
+        a.fresh = c->kv_fresh;
+        a.from = c->kv_fresh + c->kv_cap;
+        a.n_fresh = reinterpret_cast<uint32_t*>(c->kv_fresh + 2 * (size_t)c->kv_cap);
+    }
+    return a;
+}
+
+int lcs_kv_grow(lcs_ctx* c, const lcs_kv_cache* k, uint32_t n, const int32_t* seq, const int32_t* start, const int32_t* end,
+                int32_t* result, void* stream) {
+    if (!c) return LCS_ERR_INVALID_ARG;
+    const char* why = "";
+    const int rc = lcs::check_kv_requests(k, n, seq, start, end, result, lcs::kKvMaxReq, &why);
+    if (rc != LCS_OK) return fail(c, rc, why);
+    if (!c->kv_fresh) return fail(c, LCS_ERR_INVALID_ARG, "lcs_kv_grow without lcs_kv_reserve");
+    if (n == 0) return LCS_OK;
+    lcs::KvArgs a = kv_args(c, k, n, seq, result);
+    a.start = start;
+    a.end = end;
+    DeviceGuard g(c->device);
+    const hipError_t e = lcs::launch_kv_grow(a, static_cast<hipStream_t>(stream));
+    return e == hipSuccess ? LCS_OK : hip_fail(c, e, "page kernels launch");
+}
+
+int lcs_kv_fork(lcs_ctx* c, const lcs_kv_cache* k, uint32_t n, const int32_t* src, const int32_t* dst, const int32_t* tokens,
+                int32_t* result, void* stream) {
+    if (!c) return LCS_ERR_INVALID_ARG;
+    const char* why = "";
+    const int rc = lcs::check_kv_requests(k, n, src, dst, tokens, result, lcs::kKvMaxReq, &why);
+    if (rc != LCS_OK) return fail(c, rc, why);
+    if (n == 0) return LCS_OK;
+    lcs::KvArgs a = kv_args(c, k, n, src, result);
+    a.dst = dst;
+    a.end = tokens;
+    DeviceGuard g(c->device);
+    const hipError_t e = lcs::launch_kv_fork(a, static_cast<hipStream_t>(stream));
+    return e == hipSuccess ? LCS_OK : hip_fail(c, e, "fork kernel launch");
+}
+
+int lcs_kv_free(lcs_ctx* c, const lcs_kv_cache* k, uint32_t n, const int32_t* seq, const int32_t* keep, int32_t* result,
+                void* stream) {
+    if (!c) return LCS_ERR_INVALID_ARG;
+    const char* why = "";
+    const int rc = lcs::check_kv_requests(k, n, seq, seq, keep ? keep : seq, result, lcs::kKvMaxReq, &why);
+    if (rc != LCS_OK) return fail(c, rc, why);
+    if (n == 0) return LCS_OK;
+    lcs::KvArgs a = kv_args(c, k, n, seq, result);
+    a.end = keep;
+    DeviceGuard g(c->device);
+    const hipError_t e = lcs::launch_kv_free(a, static_cast<hipStream_t>(stream));
+    return e == hipSuccess ? LCS_OK : hip_fail(c, e, "free kernel launch");
+}
+
+int lcs_kv_compact(lcs_ctx* c, const lcs_kv_cache* k, uint32_t n, uint32_t max_keep, const int32_t* seq, const int32_t* count,
+                   const int32_t* keep, int32_t* result, void* stream) {
+    if (!c) return LCS_ERR_INVALID_ARG;
+    const char* why = "";
+    const int rc = lcs::check_kv_compact(k, n, max_keep, seq, count, keep, result, lcs::kKvMaxReq, &why);
+    if (rc != LCS_OK) return fail(c, rc, why);
+    if (n == 0) return LCS_OK;
+    lcs::KvArgs a = kv_args(c, k, n, seq, result);
+    a.max_keep = max_keep;
+    a.count = count;
+    a.index = keep;
+    DeviceGuard g(c->device);
+    const hipError_t e = lcs::launch_kv_compact(a, static_cast<hipStream_t>(stream));
+    return e == hipSuccess ? LCS_OK : hip_fail(c, e, "compaction kernels launch");
+}
+
+int lcs_kv_append(lcs_ctx* c, const lcs_kv_cache* k, const lcs_kv_append_batch* b, void* stream) {
+    if (!c) return LCS_ERR_INVALID_ARG;
+    const char* why = "";
+    const int rc = lcs::check_kv_append(k, b, lcs::kKvMaxReq, &why);
+    if (rc != LCS_OK) return fail(c, rc, why);
+    if (b->n_seq == 0 || b->n_layers == 0) return LCS_OK;
+    lcs::KvAppendArgs p{};
+    p.a = kv_args(c, k, b->n_seq, b->seq, nullptr);
+    p.a.layer = b->layer;
+    p.a.start = b->pos;
+    p.a.count = b->count;
+    p.a.index = b->index;
+    p.k = b->k;
+    p.v = b->v;
+    p.new_layer_stride = b->n_layers > 1 ? b->layer_stride : 0u;
+    p.k_stride = b->k_stride;
+    p.v_stride = b->v_stride;
+    p.rows_per_seq = b->rows_per_seq;
+    p.n_layers = b->n_layers;
+    DeviceGuard g(c->device);
+    const hipError_t e = lcs::launch_kv_append(p, static_cast<hipStream_t>(stream));
+    return e == hipSuccess ? LCS_OK : hip_fail(c, e, "append kernel launch");
+}
+
+int lcs_tree_attn(lcs_ctx* c, const lcs_tree_attn_batch* b, const lcs_tree_attn_out* o, void* stream) {
+    if (!c) return LCS_ERR_INVALID_ARG;
+    const char* why = "";
+    const int rc = lcs::check_tree_attn(b, o, lcs::kKvMaxReq, &why);
+    if (rc != LCS_OK) return fail(c, rc, why);
+    if (!c->kv_fresh) return fail(c, LCS_ERR_INVALID_ARG, "lcs_tree_attn without lcs_kv_reserve");
+    if (b->n_seq == 0) return LCS_OK;
+    lcs::TreeArgs a{};
+    a.c = kv_args(c, b->cache, b->n_seq, b->seq, nullptr);
+    a.c.layer = b->layer;
+    a.rows_per_seq = b->rows_per_seq;
+    a.heads = b->heads;
+    a.group = b->heads / b->cache->kv_heads;
+    a.mask_words = b->mask_words;
+    a.scale = b->scale;
+    a.q = static_cast<const uint16_t*>(b->q);
+    a.k = static_cast<const uint16_t*>(b->k);
+    a.v = static_cast<const uint16_t*>(b->v);
+    a.q_stride = b->q_stride;
+    a.k_stride = b->k_stride;
+    a.v_stride = b->v_stride;
+    a.o_stride = o->o_stride;
+    a.length = b->length;
+    a.mask = b->mask;
+    a.o = static_cast<uint16_t*>(o->o);
+    a.lse = o->lse;
+    DeviceGuard g(c->device);
+    const hipError_t e = lcs::launch_tree_attn(a, static_cast<hipStream_t>(stream));
+    return e == hipSuccess ? LCS_OK : hip_fail(c, e, "attention kernel launch");
+}
+
+int lcs_tree_verify(lcs_ctx* c, const lcs_tree_verify_batch* b, const lcs_tree_verify_out* o, void* stream) {
+    if (!c) return LCS_ERR_INVALID_ARG;
+    const char* why = "";
+    const int rc = lcs::check_tree_verify(b, o, &why);
+    if (rc != LCS_OK) return fail(c, rc, why);
+    if (b->n_seq == 0) return LCS_OK;
+    lcs::TreeVerifyArgs a{};
+    a.logits = b->logits;
+    a.row_stride = b->row_stride;
+    a.n_seq = b->n_seq;
+    a.rows_per_seq = b->rows_per_seq;
+    a.vocab = b->vocab;
+    a.dtype = b->dtype;
+    a.tokens = b->tokens;
+    a.parent = b->parent;
+    a.length = b->length;
+    a.argmax_ids = o->argmax_ids;
+    a.node_lp = o->node_lp;
+    a.path = o->path;
+    a.n_path = o->n_path;
+    a.next_id = o->next_id;
+    a.new_length = o->length;
+    DeviceGuard g(c->device);
+    const hipError_t e = lcs::launch_tree_verify(a, static_cast<hipStream_t>(stream));
+    return e == hipSuccess ? LCS_OK : hip_fail(c, e, "verify kernel launch");
 }
 
 int lcs_get_status(lcs_ctx* c, uint32_t* status_out, int reset) {

@@ -305,9 +305,78 @@ struct NormArgs {
     uint32_t waves, per;            // waves a row, rows a workgroup (launch_add_rmsnorm)
 };
 
+// paged cache (lcs_kv.hip)
+constexpr uint32_t kKvMaxReq = 1024;    // requests a call
+struct KvArgs {
+    uint32_t layers, pages, page_tokens, page_shift, kv_heads, head_dim, seqs, max_pages;
+    uint32_t f8;                    // 1: e4m3 rows with scales
+    uint32_t n, layer;              // requests; the layer (append, attention)
+    uint32_t max_keep;
+    uint32_t chunks, cp;            // 16-byte chunks of a row, lanes a row (a power of two)
+    uint32_t cap;                   // what fresh and from hold
+    void* k;
+    void* v;
+    float* k_scale;
+    float* v_scale;
+    uint64_t layer_stride, page_stride, head_stride, token_stride;   // elements
+    int32_t* table;
+    int32_t* refs;
+    const int32_t* seq;             // n: slots (fork: the sources)
+    const int32_t* dst;             // n (fork)
+    const int32_t* start;           // n: grow's start, append's position
+    const int32_t* end;             // n: grow's end, fork's tokens, free's keep (or NULL)
+    const int32_t* count;           // n: compact's, append's (or NULL)
+    const int32_t* index;           // compact's keep, append's index (or NULL)
+    int32_t* result;                // n
+    uint32_t* status;
+    int32_t* fresh;                 // the pages a grow call gives out
+    int32_t* from;                  // the page each one copies, or -1
+    uint32_t* n_fresh;
+};
+struct KvAppendArgs {
+    KvArgs a;
+    const void* k;
+    const void* v;
+    uint64_t new_layer_stride, k_stride, v_stride;
+    uint32_t rows_per_seq, n_layers, blocks;
+};
+
+// attention over the cache and a step's new tokens (lcs_tree.hip)
+struct TreeArgs {
+    KvArgs c;                       // the cache; seq, n and layer of the batch
+    uint32_t rows_per_seq, heads, group, mask_words;
+    float scale;
+    const uint16_t* q;
+    const uint16_t* k;
+    const uint16_t* v;
+    uint64_t q_stride, k_stride, v_stride, o_stride;
+    const int32_t* length;
+    const uint32_t* mask;           // or NULL: chains
+    uint16_t* o;
+    float* lse;                     // or NULL
+};
+
+// a tree's verdict (lcs_verify.hip)
+constexpr uint32_t kTreeMax = 256;      // nodes of a sequence
+struct TreeVerifyArgs {
+    const void* logits;             // or NULL
+    uint64_t row_stride;
+    uint32_t n_seq, rows_per_seq, vocab, dtype;
+    const int32_t* tokens;
+    const int32_t* parent;
+    const int32_t* length;
+    int32_t* argmax_ids;
+    float* node_lp;
+    int32_t* path;
+    int32_t* n_path;
+    int32_t* next_id;
+    int32_t* new_length;
+};
+
 // status bits
 constexpr uint32_t kStatusHistCap = 1u;   // a penalty window exceeded the capacity
 constexpr uint32_t kStatusBinCap = 2u;    // selection could not narrow a bin (unexpected)
 constexpr uint32_t kStatusWindow = 4u;    // a device-resident window did not match its row
+constexpr uint32_t kStatusPages = 8u;     // a cache request was refused, or a page was missing
 
 }  // namespace lcs

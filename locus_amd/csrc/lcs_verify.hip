@@ -315,17 +315,95 @@ __global__ __launch_bounds__(kAcceptSeqs * kWave) void accept_kernel(VerifyArgs 
     if (lane == 0u) a.accept_len[seq] = acc;
 }
 
-template <int G, int NT>
-static void launch_nt(const VerifyArgs& a, uint32_t rows, hipStream_t st) {
+// ---- a tree's verdict (lcs_tree_verify) ----
+// tree_rows streams the rows as verify_kernel does; a row's workgroup also writes the
+// log-probabilities of the nodes whose parent it is (the root's row those of the nodes
+// that have none). tree_walk then follows the accepted nodes: a wave per sequence, four
+// nodes a lane, one ballot per 64 nodes and step.
+__device__ __forceinline__ bool tree_child(uint32_t j, int32_t parent) { return parent >= 0 && (uint32_t)parent < j; }
+
+template <int G, int NT, RowForm F>
+__global__ __launch_bounds__(NT) void tree_rows(TreeVerifyArgs a) {
+    __shared__ float redf[NT / kWave];
+    __shared__ uint32_t redu[NT / kWave];
+    __shared__ double redd[NT / kWave];
+    const uint32_t row = wg_x(), V = a.vocab, R = a.rows_per_seq;
+    if (row >= a.n_seq * R) return;
+    const void* rowp = static_cast<const char*>(a.logits) + (uint64_t)row * a.row_stride * (16u / G);
+    const RowLane l = stream_row<G, NT, F>(rowp, V);
+    float bm;
+    uint32_t idx;
+    const double z = reduce_row<G, NT>(l, rowp, V, bm, idx, redf, redu, redd);
+    if (tid_x() == 0) a.argmax_ids[row] = (int32_t)(idx < V ? idx : 0u);
+    if (!a.node_lp) return;
+    const uint32_t first = row / R * R, me = row - first;
+    for (uint32_t j = tid_x(); j < R; j += NT) {
+        const int32_t p = a.parent[first + j], d = a.tokens[first + j];
+        const bool child = tree_child(j, p);
+        if (child ? (uint32_t)p != me : me != 0u) continue;
+        float lp = 0.0f;
+        if (child && d >= 0 && (uint32_t)d < V) lp = (float)((double)load_elem(rowp, a.dtype, (uint32_t)d) - (log(z) + (double)bm));
+        a.node_lp[first + j] = lp;
+    }
+}
+
+__global__ __launch_bounds__(kAcceptSeqs * kWave) void tree_walk(TreeVerifyArgs a) {
+    constexpr uint32_t NK = kTreeMax / kWave;
+    const uint32_t seq = wg_x() * kAcceptSeqs + tid_x() / kWave;
+    if (seq >= a.n_seq) return;
+    const uint32_t lane = (uint32_t)lane_id(), R = a.rows_per_seq;
+    const uint64_t first = (uint64_t)seq * R;
+    int32_t up[NK];   // a node's parent where it is what that says, else -1
+#pragma unroll
+    for (uint32_t k = 0; k < NK; ++k) {
+        const uint32_t j = lane + k * kWave;
+        up[k] = -1;
+        if (j < R) {
+            const int32_t p = a.parent[first + j];
+            if (tree_child(j, p) && a.argmax_ids[first + (uint32_t)p] == a.tokens[first + j]) up[k] = p;
+        }
+    }
+    int32_t cur = 0;
+    uint32_t n = 0;
+    for (;;) {   // (a child's number is above its parent's: at most R steps)
+        if (lane == 0u) a.path[first + n] = cur;
+        ++n;
+        int32_t next = -1;
+#pragma unroll
+        for (int k = (int)NK - 1; k >= 0; --k) {
+            const uint64_t m = ballot(up[k] == cur);
+            next = m ? (int32_t)(k * kWave) + __builtin_ctzll(m) : next;
+        }
+        if (next < 0 || n >= R) break;
+        cur = next;
+    }
+    for (uint32_t j = n + lane; j < R; j += kWave) a.path[first + j] = -1;
+    if (lane == 0u) {
+        a.n_path[seq] = (int32_t)n;
+        a.next_id[seq] = a.argmax_ids[first + (uint32_t)cur];
+        if (a.new_length) a.new_length[seq] = a.length[seq] + (int32_t)n;
+    }
+}
+
+template <int G, int NT, RowForm F>
+static void launch_form(const VerifyArgs& a, uint32_t rows, hipStream_t st) {
+    hipLaunchKernelGGL((verify_kernel<G, NT, F>), dim3(rows), dim3(NT), 0, st, a);
+}
+template <int G, int NT, RowForm F>
+static void launch_form(const TreeVerifyArgs& a, uint32_t rows, hipStream_t st) {
+    hipLaunchKernelGGL((tree_rows<G, NT, F>), dim3(rows), dim3(NT), 0, st, a);
+}
+template <int G, int NT, class Args>
+static void launch_nt(const Args& a, uint32_t rows, hipStream_t st) {
     const RowForm f = row_form<G>(a.vocab, NT);
     if constexpr (NT == 256) {   // (512 threads take long rows only)
         if (f == kRowShort) {
-            hipLaunchKernelGGL((verify_kernel<G, NT, kRowShort>), dim3(rows), dim3(NT), 0, st, a);
+            launch_form<G, NT, kRowShort>(a, rows, st);
             return;
         }
     }
-    if (f == kRowRounds) hipLaunchKernelGGL((verify_kernel<G, NT, kRowRounds>), dim3(rows), dim3(NT), 0, st, a);
-    else hipLaunchKernelGGL((verify_kernel<G, NT, kRowTail>), dim3(rows), dim3(NT), 0, st, a);
+    if (f == kRowRounds) launch_form<G, NT, kRowRounds>(a, rows, st);
+    else launch_form<G, NT, kRowTail>(a, rows, st);
 }
 
 // Threads per row (us a call with 256 / 512 threads). Up to a row a CU, a row
@@ -336,8 +414,8 @@ static void launch_nt(const VerifyArgs& a, uint32_t rows, hipStream_t st) {
 // 27.9 / 32.9, 512 rows 42.7 / 45.2; bf16, V 163840, 300 rows 23.5 / 26.2, 1024
 // rows 59.3 / 60.7; 2048 rows of V 5000 10.1 / 16.7), except for thousands of
 // long bf16 rows (V 163840, 1536 rows 93.1 / 90.7, 4096 rows 229.7 / 228.8).
-template <int G>
-static void launch_rows(const VerifyArgs& a, hipStream_t st) {
+template <int G, class Args>
+static void launch_rows(const Args& a, hipStream_t st) {
     const uint32_t rows = a.n_seq * a.rows_per_seq, ng = (a.vocab + G - 1u) / G;
     const bool wide = ng > 8192u && (rows <= 256u || (G == 8 && rows > 1024u && ng > 16384u));
     if (wide) launch_nt<G, 512>(a, rows, st);
@@ -350,6 +428,17 @@ hipError_t launch_verify(const VerifyArgs& a, hipStream_t st) {
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     hipLaunchKernelGGL(accept_kernel, dim3((a.n_seq + kAcceptSeqs - 1u) / kAcceptSeqs), dim3(kAcceptSeqs * kWave), 0, st, a);
+    return hipGetLastError();
+}
+
+hipError_t launch_tree_verify(const TreeVerifyArgs& a, hipStream_t st) {
+    if (a.logits) {
+        if (a.dtype == LCS_BF16) launch_rows<8>(a, st);
+        else launch_rows<4>(a, st);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    hipLaunchKernelGGL(tree_walk, dim3((a.n_seq + kAcceptSeqs - 1u) / kAcceptSeqs), dim3(kAcceptSeqs * kWave), 0, st, a);
     return hipGetLastError();
 }
 

@@ -90,6 +90,40 @@ class _NOut(C.Structure):
     _fields_ = [("y", _P), ("y_scale", _P), ("sum", _P), ("y_stride", C.c_uint64), ("sum_stride", C.c_uint64)]
 
 
+class _KvCache(C.Structure):
+    _fields_ = [("layers", C.c_uint32), ("pages", C.c_uint32), ("page_tokens", C.c_uint32), ("kv_heads", C.c_uint32),
+                ("head_dim", C.c_uint32), ("dtype", C.c_uint32), ("seqs", C.c_uint32), ("max_pages", C.c_uint32),
+                ("k", _P), ("v", _P), ("k_scale", _P), ("v_scale", _P), ("layer_stride", C.c_uint64),
+                ("page_stride", C.c_uint64), ("head_stride", C.c_uint64), ("token_stride", C.c_uint64),
+                ("table", _P), ("refs", _P)]
+
+
+class _TreeBatch(C.Structure):
+    _fields_ = [("n_seq", C.c_uint32), ("rows_per_seq", C.c_uint32), ("heads", C.c_uint32), ("layer", C.c_uint32),
+                ("scale", C.c_float), ("mask_words", C.c_uint32), ("cache", C.POINTER(_KvCache)), ("q", _P), ("k", _P),
+                ("v", _P), ("q_stride", C.c_uint64), ("k_stride", C.c_uint64), ("v_stride", C.c_uint64), ("seq", _P),
+                ("length", _P), ("mask", _P)]
+
+
+class _TreeOut(C.Structure):
+    _fields_ = [("o", _P), ("o_stride", C.c_uint64), ("lse", _P)]
+
+
+class _TreeVBatch(C.Structure):
+    _fields_ = [("n_seq", C.c_uint32), ("rows_per_seq", C.c_uint32), ("vocab", C.c_uint32), ("dtype", C.c_uint32),
+                ("row_stride", C.c_uint64), ("logits", _P), ("tokens", _P), ("parent", _P), ("length", _P)]
+
+
+class _TreeVOut(C.Structure):
+    _fields_ = [("argmax_ids", _P), ("node_lp", _P), ("path", _P), ("n_path", _P), ("next_id", _P), ("length", _P)]
+
+
+class _AppendBatch(C.Structure):
+    _fields_ = [("n_seq", C.c_uint32), ("rows_per_seq", C.c_uint32), ("layer", C.c_uint32), ("n_layers", C.c_uint32),
+                ("k", _P), ("v", _P), ("layer_stride", C.c_uint64), ("k_stride", C.c_uint64), ("v_stride", C.c_uint64),
+                ("seq", _P), ("pos", _P), ("count", _P), ("index", _P)]
+
+
 class SamplerError(RuntimeError):
     pass
 
@@ -124,6 +158,42 @@ class Adapters:
         self._c = _Adapters(n, self.wide, a.data_ptr(), b.data_ptr(), _addr(rank), _addr(scale))
 
 
+class KvCache:
+    """A paged cache for kv_*_dev and tree_attn_dev: `k` and `v` (layers, pages,
+    kv_heads, page_tokens, head_dim), bf16 or float8_e4m3fn, of the same strides (any,
+    with a head's elements together); `table` (seqs, max_pages) int32, -1 where a slot
+    has no page; `refs` (pages,) int32; for 8 bits `k_scale` and `v_scale` (layers,
+    pages, kv_heads, page_tokens) f32. Device tensors; nothing is copied."""
+
+    def __init__(self, k, v, table, refs, k_scale=None, v_scale=None):
+        import torch
+        types = {torch.bfloat16: LCS_BF16, torch.float8_e4m3fn: LCS_E4M3}
+        if k.dtype not in types or v.dtype != k.dtype:
+            raise SamplerError("cache: k and v must both be bfloat16 or both float8_e4m3fn")
+        if k.dim() != 5 or v.shape != k.shape:
+            raise SamplerError("cache: k and v must be (layers, pages, kv_heads, page_tokens, head_dim)")
+        ks, vs = k.stride(), v.stride()
+        if ks[4] != 1 or any(a != b and n > 1 for a, b, n in zip(ks, vs, k.shape)):
+            raise SamplerError("cache: k and v must have the same strides, a head's elements together")
+        layers, pages, heads, tokens, dim = k.shape
+        self.device, self.shape = k.get_device(), tuple(k.shape)
+        if table.dim() != 2 or table.dtype != torch.int32 or not table.is_contiguous():
+            raise SamplerError("cache: table must be (seqs, max_pages) int32, contiguous")
+        if refs.dim() != 1 or refs.dtype != torch.int32 or refs.numel() != pages or not refs.is_contiguous():
+            raise SamplerError(f"cache: refs must be ({pages},) int32, contiguous")
+        for t, name in ((k_scale, "k_scale"), (v_scale, "v_scale")):
+            if (t is not None) != (k.dtype == torch.float8_e4m3fn):
+                raise SamplerError(f"cache: {name} goes with float8_e4m3fn")
+            if t is not None and (t.dtype != torch.float32 or t.shape != k.shape[:4] or not t.is_contiguous()):
+                raise SamplerError(f"cache: {name} must be (layers, pages, kv_heads, page_tokens) f32, contiguous")
+        if any(t is not None and t.get_device() != self.device for t in (v, table, refs, k_scale, v_scale)):
+            raise SamplerError("cache: tensors on different devices")
+        self._keep = (k, v, table, refs, k_scale, v_scale)
+        self._c = _KvCache(layers, pages, tokens, heads, dim, types[k.dtype], table.shape[0], table.shape[1], k.data_ptr(),
+                           v.data_ptr(), _addr(k_scale), _addr(v_scale), ks[0], ks[1], ks[2], ks[3], table.data_ptr(),
+                           refs.data_ptr())
+
+
 _lib = None
 
 
@@ -154,6 +224,22 @@ def lib():
         L.lcs_lmhead_ex.argtypes = [_P, C.POINTER(_LExBatch), C.POINTER(_LOut), _P]
         L.lcs_add_rmsnorm.restype = C.c_int
         L.lcs_add_rmsnorm.argtypes = [_P, C.POINTER(_NBatch), C.POINTER(_NOut), _P]
+        cache, i32 = C.POINTER(_KvCache), C.c_uint32
+        L.lcs_kv_reserve.restype = C.c_int
+        L.lcs_kv_reserve.argtypes = [_P, i32]
+        for name in ("lcs_kv_grow", "lcs_kv_fork"):
+            getattr(L, name).restype = C.c_int
+            getattr(L, name).argtypes = [_P, cache, i32, _P, _P, _P, _P, _P]
+        L.lcs_kv_free.restype = C.c_int
+        L.lcs_kv_free.argtypes = [_P, cache, i32, _P, _P, _P, _P]
+        L.lcs_kv_compact.restype = C.c_int
+        L.lcs_kv_compact.argtypes = [_P, cache, i32, i32, _P, _P, _P, _P, _P]
+        L.lcs_kv_append.restype = C.c_int
+        L.lcs_kv_append.argtypes = [_P, cache, C.POINTER(_AppendBatch), _P]
+        L.lcs_tree_attn.restype = C.c_int
+        L.lcs_tree_attn.argtypes = [_P, C.POINTER(_TreeBatch), C.POINTER(_TreeOut), _P]
+        L.lcs_tree_verify.restype = C.c_int
+        L.lcs_tree_verify.argtypes = [_P, C.POINTER(_TreeVBatch), C.POINTER(_TreeVOut), _P]
         L.lcs_last_error.restype = C.c_char_p
         L.lcs_last_error.argtypes = [_P]
         L.lcs_logprobs.restype = C.c_int
@@ -528,7 +614,7 @@ class Sampler:
             out["stats"] = torch.full((rows, 2), -7.0, dtype=torch.float64, device=dev)
         return out
 
-    # (a serving step makes these two calls once a token: their checks read each
+    # (a serving step makes these calls once a token: their checks read each
     # tensor's attributes once, and messages are put together where one is raised)
     def _vec(self, t, n: int, dtype, name: str):
         """The address of an optional (n,) device vector."""
@@ -629,6 +715,163 @@ class Sampler:
         b = _NBatch(rows, hidden, xt, yt, eps, xp, rp, self._vec(weight, hidden, dtype, "weight"), xs, rs)
         o = _NOut(yp, self._vec(out.get("y_scale"), rows, self.torch.float32, "y_scale"), sp, ys, ss)
         rc = _lib.lcs_add_rmsnorm(self.ctx, b, o, self._raw_stream(stream))
+        if rc != LCS_OK:
+            self._check(rc)
+
+    # ------------------------------------------- a paged cache and trees of drafts
+    def kv_reserve(self, new_pages: int):
+        """The workspace of the calls below (lcs_kv_reserve), once, ahead of the loop:
+        new_pages bounds what one kv_grow_dev call may allocate."""
+        self._check(lib().lcs_kv_reserve(self.ctx, new_pages))
+
+    def _cache(self, cache):
+        if not isinstance(cache, KvCache) or cache.device != self.device:
+            raise SamplerError("cache must be a KvCache on the sampler's device")
+        return cache._c
+
+    def _requests(self, *named):
+        """The number of requests and the addresses of their (n,) int32 vectors."""
+        n = named[0][0].numel()
+        return n, *(self._vec(t, n, self.torch.int32, name) for t, name in named)
+
+    def kv_grow_dev(self, cache, seq, start, end, result, stream=None):
+        """Pages of their own for slots seq[i] at tokens [start[i], end[i])
+        (lcs_kv_grow): missing ones allocated, shared ones replaced by copies.
+        All (n,) int32; result[i] is 0, or -1 where a request was refused."""
+        n, q, s, e, r = self._requests((seq, "seq"), (start, "start"), (end, "end"), (result, "result"))
+        rc = _lib.lcs_kv_grow(self.ctx, self._cache(cache), n, q, s, e, r, self._raw_stream(stream))
+        if rc != LCS_OK:
+            self._check(rc)
+
+    def kv_fork_dev(self, cache, src, dst, tokens, result, stream=None):
+        """Slots dst[i], which hold nothing, share the first tokens[i] tokens of
+        slots src[i] (lcs_kv_fork). All (n,) int32; result as kv_grow_dev."""
+        n, s, d, t, r = self._requests((src, "src"), (dst, "dst"), (tokens, "tokens"), (result, "result"))
+        rc = _lib.lcs_kv_fork(self.ctx, self._cache(cache), n, s, d, t, r, self._raw_stream(stream))
+        if rc != LCS_OK:
+            self._check(rc)
+
+    def kv_free_dev(self, cache, seq, keep, result, stream=None):
+        """Slots seq[i] give up their pages past their first keep[i] tokens (keep
+        None: all) (lcs_kv_free). All (n,) int32; result as kv_grow_dev."""
+        n, s, k, r = self._requests((seq, "seq"), (keep, "keep"), (result, "result"))
+        rc = _lib.lcs_kv_free(self.ctx, self._cache(cache), n, s, k, r, self._raw_stream(stream))
+        if rc != LCS_OK:
+            self._check(rc)
+
+    def kv_compact_dev(self, cache, seq, count, keep, result, stream=None):
+        """Slots seq[i] keep the count[i] tokens that keep[i] names, ascending, moved
+        to their front in all layers (lcs_kv_compact). seq, count, result (n,)
+        and keep (n, max_keep) int32, contiguous; result as kv_grow_dev."""
+        n, s, c, r = self._requests((seq, "seq"), (count, "count"), (result, "result"))
+        if (keep.dtype != self.torch.int32 or keep.dim() != 2 or keep.shape[0] != n or not keep.is_contiguous() or
+                keep.get_device() != self.device):
+            raise SamplerError(f"keep must be ({n}, max_keep) int32, contiguous, on the sampler's device")
+        rc = _lib.lcs_kv_compact(self.ctx, self._cache(cache), n, keep.shape[1], s, c, keep.data_ptr(), r,
+                                 self._raw_stream(stream))
+        if rc != LCS_OK:
+            self._check(rc)
+
+    def _heads(self, t, rows: int, heads: int, dim: int, name: str):
+        """Address and row stride of (rows, heads, dim) bf16 rows, a row's heads together."""
+        if t.dtype != self.torch.bfloat16 or t.shape != (rows, heads, dim) or t.get_device() != self.device:
+            raise SamplerError(f"{name} must be ({rows}, {heads}, {dim}) bfloat16 on the sampler's device")
+        per, head, one = t.stride()
+        if (one != 1 and dim > 1) or (head != dim and heads > 1):
+            raise SamplerError(f"{name}: a row's heads must be contiguous")
+        return t.data_ptr(), per if rows > 1 else heads * dim
+
+    def kv_append_dev(self, cache, k, v, seq, pos, count=None, rows_per_seq: int = 1, index=None, layer: int = 0,
+                      stream=None):
+        """New rows of a cache (lcs_kv_append): token j < count[i] (None:
+        rows_per_seq) of slot seq[i] to position pos[i] + j, from row index[i, j]
+        (None: j) of sequence i's rows_per_seq ones. k and v (layers, n *
+        rows_per_seq, kv_heads, head_dim) bf16 for the layers from `layer` on, or of
+        one layer without the first dimension."""
+        c, i32, vec = self._cache(cache), self.torch.int32, self._vec
+        n = seq.numel()
+        if k.dim() == 3 and v.dim() == 3:
+            k, v = k[None], v[None]
+        if k.dim() != 4 or v.dim() != 4 or k.shape[0] != v.shape[0] or k.shape[0] == 0:
+            raise SamplerError("k and v must be (layers, rows, kv_heads, head_dim) of as many layers, one at least")
+        layers, rows = k.shape[0], n * rows_per_seq
+        (kp, ks), (vp, vs) = (self._heads(t[0], rows, c.kv_heads, c.head_dim, name) for t, name in ((k, "k"), (v, "v")))
+        if layers > 1 and k.stride(0) != v.stride(0):
+            raise SamplerError("k and v must have the same layer stride")
+        if index is not None and (index.dtype != i32 or index.numel() != rows or not index.is_contiguous() or
+                                  index.get_device() != self.device):
+            raise SamplerError(f"index must be ({n}, {rows_per_seq}) int32, contiguous, on the sampler's device")
+        b = _AppendBatch(n, rows_per_seq, layer, layers, kp, vp, k.stride(0), ks, vs, vec(seq, n, i32, "seq"),
+                         vec(pos, n, i32, "pos"), vec(count, n, i32, "count"), _addr(index))
+        rc = _lib.lcs_kv_append(self.ctx, c, b, self._raw_stream(stream))
+        if rc != LCS_OK:
+            self._check(rc)
+
+    def tree_attn_dev(self, q, k, v, cache, out, length, seq=None, rows_per_seq: int = 1, mask=None, layer: int = 0,
+                      scale: float | None = None, stream=None):
+        """Attention of a step's new tokens over their cached context and over each
+        other (lcs_tree_attn): q (rows, heads, head_dim), k and v (rows, kv_heads,
+        head_dim) bf16, any row stride, rows_per_seq rows for each sequence;
+        `length` and `seq` (n,) int32: cached tokens and slots (None: 0, 1, ..);
+        `mask` (rows, words) int32, or None for chains; scale None: head_dim ** -0.5.
+        `out` holds "o" as q, and "lse" (rows, heads) f32 if wanted."""
+        c, i32, vec = self._cache(cache), self.torch.int32, self._vec
+        n, dim = length.numel(), c.head_dim
+        rows = n * rows_per_seq
+        if q.dim() != 3:
+            raise SamplerError("q must be (rows, heads, head_dim)")
+        heads = q.shape[1]
+        qp, qs = self._heads(q, rows, heads, dim, "q")
+        kp, ks = self._heads(k, rows, c.kv_heads, dim, "k")
+        vp, vs = self._heads(v, rows, c.kv_heads, dim, "v")
+        op, os_ = self._heads(out["o"], rows, heads, dim, "o")
+        lse, words = out.get("lse"), 0
+        if lse is not None and (lse.dtype != self.torch.float32 or lse.shape != (rows, heads) or not lse.is_contiguous() or
+                                lse.get_device() != self.device):
+            raise SamplerError(f"lse must be ({rows}, {heads}) f32, contiguous, on the sampler's device")
+        if mask is not None:
+            mask = mask.view(rows, -1) if mask.is_contiguous() and rows and mask.numel() % rows == 0 else mask
+            if (mask.dtype != i32 or mask.dim() != 2 or mask.shape[0] != rows or not mask.is_contiguous() or
+                    mask.get_device() != self.device):
+                raise SamplerError(f"mask must be ({rows}, words) int32, contiguous, on the sampler's device")
+            words = mask.shape[1]
+        b = _TreeBatch(n, rows_per_seq, heads, layer, dim ** -0.5 if scale is None else scale, words, C.pointer(c), qp, kp,
+                       vp, qs, ks, vs, vec(seq, n, i32, "seq"), vec(length, n, i32, "length"), _addr(mask))
+        rc = _lib.lcs_tree_attn(self.ctx, b, _TreeOut(op, os_, _addr(lse)), self._raw_stream(stream))
+        if rc != LCS_OK:
+            self._check(rc)
+
+    def tree_verify_dev(self, tokens, parent, out, rows_per_seq: int, logits=None, length=None, stream=None):
+        """The greedy verdict on trees of drafts (lcs_tree_verify): `tokens` and
+        `parent` (n * rows_per_seq,) int32; `logits` (rows, vocab) f32 or bf16, any
+        16-byte row stride, or None where out["argmax_ids"] already holds the rows'
+        argmax. `out` holds "argmax_ids" (rows,), "path" (n, rows_per_seq),
+        "n_path" and "next_id" (n,) int32, and if wanted "node_lp" (rows,) f32 and
+        "length" (n,) int32: `length` + n_path."""
+        i32, f32, vec = self.torch.int32, self.torch.float32, self._vec
+        rows = tokens.numel()
+        if rows_per_seq < 1 or rows % rows_per_seq:
+            raise SamplerError("rows_per_seq must divide the rows")
+        n = rows // rows_per_seq
+        vocab = dtype = stride = 0
+        if logits is not None:
+            dtype = self._types.get(logits.dtype)
+            if dtype not in (LCS_F32, LCS_BF16) or logits.dim() != 2 or logits.shape[0] != rows or logits.get_device() != self.device:
+                raise SamplerError(f"logits must be ({rows}, vocab) float32 or bfloat16 on the sampler's device")
+            vocab = logits.shape[1]
+            if logits.stride(1) != 1 and vocab > 1:
+                raise SamplerError("logits must have unit column stride")
+            per = 4 if dtype == LCS_F32 else 8
+            stride = logits.stride(0) if rows > 1 else (vocab + per - 1) // per * per
+        path = out["path"]
+        if path.dtype != i32 or path.numel() != rows or not path.is_contiguous() or path.get_device() != self.device:
+            raise SamplerError(f"path must be ({n}, {rows_per_seq}) int32, contiguous, on the sampler's device")
+        b = _TreeVBatch(n, rows_per_seq, vocab, dtype, stride, _addr(logits), vec(tokens, rows, i32, "tokens"),
+                        vec(parent, rows, i32, "parent"), vec(length, n, i32, "length"))
+        o = _TreeVOut(vec(out["argmax_ids"], rows, i32, "argmax_ids"), vec(out.get("node_lp"), rows, f32, "node_lp"),
+                      path.data_ptr(), vec(out["n_path"], n, i32, "n_path"), vec(out["next_id"], n, i32, "next_id"),
+                      vec(out.get("length"), n, i32, "length"))
+        rc = _lib.lcs_tree_verify(self.ctx, b, o, self._raw_stream(stream))
         if rc != LCS_OK:
             self._check(rc)
 

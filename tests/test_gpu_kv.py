@@ -1,0 +1,315 @@
+"""The paged cache's bookkeeping and row moves on the GPU (lcs_kv_*) against the model
+of kv_util: tables, counts, results and every row bit by bit."""
+import random
+
+import pytest
+import torch
+
+from kv_util import Model, quantise
+from locus_amd import sampler as S
+
+pytestmark = pytest.mark.gpu
+STATUS_PAGES = 8
+
+
+@pytest.fixture(scope="module")
+def s():
+    x = S.Sampler(device=0, max_rows=64, max_vocab=4096, max_hist=64, max_top=4)
+    x.kv_reserve(4096)
+    yield x
+    x.close()
+
+
+def bits(t):
+    return t.contiguous().view(torch.uint8)
+
+
+class Pair:
+    """A cache on the GPU beside the model of it."""
+
+    def __init__(self, s, layers=2, pages=40, heads=3, page=16, dim=64, seqs=6, max_pages=9, f8=False, layout="head", seed=0):
+        g = torch.Generator().manual_seed(seed)
+        shape = (layers, pages, heads, page, dim)
+        k, v = (torch.randn(shape, generator=g).bfloat16() for _ in range(2))
+        k[0, 0, 0, 0, 0] = float("nan")
+        v[-1, -1, -1, -1, -1] = float("inf")
+        scales = {}
+        if f8:
+            (k, ks), (v, vs) = quantise(k.nan_to_num(1.0)), quantise(v.nan_to_num(1.0, 1.0))
+            scales = {"k_scale": ks.contiguous(), "v_scale": vs.contiguous()}
+        table = torch.full((seqs, max_pages), -1, dtype=torch.int32)
+        refs = torch.zeros(pages, dtype=torch.int32)
+        self.model = Model(k.clone(), v.clone(), table.clone(), refs.clone(), **{n: t.clone() for n, t in scales.items()})
+
+        def put(t):
+            if layout == "head":
+                return t.cuda()
+            if layout == "token":
+                return t.transpose(2, 3).contiguous().cuda().transpose(2, 3)
+            both = torch.zeros(layers, pages, 2, heads, page, dim, dtype=t.dtype)   # k and v of a page together
+            return both.cuda()
+
+        if layout == "both":
+            buf = torch.stack([k, v], 2).contiguous().cuda()
+            self.k, self.v = buf[:, :, 0], buf[:, :, 1]
+        else:
+            self.k, self.v = put(k), put(v)
+        self.scales = {n: t.cuda() for n, t in scales.items()}
+        self.table, self.refs = table.cuda(), refs.cuda()
+        self.s, self.f8 = s, f8
+        self.cache = S.KvCache(self.k, self.v, self.table, self.refs, **self.scales)
+
+    def ints(self, x):
+        return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+    def call(self, fn, want, n, *args, **kw):
+        r = torch.full((n,), 77, dtype=torch.int32, device="cuda")
+        self.s.status()
+        fn(self.cache, *args, r, **kw)
+        torch.cuda.synchronize()
+        assert r.tolist() == want
+        assert self.s.status() == (STATUS_PAGES if -1 in want else 0)
+        self.same()
+
+    def same(self):
+        m = self.model
+        assert torch.equal(self.table.cpu(), m.table)
+        assert torch.equal(self.refs.cpu(), m.refs)
+        for t, w in zip([self.k, self.v, *self.scales.values()], m.rows):
+            assert torch.equal(bits(t.cpu()), bits(w))
+
+    def grow(self, seq, start, end, cap=4096):
+        self.call(self.s.kv_grow_dev, self.model.grow(seq, start, end, cap), len(seq), self.ints(seq), self.ints(start), self.ints(end))
+
+    def fork(self, src, dst, tokens):
+        self.call(self.s.kv_fork_dev, self.model.fork(src, dst, tokens), len(src), self.ints(src), self.ints(dst), self.ints(tokens))
+
+    def free(self, seq, keep=None):
+        self.call(self.s.kv_free_dev, self.model.free(seq, keep), len(seq), self.ints(seq), None if keep is None else self.ints(keep))
+
+    def compact(self, seq, count, keep):
+        k = torch.tensor(keep, dtype=torch.int32, device="cuda")
+        self.call(self.s.kv_compact_dev, self.model.compact(seq, count, keep), len(seq), self.ints(seq), self.ints(count), k)
+
+
+@pytest.mark.parametrize("f8", [False, True])
+@pytest.mark.parametrize("layout", ["head", "token", "both"])
+@pytest.mark.parametrize("page,dim", [(16, 16), (16, 80), (32, 128), (64, 256)])
+def test_grow_fork_free(s, page, dim, layout, f8):
+    c = Pair(s, page=page, dim=dim, layout=layout, f8=f8, pages=30)
+    c.grow([0, 1, 2], [0, 0, 5], [3 * page, 2 * page + 1, page])
+    c.grow([0, 1], [3 * page, 2 * page + 1], [3 * page, 2 * page + 5])        # (nothing to do, and inside a page)
+    c.fork([0, 1, 0], [3, 4, 5], [3 * page - 1, 2 * page + 1, page])
+    c.grow([3, 4, 0], [3 * page - 1, 2 * page + 1, 0], [3 * page + 2, 3 * page, 2])   # copies: tails, and a first page
+    c.free([5, 3], [0, page])
+    c.grow([-1, 5], [0, 0], [5, 1])
+    c.free([0, 1, 2, 3, 4, 5, -1])
+    assert c.refs.sum().item() == 0
+
+
+def test_both_holders_grow(s):
+    """Two holders of a page that ask in one call both get copies, and the page is free again."""
+    c = Pair(s)
+    c.grow([0], [0], [20])
+    c.fork([0], [1], [20])
+    c.grow([0, 1], [20, 20], [21, 21])
+    assert c.refs.tolist().count(1) == 2 and c.refs.max().item() == 2
+
+
+def test_out_of_pages(s):
+    """From the first request that there are not enough pages for, none is served."""
+    c = Pair(s, pages=12)
+    c.grow([0, 1, 2, 3], [0, 0, 0, 0], [5 * 16, 5 * 16, 3 * 16, 16])    # 5 + 5 + 3 > 12: slots 2 and 3 refused
+    c.grow([3], [0], [2 * 16])
+    c.grow([4, 0], [0, 0], [1, 5 * 16])      # none left: refused, and the request after it too, though it asks for none
+    c.free([1])
+    c.grow([4], [0], [5 * 16])
+
+
+def test_few_new_pages_reserved():
+    """A call gives out no more pages than lcs_kv_reserve made room for."""
+    x = S.Sampler(device=0, max_rows=8, max_vocab=4096, max_hist=64, max_top=4)
+    x.kv_reserve(3)
+    c = Pair(x)
+    c.grow([0, 1, 2], [0, 0, 0], [32, 32, 16], cap=3)
+    c.grow([1, 2], [0, 0], [32, 16], cap=3)
+    x.kv_reserve(4)
+    c.grow([3], [0], [64], cap=4)
+    x.close()
+
+
+def test_refused_requests(s):
+    c = Pair(s, seqs=6, max_pages=4)
+    top = 4 * 16
+    c.grow([0, 6, -2, 0, 1, 2, 3], [0, 0, 0, 0, 5, -1, 0], [33, 5, 5, 9, 4, 3, top + 1])
+    c.grow([1, 2], [0, 0], [top, 1])
+    c.fork([0, 0, 3, 0, 1, 9, 0], [3, 3, 4, 2, 9, 4, 4], [33, 33, 1, 33, 16, 1, 49])   # twice, a dst, held, outside, missing
+    c.fork([0, -1, 1], [5, 3, -1], [0, 5, 5])
+    c.fork([2], [2], [1])
+    c.fork([0], [4], [-1])
+    c.free([0, 0, 7, -1, -5], [16, 0, 0, 0, 0])
+    c.free([1, 2], [1000, -3])
+
+
+@pytest.mark.parametrize("n", [1, 2, 17, 64, 200, 1024])
+def test_many_requests(s, n):
+    """Every number of lanes a request; long ranges; the pages' order over many rounds of the search."""
+    c = Pair(s, layers=1, heads=1, page=16, dim=16, pages=n * 5 + 40000, seqs=n + 1, max_pages=8)
+    rng = random.Random(n)
+    c.refs[rng.randrange(30):37000] = 1     # most of the pool held by somebody
+    c.model.refs.copy_(c.refs.cpu())
+    seq = rng.sample(range(n + 1), n)
+    start = [rng.randrange(0, 64) for _ in seq]
+    end = [min(128, a + rng.randrange(0, 80)) for a in start]
+    c.grow(seq, start, end)
+    c.free(seq[: n // 2], [rng.randrange(0, 100) for _ in seq[: n // 2]])
+    c.grow(seq, start, end)
+
+
+@pytest.mark.parametrize("f8", [False, True])
+@pytest.mark.parametrize("layout", ["head", "token", "both"])
+@pytest.mark.parametrize("page,dim", [(16, 16), (16, 96), (32, 128), (64, 256), (16, 240)])
+def test_compact(s, page, dim, layout, f8):
+    c = Pair(s, page=page, dim=dim, layout=layout, f8=f8, pages=40, max_pages=20)
+    rng = random.Random(page + dim)
+    lengths = [20 * page, 7 * page + 3, page + 1, 1]
+    c.grow([0, 1, 2, 3], [0] * 4, lengths)
+    keep = [sorted(rng.sample(range(n), max(1, n * f // 10))) for n, f in zip(lengths, (6, 5, 10, 10))]
+    wide = max(map(len, keep))
+    pad = lambda k: k + [-1] * (wide - len(k))   # noqa: E731
+    c.compact([0, 1, -1, 2, 3], [len(keep[0]), len(keep[1]), 4, len(keep[2]), 1],
+              [pad(keep[0]), pad(keep[1]), pad([]), pad(keep[2]), pad(keep[3])])
+    c.compact([0, 1], [0, -5], [pad([]), pad([])])
+    c.compact([0], [10 ** 6], [list(range(wide))])
+
+
+def test_compact_refused(s):
+    c = Pair(s, max_pages=4)
+    c.grow([0, 1], [0, 0], [64, 40])
+    c.fork([0], [2], [64])
+    c.compact([0, 1, 1, 6, -3], [2, 2, 2, 2, 2], [[0, 5], [3, 7], [3, 7], [0, 1], [0, 1]])     # shared; fine; twice; outside
+    c.compact([1, 2], [2, 2], [[0, 1], [0, 1]])               # (nothing moves: a shared page may stay)
+    c.compact([1], [3], [[0, 5, 5]])
+    c.compact([1], [3], [[4, 9, 8]])
+    c.compact([1], [2], [[-1, 3]])
+    c.compact([1], [2], [[0, 64]])
+    c.compact([1], [2], [[0, 50]])                            # (past its pages)
+    c.grow([2], [0], [64])
+    c.compact([2, 0], [2, 2], [[7, 20], [3, 4]])
+
+
+@pytest.mark.parametrize("f8", [False, True])
+@pytest.mark.parametrize("layout", ["head", "token", "both"])
+@pytest.mark.parametrize("page,dim,heads", [(16, 16, 3), (16, 80, 1), (32, 128, 8), (64, 256, 2), (128, 240, 5)])
+def test_append(s, page, dim, heads, layout, f8):
+    c = Pair(s, page=page, dim=dim, heads=heads, layout=layout, f8=f8, layers=3, pages=20, max_pages=3)
+    g = torch.Generator().manual_seed(dim)
+    seq, pos, rows = [2, -1, 0, 5], [0, 3, page - 3, 2 * page - 1], 37
+    count = [rows, 5, 20 if page > 16 else 18, 1]
+    pos = [min(p, 3 * page - n) for p, n in zip(pos, count)]
+    c.grow([2, 0, 5], [0, 0, 0], [min(3 * page, 37), min(3 * page, page + 40), 2 * page])
+    # rows cut out of a wider buffer; widths that bf16 does not hold exactly in 8 bits, a row of zeros, a NaN, an infinity
+    buf = torch.randn(2, 4 * rows, 2 * heads * dim + 16, generator=g).bfloat16()
+    buf[:, 3] = 0.0
+    buf[0, 5, 1] = float("nan")
+    buf[1, 6, 2] = float("-inf")
+    buf[:, 7] *= 1e-30
+    buf[:, 8] *= 1e30
+    new = buf.cuda()
+    k, v = (new[:, :, 8 + i * heads * dim:][:, :, : heads * dim].unflatten(2, (heads, dim)) for i in (0, 1))
+    index = torch.stack([torch.randperm(rows, generator=g) for _ in range(4)]).int()
+    for use in (None, index):
+        for cnt in (count, None):
+            if cnt is None and (page < 64 or use is None):
+                continue
+            p = pos if cnt else [0, 0, 0, 0]
+            m = c.model
+            c.s.status()
+            c.s.kv_append_dev(c.cache, k, v, c.ints(seq), c.ints(p), None if cnt is None else c.ints(cnt), rows_per_seq=rows,
+                              index=None if use is None else use.cuda(), layer=1)
+            torch.cuda.synchronize()
+            if cnt is None:
+                c.model = m
+            for i, q in enumerate(seq):
+                for j in range((cnt or [rows] * 4)[i] if q >= 0 else 0):
+                    r = i * rows + (j if use is None else int(use[i, j]))
+                    pg, off = int(m.table[q, (p[i] + j) // page]), (p[i] + j) % page
+                    for t, x in ((0, k), (1, v)):
+                        x = x[:, r].cpu()
+                        if f8:
+                            x, sc = quantise(x)
+                            m.rows[2 + t][1:3, pg, :, off] = sc
+                        m.rows[t][1:3, pg, :, off] = x
+            if f8:   # (a NaN is one whatever its bits)
+                for t, w in zip((c.k, c.v), m.rows):
+                    assert torch.equal(torch.isnan(t.float()).cpu(), torch.isnan(w.float()))
+                    assert torch.equal(t.float().cpu().nan_to_num(), w.float().nan_to_num())
+                for t, w in zip(c.scales.values(), m.rows[2:]):
+                    assert torch.equal(t.cpu(), w)
+                assert torch.equal(c.table.cpu(), m.table) and torch.equal(c.refs.cpu(), m.refs)
+            else:
+                c.same()
+            assert c.s.status() == 0
+
+
+def test_append_where_it_may_not(s):
+    """Missing and shared pages, positions and indexes out of range: nothing is written, and the status says so."""
+    c = Pair(s, max_pages=4)
+    c.grow([0, 1], [0, 0], [40, 16])
+    c.fork([1], [2], [16])
+    new = torch.randn(2, 7 * 2, 3, 64, device="cuda").bfloat16()
+    for seq, pos, count, index in [([1], [0], [2], None), ([2], [3], [1], None), ([0], [48], [2], None), ([0], [-2], [2], None),
+                                   ([0], [64], [1], None), ([0], [2 ** 31 - 1], [2], None), ([6], [0], [1], None), ([-2], [0], [1], None),
+                                   ([3], [0], [1], None), ([0], [0], [1], [[7, 0, 0, 0, 0, 0, 0]]), ([0], [0], [1], [[-1, 0, 0, 0, 0, 0, 0]])]:
+        s.status()
+        s.kv_append_dev(c.cache, new[:, :7], new[:, 7:], c.ints(seq), c.ints(pos), c.ints(count), rows_per_seq=7,
+                        index=None if index is None else c.ints(index))
+        torch.cuda.synchronize()
+        assert s.status() == STATUS_PAGES, (seq, pos)
+        c.same()
+    s.kv_append_dev(c.cache, new[:, :7], new[:, 7:], c.ints([0]), c.ints([5]), c.ints([-4]), rows_per_seq=7)
+    torch.cuda.synchronize()
+    assert s.status() == 0
+    c.same()
+
+
+def test_no_requests(s):
+    c = Pair(s)
+    none = torch.empty(0, dtype=torch.int32, device="cuda")
+    s.kv_grow_dev(c.cache, none, none, none, none)
+    s.kv_fork_dev(c.cache, none, none, none, none)
+    s.kv_free_dev(c.cache, none, None, none)
+    s.kv_append_dev(c.cache, torch.empty(2, 0, 3, 64, device="cuda", dtype=torch.bfloat16),
+                    torch.empty(2, 0, 3, 64, device="cuda", dtype=torch.bfloat16), none, none, rows_per_seq=4)
+    torch.cuda.synchronize()
+    c.same()
+
+
+def test_without_reserve():
+    x = S.Sampler(device=0, max_rows=8, max_vocab=4096, max_hist=64, max_top=4)
+    c = Pair(x)
+    one = c.ints([0])
+    with pytest.raises(S.SamplerError, match="reserve"):
+        x.kv_grow_dev(c.cache, one, one, one, one.clone())
+    x.close()
+
+
+@pytest.mark.parametrize("seed", range(4))
+def test_random_runs(s, seed):
+    """Calls of every kind in a row, good and bad requests mixed."""
+    rng = random.Random(seed)
+    c = Pair(s, layers=2, pages=rng.choice([20, 60]), heads=2, page=16, dim=32, seqs=7, max_pages=6, f8=seed % 2 == 1, seed=seed)
+    for _ in range(25):
+        n = rng.randint(1, 7)
+        seq = [rng.choice([-1, rng.randrange(7), rng.randrange(7), rng.randrange(8)]) for _ in range(n)]
+        kind = rng.choice(["grow", "grow", "fork", "free", "compact"])
+        if kind == "grow":
+            start = [rng.randrange(0, 90) for _ in seq]
+            c.grow(seq, start, [min(96, a + rng.randrange(0, 60)) for a in start])
+        elif kind == "fork":
+            c.fork([rng.randrange(7) for _ in seq], seq, [rng.randrange(0, 60) for _ in seq])
+        elif kind == "free":
+            c.free(seq, rng.choice([None, [rng.randrange(0, 90) for _ in seq]]))
+        else:
+            keep = [sorted(rng.sample(range(rng.choice([30, 60, 96])), 20)) for _ in seq]
+            c.compact(seq, [rng.randint(0, 20) for _ in seq], keep)
