@@ -316,7 +316,7 @@ typedef struct lcs_kv_cache {
  * only (lcs_kv_append puts the accepted ones there). Query head h reads kv head
  * h / (heads / kv_heads). Scores, statistics and sums are f32; a weight is rounded
  * to bf16 for the product with the values, o once at the end. A row that sees
- * nothing has o = 0 and lse = -inf. What a row does not see is no part of its
+ * nothing (or scores of -inf only) has o = 0 and lse = -inf. What a row does not see is no part of its
  * result, whatever it holds. */
 typedef struct lcs_tree_attn_batch {
     uint32_t n_seq;            /* up to 1024 */

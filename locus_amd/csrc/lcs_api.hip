@@ -36,7 +36,8 @@ hipError_t launch_kv_fork(const KvArgs& a, hipStream_t st);
 hipError_t launch_kv_grow(const KvArgs& a, hipStream_t st);
 hipError_t launch_kv_compact(const KvArgs& a, hipStream_t st);
 hipError_t launch_kv_append(const KvAppendArgs& a, hipStream_t st);
-hipError_t launch_tree_attn(const TreeArgs& a, hipStream_t st);
+hipError_t launch_tree_attn(const TreeArgs& a, uint32_t cus, hipStream_t st);
+uint64_t tree_part_floats();
 hipError_t launch_tree_verify(const TreeVerifyArgs& a, hipStream_t st);
 }  // namespace lcs
 
@@ -70,6 +71,7 @@ struct lcs_ctx {
     // each copies, and their number
     uint32_t kv_cap = 0;
     int32_t* kv_fresh = nullptr;   // kv_cap, then kv_cap for what they copy, then the number
+    float* tree_part = nullptr;    // lcs_tree_attn: 64 zeros, then the partial results
     // lcs_logprobs: greedy parameters (all fields zero) for max_rows rows, on
     // the device and on the host, and its argmax ids when the caller wants none
     lcs_params* lp_params = nullptr;
@@ -218,6 +220,7 @@ void lcs_destroy(lcs_ctx* c) {
     (void)hipFree(c->wbkt);
     (void)hipFree(c->wstage);
     (void)hipFree(c->kv_fresh);
+    (void)hipFree(c->tree_part);
     delete c;
 }
 
@@ -798,8 +801,17 @@ int lcs_kv_reserve(lcs_ctx* c, uint32_t new_pages) {
     (void)hipFree(c->kv_fresh);
     c->kv_fresh = nullptr;
     c->kv_cap = 0;
-    const hipError_t e = hipMalloc(&c->kv_fresh, ((size_t)new_pages * 2 + 1) * 4);
+    hipError_t e = hipMalloc(&c->kv_fresh, ((size_t)new_pages * 2 + 1) * 4);
+    if (e == hipSuccess && !c->tree_part) {
+        if ((e = hipMalloc(&c->tree_part, (64 + lcs::tree_part_floats()) * 4)) != hipSuccess) c->tree_part = nullptr;
+        else if ((e = hipMemset(c->tree_part, 0, 64 * 4)) == hipSuccess) e = hipDeviceSynchronize();
+        if (e != hipSuccess) {
+            (void)hipFree(c->tree_part);
+            c->tree_part = nullptr;
+        }
+    }
     if (e != hipSuccess) {
+        (void)hipFree(c->kv_fresh);
         c->kv_fresh = nullptr;
         return hip_fail(c, e, "lcs_kv_reserve");
     }
@@ -953,8 +965,10 @@ int lcs_tree_attn(lcs_ctx* c, const lcs_tree_attn_batch* b, const lcs_tree_attn_
     a.mask = b->mask;
     a.o = static_cast<uint16_t*>(o->o);
     a.lse = o->lse;
+    a.zeros = reinterpret_cast<const unsigned char*>(c->tree_part);
+    a.part = c->tree_part + 64;
     DeviceGuard g(c->device);
-    const hipError_t e = lcs::launch_tree_attn(a, static_cast<hipStream_t>(stream));
+    const hipError_t e = lcs::launch_tree_attn(a, c->cus, static_cast<hipStream_t>(stream));
     return e == hipSuccess ? LCS_OK : hip_fail(c, e, "attention kernel launch");
 }
 

@@ -354,7 +354,12 @@ struct TreeArgs {
     const uint32_t* mask;           // or NULL: chains
     uint16_t* o;
     float* lse;                     // or NULL
+    float* part;                    // partial results (tree_part_floats)
+    const unsigned char* zeros;     // 16 bytes
+    // of a launch: workgroups along the line of steps, row tiles and the first one, steps of the new tokens
+    uint32_t pieces, row_tiles, row_tile0, new_steps;
 };
+constexpr uint32_t kTreeSlots = 512;    // workgroups of a launch, at two a CU (half as many at one)
 
 // a tree's verdict (lcs_verify.hip)
 constexpr uint32_t kTreeMax = 256;      // nodes of a sequence

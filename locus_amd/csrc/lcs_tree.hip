@@ -2,13 +2,41 @@
 // (gfx950): o = sum_j p_j v_j with p = softmax_j(scale q.k_j), j over the sequence's
 // cached tokens and over the new tokens that the row's mask names.
 //
-// A wave per row and query head takes 64 keys at a time: a key's score per lane, the
-// running maximum and sum over the wave, then the values with a few elements of the
-// head per lane.
+// The cache's rows are read once and bound it: rows_per_seq x (heads / kv_heads) rows
+// share each key, and up to a few hundred of them are done before the next keys
+// arrive. So the kernel is a stream of keys and values through LDS:
+//
+// - A wave takes 32 keys at a time, their keys and values brought to its own part of
+//   LDS by 16-byte DMA loads, so that no register holds data in flight and waves need
+//   no barrier; four waves take 128 consecutive tokens, a step.
+// - Scores are computed transposed, S^T = K Q^T, with Q in registers as the B
+//   operand: a lane then holds eight keys of one row, so that its softmax is the
+//   lane's own, and the weights are already laid out as the B operand of O^T = V^T P^T.
+//   V^T comes from LDS by transposing reads. One row's statistics and sums stay in
+//   one lane column all the way.
+// - The running maximum moves only when a score exceeds it by 2^8 (wave-uniform), so
+//   that most tiles rescale nothing; weights are then up to 2^8, which f32 sums and
+//   bf16 weights hold as well as 1.
+// - The steps of all (sequence, kv head) pairs form one line that is cut into as many
+//   equal pieces as there are workgroups on the card, whatever the lengths: each
+//   workgroup finds its piece from the lengths on the device. A pair that several
+//   workgroups share is joined by a second launch from their partial sums.
+//
+// A weight is rounded to bf16 for the product with the values (2^-8 of itself at most,
+// as the values themselves are); scores, maxima, sums and the normaliser are f32.
+// e4m3 rows are widened to bf16, which is exact; a key's scale multiplies its scores, a
+// value's scale its weight ahead of the rounding.
+//
+// What is not seen must not matter: cached rows past the length and in missing pages
+// are replaced by zeros on their way to LDS and have weight 0. Among the new tokens a
+// row that some see and others do not may hold infinities or NaNs: those elements
+// are taken out of the product and added one by one to the rows that see them.
 //
 // (This file is compiled with NaNs honoured: a NaN in a row has to stay one.)
 #include <hip/hip_runtime.h>
 #include <stdint.h>
+
+#include <type_traits>
 
 #include "lcs_device.hpp"
 #include "lcs_internal.hpp"
@@ -17,109 +45,677 @@ namespace lcs {
 
 namespace {
 
-constexpr uint32_t kHeadMax = 256;
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef int i32x2 __attribute__((ext_vector_type(2)));
+#define LCS_LDS __attribute__((address_space(3)))
 
-__device__ __forceinline__ float bf16_f(uint32_t u) { return __uint_as_float(u << 16); }
-__device__ __forceinline__ float e4m3_f(uint32_t b) { return __builtin_amdgcn_cvt_f32_fp8((int)b, 0); }
-__device__ __forceinline__ uint32_t f_bf16(float v) { return (uint32_t)__builtin_bit_cast(uint16_t, (__bf16)v); }
+constexpr float kLn2 = 0.69314718055994531f, kLog2e = 1.4426950408889634f;
+constexpr float kUnset = -3.0e38f;   // the running maximum of a row that has seen nothing
+constexpr float kSlack = 8.0f;       // log2 of the weights' bound
+constexpr uint32_t kTileKeys = 32, kStepKeys = 128;
+constexpr int kTreeWaves = 4;
+
+template <int N>
+__device__ __forceinline__ void wait_vm() {
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+// 16 bytes per lane from offset vo of a buffer to LDS at dst + 16 lane (dst is wave-uniform);
+// what lies past the buffer's size arrives as zeros.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const unsigned char* p, uint32_t bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(p), 0, (int)bytes, 0x00020000);
+}
+__device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t rs, unsigned char* dst, uint32_t vo) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (LCS_LDS void*)dst, 16, (int)vo, 0, 0, 0);
+}
+__device__ __forceinline__ void dma4(const void* src, unsigned char* dst) {   // from a per-lane address to dst + 4 lane
+    __builtin_amdgcn_global_load_lds((const LCS_GLOBAL void*)src, (LCS_LDS void*)dst, 4, 0, 0);
+}
+constexpr uint32_t kNoByte = 0x80000000u;   // an offset past every buffer
+// Transposing reads of eight keys' elements by four (16-bit) or eight (8-bit) dim tiles, waited for here:
+// the compiler would have the builtins wait for every DMA load that is under way.
+template <int ROWS16>   // bytes of 16 rows
+__device__ __forceinline__ void read_tr16(const uint32_t (&at)[4], u32x4 (&o)[4]) {
+    u32x2 r[8];
+    asm volatile("ds_read_b64_tr_b16 %0, %8\n\tds_read_b64_tr_b16 %1, %8 offset:%12\n\t"
+                 "ds_read_b64_tr_b16 %2, %9\n\tds_read_b64_tr_b16 %3, %9 offset:%12\n\t"
+                 "ds_read_b64_tr_b16 %4, %10\n\tds_read_b64_tr_b16 %5, %10 offset:%12\n\t"
+                 "ds_read_b64_tr_b16 %6, %11\n\tds_read_b64_tr_b16 %7, %11 offset:%12\n\ts_waitcnt lgkmcnt(0)"
+                 : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3]), "=&v"(r[4]), "=&v"(r[5]), "=&v"(r[6]), "=&v"(r[7])
+                 : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "n"(ROWS16)
+                 : "memory");
+#pragma unroll
+    for (int k = 0; k < 4; ++k) o[k] = u32x4{r[2 * k][0], r[2 * k][1], r[2 * k + 1][0], r[2 * k + 1][1]};
+}
+__device__ __forceinline__ void read_tr8(const uint32_t (&at)[4], u32x2 (&o)[4]) {
+    asm volatile("ds_read_b64_tr_b8 %0, %4\n\tds_read_b64_tr_b8 %1, %5\n\tds_read_b64_tr_b8 %2, %6\n\tds_read_b64_tr_b8 %3, %7\n\t"
+                 "s_waitcnt lgkmcnt(0)"
+                 : "=&v"(o[0]), "=&v"(o[1]), "=&v"(o[2]), "=&v"(o[3])
+                 : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3])
+                 : "memory");
+}
+__device__ __forceinline__ uint32_t lds_at(const unsigned char* p) { return (uint32_t)(uintptr_t)(LCS_LDS const unsigned char*)p; }
+__device__ __forceinline__ float exp2_f(float x) { return __builtin_amdgcn_exp2f(x); }
+// Over the four lanes that hold a row (lane, lane ^ 16, lane ^ 32, lane ^ 48).
+template <class F>
+__device__ __forceinline__ float across(float x, F f) {
+    const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = f(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return f(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {   // to nearest even
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){a, b}, bf16x2));
+}
+__device__ __forceinline__ bool wild_bf16x2(uint32_t w) {   // either half an infinity or a NaN
+    return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
+}
+
+// A tile's row is a power of two of 16-byte chunks in LDS; chunk c of row r lies at place c
+// ^ x(r), so that the reads of a half wave cover the 64 banks once. x picks bits of r.
+template <int ROWB>   // bytes of a row
+__device__ __forceinline__ constexpr uint32_t swz_k(uint32_t r) {   // 16 rows, one chunk
+    return ROWB == 64 ? r >> 2 & 3u : ROWB == 128 ? r >> 1 & 7u : r & 15u;
+}
+template <int ROWB, bool B8>
+__device__ __forceinline__ constexpr uint32_t swz_v(uint32_t r) {
+    if (!B8) return ROWB == 128 ? 2u * (r >> 1 & 3u) : 2u * (r & 7u);   // 8 rows, two chunks
+    return ROWB == 64 ? (r >> 2 & 1u) | (r >> 3 & 2u) : ROWB == 128 ? (r >> 1 & 3u) | (r >> 2 & 4u) : (r & 7u) | (r >> 1 & 8u);   // rows 0-7 and 16-23, one chunk
+}
+
+// Where each sequence's steps lie on the line of all: lane l holds sequences per * l ..
+// per * (l + 1) - 1 (at most 16).
+struct Line {
+    uint32_t per, before, total;   // steps ahead of the lane's sequences, of all sequences
+    bool bad;
+};
+struct Seq {
+    uint32_t len, steps;   // cached tokens; steps, those of the new tokens included
+};
+__device__ __forceinline__ Seq seq_of(const TreeArgs& a, uint32_t i, bool& bad) {
+    const int32_t slot = a.c.seq ? a.c.seq[i] : (int32_t)i;
+    const uint64_t most = (uint64_t)a.c.max_pages << a.c.page_shift;
+    const int32_t n = a.length[i];
+    uint32_t len = slot == -1 || n < 0 ? 0u : (uint32_t)n;
+    if (slot < -1 || slot >= (int64_t)a.c.seqs) {
+        bad = true;
+        len = 0u;
+    } else if (len > most) {
+        bad = true;
+        len = (uint32_t)most;
+    }
+    return Seq{len, (len + kStepKeys - 1u) / kStepKeys + a.new_steps};
+}
+__device__ __forceinline__ Line line_of(const TreeArgs& a) {
+    Line l{(a.c.n + kWave - 1u) / kWave, 0u, 0u, false};
+    uint32_t sum = 0;
+    for (uint32_t k = 0; k < l.per; ++k) {
+        const uint32_t i = (uint32_t)lane_id() * l.per + k;
+        if (i < a.c.n) sum += seq_of(a, i, l.bad).steps;
+    }
+    const uint32_t incl = wave_scan_incl_u(sum);
+    l.before = incl - sum;
+    l.total = (uint32_t)__builtin_amdgcn_readlane((int)incl, kWave - 1);
+    return l;
+}
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); }
+// The steps of one workgroup's piece of the line (of total x kv_heads steps).
+__device__ __forceinline__ uint32_t share_of(const TreeArgs& a, uint32_t all) {
+    const uint32_t s = (all + a.pieces - 1u) / a.pieces;
+    return s > 1u ? s : 1u;
+}
+
+// A partial result: the rows' unnormalised sums, then their maxima (log2) and sums of weights.
+template <int DP, int MT>
+struct Part {
+    static constexpr uint32_t kRows = 16u * MT;
+    static constexpr uint32_t kFloats = kRows * DP + 2u * kRows;
+};
 
 }  // namespace
 
-template <bool F8>
-__global__ __launch_bounds__(kWave) void tree_attn(TreeArgs a) {
-    __shared__ float qs[kHeadMax], ps[kWave];
-    __shared__ uint64_t at[kWave];   // a key's element 0 in k or v
-    const uint32_t lane = tid_x(), h = wg_x() % a.heads, r = wg_x() / a.heads, i = r / a.rows_per_seq, j = r % a.rows_per_seq;
-    const uint32_t D = a.c.head_dim, kvh = h / a.group, R = a.rows_per_seq;
-    const int32_t slot = a.c.seq ? a.c.seq[i] : (int32_t)i;
-    int64_t len = slot == -1 ? 0 : max(a.length[i], 0);
-    bool bad = slot < -1 || slot >= (int64_t)a.c.seqs;
-    if (bad) len = 0;
-    const int64_t most = (int64_t)a.c.max_pages << a.c.page_shift;
-    bad = bad || len > most;
-    len = len > most ? most : len;
-    const int32_t* row = a.c.table + (uint64_t)(len > 0 ? slot : 0) * a.c.max_pages;
-    for (uint32_t d = lane; d < D; d += kWave) qs[d] = bf16_f(a.q[r * a.q_stride + h * D + d]);
-    __syncthreads();
-    float m = -__builtin_huge_valf(), z = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    // cached tokens in blocks of 64, then the new ones
-    const int64_t blocks = (len + kWave - 1) / kWave;
-    for (int64_t b = 0; b < blocks + (R + kWave - 1) / kWave; ++b) {
-        const bool fresh = b >= blocks;
-        const int64_t t = (fresh ? b - blocks : b) * kWave + lane;
-        bool see = false;
-        float s = 0.0f, vs = 1.0f;
-        uint64_t e = 0;
-        if (!fresh) {
-            if (t < len) {
-                const int32_t page = row[t >> a.c.page_shift];
-                see = (uint32_t)page < a.c.pages;
-                bad = bad || !see;
-                if (see) {
-                    const uint32_t in = (uint32_t)t & (a.c.page_tokens - 1u);
-                    e = a.c.layer * a.c.layer_stride + (uint32_t)page * a.c.page_stride + kvh * a.c.head_stride + in * a.c.token_stride;
-                    float ks = 1.0f;
-                    if (F8) {
-                        const uint64_t w = ((((uint64_t)a.c.layer * a.c.pages + (uint32_t)page) * a.c.kv_heads + kvh) << a.c.page_shift) + in;
-                        ks = a.c.k_scale[w];
-                        vs = a.c.v_scale[w];
+template <int DP, int MT, bool F8, int ST>
+__global__ __launch_bounds__(kTreeWaves * kWave, DP == 256 || (MT == 4 && DP == 128) ? 1 : 2) void tree_attn(TreeArgs a) {
+    constexpr uint32_t kRows = 16u * MT, kDT = DP / 16, kKS = DP / 32;
+    constexpr uint32_t kRowB = DP * (F8 ? 1 : 2), kNewB = DP * 2;                 // bytes of a cached row and of a new one in LDS
+    constexpr uint32_t kScaleB = F8 ? 256u : 0u;
+    constexpr uint32_t kStage = 2u * kTileKeys * kRowB + kScaleB;
+    constexpr uint32_t kMergeB = kRows * DP * 4u;
+    constexpr uint32_t kMax1 = ST * kStage > 2u * kTileKeys * kNewB ? ST * kStage : 2u * kTileKeys * kNewB;
+    constexpr uint32_t kRegion = kMax1 > kMergeB ? kMax1 : kMergeB;
+    constexpr int kNI = (int)(kTileKeys * kRowB / 1024u);      // DMA loads of a tile's keys, and of its values
+    constexpr int kNK = kNI + (F8 ? 1 : 0);
+    __shared__ __attribute__((aligned(1024))) unsigned char lds[kTreeWaves * kRegion];
+    __shared__ float stat[kTreeWaves][2][kRows];
+    const uint32_t lane = (uint32_t)lane_id(), w = uniform(tid_x() / kWave), n = lane & 15u, g = lane >> 4;
+    unsigned char* const mine = lds + w * kRegion;
+    const uint32_t b = wg_x(), piece = b / 8u / a.row_tiles * 8u + b % 8u, rt = b / 8u % a.row_tiles + a.row_tile0;
+    const Line line = line_of(a);
+    if (line.bad && b == 0u && w == 0u) atomicOr(a.c.status, kStatusPages);
+    const uint32_t H = a.c.kv_heads, all = line.total * H, share = share_of(a, all);
+    const uint32_t end = min(all, (piece + 1u) * share);   // (all < 2^31 / ...: checked on the host)
+    const uint32_t D = a.c.head_dim, N = a.rows_per_seq, R = N * a.group;
+    const uint64_t ts = a.c.token_stride * (F8 ? 1u : 2u);
+    const float sc = (a.scale == 0.0f ? 1.0f : __builtin_fabsf(a.scale)) * kLog2e;
+    // a score's dims: k-slot (ks, g, j) of the products is dim 8 chunk8(ks) + j of both operands
+    auto chunk8 = [&](uint32_t ks) -> uint32_t { return F8 ? 2u * (g + 4u * (ks / 2u)) + (ks & 1u) : 4u * ks + g; };
+
+    uint32_t x = piece * share;
+    while (x < end) {
+        // ---- the segment: the steps of one (sequence, kv head) pair in this piece ----
+        // the lane that holds the sequence is the last whose steps begin at or ahead of x
+        const uint64_t le = ballot(line.before * H <= x && lane * line.per < a.c.n);
+        const uint32_t who = 63u - (uint32_t)__builtin_clzll(le);
+        uint32_t i = who * line.per, at = uniform((uint32_t)__builtin_amdgcn_readlane((int)line.before, (int)who)) * H;
+        bool dummy = false;
+        Seq sq = seq_of(a, i, dummy);
+        while (x - at >= sq.steps * H) {
+            at += sq.steps * H;
+            sq = seq_of(a, ++i, dummy);
+        }
+        i = uniform(i);
+        const uint32_t len = uniform(sq.len), steps = uniform(sq.steps);
+        const uint32_t y = x - at, kvh = y / steps, s0 = y % steps, s1 = min(steps, s0 + (end - x));
+        const uint32_t ctx_steps = steps - a.new_steps;
+        const int32_t slot = (int32_t)uniform((uint32_t)(a.c.seq ? a.c.seq[i] : (int32_t)i));
+        const int32_t* row = a.c.table + (uint64_t)(len > 0u ? (uint32_t)slot : 0u) * a.c.max_pages;
+        const unsigned char* kb = static_cast<const unsigned char*>(a.c.k) + (a.c.layer * a.c.layer_stride + kvh * a.c.head_stride) * (F8 ? 1u : 2u);
+        const unsigned char* vb = static_cast<const unsigned char*>(a.c.v) + (a.c.layer * a.c.layer_stride + kvh * a.c.head_stride) * (F8 ? 1u : 2u);
+
+        // ---- the wave's cached tiles: tile j starts at token first + 128 j ----
+        const uint32_t c1 = min(s1, ctx_steps), first = s0 * kStepKeys + w * kTileKeys;
+        const uint32_t past = min(c1 * kStepKeys, len);
+        const uint32_t nct = s0 < c1 && first < past ? (past - first + kStepKeys - 1u) / kStepKeys : 0u;
+        struct Tile {
+            int32_t p0, p1;   // the pages of its first and last 16 tokens
+        };
+        auto pages_of = [&](uint32_t j) -> Tile {
+            const uint32_t t0 = first + (j < nct ? j : 0u) * kStepKeys;
+            const uint32_t q0 = t0 >> a.c.page_shift, q1 = min((t0 + 16u) >> a.c.page_shift, a.c.max_pages - 1u);
+            if (nct == 0u) return Tile{0, 0};
+            return Tile{scalar_load(row + q0), scalar_load(row + q1)};
+        };
+        auto mask_of = [&](const Tile& t, uint32_t j) -> uint32_t {   // the tile's keys that are there
+            const uint32_t t0 = first + j * kStepKeys, left = len - t0;
+            uint32_t m = left >= 32u ? ~0u : (1u << left) - 1u;
+            if ((uint32_t)t.p0 >= a.c.pages) m &= 0xffff0000u;
+            if ((uint32_t)t.p1 >= a.c.pages) m &= 0x0000ffffu;
+            return m;
+        };
+        // A tile's 16-row halves lie in one page each; DMA load ii of a half covers rows RPI ii + lane /
+        // CPR, a chunk per lane. A half's buffer ends with its last row that is there.
+        constexpr uint32_t CPR = kRowB / 16u, RPI = 64u / CPR;
+        constexpr int kHalf = kNI / 2;
+        const uint32_t tsb = (uint32_t)ts;
+        auto offset_of = [&](bool values, uint32_t r) -> uint32_t {   // the lane's chunk of row r
+            const uint32_t ch = (lane % CPR) ^ (values ? swz_v<kRowB, F8>(r) : swz_k<kRowB>(r));
+            return 16u * ch < D * (F8 ? 1u : 2u) ? (r & 15u) * tsb + 16u * ch : kNoByte;
+        };
+        uint32_t vo_k[kHalf], vo_v[F8 ? kNI : kHalf];   // (8-bit values: the second half is permuted by other bits)
+#pragma unroll
+        for (int ii = 0; ii < kHalf; ++ii) vo_k[ii] = offset_of(false, RPI * (uint32_t)ii + lane / CPR);
+#pragma unroll
+        for (int ii = 0; ii < (F8 ? kNI : kHalf); ++ii) vo_v[ii] = offset_of(true, RPI * (uint32_t)ii + lane / CPR);
+        auto issue_rows = [&](bool values, const Tile& t, uint32_t j, unsigned char* dst) {
+            const uint32_t t0 = first + j * kStepKeys, m = mask_of(t, j);
+            const unsigned char* base = values ? vb : kb;
+            const uint64_t ps = a.c.page_stride * (F8 ? 1u : 2u);
+#pragma unroll
+            for (uint32_t h = 0; h < 2; ++h) {
+                const uint32_t there = m >> (16u * h) & 0xffffu, page = there ? (uint32_t)(h ? t.p1 : t.p0) : 0u;
+                const __amdgpu_buffer_rsrc_t rs = buffer_of(base + page * ps + ((t0 + 16u * h) & (a.c.page_tokens - 1u)) * ts,
+                                                            (uint32_t)__builtin_popcount(there) * tsb);
+#pragma unroll
+                for (int ii = 0; ii < kHalf; ++ii)
+                    dma16(rs, dst + 1024 * (kHalf * h + ii), values ? vo_v[F8 ? kHalf * h + ii : ii] : vo_k[ii]);
+            }
+        };
+        auto issue_k = [&](const Tile& t, uint32_t j) {
+            unsigned char* dst = mine + j % ST * kStage;
+            if constexpr (F8) {   // the keys' scales by the lower half, the values' by the upper
+                const uint32_t r = lane & 31u, tok = (first + j * kStepKeys + r) & (a.c.page_tokens - 1u);
+                const uint32_t m = mask_of(t, j), pg = (uint32_t)(r < 16u ? t.p0 : t.p1);
+                const float* s = lane < 32u ? a.c.k_scale : a.c.v_scale;
+                const uint64_t e = ((((uint64_t)a.c.layer * a.c.pages + pg) * H + kvh) << a.c.page_shift) + tok;
+                dma4(m >> r & 1u ? static_cast<const void*>(s + e) : a.zeros, dst + 2u * kTileKeys * kRowB);
+            }
+            issue_rows(false, t, j, dst);
+        };
+        auto issue_v = [&](const Tile& t, uint32_t j) { issue_rows(true, t, j, mine + j % ST * kStage + kTileKeys * kRowB); };
+
+        Tile tile[ST + 1];   // of tiles j, j + 1, .. j + ST
+#pragma unroll
+        for (int k = 0; k <= ST; ++k) tile[k] = pages_of((uint32_t)k);
+        // ---- the rows: packed as (new token, query head of the group) ----
+        bf16x8 qf[MT][kKS];
+        uint32_t node[MT];
+        bool live[MT];
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+            const uint32_t pr = rt * kRows + 16u * m + n;
+            live[m] = pr < R;
+            node[m] = live[m] ? pr / a.group : 0u;
+            const uint16_t* q = a.q + ((uint64_t)i * N + node[m]) * a.q_stride + (kvh * a.group + (live[m] ? pr % a.group : 0u)) * D;
+#pragma unroll
+            for (uint32_t ks = 0; ks < kKS; ++ks) {
+                const uint32_t c = chunk8(ks);
+                u32x4 v = {0u, 0u, 0u, 0u};
+                if (live[m] && 8u * c < D && a.scale != 0.0f) v = *reinterpret_cast<const u32x4*>(q + 8u * c);
+                if (a.scale < 0.0f) v ^= 0x80008000u;
+                qf[m][ks] = __builtin_bit_cast(bf16x8, v);
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < ST; ++k) {
+            if ((uint32_t)k < nct) {
+                issue_k(tile[k], (uint32_t)k);
+                issue_v(tile[k], (uint32_t)k);
+            }
+        }
+
+        f32x4 acc[MT][kDT];
+        float top[MT], sum[MT];
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+            top[m] = kUnset;
+            sum[m] = 0.0f;
+#pragma unroll
+            for (uint32_t t = 0; t < kDT; ++t) acc[m][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+
+        // Scores of a tile to weights, packed as the second product's operand.
+        f32x4 s[MT][2];
+        bf16x8 pf[MT];
+        auto hide = [&](int m, uint32_t see) {   // bit k of see: the lane's row m sees key k
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) s[m][h][r] = see >> (16u * h + 4u * g + r) & 1u ? s[m][h][r] : -__builtin_huge_valf();
+        };
+        auto weigh = [&](const f32x4 (&vs)[2], bool scaled) {
+            float big[MT];
+            bool up = false;
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+                big[m] = -__builtin_huge_valf();
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) big[m] = f_max(big[m], s[m][h][r]);
+                up = up || big[m] * sc > top[m] + kSlack;
+            }
+            if (ballot(up) != 0ull) {   // (uniform)
+#pragma unroll
+                for (int m = 0; m < MT; ++m) {
+                    const float now = f_max(top[m], across(big[m], f_max) * sc), f = exp2_f(top[m] - now);
+                    top[m] = now;
+                    sum[m] *= f;
+#pragma unroll
+                    for (uint32_t t = 0; t < kDT; ++t) acc[m][t] *= f;
+                }
+            }
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+                u32x4 p;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        s[m][h][r] = exp2_f(__builtin_fmaf(s[m][h][r], sc, -top[m]));
+                        sum[m] += s[m][h][r];
+                        if (scaled) s[m][h][r] *= vs[h][r];
                     }
-                    for (uint32_t d = 0; d < D; ++d)
-                        s += qs[d] * (F8 ? e4m3_f(static_cast<const uint8_t*>(a.c.k)[e + d]) : bf16_f(static_cast<const uint16_t*>(a.c.k)[e + d]));
-                    s *= ks;
+                    p[2 * h] = pack_bf16(s[m][h][0], s[m][h][1]);
+                    p[2 * h + 1] = pack_bf16(s[m][h][2], s[m][h][3]);
+                }
+                pf[m] = __builtin_bit_cast(bf16x8, p);
+            }
+        };
+        const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+        // where the lane's transposing reads of dim tile t begin (the permutation repeats after kTr tiles)
+        constexpr uint32_t kTr = F8 ? (kDT < 8u || DP == 256 ? kDT : 8u) : (kDT < 8u ? kDT : 8u);
+        uint32_t tr_at[kTr];
+#pragma unroll
+        for (uint32_t t = 0; t < kTr; ++t) {
+            const uint32_t q = n >> 1, r = !F8 ? 4u * g + (n >> 2) : q < 4u ? 4u * g + q : 12u + 4u * g + q;
+            const uint32_t c = F8 ? t : 2u * t + (lane >> 1 & 1u);
+            tr_at[t] = r * kRowB + (c ^ swz_v<kRowB, F8>(r)) * 16u + 8u * (lane & 1u);
+        }
+
+        for (uint32_t j = 0; j < nct; ++j) {
+            unsigned char* const at_k = mine + j % ST * kStage;
+            unsigned char* const at_v = at_k + kTileKeys * kRowB;
+            const bool full = j + ST <= nct;   // (ST tiles are under way)
+            if (full) wait_vm<kNI + (ST - 1) * (kNK + kNI)>();
+            else wait_vm<kNI>();
+            u32x4 kc[2][F8 ? kKS / 2 : kKS];
+            f32x4 ks[2] = {zero, zero}, vs[2] = {zero, zero};
+#pragma unroll
+            for (uint32_t h = 0; h < 2; ++h) {
+                const uint32_t r = 16u * h + n;
+#pragma unroll
+                for (uint32_t c = 0; c < (F8 ? kKS / 2 : kKS); ++c)
+                    kc[h][c] = *reinterpret_cast<const u32x4*>(at_k + r * kRowB + ((4u * c + g) ^ swz_k<kRowB>(r)) * 16u);
+                if constexpr (F8) {
+                    ks[h] = *reinterpret_cast<const f32x4*>(at_k + 2u * kTileKeys * kRowB + 64u * h + 16u * g);
+                    vs[h] = *reinterpret_cast<const f32x4*>(at_k + 2u * kTileKeys * kRowB + 128u + 64u * h + 16u * g);
                 }
             }
-        } else if (t < R) {
-            see = a.mask ? a.mask[(uint64_t)r * a.mask_words + (uint32_t)t / 32u] >> (t % 32) & 1u : t <= j;
-            if (see) {
-                const uint64_t n = (uint64_t)i * R + (uint32_t)t;
-                e = n * a.v_stride + kvh * D;
-                for (uint32_t d = 0; d < D; ++d) s += qs[d] * bf16_f(a.k[n * a.k_stride + kvh * D + d]);
+            wait_lds();
+            const bool more = j + ST < nct;
+            if (more) issue_k(tile[ST], j + ST);
+#pragma unroll
+            for (int m = 0; m < MT; ++m) s[m][0] = s[m][1] = zero;
+#pragma unroll
+            for (uint32_t h = 0; h < 2; ++h)
+#pragma unroll
+                for (uint32_t k = 0; k < kKS; ++k) {
+                    bf16x8 kf;
+                    if constexpr (F8) {
+                        union { bf16x2 p[4]; bf16x8 v; } u;
+#pragma unroll
+                        for (int d = 0; d < 2; ++d) {
+                            u.p[2 * d] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(kc[h][k / 2][2 * (k & 1) + d], 1.0f, false);
+                            u.p[2 * d + 1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(kc[h][k / 2][2 * (k & 1) + d], 1.0f, true);
+                        }
+                        kf = u.v;
+                    } else {
+                        kf = __builtin_bit_cast(bf16x8, kc[h][k]);
+                    }
+#pragma unroll
+                    for (int m = 0; m < MT; ++m) s[m][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[m][k], s[m][h], 0, 0, 0);
+                }
+            if constexpr (F8) {
+#pragma unroll
+                for (int m = 0; m < MT; ++m)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) s[m][h] *= ks[h];
+            }
+            const uint32_t there = mask_of(tile[0], j);
+            if (there != ~0u) {   // (uniform)
+#pragma unroll
+                for (int m = 0; m < MT; ++m) hide(m, there);
+                const uint32_t left = len - (first + j * kStepKeys);
+                if (there != (left >= 32u ? ~0u : (1u << left) - 1u) && lane == 0u) atomicOr(a.c.status, kStatusPages);   // (a page is missing)
+            }
+            weigh(vs, F8);
+            if (!full) wait_vm<0>();
+            else if (more) wait_vm<(ST - 1) * (kNK + kNI) + kNK>();
+            else wait_vm<(ST - 1) * (kNK + kNI)>();
+            const uint32_t lv = lds_at(at_v);
+            using Raw = std::conditional_t<F8, u32x2, u32x4>;
+            Raw vc[kDT];
+#pragma unroll
+            for (uint32_t t = 0; t < kDT; t += 4u) {
+                uint32_t ad[4];
+                Raw o[4];
+#pragma unroll
+                for (uint32_t k = 0; k < 4; ++k) ad[k] = lv + tr_at[(t + k) % kTr] + (t + k) / kTr * (kTr * (F8 ? 16u : 32u));
+                if constexpr (F8) read_tr8(ad, o);
+                else read_tr16<16 * kRowB>(ad, o);
+#pragma unroll
+                for (uint32_t k = 0; k < 4; ++k) vc[t + k] = o[k];
+            }
+            if (more) issue_v(tile[ST], j + ST);
+#pragma unroll
+            for (int k = 0; k < ST; ++k) tile[k] = tile[k + 1];
+            tile[ST] = pages_of(j + 1u + ST);
+#pragma unroll
+            for (uint32_t t = 0; t < kDT; ++t) {
+                bf16x8 vf;
+                if constexpr (F8) {
+                    union { bf16x2 p[4]; bf16x8 v; } u;
+#pragma unroll
+                    for (int d = 0; d < 2; ++d) {
+                        u.p[2 * d] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(vc[t][d], 1.0f, false);
+                        u.p[2 * d + 1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(vc[t][d], 1.0f, true);
+                    }
+                    vf = u.v;
+                } else {
+                    vf = __builtin_bit_cast(bf16x8, vc[t]);
+                }
+#pragma unroll
+                for (int m = 0; m < MT; ++m) acc[m][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[m], acc[m][t], 0, 0, 0);
             }
         }
-        s = see ? s * a.scale : -__builtin_huge_valf();
-        const float top = fmaxf(m, wave_max(s));
-        const float base = top == -__builtin_huge_valf() ? 0.0f : top;
-        const float p = see ? expf(s - base) : 0.0f;
-        const float keep = expf(m - base);
-        m = top;
-        z = z * keep + wave_sum_f(p);
-        ps[lane] = p * vs;
-        at[lane] = e;
-        const uint64_t seen = ballot(see);
-        __syncthreads();
+
+        // ---- the new tokens' tiles (bf16 always) ----
+        for (uint32_t st = max(s0, ctx_steps); st < s1; ++st) {
+            const uint32_t n0 = (st - ctx_steps) * kStepKeys + w * kTileKeys;
+            if (n0 >= N) continue;   // (uniform)
+            constexpr uint32_t CPR = kNewB / 16u, RPI = 64u / CPR;   // (as above, of the new rows)
+            constexpr int NI = (int)(kTileKeys * kNewB / 1024u);
+            const uint32_t lr = lane / CPR, pl = lane % CPR;
+            unsigned char* const at_v = mine + kTileKeys * kNewB;
+            wait_lds();   // (the last tile's reads)
+            const uint64_t rw = (uint64_t)i * N + n0;
+            const uint32_t rows = min(N - n0, kTileKeys), kst = (uint32_t)a.k_stride * 2u, vst = (uint32_t)a.v_stride * 2u;
+            const __amdgpu_buffer_rsrc_t krs = buffer_of(reinterpret_cast<const unsigned char*>(a.k + rw * a.k_stride + kvh * D), (rows - 1u) * kst + 2u * D);
+            const __amdgpu_buffer_rsrc_t vrs = buffer_of(reinterpret_cast<const unsigned char*>(a.v + rw * a.v_stride + kvh * D), (rows - 1u) * vst + 2u * D);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) o[c] *= keep;
-        for (uint64_t w = seen; w; w &= w - 1u) {
-            const uint32_t x = (uint32_t)__builtin_ctzll(w);
+            for (int ii = 0; ii < NI; ++ii) {
+                const uint32_t r = RPI * (uint32_t)ii + lr, ck = pl ^ swz_k<kNewB>(r), cv = pl ^ swz_v<kNewB, false>(r);
+                dma16(krs, mine + 1024 * ii, r < rows && 8u * ck < D ? r * kst + 16u * ck : kNoByte);
+                dma16(vrs, at_v + 1024 * ii, r < rows && 8u * cv < D ? r * vst + 16u * cv : kNoByte);
+            }
+            uint32_t see[MT];
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                const uint32_t d = lane + c * kWave;
-                if (d < D) {
-                    const float v = fresh ? bf16_f(a.v[at[x] + d])
-                                    : F8  ? e4m3_f(static_cast<const uint8_t*>(a.c.v)[at[x] + d])
-                                          : bf16_f(static_cast<const uint16_t*>(a.c.v)[at[x] + d]);
-                    o[c] += ps[x] * v;
+            for (int m = 0; m < MT; ++m) {
+                if (a.mask) see[m] = live[m] ? a.mask[((uint64_t)i * N + node[m]) * a.mask_words + n0 / 32u] : 0u;
+                else see[m] = !live[m] || node[m] < n0 ? 0u : node[m] - n0 >= 31u ? ~0u : (2u << (node[m] - n0)) - 1u;
+                if (N - n0 < 32u) see[m] &= (1u << (N - n0)) - 1u;
+            }
+            wait_vm<0>();
+#pragma unroll
+            for (int m = 0; m < MT; ++m) s[m][0] = s[m][1] = zero;
+#pragma unroll
+            for (uint32_t h = 0; h < 2; ++h)
+#pragma unroll
+                for (uint32_t k = 0; k < kKS; ++k) {
+                    const uint32_t r = 16u * h + n;
+                    const bf16x8 kf = *reinterpret_cast<const bf16x8*>(mine + r * kNewB + (chunk8(k) ^ swz_k<kNewB>(r)) * 16u);
+#pragma unroll
+                    for (int m = 0; m < MT; ++m) s[m][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[m][k], s[m][h], 0, 0, 0);
+                }
+#pragma unroll
+            for (int m = 0; m < MT; ++m) hide(m, see[m]);
+            const f32x4 none[2] = {zero, zero};
+            weigh(none, false);
+            bool wild = false;
+#pragma unroll
+            for (uint32_t t = 0; t < kDT; ++t) {
+                uint32_t r = 4u * g + (n >> 2);
+                const uint32_t c = 2u * t + (lane >> 1 & 1u);
+                union { s16x4 p[2]; uint32_t w[4]; bf16x8 v; } u;
+                u.p[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                    (LCS_LDS s16x4*)(at_v + r * kNewB + (c ^ swz_v<kNewB, false>(r)) * 16u + 8u * (lane & 1u)));
+                r += 16u;
+                u.p[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                    (LCS_LDS s16x4*)(at_v + r * kNewB + (c ^ swz_v<kNewB, false>(r)) * 16u + 8u * (lane & 1u)));
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {   // (infinities and NaNs are added below)
+                    if (wild_bf16x2(u.w[k])) {
+                        wild = true;
+                        u.w[k] &= ((u.w[k] & 0x7f80u) == 0x7f80u ? 0u : 0xffffu) | ((u.w[k] & 0x7f800000u) == 0x7f800000u ? 0u : 0xffff0000u);
+                    }
+                }
+#pragma unroll
+                for (int m = 0; m < MT; ++m) acc[m][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(u.v, pf[m], acc[m][t], 0, 0, 0);
+            }
+            if (ballot(wild) != 0ull) {   // (uniform; the weights by way of the keys' place)
+                float* const wt = reinterpret_cast<float*>(mine);
+#pragma unroll
+                for (int m = 0; m < MT; ++m) {
+                    wait_lds();
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) wt[(16u * h + 4u * g + r) * 16u + n] = s[m][h][r];
+                    wait_lds();
+#pragma unroll 1
+                    for (uint32_t key = 0; key < kTileKeys; ++key) {
+                        const float p = wt[key * 16u + n];
+                        const bool seen = see[m] >> key & 1u;
+#pragma unroll
+                        for (uint32_t t = 0; t < kDT; ++t) {
+                            const uint32_t c = 2u * t + (g >> 1);
+                            const u32x2 q = *reinterpret_cast<const u32x2*>(at_v + key * kNewB + (c ^ swz_v<kNewB, false>(key)) * 16u + 8u * (g & 1u));
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) {
+                                const uint32_t e = r % 2 ? q[r / 2] & 0xffff0000u : q[r / 2] << 16;
+                                if (seen && (e & 0x7f800000u) == 0x7f800000u) acc[m][t][r] += p * __uint_as_float(e);
+                            }
+                        }
+                    }
                 }
             }
         }
-        __syncthreads();
-    }
-    const bool none = m == -__builtin_huge_valf() && z == 0.0f;
+
+        // ---- the waves' sums joined ----
+        wait_lds();
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-        const uint32_t d = lane + c * kWave;
-        if (d < D) a.o[r * a.o_stride + h * D + d] = (uint16_t)f_bf16(none ? 0.0f : o[c] / z);
+        for (int m = 0; m < MT; ++m) {
+            const float z = across(sum[m], [](float p, float q) { return p + q; });
+            if (g == 0u) {
+                stat[w][0][16u * m + n] = top[m];
+                stat[w][1][16u * m + n] = z;
+            }
+#pragma unroll
+            for (uint32_t t = 0; t < kDT; ++t)
+                *reinterpret_cast<f32x4*>(mine + (16u * m + n) * DP * 4u + ((4u * t + g) ^ n) * 16u) = acc[m][t];
+        }
+        __syncthreads();
+        const bool complete = s0 == 0u && s1 == steps;
+        // (a workgroup has at most two incomplete segments: one that begins with the piece, one that ends with it)
+        float* part = a.part + ((uint64_t)b * 2u + (x == piece * share ? 0u : 1u)) * Part<DP, MT>::kFloats;
+        for (uint32_t it = tid_x(); it < kRows * (DP / 4u); it += kTreeWaves * kWave) {
+            const uint32_t rr = it / (DP / 4u), c = it % (DP / 4u), pr = rt * kRows + rr;
+            float M = stat[0][0][rr];
+#pragma unroll
+            for (int k = 1; k < kTreeWaves; ++k) M = f_max(M, stat[k][0][rr]);
+            f32x4 o = zero;
+            float z = 0.0f;
+#pragma unroll
+            for (int k = 0; k < kTreeWaves; ++k) {
+                const float f = exp2_f(stat[k][0][rr] - M);
+                z += stat[k][1][rr] * f;
+                o += *reinterpret_cast<const f32x4*>(lds + (uint32_t)k * kRegion + rr * DP * 4u + (c ^ (rr & 15u)) * 16u) * f;
+            }
+            if (!complete) {
+                *reinterpret_cast<f32x4*>(part + rr * DP + 4u * c) = o;
+                if (c == 0u) {
+                    part[kRows * DP + rr] = M;
+                    part[kRows * DP + kRows + rr] = z;
+                }
+            } else if (pr < R && 4u * c < D) {
+                const bool empty = z == 0.0f;
+                const float f = 1.0f / z;
+                const uint64_t rw = (uint64_t)i * N + pr / a.group;
+                const uint32_t h = kvh * a.group + pr % a.group;
+                *reinterpret_cast<u32x2*>(a.o + rw * a.o_stride + h * D + 4u * c) =
+                    empty ? u32x2{0u, 0u} : u32x2{pack_bf16(o[0] * f, o[1] * f), pack_bf16(o[2] * f, o[3] * f)};
+                if (c == 0u && a.lse) a.lse[rw * a.heads + h] = empty ? -__builtin_huge_valf() : (M + __builtin_amdgcn_logf(z)) * kLn2;
+            }
+        }
+        __syncthreads();
+        x += s1 - s0;
     }
-    if (lane == 0 && a.lse) a.lse[(uint64_t)r * a.heads + h] = none ? -__builtin_huge_valf() : m + logf(z);
-    if (bad) atomicOr(a.c.status, kStatusPages);
 }
 
-hipError_t launch_tree_attn(const TreeArgs& a, hipStream_t st) {
-    const dim3 grid(a.c.n * a.rows_per_seq * a.heads);
-    if (a.c.f8) hipLaunchKernelGGL(tree_attn<true>, grid, dim3(kWave), 0, st, a);
-    else hipLaunchKernelGGL(tree_attn<false>, grid, dim3(kWave), 0, st, a);
-    return hipGetLastError();
+// Joins the partial sums of the pairs that several workgroups share: 256 threads take
+// 1024 / DP rows of a row tile, four elements each.
+template <int DP, int MT>
+__global__ __launch_bounds__(256) void tree_join(TreeArgs a) {
+    using P = Part<DP, MT>;
+    constexpr uint32_t kPer = 1024u / DP, kBlocks = P::kRows / kPer;
+    const uint32_t i = wg_x() / a.c.kv_heads, kvh = wg_x() % a.c.kv_heads;
+    const uint32_t rt = __builtin_amdgcn_workgroup_id_y() / kBlocks, rr = __builtin_amdgcn_workgroup_id_y() % kBlocks * kPer + tid_x() / (DP / 4u);
+    const uint32_t c = tid_x() % (DP / 4u), pr = (rt + a.row_tile0) * P::kRows + rr;
+    const Line line = line_of(a);
+    const uint32_t H = a.c.kv_heads, all = line.total * H, share = share_of(a, all);
+    const uint32_t who = i / line.per;
+    uint32_t at = uniform((uint32_t)__builtin_amdgcn_readlane((int)line.before, (int)who)) * H;
+    bool dummy = false;
+    for (uint32_t k = who * line.per; k < i; ++k) at += seq_of(a, k, dummy).steps * H;
+    const uint32_t steps = seq_of(a, i, dummy).steps;
+    at += kvh * steps;
+    const uint32_t p0 = at / share, p1 = (at + steps - 1u) / share;
+    if (p0 == p1 || pr >= a.rows_per_seq * a.group) return;
+    float M = kUnset, z = 0.0f;
+    f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (uint32_t p = p0; p <= p1; ++p) {
+        const uint32_t b = (p / 8u * a.row_tiles + rt) * 8u + p % 8u;
+        const float* part = a.part + ((uint64_t)b * 2u + (p * share >= at ? 0u : 1u)) * P::kFloats;
+        const float m = part[P::kRows * DP + rr], s = part[P::kRows * DP + P::kRows + rr];
+        const f32x4 v = *reinterpret_cast<const f32x4*>(part + rr * DP + 4u * c);
+        const float now = f_max(M, m), fo = exp2_f(M - now), fn = exp2_f(m - now);
+        M = now;
+        z = z * fo + s * fn;
+        o = o * fo + v * fn;
+    }
+    const uint32_t D = a.c.head_dim, h = kvh * a.group + pr % a.group;
+    if (4u * c >= D) return;
+    const bool empty = z == 0.0f;
+    const float f = 1.0f / z;
+    const uint64_t rw = (uint64_t)i * a.rows_per_seq + pr / a.group;
+    *reinterpret_cast<u32x2*>(a.o + rw * a.o_stride + h * D + 4u * c) =
+        empty ? u32x2{0u, 0u} : u32x2{pack_bf16(o[0] * f, o[1] * f), pack_bf16(o[2] * f, o[3] * f)};
+    if (c == 0u && a.lse) a.lse[rw * a.heads + h] = empty ? -__builtin_huge_valf() : (M + __builtin_amdgcn_logf(z)) * kLn2;
+}
+
+namespace {
+
+constexpr uint32_t kTreeTiles = 32;   // row tiles of a launch
+
+template <int DP, int MT, bool F8, int ST>
+hipError_t launch(TreeArgs a, uint32_t cus, hipStream_t st) {
+    constexpr uint32_t per_cu = DP == 256 || (MT == 4 && DP == 128) ? 1u : 2u;
+    const uint32_t rows = a.rows_per_seq * a.group, tiles = (rows + 16u * MT - 1u) / (16u * MT);
+    for (uint32_t t0 = 0; t0 < tiles; t0 += kTreeTiles) {
+        a.row_tile0 = t0;
+        a.row_tiles = tiles - t0 < kTreeTiles ? tiles - t0 : kTreeTiles;
+        const uint32_t most = per_cu * kTreeSlots / 2u, slots = cus * per_cu < most ? cus * per_cu : most;
+        a.pieces = slots / a.row_tiles / 8u * 8u;
+        if (a.pieces == 0u) a.pieces = 8u;
+        hipLaunchKernelGGL((tree_attn<DP, MT, F8, ST>), dim3(a.pieces * a.row_tiles), dim3(kTreeWaves * kWave), 0, st, a);
+        hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+        hipLaunchKernelGGL((tree_join<DP, MT>), dim3(a.c.n * a.c.kv_heads, a.row_tiles * (16u * MT * DP / 1024u)), dim3(256), 0, st, a);
+        if ((e = hipGetLastError()) != hipSuccess) return e;
+    }
+    return hipSuccess;
+}
+
+template <int DP, bool F8>
+hipError_t launch_rows(const TreeArgs& a, uint32_t cus, hipStream_t st) {
+    const uint32_t rows = a.rows_per_seq * a.group;
+    constexpr int ST = F8 || DP == 64 ? 2 : 1;
+    if (rows <= 16u) return launch<DP, 1, F8, ST>(a, cus, st);
+    if (rows <= 32u || DP == 256) return launch<DP, 2, F8, ST>(a, cus, st);
+    if constexpr (DP != 256) return launch<DP, 4, F8, DP == 128 && !F8 ? 2 : ST>(a, cus, st);
+    return hipErrorInvalidValue;
+}
+
+}  // namespace
+
+// Floats of a context's partial results: two results for every workgroup, the largest at two
+// workgroups a CU 64 rows of 64 (at one a CU 64 of 128 or 32 of 256, half as many).
+uint64_t tree_part_floats() { return 2ull * kTreeSlots * Part<64, 4>::kFloats; }
+static_assert(Part<32 * 4, 2>::kFloats <= Part<64, 4>::kFloats && Part<128, 4>::kFloats <= 2u * Part<64, 4>::kFloats &&
+              Part<256, 2>::kFloats <= 2u * Part<64, 4>::kFloats, "the partial results' room");
+
+hipError_t launch_tree_attn(const TreeArgs& args, uint32_t cus, hipStream_t st) {
+    TreeArgs a = args;
+    a.new_steps = (a.rows_per_seq + kStepKeys - 1u) / kStepKeys;
+    const uint32_t d = a.c.head_dim;
+    if (a.c.f8) return d <= 64 ? launch_rows<64, true>(a, cus, st) : d <= 128 ? launch_rows<128, true>(a, cus, st) : launch_rows<256, true>(a, cus, st);
+    return d <= 64 ? launch_rows<64, false>(a, cus, st) : d <= 128 ? launch_rows<128, false>(a, cus, st) : launch_rows<256, false>(a, cus, st);
 }
 
 }  // namespace lcs
