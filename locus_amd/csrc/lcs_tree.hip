@@ -30,7 +30,8 @@
 // What is not seen must not matter: cached rows past the length and in missing pages
 // are replaced by zeros on their way to LDS and have weight 0. Among the new tokens a
 // row that some see and others do not may hold infinities or NaNs: those elements
-// are taken out of the product and added one by one to the rows that see them.
+// are taken out of the product, counted for the rows that see them by another, and
+// added there.
 //
 // (This file is compiled with NaNs honoured: a NaN in a row has to stay one.)
 #include <hip/hip_runtime.h>
@@ -113,9 +114,6 @@ __device__ __forceinline__ float across(float x, F f) {
 __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {   // to nearest even
     return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){a, b}, bf16x2));
 }
-__device__ __forceinline__ bool wild_bf16x2(uint32_t w) {   // either half an infinity or a NaN
-    return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
-}
 
 // A tile's row is a power of two of 16-byte chunks in LDS; chunk c of row r lies at place c
 // ^ x(r), so that the reads of a half wave cover the 64 banks once. x picks bits of r.
@@ -171,6 +169,9 @@ __device__ __forceinline__ uint32_t share_of(const TreeArgs& a, uint32_t all) {
     return s > 1u ? s : 1u;
 }
 
+template <int DP>
+constexpr int kTreePerCu = DP == 256 ? 1 : 2;   // workgroups a CU
+
 // A partial result: the rows' unnormalised sums, then their maxima (log2) and sums of weights.
 template <int DP, int MT>
 struct Part {
@@ -181,7 +182,7 @@ struct Part {
 }  // namespace
 
 template <int DP, int MT, bool F8, int ST>
-__global__ __launch_bounds__(kTreeWaves * kWave, DP == 256 || (MT == 4 && DP == 128) ? 1 : 2) void tree_attn(TreeArgs a) {
+__global__ __launch_bounds__(kTreeWaves * kWave, kTreePerCu<DP>) void tree_attn(TreeArgs a) {
     constexpr uint32_t kRows = 16u * MT, kDT = DP / 16, kKS = DP / 32;
     constexpr uint32_t kRowB = DP * (F8 ? 1 : 2), kNewB = DP * 2;                 // bytes of a cached row and of a new one in LDS
     constexpr uint32_t kScaleB = F8 ? 256u : 0u;
@@ -276,8 +277,8 @@ __global__ __launch_bounds__(kTreeWaves * kWave, DP == 256 || (MT == 4 && DP == 
                     dma16(rs, dst + 1024 * (kHalf * h + ii), values ? vo_v[F8 ? kHalf * h + ii : ii] : vo_k[ii]);
             }
         };
-        auto issue_k = [&](const Tile& t, uint32_t j) {
-            unsigned char* dst = mine + j % ST * kStage;
+        auto issue_k = [&](const Tile& t, uint32_t j, uint32_t stage) {
+            unsigned char* dst = mine + stage;
             if constexpr (F8) {   // the keys' scales by the lower half, the values' by the upper
                 const uint32_t r = lane & 31u, tok = (first + j * kStepKeys + r) & (a.c.page_tokens - 1u);
                 const uint32_t m = mask_of(t, j), pg = (uint32_t)(r < 16u ? t.p0 : t.p1);
@@ -287,7 +288,7 @@ __global__ __launch_bounds__(kTreeWaves * kWave, DP == 256 || (MT == 4 && DP == 
             }
             issue_rows(false, t, j, dst);
         };
-        auto issue_v = [&](const Tile& t, uint32_t j) { issue_rows(true, t, j, mine + j % ST * kStage + kTileKeys * kRowB); };
+        auto issue_v = [&](const Tile& t, uint32_t j, uint32_t stage) { issue_rows(true, t, j, mine + stage + kTileKeys * kRowB); };
 
         Tile tile[ST + 1];   // of tiles j, j + 1, .. j + ST
 #pragma unroll
@@ -314,8 +315,8 @@ __global__ __launch_bounds__(kTreeWaves * kWave, DP == 256 || (MT == 4 && DP == 
 #pragma unroll
         for (int k = 0; k < ST; ++k) {
             if ((uint32_t)k < nct) {
-                issue_k(tile[k], (uint32_t)k);
-                issue_v(tile[k], (uint32_t)k);
+                issue_k(tile[k], (uint32_t)k, (uint32_t)k * kStage);
+                issue_v(tile[k], (uint32_t)k, (uint32_t)k * kStage);
             }
         }
 
@@ -388,8 +389,10 @@ __global__ __launch_bounds__(kTreeWaves * kWave, DP == 256 || (MT == 4 && DP == 
             tr_at[t] = r * kRowB + (c ^ swz_v<kRowB, F8>(r)) * 16u + 8u * (lane & 1u);
         }
 
+        uint32_t stage = 0;
+#pragma clang loop unroll(disable)
         for (uint32_t j = 0; j < nct; ++j) {
-            unsigned char* const at_k = mine + j % ST * kStage;
+            unsigned char* const at_k = mine + stage;
             unsigned char* const at_v = at_k + kTileKeys * kRowB;
             const bool full = j + ST <= nct;   // (ST tiles are under way)
             if (full) wait_vm<kNI + (ST - 1) * (kNK + kNI)>();
@@ -409,7 +412,7 @@ __global__ __launch_bounds__(kTreeWaves * kWave, DP == 256 || (MT == 4 && DP == 
             }
             wait_lds();
             const bool more = j + ST < nct;
-            if (more) issue_k(tile[ST], j + ST);
+            if (more) issue_k(tile[ST], j + ST, stage);
 #pragma unroll
             for (int m = 0; m < MT; ++m) s[m][0] = s[m][1] = zero;
 #pragma unroll
@@ -462,7 +465,8 @@ __global__ __launch_bounds__(kTreeWaves * kWave, DP == 256 || (MT == 4 && DP == 
 #pragma unroll
                 for (uint32_t k = 0; k < 4; ++k) vc[t + k] = o[k];
             }
-            if (more) issue_v(tile[ST], j + ST);
+            if (more) issue_v(tile[ST], j + ST, stage);
+            stage = stage + kStage == ST * kStage ? 0u : stage + kStage;
 #pragma unroll
             for (int k = 0; k < ST; ++k) tile[k] = tile[k + 1];
             tile[ST] = pages_of(j + 1u + ST);
@@ -491,7 +495,9 @@ __global__ __launch_bounds__(kTreeWaves * kWave, DP == 256 || (MT == 4 && DP == 
             if (n0 >= N) continue;   // (uniform)
             constexpr uint32_t CPR = kNewB / 16u, RPI = 64u / CPR;   // (as above, of the new rows)
             constexpr int NI = (int)(kTileKeys * kNewB / 1024u);
-            const uint32_t lr = lane / CPR, pl = lane % CPR;
+            uint32_t ln = lane;   // (opaque: what follows from it is not kept over the cached tiles)
+            asm volatile("" : "+v"(ln));
+            const uint32_t lr = ln / CPR, pl = ln % CPR, lane_n = ln & 15u, lg = ln >> 4;
             unsigned char* const at_v = mine + kTileKeys * kNewB;
             wait_lds();   // (the last tile's reads)
             const uint64_t rw = (uint64_t)i * N + n0;
@@ -518,8 +524,8 @@ __global__ __launch_bounds__(kTreeWaves * kWave, DP == 256 || (MT == 4 && DP == 
             for (uint32_t h = 0; h < 2; ++h)
 #pragma unroll
                 for (uint32_t k = 0; k < kKS; ++k) {
-                    const uint32_t r = 16u * h + n;
-                    const bf16x8 kf = *reinterpret_cast<const bf16x8*>(mine + r * kNewB + (chunk8(k) ^ swz_k<kNewB>(r)) * 16u);
+                    const uint32_t r = 16u * h + lane_n, c = F8 ? 2u * (lg + 4u * (k / 2u)) + (k & 1u) : 4u * k + lg;
+                    const bf16x8 kf = *reinterpret_cast<const bf16x8*>(mine + r * kNewB + (c ^ swz_k<kNewB>(r)) * 16u);
 #pragma unroll
                     for (int m = 0; m < MT; ++m) s[m][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[m][k], s[m][h], 0, 0, 0);
                 }
@@ -527,52 +533,85 @@ __global__ __launch_bounds__(kTreeWaves * kWave, DP == 256 || (MT == 4 && DP == 
             for (int m = 0; m < MT; ++m) hide(m, see[m]);
             const f32x4 none[2] = {zero, zero};
             weigh(none, false);
+            // Infinities and NaNs are kept out of the product, where a weight of 0 would not keep them
+            // from the rows that do not see them: they are replaced by 0 in LDS, and what they were noted
+            // in the keys' place (+inf 1, -inf 2, a NaN both).
             bool wild = false;
+#pragma unroll 1
+            for (int ii = 0; ii < NI; ++ii) {
+                const u32x4 v = *reinterpret_cast<const u32x4*>(at_v + 1024 * ii + 16u * ln);
 #pragma unroll
-            for (uint32_t t = 0; t < kDT; ++t) {
-                uint32_t r = 4u * g + (n >> 2);
-                const uint32_t c = 2u * t + (lane >> 1 & 1u);
-                union { s16x4 p[2]; uint32_t w[4]; bf16x8 v; } u;
-                u.p[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                    (LCS_LDS s16x4*)(at_v + r * kNewB + (c ^ swz_v<kNewB, false>(r)) * 16u + 8u * (lane & 1u)));
-                r += 16u;
-                u.p[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                    (LCS_LDS s16x4*)(at_v + r * kNewB + (c ^ swz_v<kNewB, false>(r)) * 16u + 8u * (lane & 1u)));
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {   // (infinities and NaNs are added below)
-                    if (wild_bf16x2(u.w[k])) {
-                        wild = true;
-                        u.w[k] &= ((u.w[k] & 0x7f80u) == 0x7f80u ? 0u : 0xffffu) | ((u.w[k] & 0x7f800000u) == 0x7f800000u ? 0u : 0xffff0000u);
-                    }
-                }
-#pragma unroll
-                for (int m = 0; m < MT; ++m) acc[m][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(u.v, pf[m], acc[m][t], 0, 0, 0);
+                for (int k = 0; k < 4; ++k) wild = wild || (v[k] & 0x7f80u) == 0x7f80u || (v[k] & 0x7f800000u) == 0x7f800000u;
             }
-            if (ballot(wild) != 0ull) {   // (uniform; the weights by way of the keys' place)
-                float* const wt = reinterpret_cast<float*>(mine);
+            const bool any_wild = ballot(wild) != 0ull;
+            if (any_wild) {
+                wait_lds();   // (the keys have been read)
+#pragma unroll 1
+                for (int ii = 0; ii < NI; ++ii) {
+                    u32x4* const pv = reinterpret_cast<u32x4*>(at_v + 1024 * ii + 16u * ln);
+                    u32x4 v = *pv, kind;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        auto kind_of = [](uint32_t e) -> uint32_t { return (e & 0x7f80u) != 0x7f80u ? 0u : e == 0x7f80u ? 1u : e == 0xff80u ? 2u : 3u; };
+                        const uint32_t lo = kind_of(v[k] & 0xffffu), hi = kind_of(v[k] >> 16);
+                        kind[k] = lo | hi << 16;
+                        v[k] &= (lo ? 0u : 0xffffu) | (hi ? 0u : 0xffff0000u);
+                    }
+                    *pv = v;
+                    *reinterpret_cast<u32x4*>(mine + 1024 * ii + 16u * ln) = kind;
+                }
+                wait_lds();
+            }
+            const uint32_t rv = 4u * lg + (lane_n >> 2), lv = lds_at(at_v) + rv * kNewB + 8u * (ln & 1u);
+            auto tr_of = [&](uint32_t t) -> uint32_t { return ((2u * t + (ln >> 1 & 1u)) ^ swz_v<kNewB, false>(rv)) * 16u; };
+#pragma unroll
+            for (uint32_t t0 = 0; t0 < kDT; t0 += 4u) {
+                uint32_t ad[4];
+                u32x4 v[4];
+#pragma unroll
+                for (uint32_t t = 0; t < 4u; ++t) ad[t] = lv + tr_of(t0 + t);
+                read_tr16<16 * kNewB>(ad, v);
+#pragma unroll
+                for (uint32_t t = 0; t < 4u; ++t)
+#pragma unroll
+                    for (int m = 0; m < MT; ++m)
+                        acc[m][t0 + t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, v[t]), pf[m], acc[m][t0 + t], 0, 0, 0);
+            }
+            if (any_wild) {   // 2^127 times 2 for each that is seen: infinite sums, of both signs for a NaN
+                const uint32_t lk = lv - kTileKeys * kNewB;
+                bf16x8 two[MT];
 #pragma unroll
                 for (int m = 0; m < MT; ++m) {
-                    wait_lds();
+                    u32x4 w2;
 #pragma unroll
-                    for (int h = 0; h < 2; ++h)
+                    for (int k = 0; k < 4; ++k) {
+                        const uint32_t b2 = see[m] >> (16u * (k / 2) + 4u * lg + 2u * (k % 2));
+                        w2[k] = (b2 & 1u ? 0x4000u : 0u) | (b2 & 2u ? 0x40000000u : 0u);
+                    }
+                    two[m] = __builtin_bit_cast(bf16x8, w2);
+                }
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) wt[(16u * h + 4u * g + r) * 16u + n] = s[m][h][r];
-                    wait_lds();
-#pragma unroll 1
-                    for (uint32_t key = 0; key < kTileKeys; ++key) {
-                        const float p = wt[key * 16u + n];
-                        const bool seen = see[m] >> key & 1u;
+                for (uint32_t t0 = 0; t0 < kDT; t0 += 4u) {
+                    uint32_t ad[4];
+                    u32x4 v[4];
 #pragma unroll
-                        for (uint32_t t = 0; t < kDT; ++t) {
-                            const uint32_t c = 2u * t + (g >> 1);
-                            const u32x2 q = *reinterpret_cast<const u32x2*>(at_v + key * kNewB + (c ^ swz_v<kNewB, false>(key)) * 16u + 8u * (g & 1u));
+                    for (uint32_t t = 0; t < 4u; ++t) ad[t] = lk + tr_of(t0 + t);
+                    read_tr16<16 * kNewB>(ad, v);
 #pragma unroll
-                            for (int r = 0; r < 4; ++r) {
-                                const uint32_t e = r % 2 ? q[r / 2] & 0xffff0000u : q[r / 2] << 16;
-                                if (seen && (e & 0x7f800000u) == 0x7f800000u) acc[m][t][r] += p * __uint_as_float(e);
-                            }
+                    for (uint32_t t = 0; t < 4u; ++t) {
+                        u32x4 up, down;
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            up[k] = (v[t][k] & 0x10001u) * 0x7f00u;
+                            down[k] = (v[t][k] >> 1 & 0x10001u) * 0xff00u;
+                        }
+#pragma unroll
+                        for (int m = 0; m < MT; ++m) {
+                            acc[m][t0 + t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, up), two[m], acc[m][t0 + t], 0, 0, 0);
+                            acc[m][t0 + t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, down), two[m], acc[m][t0 + t], 0, 0, 0);
                         }
                     }
+                    __builtin_amdgcn_sched_barrier(0);
                 }
             }
         }
@@ -675,7 +714,7 @@ constexpr uint32_t kTreeTiles = 32;   // row tiles of a launch
 
 template <int DP, int MT, bool F8, int ST>
 hipError_t launch(TreeArgs a, uint32_t cus, hipStream_t st) {
-    constexpr uint32_t per_cu = DP == 256 || (MT == 4 && DP == 128) ? 1u : 2u;
+    constexpr uint32_t per_cu = kTreePerCu<DP>;
     const uint32_t rows = a.rows_per_seq * a.group, tiles = (rows + 16u * MT - 1u) / (16u * MT);
     for (uint32_t t0 = 0; t0 < tiles; t0 += kTreeTiles) {
         a.row_tile0 = t0;
@@ -692,23 +731,21 @@ hipError_t launch(TreeArgs a, uint32_t cus, hipStream_t st) {
     return hipSuccess;
 }
 
+// Rows of a tile: 16, or 32 where there are more. (64 of them leave one wave a SIMD and
+// its products wait for its softmax: 64 rows a head, 32 sequences x 4096 tokens x 8 heads
+// 110 us in tiles of 32, 111 in tiles of 64; 256 rows 276 / 294.)
 template <int DP, bool F8>
 hipError_t launch_rows(const TreeArgs& a, uint32_t cus, hipStream_t st) {
-    const uint32_t rows = a.rows_per_seq * a.group;
     constexpr int ST = F8 || DP == 64 ? 2 : 1;
-    if (rows <= 16u) return launch<DP, 1, F8, ST>(a, cus, st);
-    if (rows <= 32u || DP == 256) return launch<DP, 2, F8, ST>(a, cus, st);
-    if constexpr (DP != 256) return launch<DP, 4, F8, DP == 128 && !F8 ? 2 : ST>(a, cus, st);
-    return hipErrorInvalidValue;
+    return a.rows_per_seq * a.group <= 16u ? launch<DP, 1, F8, ST>(a, cus, st) : launch<DP, 2, F8, ST>(a, cus, st);
 }
 
 }  // namespace
 
-// Floats of a context's partial results: two results for every workgroup, the largest at two
-// workgroups a CU 64 rows of 64 (at one a CU 64 of 128 or 32 of 256, half as many).
-uint64_t tree_part_floats() { return 2ull * kTreeSlots * Part<64, 4>::kFloats; }
-static_assert(Part<32 * 4, 2>::kFloats <= Part<64, 4>::kFloats && Part<128, 4>::kFloats <= 2u * Part<64, 4>::kFloats &&
-              Part<256, 2>::kFloats <= 2u * Part<64, 4>::kFloats, "the partial results' room");
+// Floats of a context's partial results: two results for every workgroup (heads of 256: one
+// workgroup a CU, half as many).
+uint64_t tree_part_floats() { return 2ull * kTreeSlots * Part<128, 2>::kFloats; }
+static_assert(Part<256, 2>::kFloats <= 2u * Part<128, 2>::kFloats, "the partial results' room");
 
 hipError_t launch_tree_attn(const TreeArgs& args, uint32_t cus, hipStream_t st) {
     TreeArgs a = args;
