@@ -312,7 +312,7 @@ struct KvArgs {
     uint32_t f8;                    // 1: e4m3 rows with scales
     uint32_t n, layer;              // requests; the layer (append, attention)
     uint32_t max_keep;
-    uint32_t chunks, cp;            // 16-byte chunks of a row, lanes a row (a power of two)
+    uint32_t chunks, cp, parts;     // 16-byte chunks of a row, lanes a row (a power of two); parts of a row (compact)
     uint32_t cap;                   // what fresh and from hold
     void* k;
     void* v;

@@ -118,25 +118,38 @@ __global__ __launch_bounds__(kKvThreads) void kv_fork(KvArgs a) {
 
 // ---- lcs_kv_grow: one workgroup decides and gives out pages ----
 // 1024 / n lanes (up to a wave) look at a request's pages. The counts do not move until
-// every request has read them.
+// every request has read them. Its time is its chain of dependent loads (table, count,
+// table), so up to kGrowLocal pages are passed on by way of LDS.
 constexpr int kGrowThreads = 1024;
 constexpr uint32_t kGrowPer = 16;   // pages a thread looks at for free ones in a round
+constexpr uint32_t kGrowLocal = 2048;
 __global__ __launch_bounds__(kGrowThreads) void kv_grow(KvArgs a) {
     constexpr uint32_t NW = kGrowThreads / kWave;
-    __shared__ int32_t slots[kKvMaxReq];
+    __shared__ __attribute__((aligned(16))) int32_t slots[kKvMaxReq];
     __shared__ uint32_t need[kKvMaxReq], off[kKvMaxReq], first[kKvMaxReq], past[kKvMaxReq];
-    __shared__ uint32_t red[NW], used;
+    __shared__ int32_t fresh_s[kGrowLocal], from_s[kGrowLocal];
+    __shared__ uint32_t red[NW], used, copies;
     const uint32_t tid = tid_x(), n = a.n;
-    const int32_t slot = tid < n ? a.seq[tid] : -1;
-    if (tid < n) slots[tid] = slot;
-    if (tid == 0) used = 0u;
+    int32_t slot = -1, s = 0, e = 0;
+    if (tid < n) {
+        slot = a.seq[tid];
+        s = a.start[tid];
+        e = a.end[tid];
+    }
+    slots[tid] = tid < n ? slot : -1;
+    if (tid == 0) used = copies = 0u;
     __syncthreads();
     bool ok = false;
     if (tid < n) {
-        const int32_t s = a.start[tid], e = a.end[tid];
         ok = slot == -1 || ((uint32_t)slot < a.seqs && s >= 0 && e >= s && (uint64_t)(uint32_t)e <= (uint64_t)a.max_pages << a.page_shift);
-        if (slot != -1)
-            for (uint32_t j = 0; j < tid; ++j) ok = ok && slots[j] != slot;
+        if (slot != -1) {
+            bool again = false;
+            for (uint32_t j = 0; j < tid; j += 4u) {
+                const int4 q = *reinterpret_cast<const int4*>(slots + j);
+                again = again || q.x == slot || (j + 1u < tid && q.y == slot) || (j + 2u < tid && q.z == slot) || (j + 3u < tid && q.w == slot);
+            }
+            ok = ok && !again;
+        }
         const bool none = !ok || slot == -1 || s == e;
         first[tid] = none ? 0u : (uint32_t)s >> a.page_shift;
         past[tid] = none ? 0u : (uint32_t)(((uint64_t)(uint32_t)e + a.page_tokens - 1u) >> a.page_shift);
@@ -155,10 +168,16 @@ __global__ __launch_bounds__(kGrowThreads) void kv_grow(KvArgs a) {
         page = p < p1 ? row[p] : 0;
         return p >= p1 ? 0u : !page_ok(a, page) ? 1u : a.refs[page] > 1 ? 2u : 0u;
     };
-    uint32_t cnt = 0;
+    uint32_t cnt = 0, w0 = 0;
+    int32_t page0 = 0;   // (the lane's first page, looked up once)
     for (uint32_t b = p0; __any(b < p1); b += L) {
         int32_t page;
-        cnt += (uint32_t)__builtin_popcountll(ballot(wants(b + sub, page) != 0u) & mine);
+        const uint32_t w = wants(b + sub, page);
+        if (b == p0) {
+            w0 = w;
+            page0 = page;
+        }
+        cnt += (uint32_t)__builtin_popcountll(ballot(w != 0u) & mine);
     }
     if (act && sub == 0u) need[req] = cnt;
     __syncthreads();
@@ -186,13 +205,17 @@ __global__ __launch_bounds__(kGrowThreads) void kv_grow(KvArgs a) {
         const uint32_t here = block_exclusive_scan<kGrowThreads>((uint32_t)__builtin_popcount(bits), at, red);
         at += found;
         while (bits != 0u && at < want) {
-            a.fresh[at++] = (int32_t)(g0 + (uint32_t)__builtin_ctz(bits));
+            const int32_t page = (int32_t)(g0 + (uint32_t)__builtin_ctz(bits));
+            if (at < kGrowLocal) fresh_s[at] = page;
+            else a.fresh[at] = page;
+            ++at;
             bits &= bits - 1u;
         }
         found += here;
     }
     found = min(found, want);
     __syncthreads();   // (the list is complete)
+    auto fresh_of = [&](uint32_t k) -> int32_t { return k < kGrowLocal ? fresh_s[k] : a.fresh[k]; };
     if (tid < n) {
         const bool served = ok && off[tid] + need[tid] <= found;
         if (served) a.result[tid] = 0;
@@ -201,28 +224,40 @@ __global__ __launch_bounds__(kGrowThreads) void kv_grow(KvArgs a) {
         if (!served) past[tid] = first[tid];
     }
     __syncthreads();
-    if (act && past[req] > first[req]) {   // (a request's lanes together; the loops below wait for none of another's)
+    if (act && past[req] > first[req]) {   // (a request's lanes together; the loop below waits for none of another's)
         uint32_t at = off[req];
         for (uint32_t b = p0; b < p1; b += L) {
-            int32_t page;
-            const uint32_t w = wants(b + sub, page);
+            int32_t page = page0;
+            const uint32_t w = b == p0 ? w0 : wants(b + sub, page);
             const uint64_t m = ballot(w != 0u) & mine;
             const uint32_t k = at + (uint32_t)__builtin_popcountll(m & below);
             if (w != 0u && k < found) {
-                const int32_t f = a.fresh[k];
-                row[b + sub] = f;
-                a.from[k] = w == 2u ? page : -1;
+                const int32_t src = w == 2u ? page : -1;
+                row[b + sub] = fresh_of(k);
+                if (k < kGrowLocal) from_s[k] = src;
+                else a.from[k] = src;
             }
             at += (uint32_t)__builtin_popcountll(m);
         }
     }
     __syncthreads();
-    for (uint32_t k = tid; k < used; k += kGrowThreads) {
-        a.refs[a.fresh[k]] = 1;
-        const int32_t f = a.from[k];
-        if (f >= 0) atomicSub(&a.refs[f], 1);
+    // the counts; and what is to be copied, in any order, moved to the front of the lists
+    const uint32_t n_used = used;
+    for (uint32_t b = 0; b < n_used; b += kGrowThreads) {
+        const uint32_t k = b + tid;
+        const int32_t src = k >= n_used ? -1 : k < kGrowLocal ? from_s[k] : a.from[k];
+        const int32_t page = k < n_used ? fresh_of(k) : 0;
+        if (k < n_used) a.refs[page] = 1;
+        if (src >= 0) atomicSub(&a.refs[src], 1);
+        __syncthreads();   // (the round's entries have been read: no more than b of them precede)
+        if (src >= 0) {
+            const uint32_t c = atomicAdd(&copies, 1u);
+            a.fresh[c] = page;
+            a.from[c] = src;
+        }
     }
-    if (tid == 0) *a.n_fresh = used;
+    __syncthreads();
+    if (tid == 0) *a.n_fresh = copies;
 }
 
 // The copies that kv_grow has planned: (copy, layer, k or v, head) by workgroup, in turn.
@@ -234,12 +269,10 @@ __global__ __launch_bounds__(kKvThreads) void kv_copy(KvArgs a) {
     const uint32_t chunk = tid_x() & (a.cp - 1u), row0 = tid_x() / a.cp, step = kKvThreads / a.cp;
     for (uint64_t it = wg_x(); it < items; it += gridDim.x) {
         const uint32_t k = (uint32_t)(it / per), r = (uint32_t)(it % per);
-        const int32_t src = a.from[k];
-        if (src < 0) continue;
-        const uint32_t dst = (uint32_t)a.fresh[k];
+        const uint32_t src = (uint32_t)a.from[k], dst = (uint32_t)a.fresh[k];
         const uint32_t head = r % a.kv_heads, kv = r / a.kv_heads & 1u, layer = r / (2u * a.kv_heads);
         unsigned char* base = static_cast<unsigned char*>(kv ? a.v : a.k);
-        const uint64_t f = place(a, layer, (uint32_t)src, head, 0), t = place(a, layer, dst, head, 0);
+        const uint64_t f = place(a, layer, src, head, 0), t = place(a, layer, dst, head, 0);
         const uint64_t ts = a.token_stride * (a.f8 ? 1u : 2u);
         if (chunk < a.chunks) {
             for (uint32_t row = row0; row < a.page_tokens; row += 4u * step) {
@@ -256,7 +289,7 @@ __global__ __launch_bounds__(kKvThreads) void kv_copy(KvArgs a) {
         }
         if (a.f8) {
             float* sc = kv ? a.v_scale : a.k_scale;
-            const uint64_t sf = scale_place(a, layer, (uint32_t)src, head, 0), st = scale_place(a, layer, dst, head, 0);
+            const uint64_t sf = scale_place(a, layer, src, head, 0), st = scale_place(a, layer, dst, head, 0);
             for (uint32_t row = tid_x(); row < a.page_tokens; row += kKvThreads) sc[st + row] = sc[sf + row];
         }
     }
@@ -297,13 +330,16 @@ __global__ __launch_bounds__(kKvThreads) void kv_compact_check(KvArgs a) {
     }
 }
 
-// A workgroup moves one head's rows of k or v of one layer of one request, in order, by rounds
-// of U rows a lane group: a round's rows are read by all its lanes before the first
-// of them is written. Rows never move up, so a round overwrites no row of a later one:
-// its places lie below the next round's first, and sources at or above their places.
+// A workgroup moves one head's rows of k or v of one layer of one request (or 16-byte chunks
+// from part * cp of them), in order, by rounds of U rows a lane group. Rows never move up:
+// a round writes below the next round's places, which lie at or below its sources, so
+// that only a round's own rows have to be read by all lanes before the first is
+// written. The next round's rows are under way meanwhile, the places of the one after it too.
 __global__ __launch_bounds__(kKvThreads) void kv_compact(KvArgs a) {
-    constexpr uint32_t U = 8;
+    constexpr uint32_t U = 4;
     uint32_t b = wg_x();
+    const uint32_t part = b % a.parts;
+    b /= a.parts;
     const uint32_t head = b % a.kv_heads;
     b /= a.kv_heads;
     const uint32_t kv = b & 1u;
@@ -314,107 +350,186 @@ __global__ __launch_bounds__(kKvThreads) void kv_compact(KvArgs a) {
     const uint32_t n = min((uint32_t)max(a.count[i], 0), a.max_keep);
     const int32_t* keep = a.index + (uint64_t)i * a.max_keep;
     const int32_t* row = a.table + (uint64_t)slot * a.max_pages;
-    const uint32_t chunk = tid_x() & (a.cp - 1u), r0 = tid_x() / a.cp, step = kKvThreads / a.cp;
-    unsigned char* base = static_cast<unsigned char*>(kv ? a.v : a.k) + 16u * chunk;
+    const uint32_t chunk = part * a.cp + (tid_x() & (a.cp - 1u)), r0 = tid_x() / a.cp, step = kKvThreads / a.cp;
+    const uint32_t es = a.f8 ? 1u : 2u, in = a.page_tokens - 1u;
+    unsigned char* base = static_cast<unsigned char*>(kv ? a.v : a.k) + (layer * a.layer_stride + head * a.head_stride) * es + 16u * chunk;
     float* sc = kv ? a.v_scale : a.k_scale;
-    const uint32_t in = a.page_tokens - 1u;
-    const bool data = chunk < a.chunks;
-    for (uint32_t j0 = 0; j0 < n; j0 += U * step) {
+    const bool data = chunk < a.chunks, scale = a.f8 && chunk == 0u;
+    struct Places {
+        uint32_t pos[U];
+        int32_t pf[U], pt[U];   // the pages that it comes from and goes to; pt -1: it stays
+    };
+    struct Rows {
         u32x4 x[U];
         float s[U];
-        uint64_t to[U], st[U];
-        bool move[U];
+    };
+    // (a row that is not moved is read where it is: no load depends on a branch)
+    auto places = [&](uint32_t j0) -> Places {
+        Places p;
 #pragma unroll
         for (uint32_t u = 0; u < U; ++u) {
             const uint32_t j = j0 + u * step + r0;
-            const uint32_t pos = j < n ? (uint32_t)keep[j] : j;
-            move[u] = j < n && pos != j;
-            s[u] = 0.0f;
-            to[u] = st[u] = 0;
-            x[u] = u32x4{0, 0, 0, 0};
-            if (move[u]) {
-                const uint32_t pf = (uint32_t)row[pos >> a.page_shift], pt = (uint32_t)row[j >> a.page_shift];
-                to[u] = place(a, layer, pt, head, j & in);
-                if (data) x[u] = *reinterpret_cast<const u32x4*>(base + place(a, layer, pf, head, pos & in));
-                if (a.f8 && chunk == 0u) {
-                    st[u] = scale_place(a, layer, pt, head, j & in);
-                    s[u] = sc[scale_place(a, layer, pf, head, pos & in)];
-                }
+            p.pos[u] = j < n ? (uint32_t)keep[j] : 0u;
+        }
+#pragma unroll
+        for (uint32_t u = 0; u < U; ++u) {
+            const uint32_t j = j0 + u * step + r0;
+            p.pf[u] = row[p.pos[u] >> a.page_shift];
+            p.pt[u] = j < n && p.pos[u] != j ? row[j >> a.page_shift] : -1;
+        }
+        return p;
+    };
+    auto read = [&](const Places& p) -> Rows {
+        Rows r;
+#pragma unroll
+        for (uint32_t u = 0; u < U; ++u) {
+            r.x[u] = u32x4{0, 0, 0, 0};
+            r.s[u] = 0.0f;
+            if (p.pt[u] >= 0) {
+                if (data) r.x[u] = *reinterpret_cast<const u32x4*>(base + ((uint32_t)p.pf[u] * a.page_stride + (p.pos[u] & in) * a.token_stride) * es);
+                if (scale) r.s[u] = sc[scale_place(a, layer, (uint32_t)p.pf[u], head, p.pos[u] & in)];
             }
         }
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // (a barrier by itself waits for no load)
+        return r;
+    };
+    const uint32_t round = U * step;
+    if (n == 0u) return;
+    Places now = places(0u), next = places(round);
+    Rows x = read(now);
+    for (uint32_t j0 = 0; j0 < n; j0 += round) {
+        const Rows y = read(next);
+        const Places then = places(j0 + 2u * round);
+#pragma unroll
+        for (uint32_t u = 0; u < U; ++u) asm volatile("" : "+v"(x.x[u]), "+v"(x.s[u]));   // (the round's rows have arrived)
         __syncthreads();
 #pragma unroll
         for (uint32_t u = 0; u < U; ++u) {
-            if (move[u]) {
-                if (data) *reinterpret_cast<u32x4*>(base + to[u]) = x[u];
-                if (a.f8 && chunk == 0u) sc[st[u]] = s[u];
+            if (now.pt[u] >= 0) {
+                const uint32_t j = j0 + u * step + r0;
+                if (data) *reinterpret_cast<u32x4*>(base + ((uint32_t)now.pt[u] * a.page_stride + (j & in) * a.token_stride) * es) = x.x[u];
+                if (scale) sc[scale_place(a, layer, (uint32_t)now.pt[u], head, j & in)] = x.s[u];
             }
         }
+        now = next;
+        next = then;
+        x = y;
     }
 }
 
 // ---- lcs_kv_append ----
 // A workgroup writes kAppendTokens tokens of one layer and sequence: cp lanes a row of 8
-// elements each, both k's and v's heads.
+// elements each, both k's and v's heads. Where each token comes from and goes to is looked
+// up once, ahead of the rows. A lane keeps its head from token to token, and quotients
+// take three operations each, since arithmetic bounds the 8-bit form (64 x 4.5 tokens of
+// 32 layers x 8 heads: 59 us with divisions for both).
 constexpr uint32_t kAppendTokens = 16;
+
+// x / scale to nearest: RN(1 / scale), a product, and its remainder's share (exact by an fma),
+// which makes the quotient the correctly rounded one. An infinite scale gives 0, and NaN
+// for an infinite x.
+struct Quotient {
+    float scale, inv;
+    __device__ __forceinline__ explicit Quotient(float s) : scale(s > 3.4e38f ? 0.0f : s), inv(fdiv(1.0f, s)) {}
+    __device__ __forceinline__ float of(float x) const {
+        const float q = fmul(x, inv);
+        return fmaf(fmaf(-q, scale, x), inv, q);
+    }
+};
+
+// The largest of cp neighbouring lanes' values (cp a power of two up to 32): pairs, quads, and
+// their mirror images, in which the quads and eights are already alike.
+__device__ __forceinline__ uint32_t row_max(uint32_t v, uint32_t cp) {
+    auto with = [](uint32_t x, int y) { return max(x, (uint32_t)y); };
+    if (cp > 1u) v = with(v, __builtin_amdgcn_mov_dpp((int)v, 0xb1, 0xf, 0xf, true));    // lane ^ 1
+    if (cp > 2u) v = with(v, __builtin_amdgcn_mov_dpp((int)v, 0x4e, 0xf, 0xf, true));    // lane ^ 2
+    if (cp > 4u) v = with(v, __builtin_amdgcn_mov_dpp((int)v, 0x141, 0xf, 0xf, true));   // 7 - lane of eight
+    if (cp > 8u) v = with(v, __builtin_amdgcn_mov_dpp((int)v, 0x140, 0xf, 0xf, true));   // 15 - lane of sixteen
+    if (cp > 16u) v = with(v, __shfl_xor((int)v, 16));
+    return v;
+}
+
 template <bool F8>
 __global__ __launch_bounds__(kKvThreads) void kv_append(KvAppendArgs p) {
+    constexpr uint32_t U = 4;
+    __shared__ int32_t page_s[kAppendTokens], src_s[kAppendTokens];
     const KvArgs& a = p.a;
     const uint32_t i = wg_x() / p.blocks, j0 = wg_x() % p.blocks * kAppendTokens, l = __builtin_amdgcn_workgroup_id_y();
     const int32_t slot = a.seq ? a.seq[i] : (int32_t)i;
-    if (slot == -1) return;
     const uint32_t n = a.count ? min((uint32_t)max(a.count[i], 0), p.rows_per_seq) : p.rows_per_seq;
-    if (j0 >= n) return;
-    if ((uint32_t)slot >= a.seqs) {
-        if (tid_x() == 0) atomicOr(a.status, kStatusPages);
-        return;
-    }
     const int32_t pos0 = a.start[i];
-    const int32_t* row = a.table + (uint64_t)slot * a.max_pages;
-    const uint32_t chunk = tid_x() & (a.cp - 1u), step = kKvThreads / a.cp;
-    const uint32_t items = min(n - j0, kAppendTokens) * 2u * a.kv_heads, elems = a.head_dim / 8u;
-    for (uint32_t it = tid_x() / a.cp; it < items; it += step) {
-        const uint32_t head = it % a.kv_heads, kv = it / a.kv_heads & 1u, j = j0 + it / (2u * a.kv_heads);
+    if (slot == -1 || j0 >= n) return;
+    const uint32_t tokens = min(n - j0, kAppendTokens);
+    if (tid_x() < tokens) {
+        const uint32_t j = j0 + tid_x();
         const int64_t pos = (int64_t)pos0 + j;
         const int32_t src = a.index ? a.index[(uint64_t)i * p.rows_per_seq + j] : (int32_t)j;
-        const bool in = pos >= 0 && (uint64_t)pos < (uint64_t)a.max_pages << a.page_shift && (uint32_t)src < p.rows_per_seq;
-        const int32_t page = in ? row[(uint64_t)pos >> a.page_shift] : -1;
-        const bool ok = page_ok(a, page) && a.refs[page_ok(a, page) ? page : 0] <= 1;
-        u32x4 x = {0, 0, 0, 0};
-        if (ok && chunk < elems) {
-            const uint64_t r = (uint64_t)i * p.rows_per_seq + (uint32_t)src;
-            const uint64_t at = (uint64_t)l * p.new_layer_stride + r * (kv ? p.v_stride : p.k_stride) + head * a.head_dim + 8u * chunk;
-            x = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(kv ? p.v : p.k) + at);
+        const bool in = (uint32_t)slot < a.seqs && pos >= 0 && (uint64_t)pos < (uint64_t)a.max_pages << a.page_shift && (uint32_t)src < p.rows_per_seq;
+        int32_t page = in ? a.table[(uint64_t)slot * a.max_pages + ((uint64_t)pos >> a.page_shift)] : -1;
+        if (!page_ok(a, page) || a.refs[page_ok(a, page) ? page : 0] > 1) {
+            page = -1;
+            atomicOr(a.status, kStatusPages);
         }
-        const uint32_t layer = a.layer + l, tok = (uint32_t)pos & (a.page_tokens - 1u);
-        unsigned char* base = static_cast<unsigned char*>(kv ? a.v : a.k);
-        if constexpr (F8) {
-            uint32_t top = 0;   // the largest |x|, by its bits (a NaN's lie above infinity's)
+        page_s[tid_x()] = page;
+        src_s[tid_x()] = src;
+    }
+    __syncthreads();
+    // a pass covers `per` whole tokens, or a part of one's rows
+    const uint32_t chunk = tid_x() & (a.cp - 1u), g = tid_x() / a.cp, step = kKvThreads / a.cp, rows = 2u * a.kv_heads;
+    const uint32_t per = step > rows ? step / rows : 1u, t0 = step > rows ? g / rows : 0u;
+    const bool data = chunk < a.head_dim / 8u;
+    if (t0 >= per) return;
+    const uint32_t layer = a.layer + l;
+    for (uint32_t r = g - t0 * rows; r < rows; r += step) {
+        const bool kv = r >= a.kv_heads;
+        const uint32_t head = kv ? r - a.kv_heads : r;
+        const uint16_t* from = static_cast<const uint16_t*>(kv ? p.v : p.k) + (uint64_t)l * p.new_layer_stride +
+                               (uint64_t)i * p.rows_per_seq * (kv ? p.v_stride : p.k_stride) + head * a.head_dim + 8u * chunk;
+        const uint64_t stride = kv ? p.v_stride : p.k_stride;
+        unsigned char* base = static_cast<unsigned char*>(kv ? a.v : a.k) + place(a, layer, 0, head, 0) + (F8 ? 8u : 16u) * chunk;
+        float* sc = F8 ? (kv ? a.v_scale : a.k_scale) + scale_place(a, layer, 0, head, 0) : nullptr;
+        for (uint32_t t = t0; t < tokens; t += U * per) {
+            u32x4 x[U];
+            int32_t page[U];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) top = max(top, max(x[k] & 0x7fffu, x[k] >> 16 & 0x7fffu));
-            for (uint32_t m = 1; m < a.cp; m <<= 1) top = max(top, (uint32_t)__shfl_xor((int)top, (int)m));
-            const float t = __uint_as_float(top << 16);
-            const float scale = t > 0.0f ? fmaxf(fdiv(t, kE4m3Max), kLeastScale) : 1.0f;   // (a NaN is not above 0)
-            uint32_t q[2];
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                float f[4];
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const uint32_t w = x[2 * h + k / 2];
-                    const float v = fdiv(__uint_as_float(k % 2 ? w & 0xffff0000u : w << 16), scale);
-                    f[k] = v > kE4m3Max ? kE4m3Max : v < -kE4m3Max ? -kE4m3Max : v;
-                }
-                int w = __builtin_amdgcn_cvt_pk_fp8_f32(f[0], f[1], 0, false);
-                q[h] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(f[2], f[3], w, true);
+            for (uint32_t u = 0; u < U; ++u) {
+                const uint32_t tu = t + u * per;
+                page[u] = tu < tokens ? page_s[tu] : -1;
+                x[u] = u32x4{0, 0, 0, 0};
+                if (page[u] >= 0 && data) x[u] = *reinterpret_cast<const u32x4*>(from + (uint32_t)src_s[tu] * stride);
             }
-            if (ok && chunk < elems) *reinterpret_cast<u32x2*>(base + place(a, layer, (uint32_t)page, head, tok) + 8u * chunk) = u32x2{q[0], q[1]};
-            if (ok && chunk == 0u) (kv ? a.v_scale : a.k_scale)[scale_place(a, layer, (uint32_t)page, head, tok)] = scale;
-        } else {
-            if (ok && chunk < elems) *reinterpret_cast<u32x4*>(base + place(a, layer, (uint32_t)page, head, tok) + 16u * chunk) = x;
+#pragma unroll
+            for (uint32_t u = 0; u < U; ++u) {
+                if (t + u * per >= tokens) break;   // (the lanes of a row together)
+                const bool ok = page[u] >= 0;
+                const uint32_t tok = ((uint32_t)pos0 + j0 + t + u * per) & (a.page_tokens - 1u);
+                const uint64_t at = ((uint32_t)page[u] * a.page_stride + tok * a.token_stride) * (F8 ? 1u : 2u);
+                if constexpr (F8) {
+                    uint32_t top = 0;   // the largest |x|, by its bits (a NaN's lie above infinity's)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) top = max(top, max(x[u][k] & 0x7fffu, x[u][k] >> 16 & 0x7fffu));
+                    top = row_max(top, a.cp);
+                    const float f = __uint_as_float(top << 16);
+                    const float scale = f > 0.0f ? fmaxf(fdiv(f, kE4m3Max), kLeastScale) : 1.0f;   // (a NaN is not above 0)
+                    const Quotient by(scale);   // (448 at most, and a rounding)
+                    uint32_t q[2];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        float e[4];
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const uint32_t w = x[u][2 * h + k / 2];
+                            e[k] = by.of(__uint_as_float(k % 2 ? w & 0xffff0000u : w << 16));
+                        }
+                        const int w = __builtin_amdgcn_cvt_pk_fp8_f32(e[0], e[1], 0, false);
+                        q[h] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(e[2], e[3], w, true);
+                    }
+                    if (ok && data) *reinterpret_cast<u32x2*>(base + at) = u32x2{q[0], q[1]};
+                    if (ok && chunk == 0u) sc[((uint64_t)(uint32_t)page[u] * a.kv_heads << a.page_shift) + tok] = scale;
+                } else {
+                    if (ok && data) *reinterpret_cast<u32x4*>(base + at) = x[u];
+                }
+            }
         }
-        if (!ok && chunk == 0u) atomicOr(a.status, kStatusPages);
     }
 }
 
@@ -452,7 +567,14 @@ hipError_t launch_kv_compact(const KvArgs& args, hipStream_t st) {
     hipLaunchKernelGGL(kv_compact_check, dim3(a.n), dim3(kKvThreads), 0, st, a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(kv_compact, dim3(a.n * a.layers * 2u * a.kv_heads), dim3(kKvThreads), 0, st, a);
+    // (few rows' heads: their chunks apart, so that the CUs have more in flight)
+    const uint32_t heads = a.n * a.layers * 2u * a.kv_heads;
+    a.parts = 1;
+    while (heads * a.parts < 2048u && a.cp > 4u) {
+        a.parts *= 2u;
+        a.cp /= 2u;
+    }
+    hipLaunchKernelGGL(kv_compact, dim3(heads * a.parts), dim3(kKvThreads), 0, st, a);
     return hipGetLastError();
 }
 

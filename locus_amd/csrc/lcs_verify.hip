@@ -318,8 +318,8 @@ __global__ __launch_bounds__(kAcceptSeqs * kWave) void accept_kernel(VerifyArgs 
 // ---- a tree's verdict (lcs_tree_verify) ----
 // tree_rows streams the rows as verify_kernel does; a row's workgroup also writes the
 // log-probabilities of the nodes whose parent it is (the root's row those of the nodes
-// that have none). tree_walk then follows the accepted nodes: a wave per sequence, four
-// nodes a lane, one ballot per 64 nodes and step.
+// that have none). tree_walk then follows the accepted nodes: a wave per sequence, a node
+// or four a lane, one ballot per 64 nodes and step, after one round of loads.
 __device__ __forceinline__ bool tree_child(uint32_t j, int32_t parent) { return parent >= 0 && (uint32_t)parent < j; }
 
 template <int G, int NT, RowForm F>
@@ -347,26 +347,39 @@ __global__ __launch_bounds__(NT) void tree_rows(TreeVerifyArgs a) {
     }
 }
 
+template <uint32_t NK>
 __global__ __launch_bounds__(kAcceptSeqs * kWave) void tree_walk(TreeVerifyArgs a) {
-    constexpr uint32_t NK = kTreeMax / kWave;
     const uint32_t seq = wg_x() * kAcceptSeqs + tid_x() / kWave;
     if (seq >= a.n_seq) return;
     const uint32_t lane = (uint32_t)lane_id(), R = a.rows_per_seq;
     const uint64_t first = (uint64_t)seq * R;
-    int32_t up[NK];   // a node's parent where it is what that says, else -1
+    int32_t up[NK], best[NK], token[NK];   // up: a node's parent where it is what that says, else -1
 #pragma unroll
     for (uint32_t k = 0; k < NK; ++k) {
-        const uint32_t j = lane + k * kWave;
-        up[k] = -1;
-        if (j < R) {
-            const int32_t p = a.parent[first + j];
-            if (tree_child(j, p) && a.argmax_ids[first + (uint32_t)p] == a.tokens[first + j]) up[k] = p;
-        }
+        const uint32_t j = lane + k * kWave, at = j < R ? j : 0u;
+        up[k] = a.parent[first + at];
+        best[k] = a.argmax_ids[first + at];
+        token[k] = a.tokens[first + at];
+        if (j >= R || !tree_child(j, up[k])) up[k] = -1;
     }
-    int32_t cur = 0;
+#pragma unroll
+    for (uint32_t k = 0; k < NK; ++k) {
+        const int src = up[k] < 0 ? 0 : up[k];
+        int32_t says = 0;
+#pragma unroll
+        for (uint32_t q = 0; q < NK; ++q) {
+            const int32_t b = __shfl(best[q], src % kWave);
+            says = (uint32_t)src / kWave == q ? b : says;
+        }
+        if (says != token[k]) up[k] = -1;
+    }
+    int32_t cur = 0, here[NK];   // here: the path's nodes, the lane's places of it
+#pragma unroll
+    for (uint32_t k = 0; k < NK; ++k) here[k] = -1;
     uint32_t n = 0;
     for (;;) {   // (a child's number is above its parent's: at most R steps)
-        if (lane == 0u) a.path[first + n] = cur;
+#pragma unroll
+        for (uint32_t k = 0; k < NK; ++k) here[k] = lane + k * kWave == n ? cur : here[k];
         ++n;
         int32_t next = -1;
 #pragma unroll
@@ -377,10 +390,17 @@ __global__ __launch_bounds__(kAcceptSeqs * kWave) void tree_walk(TreeVerifyArgs 
         if (next < 0 || n >= R) break;
         cur = next;
     }
-    for (uint32_t j = n + lane; j < R; j += kWave) a.path[first + j] = -1;
+    int32_t last = 0;
+#pragma unroll
+    for (uint32_t k = 0; k < NK; ++k) {
+        const uint32_t j = lane + k * kWave;
+        if (j < R) a.path[first + j] = here[k];
+        const int32_t b = __shfl(best[k], cur % kWave);
+        last = (uint32_t)cur / kWave == k ? b : last;
+    }
     if (lane == 0u) {
         a.n_path[seq] = (int32_t)n;
-        a.next_id[seq] = a.argmax_ids[first + (uint32_t)cur];
+        a.next_id[seq] = last;
         if (a.new_length) a.new_length[seq] = a.length[seq] + (int32_t)n;
     }
 }
@@ -438,7 +458,9 @@ hipError_t launch_tree_verify(const TreeVerifyArgs& a, hipStream_t st) {
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
     }
-    hipLaunchKernelGGL(tree_walk, dim3((a.n_seq + kAcceptSeqs - 1u) / kAcceptSeqs), dim3(kAcceptSeqs * kWave), 0, st, a);
+    const dim3 grid((a.n_seq + kAcceptSeqs - 1u) / kAcceptSeqs), block(kAcceptSeqs * kWave);
+    if (a.rows_per_seq <= (uint32_t)kWave) hipLaunchKernelGGL(tree_walk<1>, grid, block, 0, st, a);
+    else hipLaunchKernelGGL(tree_walk<kTreeMax / kWave>, grid, block, 0, st, a);
     return hipGetLastError();
 }
 
