@@ -71,7 +71,7 @@ struct lcs_ctx {
     // each copies, and their number
     uint32_t kv_cap = 0;
     int32_t* kv_fresh = nullptr;   // kv_cap, then kv_cap for what they copy, then the number
-    float* tree_part = nullptr;    // lcs_tree_attn: 64 zeros, then the partial results
+    float* tree_part = nullptr;    // lcs_tree_attn: 64 zeros, kTreePairs spans, the partial results
     // lcs_logprobs: greedy parameters (all fields zero) for max_rows rows, on
     // the device and on the host, and its argmax ids when the caller wants none
     lcs_params* lp_params = nullptr;
@@ -803,7 +803,7 @@ int lcs_kv_reserve(lcs_ctx* c, uint32_t new_pages) {
     c->kv_cap = 0;
     hipError_t e = hipMalloc(&c->kv_fresh, ((size_t)new_pages * 2 + 1) * 4);
     if (e == hipSuccess && !c->tree_part) {
-        if ((e = hipMalloc(&c->tree_part, (64 + lcs::tree_part_floats()) * 4)) != hipSuccess) c->tree_part = nullptr;
+        if ((e = hipMalloc(&c->tree_part, (64 + lcs::kTreePairs + lcs::tree_part_floats()) * 4)) != hipSuccess) c->tree_part = nullptr;
         else if ((e = hipMemset(c->tree_part, 0, 64 * 4)) == hipSuccess) e = hipDeviceSynchronize();
         if (e != hipSuccess) {
             (void)hipFree(c->tree_part);
@@ -942,7 +942,7 @@ int lcs_kv_append(lcs_ctx* c, const lcs_kv_cache* k, const lcs_kv_append_batch* 
 int lcs_tree_attn(lcs_ctx* c, const lcs_tree_attn_batch* b, const lcs_tree_attn_out* o, void* stream) {
     if (!c) return LCS_ERR_INVALID_ARG;
     const char* why = "";
-    const int rc = lcs::check_tree_attn(b, o, lcs::kKvMaxReq, &why);
+    const int rc = lcs::check_tree_attn(b, o, lcs::kKvMaxReq, lcs::kTreePairs, &why);
     if (rc != LCS_OK) return fail(c, rc, why);
     if (!c->kv_fresh) return fail(c, LCS_ERR_INVALID_ARG, "lcs_tree_attn without lcs_kv_reserve");
     if (b->n_seq == 0) return LCS_OK;
@@ -966,7 +966,8 @@ int lcs_tree_attn(lcs_ctx* c, const lcs_tree_attn_batch* b, const lcs_tree_attn_
     a.o = static_cast<uint16_t*>(o->o);
     a.lse = o->lse;
     a.zeros = reinterpret_cast<const unsigned char*>(c->tree_part);
-    a.part = c->tree_part + 64;
+    a.spans = reinterpret_cast<uint32_t*>(c->tree_part + 64);
+    a.part = c->tree_part + 64 + lcs::kTreePairs;
     DeviceGuard g(c->device);
     const hipError_t e = lcs::launch_tree_attn(a, c->cus, static_cast<hipStream_t>(stream));
     return e == hipSuccess ? LCS_OK : hip_fail(c, e, "attention kernel launch");

@@ -313,6 +313,7 @@ struct KvArgs {
     uint32_t n, layer;              // requests; the layer (append, attention)
     uint32_t max_keep;
     uint32_t chunks, cp, parts;     // 16-byte chunks of a row, lanes a row (a power of two); parts of a row (compact)
+    uint32_t pass_shift;            // log2 of the passes that copy a page's rows of one head
     uint32_t cap;                   // what fresh and from hold
     void* k;
     void* v;
@@ -355,10 +356,12 @@ struct TreeArgs {
     uint16_t* o;
     float* lse;                     // or NULL
     float* part;                    // partial results (tree_part_floats)
+    uint32_t* spans;                // kTreePairs: which pieces share a (sequence, kv head) pair
     const unsigned char* zeros;     // 16 bytes
     // of a launch: workgroups along the line of steps, row tiles and the first one, steps of the new tokens
     uint32_t pieces, row_tiles, row_tile0, new_steps;
 };
+constexpr uint32_t kTreePairs = 65536;  // sequences x kv heads of a call
 constexpr uint32_t kTreeSlots = 512;    // workgroups of a launch, at two a CU (half as many at one)
 
 // a tree's verdict (lcs_verify.hip)

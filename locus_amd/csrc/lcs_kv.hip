@@ -260,38 +260,30 @@ __global__ __launch_bounds__(kGrowThreads) void kv_grow(KvArgs a) {
     if (tid == 0) *a.n_fresh = copies;
 }
 
-// The copies that kv_grow has planned: (copy, layer, k or v, head) by workgroup, in turn.
-// CP lanes a row of 16-byte chunks.
+// The copies that kv_grow has planned, by units of 256 chunks of 16 bytes: a part of the rows of
+// one head of k or v of one layer, cp lanes a row. Many short workgroups with stores past
+// the caches (nobody reads the copies soon) come nearest to the memory's rate: 64 pages of
+// 32 tokens x 32 layers x 8 heads, us for the three calls of a fork, one unit a turn in
+// 16384 workgroups 69 and 8192 74, with plain stores 88 and 85; two units a turn in 8192
+// 74 and 88, eight in 1024 - / 112.
 __global__ __launch_bounds__(kKvThreads) void kv_copy(KvArgs a) {
-    const uint32_t used = *a.n_fresh;
-    const uint32_t per = a.layers * 2u * a.kv_heads;
-    const uint64_t items = (uint64_t)used * per;
-    const uint32_t chunk = tid_x() & (a.cp - 1u), row0 = tid_x() / a.cp, step = kKvThreads / a.cp;
-    for (uint64_t it = wg_x(); it < items; it += gridDim.x) {
-        const uint32_t k = (uint32_t)(it / per), r = (uint32_t)(it % per);
+    const uint32_t copies = *a.n_fresh;
+    const uint32_t per = a.layers * 2u * a.kv_heads, passes = 1u << a.pass_shift;
+    const uint64_t units = (uint64_t)copies * per << a.pass_shift;
+    const uint32_t chunk = tid_x() & (a.cp - 1u), row0 = tid_x() / a.cp, step = kKvThreads / a.cp, es = a.f8 ? 1u : 2u;
+    if (chunk >= a.chunks || row0 >= a.page_tokens) return;
+    for (uint64_t unit = wg_x(); unit < units; unit += gridDim.x) {
+        const uint64_t it = unit >> a.pass_shift;
+        const uint32_t k = (uint32_t)(it / per), r = (uint32_t)(it % per), row = ((uint32_t)unit & (passes - 1u)) * step + row0;
         const uint32_t src = (uint32_t)a.from[k], dst = (uint32_t)a.fresh[k];
         const uint32_t head = r % a.kv_heads, kv = r / a.kv_heads & 1u, layer = r / (2u * a.kv_heads);
-        unsigned char* base = static_cast<unsigned char*>(kv ? a.v : a.k);
-        const uint64_t f = place(a, layer, src, head, 0), t = place(a, layer, dst, head, 0);
-        const uint64_t ts = a.token_stride * (a.f8 ? 1u : 2u);
-        if (chunk < a.chunks) {
-            for (uint32_t row = row0; row < a.page_tokens; row += 4u * step) {
-                u32x4 x[4];
-#pragma unroll
-                for (uint32_t u = 0; u < 4u; ++u)
-                    if (row + u * step < a.page_tokens)
-                        x[u] = *reinterpret_cast<const u32x4*>(base + f + (row + u * step) * ts + 16u * chunk);
-#pragma unroll
-                for (uint32_t u = 0; u < 4u; ++u)
-                    if (row + u * step < a.page_tokens)
-                        *reinterpret_cast<u32x4*>(base + t + (row + u * step) * ts + 16u * chunk) = x[u];
-            }
+        unsigned char* base = static_cast<unsigned char*>(kv ? a.v : a.k) + place(a, layer, 0, head, row) + 16u * chunk;
+        const u32x4 x = *reinterpret_cast<const u32x4*>(base + src * a.page_stride * es);
+        if (a.f8 && chunk == 0u) {
+            float* sc = (kv ? a.v_scale : a.k_scale) + scale_place(a, layer, 0, head, row);
+            sc[(uint64_t)dst * a.kv_heads << a.page_shift] = sc[(uint64_t)src * a.kv_heads << a.page_shift];
         }
-        if (a.f8) {
-            float* sc = kv ? a.v_scale : a.k_scale;
-            const uint64_t sf = scale_place(a, layer, src, head, 0), st = scale_place(a, layer, dst, head, 0);
-            for (uint32_t row = tid_x(); row < a.page_tokens; row += kKvThreads) sc[st + row] = sc[sf + row];
-        }
+        __builtin_nontemporal_store(x, reinterpret_cast<u32x4*>(base + dst * a.page_stride * es));
     }
 }
 
@@ -334,9 +326,11 @@ __global__ __launch_bounds__(kKvThreads) void kv_compact_check(KvArgs a) {
 // from part * cp of them), in order, by rounds of U rows a lane group. Rows never move up:
 // a round writes below the next round's places, which lie at or below its sources, so
 // that only a round's own rows have to be read by all lanes before the first is
-// written. The next round's rows are under way meanwhile, the places of the one after it too.
+// written. The next round's rows are under way meanwhile, the places of the one after it too
+// (16 contexts of 4000 to 8192 tokens, half kept, 4 layers: 547 us without, 367 so in rounds of
+// 4 rows and plain stores, 356 of 8 and stores past the caches).
 __global__ __launch_bounds__(kKvThreads) void kv_compact(KvArgs a) {
-    constexpr uint32_t U = 4;
+    constexpr uint32_t U = 8;
     uint32_t b = wg_x();
     const uint32_t part = b % a.parts;
     b /= a.parts;
@@ -406,7 +400,7 @@ __global__ __launch_bounds__(kKvThreads) void kv_compact(KvArgs a) {
         for (uint32_t u = 0; u < U; ++u) {
             if (now.pt[u] >= 0) {
                 const uint32_t j = j0 + u * step + r0;
-                if (data) *reinterpret_cast<u32x4*>(base + ((uint32_t)now.pt[u] * a.page_stride + (j & in) * a.token_stride) * es) = x.x[u];
+                if (data) __builtin_nontemporal_store(x.x[u], reinterpret_cast<u32x4*>(base + ((uint32_t)now.pt[u] * a.page_stride + (j & in) * a.token_stride) * es));
                 if (scale) sc[scale_place(a, layer, (uint32_t)now.pt[u], head, j & in)] = x.s[u];
             }
         }
@@ -523,10 +517,10 @@ __global__ __launch_bounds__(kKvThreads) void kv_append(KvAppendArgs p) {
                         const int w = __builtin_amdgcn_cvt_pk_fp8_f32(e[0], e[1], 0, false);
                         q[h] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(e[2], e[3], w, true);
                     }
-                    if (ok && data) *reinterpret_cast<u32x2*>(base + at) = u32x2{q[0], q[1]};
+                    if (ok && data) __builtin_nontemporal_store(u32x2{q[0], q[1]}, reinterpret_cast<u32x2*>(base + at));
                     if (ok && chunk == 0u) sc[((uint64_t)(uint32_t)page[u] * a.kv_heads << a.page_shift) + tok] = scale;
                 } else {
-                    if (ok && data) *reinterpret_cast<u32x4*>(base + at) = x[u];
+                    if (ok && data) __builtin_nontemporal_store(x[u], reinterpret_cast<u32x4*>(base + at));
                 }
             }
         }
@@ -556,7 +550,11 @@ hipError_t launch_kv_grow(const KvArgs& args, hipStream_t st) {
     hipLaunchKernelGGL(kv_grow, dim3(1), dim3(kGrowThreads), 0, st, a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(kv_copy, dim3(2048), dim3(kKvThreads), 0, st, a);
+    a.pass_shift = 0;
+    while (((uint32_t)kKvThreads << a.pass_shift) < a.page_tokens * a.cp) ++a.pass_shift;
+    // (as many workgroups as a page of every request takes)
+    const uint64_t units = (uint64_t)a.n * a.layers * 2u * a.kv_heads << a.pass_shift;
+    hipLaunchKernelGGL(kv_copy, dim3(units < 16384u ? (uint32_t)units : 16384u), dim3(kKvThreads), 0, st, a);
     return hipGetLastError();
 }
 

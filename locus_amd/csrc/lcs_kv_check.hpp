@@ -109,7 +109,8 @@ inline int check_kv_append(const lcs_kv_cache* c, const lcs_kv_append_batch* b, 
     return LCS_OK;
 }
 
-inline int check_tree_attn(const lcs_tree_attn_batch* b, const lcs_tree_attn_out* o, uint32_t max_req, const char** why) {
+inline int check_tree_attn(const lcs_tree_attn_batch* b, const lcs_tree_attn_out* o, uint32_t max_req, uint32_t max_pairs,
+                           const char** why) {
     const Why w{why};
     if (!b || !o) return w.no("null attention argument");
     const lcs_kv_cache* c = b->cache;
@@ -136,6 +137,7 @@ inline int check_tree_attn(const lcs_tree_attn_batch* b, const lcs_tree_attn_out
     if (b->q_stride % 8u || b->k_stride % 8u || b->v_stride % 8u || o->o_stride % 8u) return w.no("strides must be multiples of 16 bytes");
     if (b->k_stride > 1u << 25 || b->v_stride > 1u << 25) return w.no("k_stride and v_stride must be at most 2^25");
     if ((uint64_t)b->n_seq * b->rows_per_seq * b->heads > 0x7fffffffull) return w.over("too many rows and heads for a call");
+    if ((uint64_t)b->n_seq * c->kv_heads > max_pairs) return w.over("at most 65536 sequences x kv heads a call");
     // (steps of 128 tokens, of every sequence and kv head)
     const uint64_t steps = ((uint64_t)c->max_pages * c->page_tokens + 127u) / 128u + 2u;
     if (steps > 0x40000000ull || steps * b->n_seq * c->kv_heads > 0x40000000ull) return w.over("sequences, table and heads beyond 2^30 steps of 128 tokens");

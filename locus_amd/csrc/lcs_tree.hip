@@ -129,12 +129,14 @@ __device__ __forceinline__ constexpr uint32_t swz_v(uint32_t r) {
 
 // Where each sequence's steps lie on the line of all: lane l holds sequences per * l ..
 // per * (l + 1) - 1 (at most 16).
-struct Line {
-    uint32_t per, before, total;   // steps ahead of the lane's sequences, of all sequences
-    bool bad;
-};
 struct Seq {
     uint32_t len, steps;   // cached tokens; steps, those of the new tokens included
+    int32_t slot;
+};
+struct Line {
+    uint32_t per, before, total;   // steps ahead of the lane's sequences, of all sequences
+    Seq one;                       // the lane's last sequence
+    bool bad;
 };
 __device__ __forceinline__ Seq seq_of(const TreeArgs& a, uint32_t i, bool& bad) {
     const int32_t slot = a.c.seq ? a.c.seq[i] : (int32_t)i;
@@ -148,14 +150,17 @@ __device__ __forceinline__ Seq seq_of(const TreeArgs& a, uint32_t i, bool& bad) 
         bad = true;
         len = (uint32_t)most;
     }
-    return Seq{len, (len + kStepKeys - 1u) / kStepKeys + a.new_steps};
+    return Seq{len, (len + kStepKeys - 1u) / kStepKeys + a.new_steps, slot};
 }
 __device__ __forceinline__ Line line_of(const TreeArgs& a) {
-    Line l{(a.c.n + kWave - 1u) / kWave, 0u, 0u, false};
+    Line l{(a.c.n + kWave - 1u) / kWave, 0u, 0u, Seq{0u, 0u, 0}, false};
     uint32_t sum = 0;
     for (uint32_t k = 0; k < l.per; ++k) {
         const uint32_t i = (uint32_t)lane_id() * l.per + k;
-        if (i < a.c.n) sum += seq_of(a, i, l.bad).steps;
+        if (i < a.c.n) {
+            l.one = seq_of(a, i, l.bad);
+            sum += l.one.steps;
+        }
     }
     const uint32_t incl = wave_scan_incl_u(sum);
     l.before = incl - sum;
@@ -214,17 +219,24 @@ __global__ __launch_bounds__(kTreeWaves * kWave, kTreePerCu<DP>) void tree_attn(
         const uint64_t le = ballot(line.before * H <= x && lane * line.per < a.c.n);
         const uint32_t who = 63u - (uint32_t)__builtin_clzll(le);
         uint32_t i = who * line.per, at = uniform((uint32_t)__builtin_amdgcn_readlane((int)line.before, (int)who)) * H;
-        bool dummy = false;
-        Seq sq = seq_of(a, i, dummy);
-        while (x - at >= sq.steps * H) {
-            at += sq.steps * H;
-            sq = seq_of(a, ++i, dummy);
+        Seq sq;
+        if (line.per == 1u) {   // (uniform)
+            sq.len = (uint32_t)__builtin_amdgcn_readlane((int)line.one.len, (int)who);
+            sq.steps = (uint32_t)__builtin_amdgcn_readlane((int)line.one.steps, (int)who);
+            sq.slot = __builtin_amdgcn_readlane(line.one.slot, (int)who);
+        } else {
+            bool dummy = false;
+            sq = seq_of(a, i, dummy);
+            while (x - at >= sq.steps * H) {
+                at += sq.steps * H;
+                sq = seq_of(a, ++i, dummy);
+            }
         }
         i = uniform(i);
         const uint32_t len = uniform(sq.len), steps = uniform(sq.steps);
-        const uint32_t y = x - at, kvh = y / steps, s0 = y % steps, s1 = min(steps, s0 + (end - x));
+        const int32_t slot = (int32_t)uniform((uint32_t)sq.slot);
+        const uint32_t y = x - uniform(at), kvh = y / steps, s0 = y % steps, s1 = min(steps, s0 + (end - x));
         const uint32_t ctx_steps = steps - a.new_steps;
-        const int32_t slot = (int32_t)uniform((uint32_t)(a.c.seq ? a.c.seq[i] : (int32_t)i));
         const int32_t* row = a.c.table + (uint64_t)(len > 0u ? (uint32_t)slot : 0u) * a.c.max_pages;
         const unsigned char* kb = static_cast<const unsigned char*>(a.c.k) + (a.c.layer * a.c.layer_stride + kvh * a.c.head_stride) * (F8 ? 1u : 2u);
         const unsigned char* vb = static_cast<const unsigned char*>(a.c.v) + (a.c.layer * a.c.layer_stride + kvh * a.c.head_stride) * (F8 ? 1u : 2u);
@@ -631,6 +643,8 @@ __global__ __launch_bounds__(kTreeWaves * kWave, kTreePerCu<DP>) void tree_attn(
         }
         __syncthreads();
         const bool complete = s0 == 0u && s1 == steps;
+        // (who shares the pair: its first and last pieces, and whether it begins inside the first)
+        if (s0 == 0u && rt == a.row_tile0 && tid_x() == 0u) a.spans[i * H + kvh] = piece | (x + steps - 1u) / share << 15 | (x != piece * share ? 1u << 31 : 0u);
         // (a workgroup has at most two incomplete segments: one that begins with the piece, one that ends with it)
         float* part = a.part + ((uint64_t)b * 2u + (x == piece * share ? 0u : 1u)) * Part<DP, MT>::kFloats;
         for (uint32_t it = tid_x(); it < kRows * (DP / 4u); it += kTreeWaves * kWave) {
@@ -667,39 +681,74 @@ __global__ __launch_bounds__(kTreeWaves * kWave, kTreePerCu<DP>) void tree_attn(
     }
 }
 
-// Joins the partial sums of the pairs that several workgroups share: 256 threads take
-// 1024 / DP rows of a row tile, four elements each.
-template <int DP, int MT>
+// Joins the partial sums of the pairs that several workgroups share: DP / 4 threads a row, four
+// elements each, and SPLIT such groups that take the partial results in turn, eight under way
+// in each (131000 tokens of 8 heads over 512 workgroups: 25 us with one at a time, of one group).
+template <int DP, int MT, int SPLIT>
 __global__ __launch_bounds__(256) void tree_join(TreeArgs a) {
     using P = Part<DP, MT>;
-    constexpr uint32_t kPer = 1024u / DP, kBlocks = P::kRows / kPer;
+    constexpr uint32_t kPer = 1024u / DP / SPLIT, kBlocks = P::kRows / kPer, U = 8;
+    __shared__ f32x4 os[SPLIT > 1 ? 256 : 1];
+    __shared__ float ms[SPLIT > 1 ? 256 : 1], zs[SPLIT > 1 ? 256 : 1];
+    const uint32_t span = a.spans[wg_x()];
+    const uint32_t p0 = span & 0x7fffu, p1 = span >> 15 & 0xffffu;
+    if (p0 == p1) return;
     const uint32_t i = wg_x() / a.c.kv_heads, kvh = wg_x() % a.c.kv_heads;
-    const uint32_t rt = __builtin_amdgcn_workgroup_id_y() / kBlocks, rr = __builtin_amdgcn_workgroup_id_y() % kBlocks * kPer + tid_x() / (DP / 4u);
+    const uint32_t rt = __builtin_amdgcn_workgroup_id_y() / kBlocks, row = tid_x() / (DP / 4u);
+    const uint32_t rr = __builtin_amdgcn_workgroup_id_y() % kBlocks * kPer + row % kPer, split = row / kPer;
     const uint32_t c = tid_x() % (DP / 4u), pr = (rt + a.row_tile0) * P::kRows + rr;
-    const Line line = line_of(a);
-    const uint32_t H = a.c.kv_heads, all = line.total * H, share = share_of(a, all);
-    const uint32_t who = i / line.per;
-    uint32_t at = uniform((uint32_t)__builtin_amdgcn_readlane((int)line.before, (int)who)) * H;
-    bool dummy = false;
-    for (uint32_t k = who * line.per; k < i; ++k) at += seq_of(a, k, dummy).steps * H;
-    const uint32_t steps = seq_of(a, i, dummy).steps;
-    at += kvh * steps;
-    const uint32_t p0 = at / share, p1 = (at + steps - 1u) / share;
-    if (p0 == p1 || pr >= a.rows_per_seq * a.group) return;
     float M = kUnset, z = 0.0f;
     f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (uint32_t p = p0; p <= p1; ++p) {
-        const uint32_t b = (p / 8u * a.row_tiles + rt) * 8u + p % 8u;
-        const float* part = a.part + ((uint64_t)b * 2u + (p * share >= at ? 0u : 1u)) * P::kFloats;
-        const float m = part[P::kRows * DP + rr], s = part[P::kRows * DP + P::kRows + rr];
-        const f32x4 v = *reinterpret_cast<const f32x4*>(part + rr * DP + 4u * c);
-        const float now = f_max(M, m), fo = exp2_f(M - now), fn = exp2_f(m - now);
+    for (uint32_t q = p0 + split; q <= p1; q += U * SPLIT) {
+        float m[U], s[U], now = M;
+        f32x4 v[U];
+#pragma unroll
+        for (uint32_t u = 0; u < U; ++u) {
+            const uint32_t p = q + u * SPLIT, pu = p <= p1 ? p : q;
+            const uint32_t b = (pu / 8u * a.row_tiles + rt) * 8u + pu % 8u;
+            const float* part = a.part + ((uint64_t)b * 2u + (pu == p0 ? span >> 31 : 0u)) * P::kFloats;
+            m[u] = p <= p1 ? part[P::kRows * DP + rr] : kUnset;
+            s[u] = p <= p1 ? part[P::kRows * DP + P::kRows + rr] : 0.0f;
+            v[u] = *reinterpret_cast<const f32x4*>(part + rr * DP + 4u * c);
+        }
+#pragma unroll
+        for (uint32_t u = 0; u < U; ++u) now = f_max(now, m[u]);
+        const float f = exp2_f(M - now);
+        z *= f;
+        o *= f;
         M = now;
-        z = z * fo + s * fn;
-        o = o * fo + v * fn;
+#pragma unroll
+        for (uint32_t u = 0; u < U; ++u) {
+            if (q + u * SPLIT <= p1) {   // (what is not there weighs nothing, whatever it repeats)
+                const float g = exp2_f(m[u] - now);
+                z += s[u] * g;
+                o += v[u] * g;
+            }
+        }
+    }
+    if constexpr (SPLIT > 1) {
+        os[tid_x()] = o;
+        ms[tid_x()] = M;
+        zs[tid_x()] = z;
+        __syncthreads();
+        if (split != 0u) return;
+        float now = M;
+#pragma unroll
+        for (uint32_t k = 1; k < SPLIT; ++k) now = f_max(now, ms[tid_x() + k * (256u / SPLIT)]);
+        float f = exp2_f(M - now);
+        z *= f;
+        o *= f;
+#pragma unroll
+        for (uint32_t k = 1; k < SPLIT; ++k) {
+            const uint32_t at = tid_x() + k * (256u / SPLIT);
+            f = exp2_f(ms[at] - now);
+            z += zs[at] * f;
+            o += os[at] * f;
+        }
+        M = now;
     }
     const uint32_t D = a.c.head_dim, h = kvh * a.group + pr % a.group;
-    if (4u * c >= D) return;
+    if (pr >= a.rows_per_seq * a.group || 4u * c >= D) return;
     const bool empty = z == 0.0f;
     const float f = 1.0f / z;
     const uint64_t rw = (uint64_t)i * a.rows_per_seq + pr / a.group;
@@ -725,7 +774,10 @@ hipError_t launch(TreeArgs a, uint32_t cus, hipStream_t st) {
         hipLaunchKernelGGL((tree_attn<DP, MT, F8, ST>), dim3(a.pieces * a.row_tiles), dim3(kTreeWaves * kWave), 0, st, a);
         hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
-        hipLaunchKernelGGL((tree_join<DP, MT>), dim3(a.c.n * a.c.kv_heads, a.row_tiles * (16u * MT * DP / 1024u)), dim3(256), 0, st, a);
+        const uint32_t pairs = a.c.n * a.c.kv_heads, blocks = a.row_tiles * (16u * MT * DP / 1024u);
+        // (many partial results a pair: more threads for them)
+        if (pairs * 8u <= a.pieces) hipLaunchKernelGGL((tree_join<DP, MT, 4>), dim3(pairs, 4u * blocks), dim3(256), 0, st, a);
+        else hipLaunchKernelGGL((tree_join<DP, MT, 1>), dim3(pairs, blocks), dim3(256), 0, st, a);
         if ((e = hipGetLastError()) != hipSuccess) return e;
     }
     return hipSuccess;

@@ -25,7 +25,7 @@ extern "C" int requests(const lcs_kv_cache* c, uint32_t n, const int32_t* s, con
 extern "C" int compact(const lcs_kv_cache* c, uint32_t n, uint32_t m, const int32_t* s, const int32_t* a, const int32_t* b,
                        const int32_t* r, const char** why) { return check_kv_compact(c, n, m, s, a, b, r, 1024, why); }
 extern "C" int append(const lcs_kv_cache* c, const lcs_kv_append_batch* b, const char** why) { return check_kv_append(c, b, 1024, why); }
-extern "C" int attn(const lcs_tree_attn_batch* b, const lcs_tree_attn_out* o, const char** why) { return check_tree_attn(b, o, 1024, why); }
+extern "C" int attn(const lcs_tree_attn_batch* b, const lcs_tree_attn_out* o, const char** why) { return check_tree_attn(b, o, 1024, 65536, why); }
 extern "C" int verify(const lcs_tree_verify_batch* b, const lcs_tree_verify_out* o, const char** why) { return check_tree_verify(b, o, why); }
 ''')
     so = str(d / "check.so")
@@ -140,6 +140,16 @@ def test_attention(lib):
                    (dict(q_stride=6 * 64 + 4), -1), (dict(o_stride=6 * 64 + 2), -1), (dict(cache=None), -1), (dict(cache=cache(pages=0)), -1),
                    (dict(n_seq=1024, rows_per_seq=256, heads=3 * 4096, q_stride=1 << 20, o_stride=1 << 20), -4)]:
         assert call(lib.attn, *attn(**kw))[0] == rc, kw
+    wide = cache(kv_heads=128, head_stride=16 * 64, page_stride=128 * 16 * 64, layer_stride=1280 * 16 * 64)
+    many = dict(cache=wide, heads=128, q_stride=128 * 64, k_stride=128 * 64, v_stride=128 * 64, o_stride=128 * 64)
+    assert call(lib.attn, *attn(n_seq=512, **many)) == (0, "")
+    assert call(lib.attn, *attn(n_seq=513, **many))[0] == -4
+    assert call(lib.attn, *attn(k_stride=(1 << 25) + 8))[0] == -1
+    long = cache(seqs=1024, max_pages=2 ** 21 - 1, page_tokens=1024, kv_heads=64, head_dim=16, token_stride=16, head_stride=16 * 1024,
+                 page_stride=64 * 16 * 1024, layer_stride=640 * 16 * 1024)
+    few = dict(cache=long, heads=64, q_stride=1024, k_stride=1024, v_stride=1024, o_stride=1024)
+    assert call(lib.attn, *attn(n_seq=1, **few)) == (0, "")
+    assert call(lib.attn, *attn(n_seq=2, **few))[0] == -4
     b, o = attn()
     assert call(lib.attn, None, o)[0] == -1 and call(lib.attn, b, None)[0] == -1
 
