@@ -66,6 +66,14 @@ template <int N>
 __device__ __forceinline__ void wait_vm() {
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
+// A workgroup barrier for LDS: waits for no global store.
+__device__ __forceinline__ void lds_sync() {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
 __device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 // 16 bytes per lane from offset vo of a buffer to LDS at dst + 16 lane (dst is wave-uniform);
 // what lies past the buffer's size arrives as zeros.
@@ -305,8 +313,35 @@ __global__ __launch_bounds__(kTreeWaves * kWave, kTreePerCu<DP>) void tree_attn(
         Tile tile[ST + 1];   // of tiles j, j + 1, .. j + ST
 #pragma unroll
         for (int k = 0; k <= ST; ++k) tile[k] = pages_of((uint32_t)k);
+        // ---- the new tokens' tiles (bf16 always), the first one's loads issued where LDS is free ahead of it ----
+        constexpr int kNew = (int)(kTileKeys * kNewB / 1024u);   // DMA loads of a tile's keys, and of its values
+        const uint32_t st0 = max(s0, ctx_steps);
+        auto new_first = [&](uint32_t st) -> uint32_t { return (st - ctx_steps) * kStepKeys + w * kTileKeys; };
+        const bool ahead = st0 < s1 && new_first(st0) < N;
+        auto issue_new = [&](bool values, uint32_t n0, unsigned char* dst) {
+            constexpr uint32_t CPN = kNewB / 16u, RPN = 64u / CPN;
+            const uint32_t rows = min(N - n0, kTileKeys), stride = (uint32_t)(values ? a.v_stride : a.k_stride) * 2u;
+            const uint16_t* src = (values ? a.v : a.k) + ((uint64_t)i * N + n0) * (values ? a.v_stride : a.k_stride) + kvh * D;
+            const __amdgpu_buffer_rsrc_t rs = buffer_of(reinterpret_cast<const unsigned char*>(src), (rows - 1u) * stride + 2u * D);
+            uint32_t ln = lane;   // (opaque: what follows from it is not kept over the cached tiles)
+            asm volatile("" : "+v"(ln));
+#pragma unroll
+            for (int ii = 0; ii < kNew; ++ii) {
+                const uint32_t r = RPN * (uint32_t)ii + ln / CPN, c = ln % CPN ^ (values ? swz_v<kNewB, false>(r) : swz_k<kNewB>(r));
+                dma16(rs, dst + 1024 * ii, r < rows && 8u * c < D ? r * stride + 16u * c : kNoByte);
+            }
+        };
+        // their places: with one stage its keys' and values' places; with two the other stage, and
+        // for 8-bit rows (a new row takes two cached ones' room) the last tile's own for the values
+        unsigned char* new_k = mine;
+        unsigned char* new_v = mine + kTileKeys * kNewB;
+        if (ahead && nct == 0u) {
+            issue_new(false, new_first(st0), new_k);
+            issue_new(true, new_first(st0), new_v);
+        }
+
         // ---- the rows: packed as (new token, query head of the group) ----
-        bf16x8 qf[MT][kKS];
+        u32x4 qr[MT][kKS];
         uint32_t node[MT];
         bool live[MT];
 #pragma unroll
@@ -314,16 +349,11 @@ __global__ __launch_bounds__(kTreeWaves * kWave, kTreePerCu<DP>) void tree_attn(
             const uint32_t pr = rt * kRows + 16u * m + n;
             live[m] = pr < R;
             node[m] = live[m] ? pr / a.group : 0u;
-            const uint16_t* q = a.q + ((uint64_t)i * N + node[m]) * a.q_stride + (kvh * a.group + (live[m] ? pr % a.group : 0u)) * D;
+            const uint16_t* q = a.q + ((uint64_t)i * N + node[m]) * a.q_stride + (kvh * a.group + (live[m] ? pr - node[m] * a.group : 0u)) * D;
 #pragma unroll
-            for (uint32_t ks = 0; ks < kKS; ++ks) {
-                const uint32_t c = chunk8(ks);
-                u32x4 v = {0u, 0u, 0u, 0u};
-                if (live[m] && 8u * c < D && a.scale != 0.0f) v = *reinterpret_cast<const u32x4*>(q + 8u * c);
-                if (a.scale < 0.0f) v ^= 0x80008000u;
-                qf[m][ks] = __builtin_bit_cast(bf16x8, v);
-            }
+            for (uint32_t ks = 0; ks < kKS; ++ks) qr[m][ks] = *reinterpret_cast<const u32x4*>(q + (8u * chunk8(ks) < D ? 8u * chunk8(ks) : 0u));
         }
+
 #pragma unroll
         for (int k = 0; k < ST; ++k) {
             if ((uint32_t)k < nct) {
@@ -332,6 +362,19 @@ __global__ __launch_bounds__(kTreeWaves * kWave, kTreePerCu<DP>) void tree_attn(
             }
         }
 
+        // (rows past the last and dims past the head's count as zeros; so do all at a scale of 0,
+        // whose scores are 0; a scale below 0 changes the sign here)
+        bf16x8 qf[MT][kKS];
+        const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (uint32_t ks = 0; ks < kKS; ++ks) {
+                const bool in = live[m] && 8u * chunk8(ks) < D && a.scale != 0.0f;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) qr[m][ks][k] = in ? qr[m][ks][k] ^ flip : 0u;
+                qf[m][ks] = __builtin_bit_cast(bf16x8, qr[m][ks]);
+            }
         f32x4 acc[MT][kDT];
         float top[MT], sum[MT];
 #pragma unroll
@@ -424,6 +467,17 @@ __global__ __launch_bounds__(kTreeWaves * kWave, kTreePerCu<DP>) void tree_attn(
             }
             wait_lds();
             const bool more = j + ST < nct;
+            const bool then = ahead && j + 1u == nct;   // (the new tokens come next)
+            if (then) {
+                if constexpr (ST == 1) {
+                    issue_new(false, new_first(st0), new_k);
+                } else {
+                    new_k = mine + (stage ? 0u : kStage);
+                    issue_new(false, new_first(st0), new_k);
+                    new_v = F8 ? mine + stage : new_k + kTileKeys * kNewB;
+                    if constexpr (!F8) issue_new(true, new_first(st0), new_v);
+                }
+            }
             if (more) issue_k(tile[ST], j + ST, stage);
 #pragma unroll
             for (int m = 0; m < MT; ++m) s[m][0] = s[m][1] = zero;
@@ -460,7 +514,8 @@ __global__ __launch_bounds__(kTreeWaves * kWave, kTreePerCu<DP>) void tree_attn(
                 if (there != (left >= 32u ? ~0u : (1u << left) - 1u) && lane == 0u) atomicOr(a.c.status, kStatusPages);   // (a page is missing)
             }
             weigh(vs, F8);
-            if (!full) wait_vm<0>();
+            if (then) wait_vm<ST == 2 && !F8 ? 2 * kNew : kNew>();
+            else if (!full) wait_vm<0>();
             else if (more) wait_vm<(ST - 1) * (kNK + kNI) + kNK>();
             else wait_vm<(ST - 1) * (kNK + kNI)>();
             const uint32_t lv = lds_at(at_v);
@@ -476,6 +531,9 @@ __global__ __launch_bounds__(kTreeWaves * kWave, kTreePerCu<DP>) void tree_attn(
                 else read_tr16<16 * kRowB>(ad, o);
 #pragma unroll
                 for (uint32_t k = 0; k < 4; ++k) vc[t + k] = o[k];
+            }
+            if constexpr (ST == 1 || F8) {
+                if (then) issue_new(true, new_first(st0), new_v);
             }
             if (more) issue_v(tile[ST], j + ST, stage);
             stage = stage + kStage == ST * kStage ? 0u : stage + kStage;
@@ -501,27 +559,19 @@ __global__ __launch_bounds__(kTreeWaves * kWave, kTreePerCu<DP>) void tree_attn(
             }
         }
 
-        // ---- the new tokens' tiles (bf16 always) ----
-        for (uint32_t st = max(s0, ctx_steps); st < s1; ++st) {
-            const uint32_t n0 = (st - ctx_steps) * kStepKeys + w * kTileKeys;
+        // ---- the new tokens' products ----
+        for (uint32_t st = st0; st < s1; ++st) {
+            const uint32_t n0 = new_first(st);
             if (n0 >= N) continue;   // (uniform)
-            constexpr uint32_t CPR = kNewB / 16u, RPI = 64u / CPR;   // (as above, of the new rows)
-            constexpr int NI = (int)(kTileKeys * kNewB / 1024u);
-            uint32_t ln = lane;   // (opaque: what follows from it is not kept over the cached tiles)
+            uint32_t ln = lane;   // (opaque, as above)
             asm volatile("" : "+v"(ln));
-            const uint32_t lr = ln / CPR, pl = ln % CPR, lane_n = ln & 15u, lg = ln >> 4;
-            unsigned char* const at_v = mine + kTileKeys * kNewB;
-            wait_lds();   // (the last tile's reads)
-            const uint64_t rw = (uint64_t)i * N + n0;
-            const uint32_t rows = min(N - n0, kTileKeys), kst = (uint32_t)a.k_stride * 2u, vst = (uint32_t)a.v_stride * 2u;
-            const __amdgpu_buffer_rsrc_t krs = buffer_of(reinterpret_cast<const unsigned char*>(a.k + rw * a.k_stride + kvh * D), (rows - 1u) * kst + 2u * D);
-            const __amdgpu_buffer_rsrc_t vrs = buffer_of(reinterpret_cast<const unsigned char*>(a.v + rw * a.v_stride + kvh * D), (rows - 1u) * vst + 2u * D);
-#pragma unroll
-            for (int ii = 0; ii < NI; ++ii) {
-                const uint32_t r = RPI * (uint32_t)ii + lr, ck = pl ^ swz_k<kNewB>(r), cv = pl ^ swz_v<kNewB, false>(r);
-                dma16(krs, mine + 1024 * ii, r < rows && 8u * ck < D ? r * kst + 16u * ck : kNoByte);
-                dma16(vrs, at_v + 1024 * ii, r < rows && 8u * cv < D ? r * vst + 16u * cv : kNoByte);
+            const uint32_t lane_n = ln & 15u, lg = ln >> 4;
+            if (st != st0) {
+                wait_lds();   // (the last tile's reads)
+                issue_new(false, n0, new_k);
+                issue_new(true, n0, new_v);
             }
+            unsigned char* const at_v = new_v;
             uint32_t see[MT];
 #pragma unroll
             for (int m = 0; m < MT; ++m) {
@@ -537,7 +587,7 @@ __global__ __launch_bounds__(kTreeWaves * kWave, kTreePerCu<DP>) void tree_attn(
 #pragma unroll
                 for (uint32_t k = 0; k < kKS; ++k) {
                     const uint32_t r = 16u * h + lane_n, c = F8 ? 2u * (lg + 4u * (k / 2u)) + (k & 1u) : 4u * k + lg;
-                    const bf16x8 kf = *reinterpret_cast<const bf16x8*>(mine + r * kNewB + (c ^ swz_k<kNewB>(r)) * 16u);
+                    const bf16x8 kf = *reinterpret_cast<const bf16x8*>(new_k + r * kNewB + (c ^ swz_k<kNewB>(r)) * 16u);
 #pragma unroll
                     for (int m = 0; m < MT; ++m) s[m][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[m][k], s[m][h], 0, 0, 0);
                 }
@@ -550,7 +600,7 @@ __global__ __launch_bounds__(kTreeWaves * kWave, kTreePerCu<DP>) void tree_attn(
             // in the keys' place (+inf 1, -inf 2, a NaN both).
             bool wild = false;
 #pragma unroll 1
-            for (int ii = 0; ii < NI; ++ii) {
+            for (int ii = 0; ii < kNew; ++ii) {
                 const u32x4 v = *reinterpret_cast<const u32x4*>(at_v + 1024 * ii + 16u * ln);
 #pragma unroll
                 for (int k = 0; k < 4; ++k) wild = wild || (v[k] & 0x7f80u) == 0x7f80u || (v[k] & 0x7f800000u) == 0x7f800000u;
@@ -559,7 +609,7 @@ __global__ __launch_bounds__(kTreeWaves * kWave, kTreePerCu<DP>) void tree_attn(
             if (any_wild) {
                 wait_lds();   // (the keys have been read)
 #pragma unroll 1
-                for (int ii = 0; ii < NI; ++ii) {
+                for (int ii = 0; ii < kNew; ++ii) {
                     u32x4* const pv = reinterpret_cast<u32x4*>(at_v + 1024 * ii + 16u * ln);
                     u32x4 v = *pv, kind;
 #pragma unroll
@@ -570,7 +620,7 @@ __global__ __launch_bounds__(kTreeWaves * kWave, kTreePerCu<DP>) void tree_attn(
                         v[k] &= (lo ? 0u : 0xffffu) | (hi ? 0u : 0xffff0000u);
                     }
                     *pv = v;
-                    *reinterpret_cast<u32x4*>(mine + 1024 * ii + 16u * ln) = kind;
+                    *reinterpret_cast<u32x4*>(new_k + 1024 * ii + 16u * ln) = kind;
                 }
                 wait_lds();
             }
@@ -590,7 +640,7 @@ __global__ __launch_bounds__(kTreeWaves * kWave, kTreePerCu<DP>) void tree_attn(
                         acc[m][t0 + t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, v[t]), pf[m], acc[m][t0 + t], 0, 0, 0);
             }
             if (any_wild) {   // 2^127 times 2 for each that is seen: infinite sums, of both signs for a NaN
-                const uint32_t lk = lv - kTileKeys * kNewB;
+                const uint32_t lk = lds_at(new_k) + (lv - lds_at(at_v));
                 bf16x8 two[MT];
 #pragma unroll
                 for (int m = 0; m < MT; ++m) {
@@ -641,7 +691,7 @@ __global__ __launch_bounds__(kTreeWaves * kWave, kTreePerCu<DP>) void tree_attn(
             for (uint32_t t = 0; t < kDT; ++t)
                 *reinterpret_cast<f32x4*>(mine + (16u * m + n) * DP * 4u + ((4u * t + g) ^ n) * 16u) = acc[m][t];
         }
-        __syncthreads();
+        lds_sync();
         const bool complete = s0 == 0u && s1 == steps;
         // (who shares the pair: its first and last pieces, and whether it begins inside the first)
         if (s0 == 0u && rt == a.row_tile0 && tid_x() == 0u) a.spans[i * H + kvh] = piece | (x + steps - 1u) / share << 15 | (x != piece * share ? 1u << 31 : 0u);
@@ -676,7 +726,7 @@ __global__ __launch_bounds__(kTreeWaves * kWave, kTreePerCu<DP>) void tree_attn(
                 if (c == 0u && a.lse) a.lse[rw * a.heads + h] = empty ? -__builtin_huge_valf() : (M + __builtin_amdgcn_logf(z)) * kLn2;
             }
         }
-        __syncthreads();
+        lds_sync();
         x += s1 - s0;
     }
 }
