@@ -194,24 +194,26 @@ struct Part {
 
 }  // namespace
 
-template <int DP, int MT, bool F8, int ST>
-__global__ __launch_bounds__(kTreeWaves * kWave, kTreePerCu<DP>) void tree_attn(TreeArgs a) {
-    constexpr uint32_t kRows = 16u * MT, kDT = DP / 16, kKS = DP / 32;
+template <int DP, int MT, bool F8, int ST, int WR>
+__global__ __launch_bounds__(kTreeWaves * WR * kWave, WR == 1 ? kTreePerCu<DP> : 1) void tree_attn(TreeArgs a) {
+    static_assert(WR == 1 || (WR == 2 && ST == 2), "the schedule of shared tiles");
+    constexpr uint32_t kMine = 16u * MT, kRows = kMine * WR, kDT = DP / 16, kKS = DP / 32;   // rows of a wave, of the workgroup
     constexpr uint32_t kRowB = DP * (F8 ? 1 : 2), kNewB = DP * 2;                 // bytes of a cached row and of a new one in LDS
     constexpr uint32_t kScaleB = F8 ? 256u : 0u;
     constexpr uint32_t kStage = 2u * kTileKeys * kRowB + kScaleB;
     constexpr uint32_t kMergeB = kRows * DP * 4u;
-    constexpr uint32_t kMax1 = ST * kStage > 2u * kTileKeys * kNewB ? ST * kStage : 2u * kTileKeys * kNewB;
+    constexpr uint32_t kNewAt = WR == 2 && F8 ? ST * kStage : 0u;   // (shared 8-bit tiles leave room for new ones beside them)
+    constexpr uint32_t kMax1 = kNewAt + 2u * kTileKeys * kNewB > ST * kStage ? kNewAt + 2u * kTileKeys * kNewB : ST * kStage;
     constexpr uint32_t kRegion = kMax1 > kMergeB ? kMax1 : kMergeB;
     constexpr int kNI = (int)(kTileKeys * kRowB / 1024u);      // DMA loads of a tile's keys, and of its values
     constexpr int kNK = kNI + (F8 ? 1 : 0);
     __shared__ __attribute__((aligned(1024))) unsigned char lds[kTreeWaves * kRegion];
     __shared__ float stat[kTreeWaves][2][kRows];
-    const uint32_t lane = (uint32_t)lane_id(), w = uniform(tid_x() / kWave), n = lane & 15u, g = lane >> 4;
+    const uint32_t lane = (uint32_t)lane_id(), wave = uniform(tid_x() / kWave), w = wave % kTreeWaves, wr = wave / kTreeWaves, n = lane & 15u, g = lane >> 4;
     unsigned char* const mine = lds + w * kRegion;
     const uint32_t b = wg_x(), piece = b / 8u / a.row_tiles * 8u + b % 8u, rt = b / 8u % a.row_tiles + a.row_tile0;
     const Line line = line_of(a);
-    if (line.bad && b == 0u && w == 0u) atomicOr(a.c.status, kStatusPages);
+    if (line.bad && b == 0u && wave == 0u) atomicOr(a.c.status, kStatusPages);
     const uint32_t H = a.c.kv_heads, all = line.total * H, share = share_of(a, all);
     const uint32_t end = min(all, (piece + 1u) * share);   // (all < 2^31 / ...: checked on the host)
     const uint32_t D = a.c.head_dim, N = a.rows_per_seq, R = N * a.group;
@@ -251,19 +253,18 @@ __global__ __launch_bounds__(kTreeWaves * kWave, kTreePerCu<DP>) void tree_attn(
 
         // ---- the wave's cached tiles: tile j starts at token first + 128 j ----
         const uint32_t c1 = min(s1, ctx_steps), first = s0 * kStepKeys + w * kTileKeys;
-        const uint32_t past = min(c1 * kStepKeys, len);
-        const uint32_t nct = s0 < c1 && first < past ? (past - first + kStepKeys - 1u) / kStepKeys : 0u;
+        const uint32_t nct = s0 < c1 ? c1 - s0 : 0u;   // (the last one may lie past the length: all zeros, unseen)
         struct Tile {
             int32_t p0, p1;   // the pages of its first and last 16 tokens
         };
         auto pages_of = [&](uint32_t j) -> Tile {
             const uint32_t t0 = first + (j < nct ? j : 0u) * kStepKeys;
-            const uint32_t q0 = t0 >> a.c.page_shift, q1 = min((t0 + 16u) >> a.c.page_shift, a.c.max_pages - 1u);
+            const uint32_t q0 = min(t0 >> a.c.page_shift, a.c.max_pages - 1u), q1 = min((t0 + 16u) >> a.c.page_shift, a.c.max_pages - 1u);
             if (nct == 0u) return Tile{0, 0};
             return Tile{scalar_load(row + q0), scalar_load(row + q1)};
         };
         auto mask_of = [&](const Tile& t, uint32_t j) -> uint32_t {   // the tile's keys that are there
-            const uint32_t t0 = first + j * kStepKeys, left = len - t0;
+            const uint32_t t0 = first + j * kStepKeys, left = t0 < len ? len - t0 : 0u;
             uint32_t m = left >= 32u ? ~0u : (1u << left) - 1u;
             if ((uint32_t)t.p0 >= a.c.pages) m &= 0xffff0000u;
             if ((uint32_t)t.p1 >= a.c.pages) m &= 0x0000ffffu;
@@ -278,23 +279,24 @@ __global__ __launch_bounds__(kTreeWaves * kWave, kTreePerCu<DP>) void tree_attn(
             const uint32_t ch = (lane % CPR) ^ (values ? swz_v<kRowB, F8>(r) : swz_k<kRowB>(r));
             return 16u * ch < D * (F8 ? 1u : 2u) ? (r & 15u) * tsb + 16u * ch : kNoByte;
         };
-        uint32_t vo_k[kHalf], vo_v[F8 ? kNI : kHalf];   // (8-bit values: the second half is permuted by other bits)
+        constexpr int kVo = F8 && WR == 1 ? kNI : kHalf;   // (8-bit values: the second half is permuted by other bits)
+        uint32_t vo_k[kHalf], vo_v[kVo];
 #pragma unroll
         for (int ii = 0; ii < kHalf; ++ii) vo_k[ii] = offset_of(false, RPI * (uint32_t)ii + lane / CPR);
 #pragma unroll
-        for (int ii = 0; ii < (F8 ? kNI : kHalf); ++ii) vo_v[ii] = offset_of(true, RPI * (uint32_t)ii + lane / CPR);
+        for (int ii = 0; ii < kVo; ++ii) vo_v[ii] = offset_of(true, RPI * (uint32_t)ii + lane / CPR + (WR == 2 ? 16u * wr : 0u));
         auto issue_rows = [&](bool values, const Tile& t, uint32_t j, unsigned char* dst) {
             const uint32_t t0 = first + j * kStepKeys, m = mask_of(t, j);
             const unsigned char* base = values ? vb : kb;
             const uint64_t ps = a.c.page_stride * (F8 ? 1u : 2u);
 #pragma unroll
-            for (uint32_t h = 0; h < 2; ++h) {
-                const uint32_t there = m >> (16u * h) & 0xffffu, page = there ? (uint32_t)(h ? t.p1 : t.p0) : 0u;
+            for (uint32_t q = 0; q < 2u / WR; ++q) {   // (two waves that share a tile bring a half each)
+                const uint32_t h = WR == 2 ? wr : q, there = m >> (16u * h) & 0xffffu, page = there ? (uint32_t)(h ? t.p1 : t.p0) : 0u;
                 const __amdgpu_buffer_rsrc_t rs = buffer_of(base + page * ps + ((t0 + 16u * h) & (a.c.page_tokens - 1u)) * ts,
                                                             (uint32_t)__builtin_popcount(there) * tsb);
 #pragma unroll
                 for (int ii = 0; ii < kHalf; ++ii)
-                    dma16(rs, dst + 1024 * (kHalf * h + ii), values ? vo_v[F8 ? kHalf * h + ii : ii] : vo_k[ii]);
+                    dma16(rs, dst + 1024 * (kHalf * h + ii), values ? vo_v[F8 && WR == 1 ? kHalf * q + ii : ii] : vo_k[ii]);
             }
         };
         auto issue_k = [&](const Tile& t, uint32_t j, uint32_t stage) {
@@ -326,15 +328,16 @@ __global__ __launch_bounds__(kTreeWaves * kWave, kTreePerCu<DP>) void tree_attn(
             uint32_t ln = lane;   // (opaque: what follows from it is not kept over the cached tiles)
             asm volatile("" : "+v"(ln));
 #pragma unroll
-            for (int ii = 0; ii < kNew; ++ii) {
+            for (int q = 0; q < kNew / WR; ++q) {
+                const int ii = q + (WR == 2 ? (int)wr * (kNew / 2) : 0);
                 const uint32_t r = RPN * (uint32_t)ii + ln / CPN, c = ln % CPN ^ (values ? swz_v<kNewB, false>(r) : swz_k<kNewB>(r));
                 dma16(rs, dst + 1024 * ii, r < rows && 8u * c < D ? r * stride + 16u * c : kNoByte);
             }
         };
         // their places: with one stage its keys' and values' places; with two the other stage, and
         // for 8-bit rows (a new row takes two cached ones' room) the last tile's own for the values
-        unsigned char* new_k = mine;
-        unsigned char* new_v = mine + kTileKeys * kNewB;
+        unsigned char* new_k = mine + kNewAt;
+        unsigned char* new_v = mine + kNewAt + kTileKeys * kNewB;
         if (ahead && nct == 0u) {
             issue_new(false, new_first(st0), new_k);
             issue_new(true, new_first(st0), new_v);
@@ -346,7 +349,7 @@ __global__ __launch_bounds__(kTreeWaves * kWave, kTreePerCu<DP>) void tree_attn(
         bool live[MT];
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
-            const uint32_t pr = rt * kRows + 16u * m + n;
+            const uint32_t pr = rt * kRows + wr * kMine + 16u * m + n;
             live[m] = pr < R;
             node[m] = live[m] ? pr / a.group : 0u;
             const uint16_t* q = a.q + ((uint64_t)i * N + node[m]) * a.q_stride + (kvh * a.group + (live[m] ? pr - node[m] * a.group : 0u)) * D;
@@ -358,7 +361,7 @@ __global__ __launch_bounds__(kTreeWaves * kWave, kTreePerCu<DP>) void tree_attn(
         for (int k = 0; k < ST; ++k) {
             if ((uint32_t)k < nct) {
                 issue_k(tile[k], (uint32_t)k, (uint32_t)k * kStage);
-                issue_v(tile[k], (uint32_t)k, (uint32_t)k * kStage);
+                if (WR == 1 || k + 1 < ST) issue_v(tile[k], (uint32_t)k, (uint32_t)k * kStage);
             }
         }
 
@@ -450,8 +453,19 @@ __global__ __launch_bounds__(kTreeWaves * kWave, kTreePerCu<DP>) void tree_attn(
             unsigned char* const at_k = mine + stage;
             unsigned char* const at_v = at_k + kTileKeys * kRowB;
             const bool full = j + ST <= nct;   // (ST tiles are under way)
-            if (full) wait_vm<kNI + (ST - 1) * (kNK + kNI)>();
-            else wait_vm<kNI>();
+            constexpr int kIK = WR == 2 ? kHalf + (kNK - kNI) : kNK, kIV = WR == 2 ? kHalf : kNI;   // loads of a wave
+            if constexpr (WR == 2) {
+                // A step of shared tiles: the next values go out once all have taken the last ones', the keys
+                // after the next once all have read these, so that three half steps are under way.
+                if (full) wait_vm<kIV + kIK>();
+                else wait_vm<kIV>();
+                lds_sync();
+                if (j + 1u < nct) issue_v(tile[1], j + 1u, stage ? 0u : kStage);
+            } else if (full) {
+                wait_vm<kNI + (ST - 1) * (kNK + kNI)>();
+            } else {
+                wait_vm<kNI>();
+            }
             u32x4 kc[2][F8 ? kKS / 2 : kKS];
             f32x4 ks[2] = {zero, zero}, vs[2] = {zero, zero};
 #pragma unroll
@@ -469,7 +483,14 @@ __global__ __launch_bounds__(kTreeWaves * kWave, kTreePerCu<DP>) void tree_attn(
             const bool more = j + ST < nct;
             const bool then = ahead && j + 1u == nct;   // (the new tokens come next)
             if (then) {
-                if constexpr (ST == 1) {
+                if constexpr (WR == 2) {
+                    if constexpr (!F8) {
+                        new_k = mine + (stage ? 0u : kStage);
+                        new_v = new_k + kTileKeys * kNewB;
+                    }
+                    issue_new(false, new_first(st0), new_k);
+                    issue_new(true, new_first(st0), new_v);
+                } else if constexpr (ST == 1) {
                     issue_new(false, new_first(st0), new_k);
                 } else {
                     new_k = mine + (stage ? 0u : kStage);
@@ -478,7 +499,7 @@ __global__ __launch_bounds__(kTreeWaves * kWave, kTreePerCu<DP>) void tree_attn(
                     if constexpr (!F8) issue_new(true, new_first(st0), new_v);
                 }
             }
-            if (more) issue_k(tile[ST], j + ST, stage);
+            if (WR == 1 && more) issue_k(tile[ST], j + ST, stage);
 #pragma unroll
             for (int m = 0; m < MT; ++m) s[m][0] = s[m][1] = zero;
 #pragma unroll
@@ -510,11 +531,17 @@ __global__ __launch_bounds__(kTreeWaves * kWave, kTreePerCu<DP>) void tree_attn(
             if (there != ~0u) {   // (uniform)
 #pragma unroll
                 for (int m = 0; m < MT; ++m) hide(m, there);
-                const uint32_t left = len - (first + j * kStepKeys);
+                const uint32_t t0 = first + j * kStepKeys, left = t0 < len ? len - t0 : 0u;
                 if (there != (left >= 32u ? ~0u : (1u << left) - 1u) && lane == 0u) atomicOr(a.c.status, kStatusPages);   // (a page is missing)
             }
             weigh(vs, F8);
-            if (then) wait_vm<ST == 2 && !F8 ? 2 * kNew : kNew>();
+            if constexpr (WR == 2) {
+                if (then) wait_vm<kNew>();   // (halves of both)
+                else if (full) wait_vm<kIK + kIV>();
+                else wait_vm<0>();
+                lds_sync();
+                if (more) issue_k(tile[ST], j + ST, stage);
+            } else if (then) wait_vm<ST == 2 && !F8 ? 2 * kNew : kNew>();
             else if (!full) wait_vm<0>();
             else if (more) wait_vm<(ST - 1) * (kNK + kNI) + kNK>();
             else wait_vm<(ST - 1) * (kNK + kNI)>();
@@ -532,10 +559,10 @@ __global__ __launch_bounds__(kTreeWaves * kWave, kTreePerCu<DP>) void tree_attn(
 #pragma unroll
                 for (uint32_t k = 0; k < 4; ++k) vc[t + k] = o[k];
             }
-            if constexpr (ST == 1 || F8) {
+            if constexpr (WR == 1 && (ST == 1 || F8)) {
                 if (then) issue_new(true, new_first(st0), new_v);
             }
-            if (more) issue_v(tile[ST], j + ST, stage);
+            if (WR == 1 && more) issue_v(tile[ST], j + ST, stage);
             stage = stage + kStage == ST * kStage ? 0u : stage + kStage;
 #pragma unroll
             for (int k = 0; k < ST; ++k) tile[k] = tile[k + 1];
@@ -562,24 +589,33 @@ __global__ __launch_bounds__(kTreeWaves * kWave, kTreePerCu<DP>) void tree_attn(
         // ---- the new tokens' products ----
         for (uint32_t st = st0; st < s1; ++st) {
             const uint32_t n0 = new_first(st);
-            if (n0 >= N) continue;   // (uniform)
+            const bool in = n0 < N;   // (uniform over the waves that share a tile; all take part in the barriers)
+            if (WR == 1 && !in) continue;
             uint32_t ln = lane;   // (opaque, as above)
             asm volatile("" : "+v"(ln));
             const uint32_t lane_n = ln & 15u, lg = ln >> 4;
-            if (st != st0) {
-                wait_lds();   // (the last tile's reads)
-                issue_new(false, n0, new_k);
-                issue_new(true, n0, new_v);
+            if (st != st0) {   // (the last tile has been read)
+                if constexpr (WR == 2) lds_sync();
+                else wait_lds();
+                if (in) {
+                    issue_new(false, n0, new_k);
+                    issue_new(true, n0, new_v);
+                }
             }
             unsigned char* const at_v = new_v;
             uint32_t see[MT];
 #pragma unroll
             for (int m = 0; m < MT; ++m) {
+                see[m] = 0u;
+                if (!in) continue;
                 if (a.mask) see[m] = live[m] ? a.mask[((uint64_t)i * N + node[m]) * a.mask_words + n0 / 32u] : 0u;
                 else see[m] = !live[m] || node[m] < n0 ? 0u : node[m] - n0 >= 31u ? ~0u : (2u << (node[m] - n0)) - 1u;
                 if (N - n0 < 32u) see[m] &= (1u << (N - n0)) - 1u;
             }
             wait_vm<0>();
+            if constexpr (WR == 2) lds_sync();
+            bool wild = false;
+            if (in) {
 #pragma unroll
             for (int m = 0; m < MT; ++m) s[m][0] = s[m][1] = zero;
 #pragma unroll
@@ -598,16 +634,17 @@ __global__ __launch_bounds__(kTreeWaves * kWave, kTreePerCu<DP>) void tree_attn(
             // Infinities and NaNs are kept out of the product, where a weight of 0 would not keep them
             // from the rows that do not see them: they are replaced by 0 in LDS, and what they were noted
             // in the keys' place (+inf 1, -inf 2, a NaN both).
-            bool wild = false;
 #pragma unroll 1
             for (int ii = 0; ii < kNew; ++ii) {
                 const u32x4 v = *reinterpret_cast<const u32x4*>(at_v + 1024 * ii + 16u * ln);
 #pragma unroll
                 for (int k = 0; k < 4; ++k) wild = wild || (v[k] & 0x7f80u) == 0x7f80u || (v[k] & 0x7f800000u) == 0x7f800000u;
             }
+            }
             const bool any_wild = ballot(wild) != 0ull;
-            if (any_wild) {
-                wait_lds();   // (the keys have been read)
+            if constexpr (WR == 2) lds_sync();   // (keys and values have been read by both)
+            if (any_wild && wr == 0u) {
+                wait_lds();
 #pragma unroll 1
                 for (int ii = 0; ii < kNew; ++ii) {
                     u32x4* const pv = reinterpret_cast<u32x4*>(at_v + 1024 * ii + 16u * ln);
@@ -623,6 +660,10 @@ __global__ __launch_bounds__(kTreeWaves * kWave, kTreePerCu<DP>) void tree_attn(
                     *reinterpret_cast<u32x4*>(new_k + 1024 * ii + 16u * ln) = kind;
                 }
                 wait_lds();
+            }
+            if constexpr (WR == 2) {
+                lds_sync();
+                if (!in) continue;
             }
             const uint32_t rv = 4u * lg + (lane_n >> 2), lv = lds_at(at_v) + rv * kNewB + 8u * (ln & 1u);
             auto tr_of = [&](uint32_t t) -> uint32_t { return ((2u * t + (ln >> 1 & 1u)) ^ swz_v<kNewB, false>(rv)) * 16u; };
@@ -679,25 +720,26 @@ __global__ __launch_bounds__(kTreeWaves * kWave, kTreePerCu<DP>) void tree_attn(
         }
 
         // ---- the waves' sums joined ----
-        wait_lds();
+        if constexpr (WR == 2) lds_sync();   // (the tiles' place)
+        else wait_lds();
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
             const float z = across(sum[m], [](float p, float q) { return p + q; });
             if (g == 0u) {
-                stat[w][0][16u * m + n] = top[m];
-                stat[w][1][16u * m + n] = z;
+                stat[w][0][wr * kMine + 16u * m + n] = top[m];
+                stat[w][1][wr * kMine + 16u * m + n] = z;
             }
 #pragma unroll
             for (uint32_t t = 0; t < kDT; ++t)
-                *reinterpret_cast<f32x4*>(mine + (16u * m + n) * DP * 4u + ((4u * t + g) ^ n) * 16u) = acc[m][t];
+                *reinterpret_cast<f32x4*>(mine + (wr * kMine + 16u * m + n) * DP * 4u + ((4u * t + g) ^ n) * 16u) = acc[m][t];
         }
         lds_sync();
         const bool complete = s0 == 0u && s1 == steps;
         // (who shares the pair: its first and last pieces, and whether it begins inside the first)
         if (s0 == 0u && rt == a.row_tile0 && tid_x() == 0u) a.spans[i * H + kvh] = piece | (x + steps - 1u) / share << 15 | (x != piece * share ? 1u << 31 : 0u);
         // (a workgroup has at most two incomplete segments: one that begins with the piece, one that ends with it)
-        float* part = a.part + ((uint64_t)b * 2u + (x == piece * share ? 0u : 1u)) * Part<DP, MT>::kFloats;
-        for (uint32_t it = tid_x(); it < kRows * (DP / 4u); it += kTreeWaves * kWave) {
+        float* part = a.part + ((uint64_t)b * 2u + (x == piece * share ? 0u : 1u)) * Part<DP, MT * WR>::kFloats;
+        for (uint32_t it = tid_x(); it < kRows * (DP / 4u); it += kTreeWaves * WR * kWave) {
             const uint32_t rr = it / (DP / 4u), c = it % (DP / 4u), pr = rt * kRows + rr;
             float M = stat[0][0][rr];
 #pragma unroll
@@ -810,24 +852,28 @@ __global__ __launch_bounds__(256) void tree_join(TreeArgs a) {
 namespace {
 
 constexpr uint32_t kTreeTiles = 32;   // row tiles of a launch
+#ifndef WIDE
+#define WIDE 32
+#endif
+constexpr uint32_t kWideRows = WIDE;
 
-template <int DP, int MT, bool F8, int ST>
+template <int DP, int MT, bool F8, int ST, int WR>
 hipError_t launch(TreeArgs a, uint32_t cus, hipStream_t st) {
-    constexpr uint32_t per_cu = kTreePerCu<DP>;
-    const uint32_t rows = a.rows_per_seq * a.group, tiles = (rows + 16u * MT - 1u) / (16u * MT);
+    constexpr uint32_t per_cu = WR == 1 ? kTreePerCu<DP> : 1, per = 16u * MT * WR;
+    const uint32_t rows = a.rows_per_seq * a.group, tiles = (rows + per - 1u) / per;
     for (uint32_t t0 = 0; t0 < tiles; t0 += kTreeTiles) {
         a.row_tile0 = t0;
         a.row_tiles = tiles - t0 < kTreeTiles ? tiles - t0 : kTreeTiles;
         const uint32_t most = per_cu * kTreeSlots / 2u, slots = cus * per_cu < most ? cus * per_cu : most;
         a.pieces = slots / a.row_tiles / 8u * 8u;
         if (a.pieces == 0u) a.pieces = 8u;
-        hipLaunchKernelGGL((tree_attn<DP, MT, F8, ST>), dim3(a.pieces * a.row_tiles), dim3(kTreeWaves * kWave), 0, st, a);
+        hipLaunchKernelGGL((tree_attn<DP, MT, F8, ST, WR>), dim3(a.pieces * a.row_tiles), dim3(kTreeWaves * WR * kWave), 0, st, a);
         hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
-        const uint32_t pairs = a.c.n * a.c.kv_heads, blocks = a.row_tiles * (16u * MT * DP / 1024u);
+        const uint32_t pairs = a.c.n * a.c.kv_heads, blocks = a.row_tiles * (per * DP / 1024u);
         // (many partial results a pair: more threads for them)
-        if (pairs * 8u <= a.pieces) hipLaunchKernelGGL((tree_join<DP, MT, 4>), dim3(pairs, 4u * blocks), dim3(256), 0, st, a);
-        else hipLaunchKernelGGL((tree_join<DP, MT, 1>), dim3(pairs, blocks), dim3(256), 0, st, a);
+        if (pairs * 8u <= a.pieces) hipLaunchKernelGGL((tree_join<DP, MT * WR, 4>), dim3(pairs, 4u * blocks), dim3(256), 0, st, a);
+        else hipLaunchKernelGGL((tree_join<DP, MT * WR, 1>), dim3(pairs, blocks), dim3(256), 0, st, a);
         if ((e = hipGetLastError()) != hipSuccess) return e;
     }
     return hipSuccess;
@@ -839,7 +885,12 @@ hipError_t launch(TreeArgs a, uint32_t cus, hipStream_t st) {
 template <int DP, bool F8>
 hipError_t launch_rows(const TreeArgs& a, uint32_t cus, hipStream_t st) {
     constexpr int ST = F8 || DP == 64 ? 2 : 1;
-    return a.rows_per_seq * a.group <= 16u ? launch<DP, 1, F8, ST>(a, cus, st) : launch<DP, 2, F8, ST>(a, cus, st);
+    const uint32_t rows = a.rows_per_seq * a.group;
+    if (rows <= 16u) return launch<DP, 1, F8, ST, 1>(a, cus, st);
+    if constexpr (DP != 256) {
+        if (rows > kWideRows) return launch<DP, 2, F8, 2, 2>(a, cus, st);
+    }
+    return launch<DP, 2, F8, ST, 1>(a, cus, st);
 }
 
 }  // namespace
@@ -847,7 +898,7 @@ hipError_t launch_rows(const TreeArgs& a, uint32_t cus, hipStream_t st) {
 // Floats of a context's partial results: two results for every workgroup (heads of 256: one
 // workgroup a CU, half as many).
 uint64_t tree_part_floats() { return 2ull * kTreeSlots * Part<128, 2>::kFloats; }
-static_assert(Part<256, 2>::kFloats <= 2u * Part<128, 2>::kFloats, "the partial results' room");
+static_assert(Part<256, 2>::kFloats <= 2u * Part<128, 2>::kFloats && Part<128, 4>::kFloats <= 2u * Part<128, 2>::kFloats, "the partial results' room");
 
 hipError_t launch_tree_attn(const TreeArgs& args, uint32_t cus, hipStream_t st) {
     TreeArgs a = args;
