@@ -135,6 +135,7 @@ inline int check_tree_attn(const lcs_tree_attn_batch* b, const lcs_tree_attn_out
         return w.no("row strides must be at least a row's heads");
     }
     if (b->q_stride % 8u || b->k_stride % 8u || b->v_stride % 8u || o->o_stride % 8u) return w.no("strides must be multiples of 16 bytes");
+    if (c->pages > 1 && c->page_stride * (c->dtype == LCS_BF16 ? 2u : 1u) > 0xffffffffull) return w.no("the cache's pages must be less than 4 GiB apart");
     if (b->k_stride > 1u << 25 || b->v_stride > 1u << 25) return w.no("k_stride and v_stride must be at most 2^25");
     if ((uint64_t)b->n_seq * b->rows_per_seq * b->heads > 0x7fffffffull) return w.over("too many rows and heads for a call");
     if ((uint64_t)b->n_seq * c->kv_heads > max_pairs) return w.over("at most 65536 sequences x kv heads a call");

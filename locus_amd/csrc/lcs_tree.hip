@@ -9,6 +9,7 @@
 // - A wave takes 32 keys at a time, their keys and values brought to its own part of
 //   LDS by 16-byte DMA loads, so that no register holds data in flight and waves need
 //   no barrier; four waves take 128 consecutive tokens, a step.
+//   Above 128 rows a head two waves share a tile and bring a half of it each, with barriers.
 // - Scores are computed transposed, S^T = K Q^T, with Q in registers as the B
 //   operand: a lane then holds eight keys of one row, so that its softmax is the
 //   lane's own, and the weights are already laid out as the B operand of O^T = V^T P^T.
@@ -109,6 +110,24 @@ __device__ __forceinline__ void read_tr8(const uint32_t (&at)[4], u32x2 (&o)[4])
                  : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3])
                  : "memory");
 }
+// Plain reads, likewise: 16 bytes at each address and NEXT bytes behind it.
+template <int NEXT>
+__device__ __forceinline__ void read_two(const uint32_t (&at)[2], u32x4 (&lo)[2], u32x4 (&hi)[2]) {
+    asm volatile("ds_read_b128 %0, %4\n\tds_read_b128 %1, %4 offset:%6\n\tds_read_b128 %2, %5\n\tds_read_b128 %3, %5 offset:%6\n\t"
+                 "s_waitcnt lgkmcnt(0)"
+                 : "=&v"(lo[0]), "=&v"(hi[0]), "=&v"(lo[1]), "=&v"(hi[1])
+                 : "v"(at[0]), "v"(at[1]), "n"(NEXT)
+                 : "memory");
+}
+template <int NEXT>
+__device__ __forceinline__ void read_four(const uint32_t (&at)[4], u32x4 (&lo)[4], u32x4 (&hi)[4]) {
+    asm volatile("ds_read_b128 %0, %8\n\tds_read_b128 %1, %8 offset:%12\n\tds_read_b128 %2, %9\n\tds_read_b128 %3, %9 offset:%12\n\t"
+                 "ds_read_b128 %4, %10\n\tds_read_b128 %5, %10 offset:%12\n\tds_read_b128 %6, %11\n\tds_read_b128 %7, %11 offset:%12\n\t"
+                 "s_waitcnt lgkmcnt(0)"
+                 : "=&v"(lo[0]), "=&v"(hi[0]), "=&v"(lo[1]), "=&v"(hi[1]), "=&v"(lo[2]), "=&v"(hi[2]), "=&v"(lo[3]), "=&v"(hi[3])
+                 : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "n"(NEXT)
+                 : "memory");
+}
 __device__ __forceinline__ uint32_t lds_at(const unsigned char* p) { return (uint32_t)(uintptr_t)(LCS_LDS const unsigned char*)p; }
 __device__ __forceinline__ float exp2_f(float x) { return __builtin_amdgcn_exp2f(x); }
 // Over the four lanes that hold a row (lane, lane ^ 16, lane ^ 32, lane ^ 48).
@@ -196,14 +215,13 @@ struct Part {
 
 template <int DP, int MT, bool F8, int ST, int WR>
 __global__ __launch_bounds__(kTreeWaves * WR * kWave, WR == 1 ? kTreePerCu<DP> : 1) void tree_attn(TreeArgs a) {
-    static_assert(WR == 1 || (WR == 2 && ST == 2), "the schedule of shared tiles");
+    static_assert(WR == 1 || (WR == 2 && ST == 2 && !F8), "the schedule of shared tiles");
     constexpr uint32_t kMine = 16u * MT, kRows = kMine * WR, kDT = DP / 16, kKS = DP / 32;   // rows of a wave, of the workgroup
     constexpr uint32_t kRowB = DP * (F8 ? 1 : 2), kNewB = DP * 2;                 // bytes of a cached row and of a new one in LDS
     constexpr uint32_t kScaleB = F8 ? 256u : 0u;
     constexpr uint32_t kStage = 2u * kTileKeys * kRowB + kScaleB;
     constexpr uint32_t kMergeB = kRows * DP * 4u;
-    constexpr uint32_t kNewAt = WR == 2 && F8 ? ST * kStage : 0u;   // (shared 8-bit tiles leave room for new ones beside them)
-    constexpr uint32_t kMax1 = kNewAt + 2u * kTileKeys * kNewB > ST * kStage ? kNewAt + 2u * kTileKeys * kNewB : ST * kStage;
+    constexpr uint32_t kMax1 = 2u * kTileKeys * kNewB > ST * kStage ? 2u * kTileKeys * kNewB : ST * kStage;
     constexpr uint32_t kRegion = kMax1 > kMergeB ? kMax1 : kMergeB;
     constexpr int kNI = (int)(kTileKeys * kRowB / 1024u);      // DMA loads of a tile's keys, and of its values
     constexpr int kNK = kNI + (F8 ? 1 : 0);
@@ -255,20 +273,23 @@ __global__ __launch_bounds__(kTreeWaves * WR * kWave, WR == 1 ? kTreePerCu<DP> :
         const uint32_t c1 = min(s1, ctx_steps), first = s0 * kStepKeys + w * kTileKeys;
         const uint32_t nct = s0 < c1 ? c1 - s0 : 0u;   // (the last one may lie past the length: all zeros, unseen)
         struct Tile {
-            int32_t p0, p1;   // the pages of its first and last 16 tokens
+            uint32_t p0, p1;   // the pages of its first and last 16 tokens
+            uint32_t there;    // its keys that are there (settle)
         };
         auto pages_of = [&](uint32_t j) -> Tile {
             const uint32_t t0 = first + (j < nct ? j : 0u) * kStepKeys;
             const uint32_t q0 = min(t0 >> a.c.page_shift, a.c.max_pages - 1u), q1 = min((t0 + 16u) >> a.c.page_shift, a.c.max_pages - 1u);
-            if (nct == 0u) return Tile{0, 0};
-            return Tile{scalar_load(row + q0), scalar_load(row + q1)};
+            if (nct == 0u) return Tile{0u, 0u, 0u};
+            return Tile{(uint32_t)scalar_load(row + q0), (uint32_t)scalar_load(row + q1), 0u};
         };
-        auto mask_of = [&](const Tile& t, uint32_t j) -> uint32_t {   // the tile's keys that are there
+        auto expected = [&](uint32_t j) -> uint32_t {   // the keys of tile j ahead of the length
             const uint32_t t0 = first + j * kStepKeys, left = t0 < len ? len - t0 : 0u;
-            uint32_t m = left >= 32u ? ~0u : (1u << left) - 1u;
-            if ((uint32_t)t.p0 >= a.c.pages) m &= 0xffff0000u;
-            if ((uint32_t)t.p1 >= a.c.pages) m &= 0x0000ffffu;
-            return m;
+            return left >= 32u ? ~0u : (1u << left) - 1u;
+        };
+        auto settle = [&](Tile& t, uint32_t j) {   // (a page that is missing: none of its keys, page 0 in its place)
+            t.there = expected(j) & (t.p0 < a.c.pages ? ~0u : 0xffff0000u) & (t.p1 < a.c.pages ? ~0u : 0x0000ffffu);
+            t.p0 = t.p0 < a.c.pages ? t.p0 : 0u;
+            t.p1 = t.p1 < a.c.pages ? t.p1 : 0u;
         };
         // A tile's 16-row halves lie in one page each; DMA load ii of a half covers rows RPI ii + lane /
         // CPR, a chunk per lane. A half's buffer ends with its last row that is there.
@@ -279,34 +300,32 @@ __global__ __launch_bounds__(kTreeWaves * WR * kWave, WR == 1 ? kTreePerCu<DP> :
             const uint32_t ch = (lane % CPR) ^ (values ? swz_v<kRowB, F8>(r) : swz_k<kRowB>(r));
             return 16u * ch < D * (F8 ? 1u : 2u) ? (r & 15u) * tsb + 16u * ch : kNoByte;
         };
-        constexpr int kVo = F8 && WR == 1 ? kNI : kHalf;   // (8-bit values: the second half is permuted by other bits)
+        constexpr int kVo = F8 ? kNI : kHalf;   // (8-bit values: the second half is permuted by other bits)
         uint32_t vo_k[kHalf], vo_v[kVo];
 #pragma unroll
         for (int ii = 0; ii < kHalf; ++ii) vo_k[ii] = offset_of(false, RPI * (uint32_t)ii + lane / CPR);
 #pragma unroll
-        for (int ii = 0; ii < kVo; ++ii) vo_v[ii] = offset_of(true, RPI * (uint32_t)ii + lane / CPR + (WR == 2 ? 16u * wr : 0u));
+        for (int ii = 0; ii < kVo; ++ii) vo_v[ii] = offset_of(true, RPI * (uint32_t)ii + lane / CPR);
+        const uint32_t psb = (uint32_t)a.c.page_stride * (F8 ? 1u : 2u);   // (below 2^32, and so is a row's place in its page)
         auto issue_rows = [&](bool values, const Tile& t, uint32_t j, unsigned char* dst) {
-            const uint32_t t0 = first + j * kStepKeys, m = mask_of(t, j);
             const unsigned char* base = values ? vb : kb;
-            const uint64_t ps = a.c.page_stride * (F8 ? 1u : 2u);
 #pragma unroll
             for (uint32_t q = 0; q < 2u / WR; ++q) {   // (two waves that share a tile bring a half each)
-                const uint32_t h = WR == 2 ? wr : q, there = m >> (16u * h) & 0xffffu, page = there ? (uint32_t)(h ? t.p1 : t.p0) : 0u;
-                const __amdgpu_buffer_rsrc_t rs = buffer_of(base + page * ps + ((t0 + 16u * h) & (a.c.page_tokens - 1u)) * ts,
-                                                            (uint32_t)__builtin_popcount(there) * tsb);
+                const uint32_t h = WR == 2 ? wr : q, first_page = t.p0, second_page = t.p1, in_page = ((first + j * kStepKeys + 16u * h) & (a.c.page_tokens - 1u)) * tsb;
+                const __amdgpu_buffer_rsrc_t rs = buffer_of(base + (uint64_t)(h ? second_page : first_page) * psb + in_page,
+                                                            (uint32_t)__builtin_popcount(t.there >> (16u * h) & 0xffffu) * tsb);
 #pragma unroll
                 for (int ii = 0; ii < kHalf; ++ii)
-                    dma16(rs, dst + 1024 * (kHalf * h + ii), values ? vo_v[F8 && WR == 1 ? kHalf * q + ii : ii] : vo_k[ii]);
+                    dma16(rs, dst + 1024 * (kHalf * h + ii), values ? vo_v[F8 ? kHalf * q + ii : ii] : vo_k[ii]);
             }
         };
         auto issue_k = [&](const Tile& t, uint32_t j, uint32_t stage) {
             unsigned char* dst = mine + stage;
             if constexpr (F8) {   // the keys' scales by the lower half, the values' by the upper
-                const uint32_t r = lane & 31u, tok = (first + j * kStepKeys + r) & (a.c.page_tokens - 1u);
-                const uint32_t m = mask_of(t, j), pg = (uint32_t)(r < 16u ? t.p0 : t.p1);
+                const uint32_t r = lane & 31u, tok = (first + j * kStepKeys + r) & (a.c.page_tokens - 1u), first_page = t.p0, second_page = t.p1;
                 const float* s = lane < 32u ? a.c.k_scale : a.c.v_scale;
-                const uint64_t e = ((((uint64_t)a.c.layer * a.c.pages + pg) * H + kvh) << a.c.page_shift) + tok;
-                dma4(m >> r & 1u ? static_cast<const void*>(s + e) : a.zeros, dst + 2u * kTileKeys * kRowB);
+                const uint64_t e = ((((uint64_t)a.c.layer * a.c.pages + (r < 16u ? first_page : second_page)) * H + kvh) << a.c.page_shift) + tok;
+                dma4(t.there >> r & 1u ? static_cast<const void*>(s + e) : a.zeros, dst + 2u * kTileKeys * kRowB);
             }
             issue_rows(false, t, j, dst);
         };
@@ -315,6 +334,8 @@ __global__ __launch_bounds__(kTreeWaves * WR * kWave, WR == 1 ? kTreePerCu<DP> :
         Tile tile[ST + 1];   // of tiles j, j + 1, .. j + ST
 #pragma unroll
         for (int k = 0; k <= ST; ++k) tile[k] = pages_of((uint32_t)k);
+#pragma unroll
+        for (int k = 0; k < ST; ++k) settle(tile[k], (uint32_t)k);
         // ---- the new tokens' tiles (bf16 always), the first one's loads issued where LDS is free ahead of it ----
         constexpr int kNew = (int)(kTileKeys * kNewB / 1024u);   // DMA loads of a tile's keys, and of its values
         const uint32_t st0 = max(s0, ctx_steps);
@@ -336,12 +357,8 @@ __global__ __launch_bounds__(kTreeWaves * WR * kWave, WR == 1 ? kTreePerCu<DP> :
         };
         // their places: with one stage its keys' and values' places; with two the other stage, and
         // for 8-bit rows (a new row takes two cached ones' room) the last tile's own for the values
-        unsigned char* new_k = mine + kNewAt;
-        unsigned char* new_v = mine + kNewAt + kTileKeys * kNewB;
-        if (ahead && nct == 0u) {
-            issue_new(false, new_first(st0), new_k);
-            issue_new(true, new_first(st0), new_v);
-        }
+        unsigned char* new_k = mine;
+        unsigned char* new_v = mine + kTileKeys * kNewB;
 
         // ---- the rows: packed as (new token, query head of the group) ----
         u32x4 qr[MT][kKS];
@@ -357,27 +374,38 @@ __global__ __launch_bounds__(kTreeWaves * WR * kWave, WR == 1 ? kTreePerCu<DP> :
             for (uint32_t ks = 0; ks < kKS; ++ks) qr[m][ks] = *reinterpret_cast<const u32x4*>(q + (8u * chunk8(ks) < D ? 8u * chunk8(ks) : 0u));
         }
 
-#pragma unroll
-        for (int k = 0; k < ST; ++k) {
-            if ((uint32_t)k < nct) {
-                issue_k(tile[k], (uint32_t)k, (uint32_t)k * kStage);
-                if (WR == 1 || k + 1 < ST) issue_v(tile[k], (uint32_t)k, (uint32_t)k * kStage);
-            }
-        }
-
         // (rows past the last and dims past the head's count as zeros; so do all at a scale of 0,
         // whose scores are 0; a scale below 0 changes the sign here)
         bf16x8 qf[MT][kKS];
-        const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;
+        auto take_q = [&] {
+            const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
+            for (int m = 0; m < MT; ++m)
 #pragma unroll
-            for (uint32_t ks = 0; ks < kKS; ++ks) {
-                const bool in = live[m] && 8u * chunk8(ks) < D && a.scale != 0.0f;
+                for (uint32_t ks = 0; ks < kKS; ++ks) {
+                    const bool in = live[m] && 8u * chunk8(ks) < D && a.scale != 0.0f;
 #pragma unroll
-                for (int k = 0; k < 4; ++k) qr[m][ks][k] = in ? qr[m][ks][k] ^ flip : 0u;
-                qf[m][ks] = __builtin_bit_cast(bf16x8, qr[m][ks]);
+                    for (int k = 0; k < 4; ++k) qr[m][ks][k] = in ? qr[m][ks][k] ^ flip : 0u;
+                    qf[m][ks] = __builtin_bit_cast(bf16x8, qr[m][ks]);
+                }
+        };
+        // (the queries are waited for where the loads behind them are the same on every path: the
+        // compiler counts those that surely follow)
+        if (nct != 0u) {
+            issue_k(tile[0], 0u, 0u);
+            issue_v(tile[0], 0u, 0u);
+            take_q();
+            if (ST == 2 && nct > 1u) {
+                issue_k(tile[1], 1u, kStage);
+                if (WR == 1) issue_v(tile[1], 1u, kStage);
             }
+        } else {
+            if (ahead) {
+                issue_new(false, new_first(st0), new_k);
+                issue_new(true, new_first(st0), new_v);
+            }
+            take_q();
+        }
         f32x4 acc[MT][kDT];
         float top[MT], sum[MT];
 #pragma unroll
@@ -450,17 +478,19 @@ __global__ __launch_bounds__(kTreeWaves * WR * kWave, WR == 1 ? kTreePerCu<DP> :
         uint32_t stage = 0;
 #pragma clang loop unroll(disable)
         for (uint32_t j = 0; j < nct; ++j) {
+            uint32_t fresh_stage = stage;   // (opaque: the loads' LDS places follow from it by additions, and take no registers)
+            asm volatile("" : "+s"(fresh_stage));
             unsigned char* const at_k = mine + stage;
             unsigned char* const at_v = at_k + kTileKeys * kRowB;
             const bool full = j + ST <= nct;   // (ST tiles are under way)
-            constexpr int kIK = WR == 2 ? kHalf + (kNK - kNI) : kNK, kIV = WR == 2 ? kHalf : kNI;   // loads of a wave
+            constexpr int kIK = kHalf, kIV = kHalf;   // (WR 2) loads of a wave
             if constexpr (WR == 2) {
                 // A step of shared tiles: the next values go out once all have taken the last ones', the keys
                 // after the next once all have read these, so that three half steps are under way.
                 if (full) wait_vm<kIV + kIK>();
                 else wait_vm<kIV>();
                 lds_sync();
-                if (j + 1u < nct) issue_v(tile[1], j + 1u, stage ? 0u : kStage);
+                if (j + 1u < nct) issue_v(tile[1], j + 1u, fresh_stage ? 0u : kStage);
             } else if (full) {
                 wait_vm<kNI + (ST - 1) * (kNK + kNI)>();
             } else {
@@ -468,26 +498,49 @@ __global__ __launch_bounds__(kTreeWaves * WR * kWave, WR == 1 ? kTreePerCu<DP> :
             }
             u32x4 kc[2][F8 ? kKS / 2 : kKS];
             f32x4 ks[2] = {zero, zero}, vs[2] = {zero, zero};
+            constexpr uint32_t kKC = F8 ? kKS / 2 : kKS;   // 16-byte chunks of a key that a lane takes
+            const uint32_t lk = lds_at(at_k) + n * kRowB;
 #pragma unroll
-            for (uint32_t h = 0; h < 2; ++h) {
-                const uint32_t r = 16u * h + n;
+            for (uint32_t c0 = 0; c0 < kKC; c0 += 4u) {
+                constexpr uint32_t kAt = kKC < 4u ? kKC : 4u;
+                uint32_t ad[kAt];
+                u32x4 lo[kAt], hi[kAt];
 #pragma unroll
-                for (uint32_t c = 0; c < (F8 ? kKS / 2 : kKS); ++c)
-                    kc[h][c] = *reinterpret_cast<const u32x4*>(at_k + r * kRowB + ((4u * c + g) ^ swz_k<kRowB>(r)) * 16u);
-                if constexpr (F8) {
-                    ks[h] = *reinterpret_cast<const f32x4*>(at_k + 2u * kTileKeys * kRowB + 64u * h + 16u * g);
-                    vs[h] = *reinterpret_cast<const f32x4*>(at_k + 2u * kTileKeys * kRowB + 128u + 64u * h + 16u * g);
+                for (uint32_t c = 0; c < kAt; ++c) ad[c] = lk + ((4u * (c0 + c) + g) ^ swz_k<kRowB>(n)) * 16u;
+                if constexpr (kAt == 4u) {
+                    read_four<16 * kRowB>(ad, lo, hi);
+                } else if constexpr (kAt == 2u) {
+                    read_two<16 * kRowB>(ad, lo, hi);
+                } else {
+                    const uint32_t twice[2] = {ad[0], ad[0]};
+                    u32x4 l2[2], h2[2];
+                    read_two<16 * kRowB>(twice, l2, h2);
+                    lo[0] = l2[0];
+                    hi[0] = h2[0];
+                }
+#pragma unroll
+                for (uint32_t c = 0; c < kAt; ++c) {
+                    kc[0][c0 + c] = lo[c];
+                    kc[1][c0 + c] = hi[c];
                 }
             }
-            wait_lds();
+            if constexpr (F8) {   // the scales of keys 4 g .. and 16 + 4 g ..; the values' 128 bytes behind
+                const uint32_t sa = lds_at(at_k) + 2u * kTileKeys * kRowB + 16u * g, ad[2] = {sa, sa + 64u};
+                u32x4 lo[2], hi[2];
+                read_two<128>(ad, lo, hi);
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    ks[h] = __builtin_bit_cast(f32x4, lo[h]);
+                    vs[h] = __builtin_bit_cast(f32x4, hi[h]);
+                }
+            }
             const bool more = j + ST < nct;
+            settle(tile[ST], j + ST);
             const bool then = ahead && j + 1u == nct;   // (the new tokens come next)
             if (then) {
                 if constexpr (WR == 2) {
-                    if constexpr (!F8) {
-                        new_k = mine + (stage ? 0u : kStage);
-                        new_v = new_k + kTileKeys * kNewB;
-                    }
+                    new_k = mine + (stage ? 0u : kStage);
+                    new_v = new_k + kTileKeys * kNewB;
                     issue_new(false, new_first(st0), new_k);
                     issue_new(true, new_first(st0), new_v);
                 } else if constexpr (ST == 1) {
@@ -499,7 +552,7 @@ __global__ __launch_bounds__(kTreeWaves * WR * kWave, WR == 1 ? kTreePerCu<DP> :
                     if constexpr (!F8) issue_new(true, new_first(st0), new_v);
                 }
             }
-            if (WR == 1 && more) issue_k(tile[ST], j + ST, stage);
+            if (WR == 1 && more) issue_k(tile[ST], j + ST, fresh_stage);
 #pragma unroll
             for (int m = 0; m < MT; ++m) s[m][0] = s[m][1] = zero;
 #pragma unroll
@@ -527,12 +580,10 @@ __global__ __launch_bounds__(kTreeWaves * WR * kWave, WR == 1 ? kTreePerCu<DP> :
 #pragma unroll
                     for (int h = 0; h < 2; ++h) s[m][h] *= ks[h];
             }
-            const uint32_t there = mask_of(tile[0], j);
-            if (there != ~0u) {   // (uniform)
+            if (tile[0].there != ~0u) {   // (uniform)
 #pragma unroll
-                for (int m = 0; m < MT; ++m) hide(m, there);
-                const uint32_t t0 = first + j * kStepKeys, left = t0 < len ? len - t0 : 0u;
-                if (there != (left >= 32u ? ~0u : (1u << left) - 1u) && lane == 0u) atomicOr(a.c.status, kStatusPages);   // (a page is missing)
+                for (int m = 0; m < MT; ++m) hide(m, tile[0].there);
+                if (tile[0].there != expected(j) && lane == 0u) atomicOr(a.c.status, kStatusPages);   // (a page is missing)
             }
             weigh(vs, F8);
             if constexpr (WR == 2) {
@@ -540,7 +591,7 @@ __global__ __launch_bounds__(kTreeWaves * WR * kWave, WR == 1 ? kTreePerCu<DP> :
                 else if (full) wait_vm<kIK + kIV>();
                 else wait_vm<0>();
                 lds_sync();
-                if (more) issue_k(tile[ST], j + ST, stage);
+                if (more) issue_k(tile[ST], j + ST, fresh_stage);
             } else if (then) wait_vm<ST == 2 && !F8 ? 2 * kNew : kNew>();
             else if (!full) wait_vm<0>();
             else if (more) wait_vm<(ST - 1) * (kNK + kNI) + kNK>();
@@ -562,7 +613,7 @@ __global__ __launch_bounds__(kTreeWaves * WR * kWave, WR == 1 ? kTreePerCu<DP> :
             if constexpr (WR == 1 && (ST == 1 || F8)) {
                 if (then) issue_new(true, new_first(st0), new_v);
             }
-            if (WR == 1 && more) issue_v(tile[ST], j + ST, stage);
+            if (WR == 1 && more) issue_v(tile[ST], j + ST, fresh_stage);
             stage = stage + kStage == ST * kStage ? 0u : stage + kStage;
 #pragma unroll
             for (int k = 0; k < ST; ++k) tile[k] = tile[k + 1];
@@ -852,10 +903,7 @@ __global__ __launch_bounds__(256) void tree_join(TreeArgs a) {
 namespace {
 
 constexpr uint32_t kTreeTiles = 32;   // row tiles of a launch
-#ifndef WIDE
-#define WIDE 32
-#endif
-constexpr uint32_t kWideRows = WIDE;
+constexpr uint32_t kWideRows = 128;   // rows a head above which waves share tiles
 
 template <int DP, int MT, bool F8, int ST, int WR>
 hipError_t launch(TreeArgs a, uint32_t cus, hipStream_t st) {
@@ -879,15 +927,18 @@ hipError_t launch(TreeArgs a, uint32_t cus, hipStream_t st) {
     return hipSuccess;
 }
 
-// Rows of a tile: 16, or 32 where there are more. (64 of them leave one wave a SIMD and
-// its products wait for its softmax: 64 rows a head, 32 sequences x 4096 tokens x 8 heads
-// 110 us in tiles of 32, 111 in tiles of 64; 256 rows 276 / 294.)
+// Rows of a wave: 16, or 32 where there are more (64 leave one wave a SIMD, whose products
+// wait for its softmax: 256 rows a head, 32 sequences x 4096 tokens x 8 heads 294 us, of 32
+// 276). Above 128 rows over bf16 two waves share each tile, which halves what the L2 and LDS
+// bring (the same 273 -> 244 us; 512 rows, 8 sequences x 8192 tokens 252 -> 234); for
+// fewer rows, and for 8 bits, whose tiles are half as large, its barriers cost what that
+// saves (64 rows over up to 6000 tokens 69 -> 73, 256 rows over e4m3 261 -> 276).
 template <int DP, bool F8>
 hipError_t launch_rows(const TreeArgs& a, uint32_t cus, hipStream_t st) {
     constexpr int ST = F8 || DP == 64 ? 2 : 1;
     const uint32_t rows = a.rows_per_seq * a.group;
     if (rows <= 16u) return launch<DP, 1, F8, ST, 1>(a, cus, st);
-    if constexpr (DP != 256) {
+    if constexpr (DP != 256 && !F8) {
         if (rows > kWideRows) return launch<DP, 2, F8, 2, 2>(a, cus, st);
     }
     return launch<DP, 2, F8, ST, 1>(a, cus, st);

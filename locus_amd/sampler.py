@@ -192,6 +192,7 @@ class KvCache:
         self._c = _KvCache(layers, pages, tokens, heads, dim, types[k.dtype], table.shape[0], table.shape[1], k.data_ptr(),
                            v.data_ptr(), _addr(k_scale), _addr(v_scale), ks[0], ks[1], ks[2], ks[3], table.data_ptr(),
                            refs.data_ptr())
+        self._p = C.pointer(self._c)
 
 
 _lib = None
@@ -278,6 +279,7 @@ class Sampler:
         self.torch = torch
         self.device = device
         self._types = {torch.float32: LCS_F32, torch.bfloat16: LCS_BF16, torch.float8_e4m3fn: LCS_E4M3}
+        self._bf16, self._i32, self._f32 = torch.bfloat16, torch.int32, torch.float32
         self._current = getattr(torch._C, "_cuda_getCurrentRawStream", None)
         L = lib()
         self.ctx = L.lcs_create(device, max_rows, max_vocab, max_hist, max_top)
@@ -731,8 +733,8 @@ class Sampler:
 
     def _requests(self, *named):
         """The number of requests and the addresses of their (n,) int32 vectors."""
-        n = named[0][0].numel()
-        return n, *(self._vec(t, n, self.torch.int32, name) for t, name in named)
+        n, i32, vec = named[0][0].numel(), self._i32, self._vec
+        return n, *[vec(t, n, i32, name) for t, name in named]
 
     def kv_grow_dev(self, cache, seq, start, end, result, stream=None):
         """Pages of their own for slots seq[i] at tokens [start[i], end[i])
@@ -772,14 +774,15 @@ class Sampler:
         if rc != LCS_OK:
             self._check(rc)
 
-    def _heads(self, t, rows: int, heads: int, dim: int, name: str):
-        """Address and row stride of (rows, heads, dim) bf16 rows, a row's heads together."""
-        if t.dtype != self.torch.bfloat16 or t.shape != (rows, heads, dim) or t.get_device() != self.device:
-            raise SamplerError(f"{name} must be ({rows}, {heads}, {dim}) bfloat16 on the sampler's device")
-        per, head, one = t.stride()
-        if (one != 1 and dim > 1) or (head != dim and heads > 1):
+    def _heads(self, t, shape, name: str):
+        """Address and row stride of bf16 rows (..., rows, heads, dim), a row's heads together."""
+        if t.dtype != self._bf16 or t.shape != shape or t.get_device() != self.device:
+            raise SamplerError(f"{name} must be {shape} bfloat16 on the sampler's device")
+        at = t.stride()
+        heads, dim = shape[-2], shape[-1]
+        if (at[-1] != 1 and dim > 1) or (at[-2] != dim and heads > 1):
             raise SamplerError(f"{name}: a row's heads must be contiguous")
-        return t.data_ptr(), per if rows > 1 else heads * dim
+        return t.data_ptr(), at[-3] if shape[-3] > 1 else heads * dim
 
     def kv_append_dev(self, cache, k, v, seq, pos, count=None, rows_per_seq: int = 1, index=None, layer: int = 0,
                       stream=None):
@@ -788,20 +791,23 @@ class Sampler:
         (None: j) of sequence i's rows_per_seq ones. k and v (layers, n *
         rows_per_seq, kv_heads, head_dim) bf16 for the layers from `layer` on, or of
         one layer without the first dimension."""
-        c, i32, vec = self._cache(cache), self.torch.int32, self._vec
+        c, i32, vec = self._cache(cache), self._i32, self._vec
         n = seq.numel()
-        if k.dim() == 3 and v.dim() == 3:
-            k, v = k[None], v[None]
-        if k.dim() != 4 or v.dim() != 4 or k.shape[0] != v.shape[0] or k.shape[0] == 0:
-            raise SamplerError("k and v must be (layers, rows, kv_heads, head_dim) of as many layers, one at least")
-        layers, rows = k.shape[0], n * rows_per_seq
-        (kp, ks), (vp, vs) = (self._heads(t[0], rows, c.kv_heads, c.head_dim, name) for t, name in ((k, "k"), (v, "v")))
-        if layers > 1 and k.stride(0) != v.stride(0):
-            raise SamplerError("k and v must have the same layer stride")
+        rows = n * rows_per_seq
+        shape, layers, apart = (rows, cache.shape[2], cache.shape[4]), 1, 0
+        if k.dim() == 4:
+            layers, apart = k.shape[0], k.stride(0)
+            if layers == 0:
+                raise SamplerError("k and v must have a layer at least")
+            shape = (layers, *shape)
+            if layers > 1 and (v.dim() != 4 or v.stride(0) != apart):
+                raise SamplerError("k and v must have the same layer stride")
+        kp, ks = self._heads(k, shape, "k")
+        vp, vs = self._heads(v, shape, "v")
         if index is not None and (index.dtype != i32 or index.numel() != rows or not index.is_contiguous() or
                                   index.get_device() != self.device):
             raise SamplerError(f"index must be ({n}, {rows_per_seq}) int32, contiguous, on the sampler's device")
-        b = _AppendBatch(n, rows_per_seq, layer, layers, kp, vp, k.stride(0), ks, vs, vec(seq, n, i32, "seq"),
+        b = _AppendBatch(n, rows_per_seq, layer, layers, kp, vp, apart, ks, vs, vec(seq, n, i32, "seq"),
                          vec(pos, n, i32, "pos"), vec(count, n, i32, "count"), _addr(index))
         rc = _lib.lcs_kv_append(self.ctx, c, b, self._raw_stream(stream))
         if rc != LCS_OK:
@@ -815,16 +821,17 @@ class Sampler:
         `length` and `seq` (n,) int32: cached tokens and slots (None: 0, 1, ..);
         `mask` (rows, words) int32, or None for chains; scale None: head_dim ** -0.5.
         `out` holds "o" as q, and "lse" (rows, heads) f32 if wanted."""
-        c, i32, vec = self._cache(cache), self.torch.int32, self._vec
-        n, dim = length.numel(), c.head_dim
+        c, i32, vec = self._cache(cache), self._i32, self._vec
+        n, kv_heads, dim = length.numel(), cache.shape[2], cache.shape[4]
         rows = n * rows_per_seq
         if q.dim() != 3:
             raise SamplerError("q must be (rows, heads, head_dim)")
         heads = q.shape[1]
-        qp, qs = self._heads(q, rows, heads, dim, "q")
-        kp, ks = self._heads(k, rows, c.kv_heads, dim, "k")
-        vp, vs = self._heads(v, rows, c.kv_heads, dim, "v")
-        op, os_ = self._heads(out["o"], rows, heads, dim, "o")
+        shape, new = (rows, heads, dim), (rows, kv_heads, dim)
+        qp, qs = self._heads(q, shape, "q")
+        kp, ks = self._heads(k, new, "k")
+        vp, vs = self._heads(v, new, "v")
+        op, os_ = self._heads(out["o"], shape, "o")
         lse, words = out.get("lse"), 0
         if lse is not None and (lse.dtype != self.torch.float32 or lse.shape != (rows, heads) or not lse.is_contiguous() or
                                 lse.get_device() != self.device):
@@ -835,7 +842,7 @@ class Sampler:
                     mask.get_device() != self.device):
                 raise SamplerError(f"mask must be ({rows}, words) int32, contiguous, on the sampler's device")
             words = mask.shape[1]
-        b = _TreeBatch(n, rows_per_seq, heads, layer, dim ** -0.5 if scale is None else scale, words, C.pointer(c), qp, kp,
+        b = _TreeBatch(n, rows_per_seq, heads, layer, dim ** -0.5 if scale is None else scale, words, cache._p, qp, kp,
                        vp, qs, ks, vs, vec(seq, n, i32, "seq"), vec(length, n, i32, "length"), _addr(mask))
         rc = _lib.lcs_tree_attn(self.ctx, b, _TreeOut(op, os_, _addr(lse)), self._raw_stream(stream))
         if rc != LCS_OK:
@@ -848,7 +855,7 @@ class Sampler:
         argmax. `out` holds "argmax_ids" (rows,), "path" (n, rows_per_seq),
         "n_path" and "next_id" (n,) int32, and if wanted "node_lp" (rows,) f32 and
         "length" (n,) int32: `length` + n_path."""
-        i32, f32, vec = self.torch.int32, self.torch.float32, self._vec
+        i32, f32, vec = self._i32, self._f32, self._vec
         rows = tokens.numel()
         if rows_per_seq < 1 or rows % rows_per_seq:
             raise SamplerError("rows_per_seq must divide the rows")
