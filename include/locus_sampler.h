@@ -46,7 +46,7 @@ enum lcs_status {
 enum lcs_dtype {
     LCS_F32 = 0,
     LCS_BF16 = 1,
-    LCS_E4M3 = 2              /* 8 bits (OCP e4m3, no infinities): lcs_add_rmsnorm, lcs_lmhead_ex */
+    LCS_E4M3 = 2              /* 8 bits (OCP e4m3, no infinities): lcs_add_rmsnorm, lcs_lmhead_ex, lcs_kv_cache */
 };
 
 enum lcs_flags {
@@ -319,17 +319,17 @@ typedef struct lcs_kv_cache {
  * nothing (or scores of -inf only) has o = 0 and lse = -inf. What a row does not see is no part of its
  * result, whatever it holds. */
 typedef struct lcs_tree_attn_batch {
-    uint32_t n_seq;            /* up to 1024 */
+    uint32_t n_seq;            /* up to 1024, and n_seq * kv_heads up to 65536 */
     uint32_t rows_per_seq;     /* 1..256 */
     uint32_t heads;            /* a multiple of the cache's kv_heads */
     uint32_t layer;
-    float scale;               /* finite */
+    float scale;               /* at most 1e30, of either sign */
     uint32_t mask_words;       /* >= ceil(rows_per_seq / 32) when mask != NULL */
     const lcs_kv_cache* cache; /* host struct */
     const void* q;             /* row r = i * rows_per_seq + j, head h: q + r * q_stride + h * head_dim; bf16 */
     const void* k;             /* likewise, kv_heads a row */
     const void* v;
-    uint64_t q_stride;         /* elements; bases and strides are multiples of 16 bytes */
+    uint64_t q_stride;         /* elements; bases and strides are multiples of 16 bytes, k's and v's at most 2^25 */
     uint64_t k_stride;
     uint64_t v_stride;
     const int32_t* seq;        /* n_seq: the sequence's slot of the cache, -1: no context; NULL: i */
@@ -471,9 +471,12 @@ int lcs_lmhead_ex(lcs_ctx* ctx, const lcs_lmhead_ex_batch* batch, const lcs_lmhe
  * nothing and uses no context workspace: rows are not bounded by max_rows. */
 int lcs_add_rmsnorm(lcs_ctx* ctx, const lcs_norm_batch* batch, const lcs_norm_out* out, void* stream);
 
-/* The workspace of the calls below: room for `new_pages` pages that one lcs_kv_grow
- * call may allocate, and for the partial results of lcs_tree_attn (about 17 MB).
- * Allocates once, ahead of the hot loop (a call with a larger limit reallocates). */
+/* The workspace of lcs_kv_grow and lcs_tree_attn: room for `new_pages` pages that one
+ * lcs_kv_grow call may allocate, and for the partial results of lcs_tree_attn (34 MB).
+ * Allocates once, ahead of the hot loop; a call with a larger limit reallocates, and
+ * graphs that were captured ahead of it are then to be captured anew. Nothing in it
+ * outlives a call, but calls on one context share it: issue them, and graphs that hold
+ * them, on one stream, or order the streams. */
 int lcs_kv_reserve(lcs_ctx* ctx, uint32_t new_pages);
 
 /* The bookkeeping of a paged cache, on the device, for n <= 1024 requests per call. Slots

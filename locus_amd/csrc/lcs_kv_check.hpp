@@ -80,7 +80,7 @@ inline int check_kv_requests(const lcs_kv_cache* c, uint32_t n, const int32_t* s
 inline int check_kv_compact(const lcs_kv_cache* c, uint32_t n, uint32_t max_keep, const int32_t* seq, const int32_t* count,
                             const int32_t* keep, const int32_t* result, uint32_t max_req, const char** why) {
     const Why w{why};
-    const int rc = check_kv_requests(c, n, seq, count, keep, result, max_req, why);
+    const int rc = check_kv_requests(c, n, seq, count, max_keep ? keep : count, result, max_req, why);
     if (rc != LCS_OK) return rc;
     if (max_keep > 0x7fffffffu) return w.no("max_keep must be below 2^31");
     if ((uint64_t)n * c->layers * 2u * c->kv_heads > 0x7fffffffull) return w.over("too many requests, layers and heads for a call");
@@ -121,7 +121,7 @@ inline int check_tree_attn(const lcs_tree_attn_batch* b, const lcs_tree_attn_out
     if (b->rows_per_seq == 0 || b->rows_per_seq > 256) return w.no("rows_per_seq must be 1..256");
     if (b->heads == 0 || b->heads % c->kv_heads != 0 || b->heads > 65536) return w.no("heads must be a multiple of kv_heads, up to 65536");
     if (b->layer >= c->layers) return w.no("layer outside the cache's");
-    if (!finite_bits(b->scale)) return w.no("scale must be finite");
+    if (!finite_bits(b->scale) || b->scale > 1e30f || b->scale < -1e30f) return w.no("scale must be a number of at most 1e30");
     if (!b->q || !b->k || !b->v || !b->length || !o->o) return w.no("null q / k / v / length / o");
     if (misaligned(b->q, 16u) || misaligned(b->k, 16u) || misaligned(b->v, 16u) || misaligned(o->o, 16u)) {
         return w.no("q, k, v and o must be 16-byte aligned");

@@ -161,9 +161,11 @@ struct Seq {
     int32_t slot;
 };
 struct Line {
-    uint32_t per, before, total;   // steps ahead of the lane's sequences, of all sequences
+    uint32_t per, before, total;   // units ahead of the lane's sequences, of all sequences (of one kv head)
+    uint32_t unit, share;          // steps of a unit; units of a piece
     Seq one;                       // the lane's last sequence
     bool bad;
+    __device__ __forceinline__ uint32_t units(const Seq& q) const { return unit == 1u ? q.steps : (q.steps + unit - 1u) / unit; }
 };
 __device__ __forceinline__ Seq seq_of(const TreeArgs& a, uint32_t i, bool& bad) {
     const int32_t slot = a.c.seq ? a.c.seq[i] : (int32_t)i;
@@ -179,8 +181,15 @@ __device__ __forceinline__ Seq seq_of(const TreeArgs& a, uint32_t i, bool& bad) 
     }
     return Seq{len, (len + kStepKeys - 1u) / kStepKeys + a.new_steps, slot};
 }
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); }
+// The line is cut into a.pieces equal pieces, of `share` steps each. A piece that begins with one
+// pair's end and goes on with another's start pays twice for what a pair costs by itself
+// (about three steps), so where pieces are short, pairs are cut by themselves instead, into
+// units of `share` or one more steps, a piece each, if there are pieces enough (7 trees of
+// 13 nodes over up to 1777 tokens, 5 kv heads: 24.3 -> 19.5 us).
+constexpr uint32_t kShortShare = 4;
 __device__ __forceinline__ Line line_of(const TreeArgs& a) {
-    Line l{(a.c.n + kWave - 1u) / kWave, 0u, 0u, Seq{0u, 0u, 0}, false};
+    Line l{(a.c.n + kWave - 1u) / kWave, 0u, 0u, 1u, 0u, Seq{0u, 0u, 0}, false};
     uint32_t sum = 0;
     for (uint32_t k = 0; k < l.per; ++k) {
         const uint32_t i = (uint32_t)lane_id() * l.per + k;
@@ -189,16 +198,26 @@ __device__ __forceinline__ Line line_of(const TreeArgs& a) {
             sum += l.one.steps;
         }
     }
-    const uint32_t incl = wave_scan_incl_u(sum);
+    uint32_t incl = wave_scan_incl_u(sum);
     l.before = incl - sum;
     l.total = (uint32_t)__builtin_amdgcn_readlane((int)incl, kWave - 1);
+    const uint32_t H = a.c.kv_heads;
+    l.share = max((l.total * H + a.pieces - 1u) / a.pieces, 1u);
+    if (l.per == 1u && l.share > 1u && l.share <= kShortShare) {   // (uniform; lanes without a sequence have 0 steps)
+        for (uint32_t unit = l.share; unit <= l.share + 1u; ++unit) {
+            const uint32_t mine = (l.one.steps + unit - 1u) / unit;
+            incl = wave_scan_incl_u(mine);
+            const uint32_t total = (uint32_t)__builtin_amdgcn_readlane((int)incl, kWave - 1);
+            if (total * H <= a.pieces) {
+                l.before = incl - mine;
+                l.total = total;
+                l.unit = unit;
+                l.share = 1u;
+                break;
+            }
+        }
+    }
     return l;
-}
-__device__ __forceinline__ uint32_t uniform(uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); }
-// The steps of one workgroup's piece of the line (of total x kv_heads steps).
-__device__ __forceinline__ uint32_t share_of(const TreeArgs& a, uint32_t all) {
-    const uint32_t s = (all + a.pieces - 1u) / a.pieces;
-    return s > 1u ? s : 1u;
 }
 
 template <int DP>
@@ -232,7 +251,7 @@ __global__ __launch_bounds__(kTreeWaves * WR * kWave, WR == 1 ? kTreePerCu<DP> :
     const uint32_t b = wg_x(), piece = b / 8u / a.row_tiles * 8u + b % 8u, rt = b / 8u % a.row_tiles + a.row_tile0;
     const Line line = line_of(a);
     if (line.bad && b == 0u && wave == 0u) atomicOr(a.c.status, kStatusPages);
-    const uint32_t H = a.c.kv_heads, all = line.total * H, share = share_of(a, all);
+    const uint32_t H = a.c.kv_heads, all = line.total * H, share = line.share;
     const uint32_t end = min(all, (piece + 1u) * share);   // (all < 2^31 / ...: checked on the host)
     const uint32_t D = a.c.head_dim, N = a.rows_per_seq, R = N * a.group;
     const uint64_t ts = a.c.token_stride * (F8 ? 1u : 2u);
@@ -255,7 +274,7 @@ __global__ __launch_bounds__(kTreeWaves * WR * kWave, WR == 1 ? kTreePerCu<DP> :
         } else {
             bool dummy = false;
             sq = seq_of(a, i, dummy);
-            while (x - at >= sq.steps * H) {
+            while (x - at >= sq.steps * H) {   // (units of one step)
                 at += sq.steps * H;
                 sq = seq_of(a, ++i, dummy);
             }
@@ -263,7 +282,8 @@ __global__ __launch_bounds__(kTreeWaves * WR * kWave, WR == 1 ? kTreePerCu<DP> :
         i = uniform(i);
         const uint32_t len = uniform(sq.len), steps = uniform(sq.steps);
         const int32_t slot = (int32_t)uniform((uint32_t)sq.slot);
-        const uint32_t y = x - uniform(at), kvh = y / steps, s0 = y % steps, s1 = min(steps, s0 + (end - x));
+        const uint32_t units = line.units(Seq{len, steps, slot}), y = x - uniform(at), kvh = y / units, u0 = y % units, u1 = min(units, u0 + (end - x));
+        const uint32_t s0 = u0 * line.unit, s1 = min(steps, u1 * line.unit);
         const uint32_t ctx_steps = steps - a.new_steps;
         const int32_t* row = a.c.table + (uint64_t)(len > 0u ? (uint32_t)slot : 0u) * a.c.max_pages;
         const unsigned char* kb = static_cast<const unsigned char*>(a.c.k) + (a.c.layer * a.c.layer_stride + kvh * a.c.head_stride) * (F8 ? 1u : 2u);
@@ -787,7 +807,7 @@ __global__ __launch_bounds__(kTreeWaves * WR * kWave, WR == 1 ? kTreePerCu<DP> :
         lds_sync();
         const bool complete = s0 == 0u && s1 == steps;
         // (who shares the pair: its first and last pieces, and whether it begins inside the first)
-        if (s0 == 0u && rt == a.row_tile0 && tid_x() == 0u) a.spans[i * H + kvh] = piece | (x + steps - 1u) / share << 15 | (x != piece * share ? 1u << 31 : 0u);
+        if (s0 == 0u && rt == a.row_tile0 && tid_x() == 0u) a.spans[i * H + kvh] = piece | (x + units - 1u) / share << 15 | (x != piece * share ? 1u << 31 : 0u);
         // (a workgroup has at most two incomplete segments: one that begins with the piece, one that ends with it)
         float* part = a.part + ((uint64_t)b * 2u + (x == piece * share ? 0u : 1u)) * Part<DP, MT * WR>::kFloats;
         for (uint32_t it = tid_x(); it < kRows * (DP / 4u); it += kTreeWaves * WR * kWave) {
@@ -820,7 +840,7 @@ __global__ __launch_bounds__(kTreeWaves * WR * kWave, WR == 1 ? kTreePerCu<DP> :
             }
         }
         lds_sync();
-        x += s1 - s0;
+        x += u1 - u0;
     }
 }
 

@@ -94,6 +94,8 @@ def test_requests(lib):
     assert call(lib.requests, cache(pages=0), 3, A, A, A, A)[0] == -1
     assert call(lib.compact, c, 3, 7, A, A, A, A) == (0, "")
     assert call(lib.compact, c, 3, 1 << 31, A, A, A, A)[0] == -1
+    assert call(lib.compact, c, 3, 0, A, A, None, A) == (0, "")
+    assert call(lib.compact, c, 3, 1, A, A, None, A)[0] == -1
     big = dict(layers=4096, kv_heads=1024, pages=1, head_stride=16 * 64, page_stride=0, layer_stride=1024 * 16 * 64)
     assert call(lib.compact, cache(**big), 200, 7, A, A, A, A) == (0, "")
     assert call(lib.compact, cache(**big), 300, 7, A, A, A, A)[0] == -4
@@ -130,10 +132,10 @@ def attn(**kw):
 
 def test_attention(lib):
     for kw in [{}, dict(n_seq=0, q=None), dict(lse=None), dict(seq=A, mask=A, mask_words=1), dict(rows_per_seq=256, mask=A, mask_words=8),
-               dict(scale=-1.0), dict(scale=0.0), dict(layer=1), dict(q_stride=1000, o_stride=392, k_stride=1000), dict(heads=3)]:
+               dict(scale=-1.0), dict(scale=0.0), dict(scale=-9e29), dict(layer=1), dict(q_stride=1000, o_stride=392, k_stride=1000), dict(heads=3)]:
         assert call(lib.attn, *attn(**kw)) == (0, ""), kw
     for kw, rc in [(dict(n_seq=1025), -4), (dict(rows_per_seq=0), -1), (dict(rows_per_seq=257), -1), (dict(heads=0), -1), (dict(heads=7), -1),
-                   (dict(heads=3 << 20), -1), (dict(layer=2), -1), (dict(scale=float("nan")), -1), (dict(scale=float("inf")), -1), (dict(q=None), -1),
+                   (dict(heads=3 << 20), -1), (dict(layer=2), -1), (dict(scale=float("nan")), -1), (dict(scale=float("inf")), -1), (dict(scale=1.1e30), -1), (dict(scale=-1.1e30), -1), (dict(q=None), -1),
                    (dict(k=None), -1), (dict(v=None), -1), (dict(length=None), -1), (dict(o=None), -1), (dict(q=A + 8), -1), (dict(o=A + 2), -1),
                    (dict(seq=A + 2), -1), (dict(lse=A + 1), -1), (dict(mask=A), -1), (dict(rows_per_seq=33, mask=A, mask_words=1), -1),
                    (dict(q_stride=6 * 64 - 8), -1), (dict(o_stride=6 * 64 - 8), -1), (dict(k_stride=184), -1), (dict(v_stride=196), -1),
