@@ -112,6 +112,13 @@ __device__ __forceinline__ void read_tr8(const uint32_t (&at)[4], u32x2 (&o)[4])
 }
 // Plain reads, likewise: 16 bytes at each address and NEXT bytes behind it.
 template <int NEXT>
+__device__ __forceinline__ void read_one(const uint32_t (&at)[1], u32x4 (&lo)[1], u32x4 (&hi)[1]) {
+    asm volatile("ds_read_b128 %0, %2\n\tds_read_b128 %1, %2 offset:%3\n\ts_waitcnt lgkmcnt(0)"
+                 : "=&v"(lo[0]), "=&v"(hi[0])
+                 : "v"(at[0]), "n"(NEXT)
+                 : "memory");
+}
+template <int NEXT>
 __device__ __forceinline__ void read_two(const uint32_t (&at)[2], u32x4 (&lo)[2], u32x4 (&hi)[2]) {
     asm volatile("ds_read_b128 %0, %4\n\tds_read_b128 %1, %4 offset:%6\n\tds_read_b128 %2, %5\n\tds_read_b128 %3, %5 offset:%6\n\t"
                  "s_waitcnt lgkmcnt(0)"
@@ -532,11 +539,7 @@ __global__ __launch_bounds__(kTreeWaves * WR * kWave, WR == 1 ? kTreePerCu<DP> :
                 } else if constexpr (kAt == 2u) {
                     read_two<16 * kRowB>(ad, lo, hi);
                 } else {
-                    const uint32_t twice[2] = {ad[0], ad[0]};
-                    u32x4 l2[2], h2[2];
-                    read_two<16 * kRowB>(twice, l2, h2);
-                    lo[0] = l2[0];
-                    hi[0] = h2[0];
+                    read_one<16 * kRowB>(ad, lo, hi);
                 }
 #pragma unroll
                 for (uint32_t c = 0; c < kAt; ++c) {
