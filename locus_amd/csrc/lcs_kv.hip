@@ -288,8 +288,11 @@ __global__ __launch_bounds__(kKvThreads) void kv_copy(KvArgs a) {
 }
 
 // ---- lcs_kv_compact ----
-// Whether a request can be served, a workgroup each.
-__global__ __launch_bounds__(kKvThreads) void kv_compact_check(KvArgs a) {
+// Whether a request can be served, a workgroup each. Its time is the chain of place, table and
+// count that a thread walks every kCheckThreads rows (16 contexts cut to 4096 rows:
+// 357 us for the whole call by 256 threads, 347 by 1024; 610 rows 11.0 by either).
+constexpr int kCheckThreads = 1024;
+__global__ __launch_bounds__(kCheckThreads) void kv_compact_check(KvArgs a) {
     const uint32_t i = wg_x();
     const int32_t slot = a.seq[i];
     if (slot == -1) {
@@ -302,7 +305,7 @@ __global__ __launch_bounds__(kKvThreads) void kv_compact_check(KvArgs a) {
         const uint32_t n = min((uint32_t)max(a.count[i], 0), a.max_keep);
         const int32_t* keep = a.index + (uint64_t)i * a.max_keep;
         const int32_t* row = a.table + (uint64_t)slot * a.max_pages;
-        for (uint32_t j = tid_x(); j < n; j += kKvThreads) {
+        for (uint32_t j = tid_x(); j < n; j += kCheckThreads) {
             const int32_t pos = keep[j], last = j ? keep[j - 1u] : -1;
             const uint32_t pp = (uint32_t)pos >> a.page_shift, pj = j >> a.page_shift;
             if (pos <= last || pos < (int32_t)j || pp >= a.max_pages) {
@@ -416,7 +419,11 @@ __global__ __launch_bounds__(kKvThreads) void kv_compact(KvArgs a) {
 // up once, ahead of the rows. A lane keeps its head from token to token, and quotients
 // take three operations each, since arithmetic bounds the 8-bit form (64 x 4.5 tokens of
 // 32 layers x 8 heads: 59 us with divisions for both).
-constexpr uint32_t kAppendTokens = 16;
+// (Few tokens a workgroup, the layers of one sequence side by side: CUs then take like shares
+// where the sequences' counts differ. 64 sequences of 0 to 16 kept tokens, 32 layers, with
+// the verdict and the pages: 88.9 us; 16 tokens a workgroup, one layer's sequences side
+// by side 90.7. All 16 kept: 39 us by either, 5.2 TB/s.)
+constexpr uint32_t kAppendTokens = 4;
 
 // x / scale to nearest: RN(1 / scale), a product, and its remainder's share (exact by an fma),
 // which makes the quotient the correctly rounded one. An infinite scale gives 0, and NaN
@@ -447,7 +454,8 @@ __global__ __launch_bounds__(kKvThreads) void kv_append(KvAppendArgs p) {
     constexpr uint32_t U = 4;
     __shared__ int32_t page_s[kAppendTokens], src_s[kAppendTokens];
     const KvArgs& a = p.a;
-    const uint32_t i = wg_x() / p.blocks, j0 = wg_x() % p.blocks * kAppendTokens, l = __builtin_amdgcn_workgroup_id_y();
+    const uint32_t id = wg_x() + __builtin_amdgcn_workgroup_id_y() * p.a.n * p.blocks;   // (n_layers * n * blocks of them: below 2^32)
+    const uint32_t l = id % p.n_layers, wg = id / p.n_layers, i = wg / p.blocks, j0 = wg % p.blocks * kAppendTokens;
     const int32_t slot = a.seq ? a.seq[i] : (int32_t)i;
     const uint32_t n = a.count ? min((uint32_t)max(a.count[i], 0), p.rows_per_seq) : p.rows_per_seq;
     const int32_t pos0 = a.start[i];
@@ -562,7 +570,7 @@ hipError_t launch_kv_compact(const KvArgs& args, hipStream_t st) {
     KvArgs a = args;
     a.chunks = a.head_dim * (a.f8 ? 1u : 2u) / 16u;
     a.cp = pow2_from(a.chunks);
-    hipLaunchKernelGGL(kv_compact_check, dim3(a.n), dim3(kKvThreads), 0, st, a);
+    hipLaunchKernelGGL(kv_compact_check, dim3(a.n), dim3(kCheckThreads), 0, st, a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     // (few rows' heads: their chunks apart, so that the CUs have more in flight)
