@@ -518,7 +518,8 @@ int lcs_kv_compact(lcs_ctx* ctx, const lcs_kv_cache* cache, uint32_t n, uint32_t
  * Allocates nothing and uses no context workspace. */
 int lcs_kv_append(lcs_ctx* ctx, const lcs_kv_cache* cache, const lcs_kv_append_batch* batch, void* stream);
 
-/* Attention over the cache and the new tokens (see lcs_tree_attn_batch). Allocates nothing.
+/* Attention over the cache and the new tokens (see lcs_tree_attn_batch), after
+ * lcs_kv_reserve. Allocates nothing.
  * A page that is missing below length[i] counts as not seen and sets LCS_STATUS_PAGES, as
  * does a slot outside [-1, seqs) or a length past the table. */
 int lcs_tree_attn(lcs_ctx* ctx, const lcs_tree_attn_batch* batch, const lcs_tree_attn_out* out, void* stream);
