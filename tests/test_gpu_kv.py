@@ -313,3 +313,88 @@ def test_random_runs(s, seed):
         else:
             keep = [sorted(rng.sample(range(rng.choice([30, 60, 96])), 20)) for _ in seq]
             c.compact(seq, [rng.randint(0, 20) for _ in seq], keep)
+
+
+@pytest.mark.parametrize("f8", [False, True])
+def test_far_pages(s, f8):
+    """Places past 2^32 bytes: rows appended to the last pages of a large pool, copied on write and compacted there."""
+    pages, heads, page, dim = (24576, 8, 128, 128) if not f8 else (36864, 8, 128, 128)
+    shape = (1, pages, heads, page, dim)
+    k, v = (torch.empty(shape, dtype=torch.float8_e4m3fn if f8 else torch.bfloat16, device="cuda") for _ in range(2))
+    assert k.numel() * k.element_size() > 1 << 32
+    scales = {n: torch.empty(shape[:4], device="cuda") for n in ("k_scale", "v_scale")} if f8 else {}
+    refs = torch.ones(pages, dtype=torch.int32, device="cuda")
+    refs[-5:] = 0
+    table = torch.full((2, 3), -1, dtype=torch.int32, device="cuda")
+    c = S.KvCache(k, v, table, refs, **scales)
+    ints = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")   # noqa: E731
+    g = torch.Generator().manual_seed(1)
+    new = [torch.randn(1, 200, heads, dim, generator=g).bfloat16() for _ in range(2)]
+    r = [ints(9) for _ in range(4)]
+    s.status()
+    s.kv_grow_dev(c, ints(0), ints(0), ints(200), r[0])
+    s.kv_append_dev(c, new[0].cuda(), new[1].cuda(), ints(0), ints(0), rows_per_seq=200)
+    s.kv_fork_dev(c, ints(0), ints(1), ints(200), r[1])
+    s.kv_grow_dev(c, ints(1), ints(0), ints(200), r[2])
+    keep = sorted(random.Random(2).sample(range(200), 150))
+    s.kv_compact_dev(c, ints(1), ints(150), torch.tensor([keep], dtype=torch.int32, device="cuda"), r[3])
+    torch.cuda.synchronize()
+    assert [int(x) for x in r] == [0] * 4 and s.status() == 0
+    assert table.tolist() == [[pages - 5, pages - 4, -1], [pages - 3, pages - 2, -1]] and refs[-5:].tolist() == [1, 1, 1, 1, 0]
+    for slot, rows in ((0, list(range(200))), (1, keep)):
+        at = table[slot, :2].long()
+        for t, n, sc in ((k, new[0], "k_scale"), (v, new[1], "v_scale")):
+            want, scale = quantise(n[0, rows]) if f8 else (n[0, rows], None)
+            held = t[0, at].permute(0, 2, 1, 3).reshape(2 * page, heads, dim)[: len(rows)].cpu()
+            assert torch.equal(bits(held), bits(want))
+            if f8:
+                assert torch.equal(scales[sc][0, at].permute(0, 2, 1).reshape(2 * page, heads)[: len(rows)].cpu(), scale)
+
+
+def test_side_stream_and_graph(s):
+    """Pages and rows on a side stream, and in two graphs of one context that are replayed in turn with eager calls between."""
+    pairs = [Pair(s, pages=60, max_pages=6, seed=i) for i in range(4)]
+    rows, dim = 9, 64
+    g = torch.Generator().manual_seed(4)
+    k, v = (torch.randn(2, 3 * rows, 3, dim, generator=g).bfloat16().cuda() for _ in range(2))
+    seq = pairs[0].ints([2, 0, 5])
+    state = [{"start": c.ints([0, 3, 40]), "end": c.ints([9, 12, 49]), "res": c.ints([9] * 3)} for c in pairs]
+
+    def step(c, st, stream=None):
+        s.kv_grow_dev(c.cache, seq, st["start"], st["end"], st["res"], stream=stream)
+        s.kv_append_dev(c.cache, k, v, seq, st["start"], rows_per_seq=rows, stream=stream)
+
+    graphs = []
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for c, st in zip(pairs[:2], state):
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            step(c, st)
+        graphs.append(gr)
+    for i in range(4):
+        for a in (0, 1):
+            if i == 2:
+                step(pairs[a], state[a], side)
+                side.synchronize()
+            else:
+                graphs[a].replay()
+            torch.cuda.synchronize()
+            step(pairs[2 + a], state[2 + a])
+            torch.cuda.synchronize()
+            assert torch.equal(state[a]["res"], state[2 + a]["res"])
+            assert torch.equal(pairs[a].table, pairs[2 + a].table) and torch.equal(pairs[a].refs, pairs[2 + a].refs)
+            used = pairs[a].table[pairs[a].table >= 0].long()
+            for x, y in ((pairs[a].k, pairs[2 + a].k), (pairs[a].v, pairs[2 + a].v)):
+                x, y = x[:, used], y[:, used]
+                same = x.view(torch.int16) == y.view(torch.int16)
+                filled = torch.zeros(x.shape[:4], dtype=torch.bool, device="cuda")
+                for j, q in enumerate(seq.tolist()):
+                    for p in range(int(state[a]["start"][j]), int(state[a]["end"][j])):
+                        page = int(pairs[a].table[q, p // 16])
+                        filled[:, (used == page).nonzero()[0, 0], :, p % 16] = True
+                assert bool(same[filled].all())
+        for st in state:
+            st["start"] += 9
+            st["end"] += 9
+    assert s.status() == 0
