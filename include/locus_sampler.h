@@ -472,7 +472,7 @@ int lcs_lmhead_ex(lcs_ctx* ctx, const lcs_lmhead_ex_batch* batch, const lcs_lmhe
 int lcs_add_rmsnorm(lcs_ctx* ctx, const lcs_norm_batch* batch, const lcs_norm_out* out, void* stream);
 
 /* The workspace of lcs_kv_grow and lcs_tree_attn: room for `new_pages` pages that one
- * lcs_kv_grow call may allocate, and for the partial results of lcs_tree_attn (17 MB).
+ * lcs_kv_grow call may allocate, and for the partial results of lcs_tree_attn (34 MB).
  * Allocates once, ahead of the hot loop; a call with a larger limit reallocates, and
  * graphs that were captured ahead of it are then to be captured anew. Nothing in it
  * outlives a call, but calls on one context share it: issue them, and graphs that hold

@@ -9,7 +9,7 @@
 // - A wave takes 32 keys at a time, their keys and values brought to its own part of
 //   LDS by 16-byte DMA loads, so that no register holds data in flight and waves need
 //   no barrier; four waves take 128 consecutive tokens, a step.
-//   Above 128 rows a head two waves share a tile and bring a half of it each, with barriers.
+//   Above 64 rows a head two or four waves share a tile, of which each brings its part, with barriers.
 // - Scores are computed transposed, S^T = K Q^T, with Q in registers as the B
 //   operand: a lane then holds eight keys of one row, so that its softmax is the
 //   lane's own, and the weights are already laid out as the B operand of O^T = V^T P^T.
@@ -239,9 +239,15 @@ struct Part {
 
 }  // namespace
 
+// Tiles that a workgroup has before it at once, each shared by WR waves.
+template <int WR>
+constexpr int kTilesOf = WR == 4 ? 2 : kTreeWaves;
+
 template <int DP, int MT, bool F8, int ST, int WR>
-__global__ __launch_bounds__(kTreeWaves * WR * kWave, WR == 1 ? kTreePerCu<DP> : 1) void tree_attn(TreeArgs a) {
-    static_assert(WR == 1 || (WR == 2 && ST == 2 && !F8), "the schedule of shared tiles");
+__global__ __launch_bounds__(kTilesOf<WR> * WR * kWave, WR == 1 ? kTreePerCu<DP> : 1) void tree_attn(TreeArgs a) {
+    static_assert(WR == 1 || ((WR == 2 || WR == 4) && ST == 2 && !F8), "the schedule of shared tiles");
+    constexpr int NW = kTilesOf<WR>;
+    constexpr uint32_t kStride = NW * kTileKeys, kPer = kStepKeys / kStride;   // keys from tile to tile of a wave, its tiles a step
     constexpr uint32_t kMine = 16u * MT, kRows = kMine * WR, kDT = DP / 16, kKS = DP / 32;   // rows of a wave, of the workgroup
     constexpr uint32_t kRowB = DP * (F8 ? 1 : 2), kNewB = DP * 2;                 // bytes of a cached row and of a new one in LDS
     constexpr uint32_t kScaleB = F8 ? 256u : 0u;
@@ -251,9 +257,9 @@ __global__ __launch_bounds__(kTreeWaves * WR * kWave, WR == 1 ? kTreePerCu<DP> :
     constexpr uint32_t kRegion = kMax1 > kMergeB ? kMax1 : kMergeB;
     constexpr int kNI = (int)(kTileKeys * kRowB / 1024u);      // DMA loads of a tile's keys, and of its values
     constexpr int kNK = kNI + (F8 ? 1 : 0);
-    __shared__ __attribute__((aligned(1024))) unsigned char lds[kTreeWaves * kRegion];
-    __shared__ float stat[kTreeWaves][2][kRows];
-    const uint32_t lane = (uint32_t)lane_id(), wave = uniform(tid_x() / kWave), w = wave % kTreeWaves, wr = wave / kTreeWaves, n = lane & 15u, g = lane >> 4;
+    __shared__ __attribute__((aligned(1024))) unsigned char lds[NW * kRegion];
+    __shared__ float stat[NW][2][kRows];
+    const uint32_t lane = (uint32_t)lane_id(), wave = uniform(tid_x() / kWave), w = wave % NW, wr = wave / NW, n = lane & 15u, g = lane >> 4;
     unsigned char* const mine = lds + w * kRegion;
     const uint32_t b = wg_x(), piece = b / 8u / a.row_tiles * 8u + b % 8u, rt = b / 8u % a.row_tiles + a.row_tile0;
     const Line line = line_of(a);
@@ -296,21 +302,21 @@ __global__ __launch_bounds__(kTreeWaves * WR * kWave, WR == 1 ? kTreePerCu<DP> :
         const unsigned char* kb = static_cast<const unsigned char*>(a.c.k) + (a.c.layer * a.c.layer_stride + kvh * a.c.head_stride) * (F8 ? 1u : 2u);
         const unsigned char* vb = static_cast<const unsigned char*>(a.c.v) + (a.c.layer * a.c.layer_stride + kvh * a.c.head_stride) * (F8 ? 1u : 2u);
 
-        // ---- the wave's cached tiles: tile j starts at token first + 128 j ----
+        // ---- the wave's cached tiles: tile j starts at token first + kStride j ----
         const uint32_t c1 = min(s1, ctx_steps), first = s0 * kStepKeys + w * kTileKeys;
-        const uint32_t nct = s0 < c1 ? c1 - s0 : 0u;   // (the last one may lie past the length: all zeros, unseen)
+        const uint32_t nct = s0 < c1 ? (c1 - s0) * kPer : 0u;   // (the last ones may lie past the length: all zeros, unseen)
         struct Tile {
             uint32_t p0, p1;   // the pages of its first and last 16 tokens
             uint32_t there;    // its keys that are there (settle)
         };
         auto pages_of = [&](uint32_t j) -> Tile {
-            const uint32_t t0 = first + (j < nct ? j : 0u) * kStepKeys;
+            const uint32_t t0 = first + (j < nct ? j : 0u) * kStride;
             const uint32_t q0 = min(t0 >> a.c.page_shift, a.c.max_pages - 1u), q1 = min((t0 + 16u) >> a.c.page_shift, a.c.max_pages - 1u);
             if (nct == 0u) return Tile{0u, 0u, 0u};
             return Tile{(uint32_t)scalar_load(row + q0), (uint32_t)scalar_load(row + q1), 0u};
         };
         auto expected = [&](uint32_t j) -> uint32_t {   // the keys of tile j ahead of the length
-            const uint32_t t0 = first + j * kStepKeys, left = t0 < len ? len - t0 : 0u;
+            const uint32_t t0 = first + j * kStride, left = t0 < len ? len - t0 : 0u;
             return left >= 32u ? ~0u : (1u << left) - 1u;
         };
         auto settle = [&](Tile& t, uint32_t j) {   // (a page that is missing: none of its keys, page 0 in its place)
@@ -321,35 +327,37 @@ __global__ __launch_bounds__(kTreeWaves * WR * kWave, WR == 1 ? kTreePerCu<DP> :
         // A tile's 16-row halves lie in one page each; DMA load ii of a half covers rows RPI ii + lane /
         // CPR, a chunk per lane. A half's buffer ends with its last row that is there.
         constexpr uint32_t CPR = kRowB / 16u, RPI = 64u / CPR;
-        constexpr int kHalf = kNI / 2;
+        constexpr int kHalf = kNI / 2, kShare = WR == 4 ? kHalf / 2 : kHalf;   // DMA loads of a half, and those of it that the wave issues
+        static_assert(kShare > 0, "a load for each wave");
+        const uint32_t part0 = WR == 4 ? (wr & 1u) * (uint32_t)kShare : 0u;
         const uint32_t tsb = (uint32_t)ts;
         auto offset_of = [&](bool values, uint32_t r) -> uint32_t {   // the lane's chunk of row r
             const uint32_t ch = (lane % CPR) ^ (values ? swz_v<kRowB, F8>(r) : swz_k<kRowB>(r));
             return 16u * ch < D * (F8 ? 1u : 2u) ? (r & 15u) * tsb + 16u * ch : kNoByte;
         };
-        constexpr int kVo = F8 ? kNI : kHalf;   // (8-bit values: the second half is permuted by other bits)
-        uint32_t vo_k[kHalf], vo_v[kVo];
+        constexpr int kVo = F8 ? kNI : kShare;   // (8-bit values: the second half is permuted by other bits)
+        uint32_t vo_k[kShare], vo_v[kVo];
 #pragma unroll
-        for (int ii = 0; ii < kHalf; ++ii) vo_k[ii] = offset_of(false, RPI * (uint32_t)ii + lane / CPR);
+        for (int ii = 0; ii < kShare; ++ii) vo_k[ii] = offset_of(false, RPI * (part0 + (uint32_t)ii) + lane / CPR);
 #pragma unroll
-        for (int ii = 0; ii < kVo; ++ii) vo_v[ii] = offset_of(true, RPI * (uint32_t)ii + lane / CPR);
+        for (int ii = 0; ii < kVo; ++ii) vo_v[ii] = offset_of(true, RPI * (part0 + (uint32_t)ii) + lane / CPR);
         const uint32_t psb = (uint32_t)a.c.page_stride * (F8 ? 1u : 2u);   // (below 2^32, and so is a row's place in its page)
         auto issue_rows = [&](bool values, const Tile& t, uint32_t j, unsigned char* dst) {
             const unsigned char* base = values ? vb : kb;
 #pragma unroll
-            for (uint32_t q = 0; q < 2u / WR; ++q) {   // (two waves that share a tile bring a half each)
-                const uint32_t h = WR == 2 ? wr : q, first_page = t.p0, second_page = t.p1, in_page = ((first + j * kStepKeys + 16u * h) & (a.c.page_tokens - 1u)) * tsb;
+            for (uint32_t q = 0; q < (WR == 1 ? 2u : 1u); ++q) {   // (waves that share a tile bring a half or a quarter each)
+                const uint32_t h = WR == 1 ? q : wr / (WR / 2u), first_page = t.p0, second_page = t.p1, in_page = ((first + j * kStride + 16u * h) & (a.c.page_tokens - 1u)) * tsb;
                 const __amdgpu_buffer_rsrc_t rs = buffer_of(base + (uint64_t)(h ? second_page : first_page) * psb + in_page,
                                                             (uint32_t)__builtin_popcount(t.there >> (16u * h) & 0xffffu) * tsb);
 #pragma unroll
-                for (int ii = 0; ii < kHalf; ++ii)
-                    dma16(rs, dst + 1024 * (kHalf * h + ii), values ? vo_v[F8 ? kHalf * q + ii : ii] : vo_k[ii]);
+                for (int ii = 0; ii < kShare; ++ii)
+                    dma16(rs, dst + 1024 * (kHalf * h + part0 + ii), values ? vo_v[F8 ? kHalf * q + ii : ii] : vo_k[ii]);
             }
         };
         auto issue_k = [&](const Tile& t, uint32_t j, uint32_t stage) {
             unsigned char* dst = mine + stage;
             if constexpr (F8) {   // the keys' scales by the lower half, the values' by the upper
-                const uint32_t r = lane & 31u, tok = (first + j * kStepKeys + r) & (a.c.page_tokens - 1u), first_page = t.p0, second_page = t.p1;
+                const uint32_t r = lane & 31u, tok = (first + j * kStride + r) & (a.c.page_tokens - 1u), first_page = t.p0, second_page = t.p1;
                 const float* s = lane < 32u ? a.c.k_scale : a.c.v_scale;
                 const uint64_t e = ((((uint64_t)a.c.layer * a.c.pages + (r < 16u ? first_page : second_page)) * H + kvh) << a.c.page_shift) + tok;
                 dma4(t.there >> r & 1u ? static_cast<const void*>(s + e) : a.zeros, dst + 2u * kTileKeys * kRowB);
@@ -366,7 +374,7 @@ __global__ __launch_bounds__(kTreeWaves * WR * kWave, WR == 1 ? kTreePerCu<DP> :
         // ---- the new tokens' tiles (bf16 always), the first one's loads issued where LDS is free ahead of it ----
         constexpr int kNew = (int)(kTileKeys * kNewB / 1024u);   // DMA loads of a tile's keys, and of its values
         const uint32_t st0 = max(s0, ctx_steps);
-        auto new_first = [&](uint32_t st) -> uint32_t { return (st - ctx_steps) * kStepKeys + w * kTileKeys; };
+        auto new_first = [&](uint32_t st) -> uint32_t { return (st - ctx_steps) * kStepKeys + w * kTileKeys; };   // (and every kStride on)
         const bool ahead = st0 < s1 && new_first(st0) < N;
         auto issue_new = [&](bool values, uint32_t n0, unsigned char* dst) {
             constexpr uint32_t CPN = kNewB / 16u, RPN = 64u / CPN;
@@ -377,7 +385,7 @@ __global__ __launch_bounds__(kTreeWaves * WR * kWave, WR == 1 ? kTreePerCu<DP> :
             asm volatile("" : "+v"(ln));
 #pragma unroll
             for (int q = 0; q < kNew / WR; ++q) {
-                const int ii = q + (WR == 2 ? (int)wr * (kNew / 2) : 0);
+                const int ii = q + (int)wr * (kNew / WR);
                 const uint32_t r = RPN * (uint32_t)ii + ln / CPN, c = ln % CPN ^ (values ? swz_v<kNewB, false>(r) : swz_k<kNewB>(r));
                 dma16(rs, dst + 1024 * ii, r < rows && 8u * c < D ? r * stride + 16u * c : kNoByte);
             }
@@ -510,8 +518,8 @@ __global__ __launch_bounds__(kTreeWaves * WR * kWave, WR == 1 ? kTreePerCu<DP> :
             unsigned char* const at_k = mine + stage;
             unsigned char* const at_v = at_k + kTileKeys * kRowB;
             const bool full = j + ST <= nct;   // (ST tiles are under way)
-            constexpr int kIK = kHalf, kIV = kHalf;   // (WR 2) loads of a wave
-            if constexpr (WR == 2) {
+            constexpr int kIK = kShare, kIV = kShare;   // (shared tiles) loads of a wave
+            if constexpr (WR > 1) {
                 // A step of shared tiles: the next values go out once all have taken the last ones', the keys
                 // after the next once all have read these, so that three half steps are under way.
                 if (full) wait_vm<kIV + kIK>();
@@ -561,7 +569,7 @@ __global__ __launch_bounds__(kTreeWaves * WR * kWave, WR == 1 ? kTreePerCu<DP> :
             settle(tile[ST], j + ST);
             const bool then = ahead && j + 1u == nct;   // (the new tokens come next)
             if (then) {
-                if constexpr (WR == 2) {
+                if constexpr (WR > 1) {
                     new_k = mine + (stage ? 0u : kStage);
                     new_v = new_k + kTileKeys * kNewB;
                     issue_new(false, new_first(st0), new_k);
@@ -609,8 +617,8 @@ __global__ __launch_bounds__(kTreeWaves * WR * kWave, WR == 1 ? kTreePerCu<DP> :
                 if (tile[0].there != expected(j) && lane == 0u) atomicOr(a.c.status, kStatusPages);   // (a page is missing)
             }
             weigh(vs, F8);
-            if constexpr (WR == 2) {
-                if (then) wait_vm<kNew>();   // (halves of both)
+            if constexpr (WR > 1) {
+                if (then) wait_vm<2 * kNew / WR>();   // (its shares of both)
                 else if (full) wait_vm<kIK + kIV>();
                 else wait_vm<0>();
                 lds_sync();
@@ -661,15 +669,17 @@ __global__ __launch_bounds__(kTreeWaves * WR * kWave, WR == 1 ? kTreePerCu<DP> :
         }
 
         // ---- the new tokens' products ----
-        for (uint32_t st = st0; st < s1; ++st) {
-            const uint32_t n0 = new_first(st);
+        const uint32_t nnt = st0 < s1 ? (s1 - st0) * kPer : 0u;
+        for (uint32_t jn = 0; jn < nnt; ++jn) {
+            const uint32_t n0 = new_first(st0) + jn * kStride;
+            if (n0 - w * kTileKeys >= N) break;   // (uniform over the workgroup)
             const bool in = n0 < N;   // (uniform over the waves that share a tile; all take part in the barriers)
             if (WR == 1 && !in) continue;
             uint32_t ln = lane;   // (opaque, as above)
             asm volatile("" : "+v"(ln));
             const uint32_t lane_n = ln & 15u, lg = ln >> 4;
-            if (st != st0) {   // (the last tile has been read)
-                if constexpr (WR == 2) lds_sync();
+            if (jn != 0u) {   // (the last tile has been read)
+                if constexpr (WR > 1) lds_sync();
                 else wait_lds();
                 if (in) {
                     issue_new(false, n0, new_k);
@@ -687,7 +697,7 @@ __global__ __launch_bounds__(kTreeWaves * WR * kWave, WR == 1 ? kTreePerCu<DP> :
                 if (N - n0 < 32u) see[m] &= (1u << (N - n0)) - 1u;
             }
             wait_vm<0>();
-            if constexpr (WR == 2) lds_sync();
+            if constexpr (WR > 1) lds_sync();
             bool wild = false;
             if (in) {
 #pragma unroll
@@ -716,7 +726,7 @@ __global__ __launch_bounds__(kTreeWaves * WR * kWave, WR == 1 ? kTreePerCu<DP> :
             }
             }
             const bool any_wild = ballot(wild) != 0ull;
-            if constexpr (WR == 2) lds_sync();   // (keys and values have been read by both)
+            if constexpr (WR > 1) lds_sync();   // (keys and values have been read by both)
             if (any_wild && wr == 0u) {
                 wait_lds();
 #pragma unroll 1
@@ -735,7 +745,7 @@ __global__ __launch_bounds__(kTreeWaves * WR * kWave, WR == 1 ? kTreePerCu<DP> :
                 }
                 wait_lds();
             }
-            if constexpr (WR == 2) {
+            if constexpr (WR > 1) {
                 lds_sync();
                 if (!in) continue;
             }
@@ -794,7 +804,7 @@ __global__ __launch_bounds__(kTreeWaves * WR * kWave, WR == 1 ? kTreePerCu<DP> :
         }
 
         // ---- the waves' sums joined ----
-        if constexpr (WR == 2) lds_sync();   // (the tiles' place)
+        if constexpr (WR > 1) lds_sync();   // (the tiles' place)
         else wait_lds();
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
@@ -813,15 +823,15 @@ __global__ __launch_bounds__(kTreeWaves * WR * kWave, WR == 1 ? kTreePerCu<DP> :
         if (s0 == 0u && rt == a.row_tile0 && tid_x() == 0u) a.spans[i * H + kvh] = piece | (x + units - 1u) / share << 15 | (x != piece * share ? 1u << 31 : 0u);
         // (a workgroup has at most two incomplete segments: one that begins with the piece, one that ends with it)
         float* part = a.part + ((uint64_t)b * 2u + (x == piece * share ? 0u : 1u)) * Part<DP, MT * WR>::kFloats;
-        for (uint32_t it = tid_x(); it < kRows * (DP / 4u); it += kTreeWaves * WR * kWave) {
+        for (uint32_t it = tid_x(); it < kRows * (DP / 4u); it += NW * WR * kWave) {
             const uint32_t rr = it / (DP / 4u), c = it % (DP / 4u), pr = rt * kRows + rr;
             float M = stat[0][0][rr];
 #pragma unroll
-            for (int k = 1; k < kTreeWaves; ++k) M = f_max(M, stat[k][0][rr]);
+            for (int k = 1; k < NW; ++k) M = f_max(M, stat[k][0][rr]);
             f32x4 o = zero;
             float z = 0.0f;
 #pragma unroll
-            for (int k = 0; k < kTreeWaves; ++k) {
+            for (int k = 0; k < NW; ++k) {
                 const float f = exp2_f(stat[k][0][rr] - M);
                 z += stat[k][1][rr] * f;
                 o += *reinterpret_cast<const f32x4*>(lds + (uint32_t)k * kRegion + rr * DP * 4u + (c ^ (rr & 15u)) * 16u) * f;
@@ -926,7 +936,7 @@ __global__ __launch_bounds__(256) void tree_join(TreeArgs a) {
 namespace {
 
 constexpr uint32_t kTreeTiles = 32;   // row tiles of a launch
-constexpr uint32_t kWideRows = 128;   // rows a head above which waves share tiles
+constexpr uint32_t kWideRows = 128;   // rows a head above which two waves share a tile
 
 template <int DP, int MT, bool F8, int ST, int WR>
 hipError_t launch(TreeArgs a, uint32_t cus, hipStream_t st) {
@@ -938,7 +948,7 @@ hipError_t launch(TreeArgs a, uint32_t cus, hipStream_t st) {
         const uint32_t most = per_cu * kTreeSlots / 2u, slots = cus * per_cu < most ? cus * per_cu : most;
         a.pieces = slots / a.row_tiles / 8u * 8u;
         if (a.pieces == 0u) a.pieces = 8u;
-        hipLaunchKernelGGL((tree_attn<DP, MT, F8, ST, WR>), dim3(a.pieces * a.row_tiles), dim3(kTreeWaves * WR * kWave), 0, st, a);
+        hipLaunchKernelGGL((tree_attn<DP, MT, F8, ST, WR>), dim3(a.pieces * a.row_tiles), dim3(kTilesOf<WR> * WR * kWave), 0, st, a);
         hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
         const uint32_t pairs = a.c.n * a.c.kv_heads, blocks = a.row_tiles * (per * DP / 1024u);
@@ -952,16 +962,23 @@ hipError_t launch(TreeArgs a, uint32_t cus, hipStream_t st) {
 
 // Rows of a wave: 16, or 32 where there are more (64 leave one wave a SIMD, whose products
 // wait for its softmax: 256 rows a head, 32 sequences x 4096 tokens x 8 heads 294 us, of 32
-// 276). Above 128 rows over bf16 two waves share each tile, which halves what the L2 and LDS
-// bring (the same 273 -> 244 us; 512 rows, 8 sequences x 8192 tokens 252 -> 234); for
-// fewer rows, and for 8 bits, whose tiles are half as large, its barriers cost what that
-// saves (64 rows over up to 6000 tokens 69 -> 73, 256 rows over e4m3 261 -> 276).
+// 276). Over bf16, waves share tiles where there are enough rows: what the L2 and LDS's
+// write side bring is by a workgroup then and not by a wave. Four waves share a tile, 128 rows a
+// workgroup, where the last 128 are more than half full, else two waves, 64 rows (the same
+// sequences, us of one wave / two / four a tile: 72 rows 154 / - / 120, 128 rows 164 / - / 117,
+// 192 rows - / 206 / 200, 256 rows 273 / 250 / 226; 512 rows, 8 x 8192 tokens 252 / 234 / 217;
+// 320 rows, 16 x 4096 - / 167 / 182). Up to 64 rows its barriers cost more than that saves
+// (40 rows 105 / - / 139, 64 rows 110 / - / 131; over up to 6000 tokens 69 / 73 / -), as with
+// heads of 64 up to 128 rows (16 x 6000 tokens 58 / - / 63), and for 8 bits, whose tiles are half
+// as large (256 rows 261 / 276 / -). One short context is 1 us slower by four (72 rows over 1000
+// tokens 14.3 / - / 15.5 to 16.7): the lengths are known on the device only.
 template <int DP, bool F8>
 hipError_t launch_rows(const TreeArgs& a, uint32_t cus, hipStream_t st) {
     constexpr int ST = F8 || DP == 64 ? 2 : 1;
     const uint32_t rows = a.rows_per_seq * a.group;
     if (rows <= 16u) return launch<DP, 1, F8, ST, 1>(a, cus, st);
     if constexpr (DP != 256 && !F8) {
+        if (rows > (DP == 64 ? kWideRows : 64u) && (rows - 1u) % 128u >= 64u) return launch<DP, 2, F8, 2, 4>(a, cus, st);
         if (rows > kWideRows) return launch<DP, 2, F8, 2, 2>(a, cus, st);
     }
     return launch<DP, 2, F8, ST, 1>(a, cus, st);
@@ -971,8 +988,8 @@ hipError_t launch_rows(const TreeArgs& a, uint32_t cus, hipStream_t st) {
 
 // Floats of a context's partial results: two results for every workgroup (heads of 256: one
 // workgroup a CU, half as many).
-uint64_t tree_part_floats() { return 2ull * kTreeSlots * Part<128, 2>::kFloats; }
-static_assert(Part<256, 2>::kFloats <= 2u * Part<128, 2>::kFloats && Part<128, 4>::kFloats <= 2u * Part<128, 2>::kFloats, "the partial results' room");
+uint64_t tree_part_floats() { return 4ull * kTreeSlots * Part<128, 2>::kFloats; }
+static_assert(Part<256, 2>::kFloats <= 2u * Part<128, 2>::kFloats && Part<128, 8>::kFloats <= 4u * Part<128, 2>::kFloats, "the partial results' room");
 
 hipError_t launch_tree_attn(const TreeArgs& args, uint32_t cus, hipStream_t st) {
     TreeArgs a = args;

@@ -377,3 +377,34 @@ def test_binding_refusals(s):
         s.tree_attn_dev(q, k, v, None, c.out, **kw)
     s.tree_attn_dev(q, k, v, c.cache, {"o": c.out["o"]}, **(kw | {"scale": None}))
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("dim", [64, 112, 128])
+@pytest.mark.parametrize("lengths,rows,heads,kv,page,mask,layout", [
+    ([5000, 0, 63, 64, 65], 13, 10, 2, 16, "tree", "head"),       # 65 rows a head
+    ([700, 129], 24, 3, 1, 32, "any", "token"),                   # 72
+    ([33, 2000], 128, 2, 2, 64, "tree", "head"),                  # 128, new tokens of a whole step
+    ([1, 95, 4000], 129, 1, 1, 16, "chain", "head"),              # 129, of more than a step
+    ([300, 3001], 97, 4, 2, 16, "tree", "token"),                 # 194
+    ([8000], 64, 8, 2, 128, "tree", "head"),                      # 256, one sequence over all workgroups
+    ([40, 0], 256, 3, 1, 16, "any", "head"),                      # 768
+    ([1500] * 66, 33, 4, 2, 16, "chain", "head"),                 # 66, several sequences a lane
+])
+def test_shared_tiles(s, lengths, rows, heads, kv, page, mask, layout, dim):
+    """Rows a head on both sides of what makes two or four waves share a tile."""
+    Case(lengths, rows, heads, kv, dim, page, False, layout, mask, seed=dim + rows).run(s).check()
+    assert s.status() == 0
+
+
+@pytest.mark.parametrize("rows,heads,kv", [(70, 2, 2), (70, 2, 1), (100, 2, 1)])
+def test_masked_nan_in_shared_tiles(s, rows, heads, kv):
+    """NaN and infinities in new tokens that some rows see and others do not, in every tile; a missing page."""
+    c = Case([90, 0, 333], rows, heads, kv, 128, 16, seed=rows)
+    for i in range(3):
+        for j, what in ((2, NAN), (4, INF), (33, -INF), (40, NAN), (64, INF), (69, -INF)):
+            c.v_new[i * rows + j, :, j % 5::3] = what
+        c.see[i][:, rows - 1] = False
+        c.k_new[i * rows + rows - 1] = NAN
+        c.v_new[i * rows + rows - 1] = NAN
+    c.mask = torch.cat([words(x) for x in c.see])
+    c.run(s).check()
