@@ -61,7 +61,6 @@ constexpr float kLn2 = 0.69314718055994531f, kLog2e = 1.4426950408889634f;
 constexpr float kUnset = -3.0e38f;   // the running maximum of a row that has seen nothing
 constexpr float kSlack = 8.0f;       // log2 of the weights' bound
 constexpr uint32_t kTileKeys = 32, kStepKeys = 128;
-constexpr int kTreeWaves = 4;
 
 template <int N>
 __device__ __forceinline__ void wait_vm() {
@@ -191,10 +190,11 @@ __device__ __forceinline__ Seq seq_of(const TreeArgs& a, uint32_t i, bool& bad) 
 __device__ __forceinline__ uint32_t uniform(uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); }
 // The line is cut into a.pieces equal pieces, of `share` steps each. A piece that begins with one
 // pair's end and goes on with another's start pays twice for what a pair costs by itself
-// (about three steps), so where pieces are short, pairs are cut by themselves instead, into
-// units of `share` or one more steps, a piece each, if there are pieces enough (7 trees of
-// 13 nodes over up to 1777 tokens, 5 kv heads: 24.3 -> 19.5 us).
-constexpr uint32_t kShortShare = 4;
+// (about three steps), so pairs are cut by themselves instead, into units of up to kMoreShare
+// steps more than `share`, a piece each, if there are pieces enough (16 trees of 16 nodes over
+// 300 to 6000 tokens, 8 kv heads: 64.7 -> 59.5 us; 16 of 48 over 600: 40.3 -> 31.1; 32 single
+// tokens over 4096: 106 -> 99; 7 trees of 13 over up to 1777, 5 heads: 24.3 -> 19.5).
+constexpr uint32_t kMoreShare = 3;
 __device__ __forceinline__ Line line_of(const TreeArgs& a) {
     Line l{(a.c.n + kWave - 1u) / kWave, 0u, 0u, 1u, 0u, Seq{0u, 0u, 0}, false};
     uint32_t sum = 0;
@@ -210,8 +210,8 @@ __device__ __forceinline__ Line line_of(const TreeArgs& a) {
     l.total = (uint32_t)__builtin_amdgcn_readlane((int)incl, kWave - 1);
     const uint32_t H = a.c.kv_heads;
     l.share = max((l.total * H + a.pieces - 1u) / a.pieces, 1u);
-    if (l.per == 1u && l.share > 1u && l.share <= kShortShare) {   // (uniform; lanes without a sequence have 0 steps)
-        for (uint32_t unit = l.share; unit <= l.share + 1u; ++unit) {
+    if (l.per == 1u && l.share > 1u) {   // (uniform; lanes without a sequence have 0 steps)
+        for (uint32_t unit = l.share; unit <= l.share + kMoreShare; ++unit) {
             const uint32_t mine = (l.one.steps + unit - 1u) / unit;
             incl = wave_scan_incl_u(mine);
             const uint32_t total = (uint32_t)__builtin_amdgcn_readlane((int)incl, kWave - 1);
@@ -239,14 +239,10 @@ struct Part {
 
 }  // namespace
 
-// Tiles that a workgroup has before it at once, each shared by WR waves.
-template <int WR>
-constexpr int kTilesOf = WR == 4 ? 2 : kTreeWaves;
-
-template <int DP, int MT, bool F8, int ST, int WR>
-__global__ __launch_bounds__(kTilesOf<WR> * WR * kWave, WR == 1 ? kTreePerCu<DP> : 1) void tree_attn(TreeArgs a) {
+// A workgroup has NW tiles before it at once, each shared by WR waves of 16 MT rows.
+template <int DP, int MT, bool F8, int ST, int WR, int NW>
+__global__ __launch_bounds__(NW * WR * kWave, NW * WR == 4 ? kTreePerCu<DP> : 1) void tree_attn(TreeArgs a) {
     static_assert(WR == 1 || ((WR == 2 || WR == 4) && ST == 2 && !F8), "the schedule of shared tiles");
-    constexpr int NW = kTilesOf<WR>;
     constexpr uint32_t kStride = NW * kTileKeys, kPer = kStepKeys / kStride;   // keys from tile to tile of a wave, its tiles a step
     constexpr uint32_t kMine = 16u * MT, kRows = kMine * WR, kDT = DP / 16, kKS = DP / 32;   // rows of a wave, of the workgroup
     constexpr uint32_t kRowB = DP * (F8 ? 1 : 2), kNewB = DP * 2;                 // bytes of a cached row and of a new one in LDS
@@ -936,11 +932,10 @@ __global__ __launch_bounds__(256) void tree_join(TreeArgs a) {
 namespace {
 
 constexpr uint32_t kTreeTiles = 32;   // row tiles of a launch
-constexpr uint32_t kWideRows = 128;   // rows a head above which two waves share a tile
 
-template <int DP, int MT, bool F8, int ST, int WR>
+template <int DP, int MT, bool F8, int ST, int WR, int NW>
 hipError_t launch(TreeArgs a, uint32_t cus, hipStream_t st) {
-    constexpr uint32_t per_cu = WR == 1 ? kTreePerCu<DP> : 1, per = 16u * MT * WR;
+    constexpr uint32_t per_cu = NW * WR == 4 ? kTreePerCu<DP> : 1, per = 16u * MT * WR;
     const uint32_t rows = a.rows_per_seq * a.group, tiles = (rows + per - 1u) / per;
     for (uint32_t t0 = 0; t0 < tiles; t0 += kTreeTiles) {
         a.row_tile0 = t0;
@@ -948,7 +943,7 @@ hipError_t launch(TreeArgs a, uint32_t cus, hipStream_t st) {
         const uint32_t most = per_cu * kTreeSlots / 2u, slots = cus * per_cu < most ? cus * per_cu : most;
         a.pieces = slots / a.row_tiles / 8u * 8u;
         if (a.pieces == 0u) a.pieces = 8u;
-        hipLaunchKernelGGL((tree_attn<DP, MT, F8, ST, WR>), dim3(a.pieces * a.row_tiles), dim3(kTilesOf<WR> * WR * kWave), 0, st, a);
+        hipLaunchKernelGGL((tree_attn<DP, MT, F8, ST, WR, NW>), dim3(a.pieces * a.row_tiles), dim3(NW * WR * kWave), 0, st, a);
         hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
         const uint32_t pairs = a.c.n * a.c.kv_heads, blocks = a.row_tiles * (per * DP / 1024u);
@@ -963,25 +958,28 @@ hipError_t launch(TreeArgs a, uint32_t cus, hipStream_t st) {
 // Rows of a wave: 16, or 32 where there are more (64 leave one wave a SIMD, whose products
 // wait for its softmax: 256 rows a head, 32 sequences x 4096 tokens x 8 heads 294 us, of 32
 // 276). Over bf16, waves share tiles where there are enough rows: what the L2 and LDS's
-// write side bring is by a workgroup then and not by a wave. Four waves share a tile, 128 rows a
-// workgroup, where the last 128 are more than half full, else two waves, 64 rows (the same
-// sequences, us of one wave / two / four a tile: 72 rows 154 / - / 120, 128 rows 164 / - / 117,
-// 192 rows - / 206 / 200, 256 rows 273 / 250 / 226; 512 rows, 8 x 8192 tokens 252 / 234 / 217;
-// 320 rows, 16 x 4096 - / 167 / 182). Up to 64 rows its barriers cost more than that saves
-// (40 rows 105 / - / 139, 64 rows 110 / - / 131; over up to 6000 tokens 69 / 73 / -), as with
-// heads of 64 up to 128 rows (16 x 6000 tokens 58 / - / 63), and for 8 bits, whose tiles are half
-// as large (256 rows 261 / 276 / -). One short context is 1 us slower by four (72 rows over 1000
-// tokens 14.3 / - / 15.5 to 16.7): the lengths are known on the device only.
+// write side bring is by a workgroup then and not by a wave.
+// - Four a tile, 128 rows a workgroup, where the last 128 are more than half full (the same
+//   sequences, us of one wave / four a tile: 72 rows 154 / 120, 128 rows 164 / 117, 256 rows
+//   250 (of two) / 226; 512 rows, 8 x 8192 tokens 234 (of two) / 217). One short context is slower
+//   (72 rows over 1000 tokens 14.3 / 16), and heads of 64 up to 128 rows (16 x 6000 tokens
+//   58 / 63).
+// - Else two, 64 rows: above 128 rows (136 rows 214 of four / 192, 320 rows over 16 x 4096 tokens
+//   182 of four / 160), and up to there where the pairs are a quarter of the workgroups or more,
+//   whose lengths then matter little (us of one / two a tile, 40 or 64 rows, 8 kv heads: 64
+//   sequences over up to 1300 tokens 73 / 56, 32 over up to 4096 81 / 69, all of 4096 105 / 112;
+//   16 over up to 6000 67 / 60; fewer: 8 over up to 8000 40 / 43, 1 over 100000 87 / 90).
+// - Not for 8 bits, whose tiles are half as large (256 rows 261 / 276 of two).
 template <int DP, bool F8>
 hipError_t launch_rows(const TreeArgs& a, uint32_t cus, hipStream_t st) {
     constexpr int ST = F8 || DP == 64 ? 2 : 1;
-    const uint32_t rows = a.rows_per_seq * a.group;
-    if (rows <= 16u) return launch<DP, 1, F8, ST, 1>(a, cus, st);
+    const uint32_t rows = a.rows_per_seq * a.group, pairs = a.c.n * a.c.kv_heads;
+    if (rows <= 16u) return launch<DP, 1, F8, ST, 1, 4>(a, cus, st);
     if constexpr (DP != 256 && !F8) {
-        if (rows > (DP == 64 ? kWideRows : 64u) && (rows - 1u) % 128u >= 64u) return launch<DP, 2, F8, 2, 4>(a, cus, st);
-        if (rows > kWideRows) return launch<DP, 2, F8, 2, 2>(a, cus, st);
+        if (rows > (DP == 64 ? 128u : 64u) && (rows - 1u) % 128u >= 64u) return launch<DP, 2, F8, 2, 4, 2>(a, cus, st);
+        if (rows > 128u || (rows > 32u && pairs * 2u >= cus)) return launch<DP, 2, F8, 2, 2, 2>(a, cus, st);
     }
-    return launch<DP, 2, F8, ST, 1>(a, cus, st);
+    return launch<DP, 2, F8, ST, 1, 4>(a, cus, st);
 }
 
 }  // namespace

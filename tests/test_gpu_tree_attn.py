@@ -408,3 +408,11 @@ def test_masked_nan_in_shared_tiles(s, rows, heads, kv):
         c.v_new[i * rows + rows - 1] = NAN
     c.mask = torch.cat([words(x) for x in c.see])
     c.run(s).check()
+
+
+@pytest.mark.parametrize("dim", [48, 64, 128])
+@pytest.mark.parametrize("rows,heads,page,mask", [(10, 32, 16, "tree"), (64, 8, 64, "any"), (33, 8, 32, "chain")])
+def test_many_pairs_of_uneven_lengths(s, rows, heads, page, mask, dim):
+    lengths = [(37 * i * i) % 1500 if i % 5 else i for i in range(17)]
+    Case(lengths, rows, heads, 8, dim, page, mask=mask, seed=dim + rows).run(s).check()
+    assert s.status() == 0
