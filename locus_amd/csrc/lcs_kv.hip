@@ -290,7 +290,7 @@ __global__ __launch_bounds__(kKvThreads) void kv_copy(KvArgs a) {
 // ---- lcs_kv_compact ----
 // Whether a request can be served, a workgroup each. Its time is the chain of place, table and
 // count that a thread walks every kCheckThreads rows (16 contexts cut to 4096 rows:
-// 357 us for the whole call by 256 threads, 347 by 1024; 610 rows 11.0 by either).
+// 10 us more for the call by 256 threads than by 1024; 610 rows alike).
 constexpr int kCheckThreads = 1024;
 __global__ __launch_bounds__(kCheckThreads) void kv_compact_check(KvArgs a) {
     const uint32_t i = wg_x();
@@ -330,10 +330,15 @@ __global__ __launch_bounds__(kCheckThreads) void kv_compact_check(KvArgs a) {
 // a round writes below the next round's places, which lie at or below its sources, so
 // that only a round's own rows have to be read by all lanes before the first is
 // written. The next round's rows are under way meanwhile, the places of the one after it too
-// (16 contexts of 4000 to 8192 tokens, half kept, 4 layers: 547 us without, 367 so in rounds of
-// 4 rows and plain stores, 356 of 8 and stores past the caches).
-__global__ __launch_bounds__(kKvThreads) void kv_compact(KvArgs a) {
-    constexpr uint32_t U = 8;
+// (16 contexts of 4000 to 8192 tokens, half kept, 4 layers: 547 us without, 367 so, 356 with
+// stores past the caches). The rounds of a workgroup follow each other, so a long list is
+// walked by 1024 threads; a short one by 256, which start sooner (us of 256 / 1024: the same
+// 350 / 332; 10 contexts of 13000 tokens, one layer, 276 / 192; one of 3000, 6 layers, 64 / 31; 3 of up
+// to 777, 5 layers, 13.2 / 9.3; 5 of 200, a third kept, 13 layers, 9.7 / 20; 10 of 30, 3 layers, 9.9 / 17).
+// 8 rows of a lane are no faster by 256 threads (346; 230 of 10 contexts) and spill by 1024 (550).
+template <int NT>
+__global__ __launch_bounds__(NT) void kv_compact(KvArgs a) {
+    constexpr uint32_t U = 4;
     uint32_t b = wg_x();
     const uint32_t part = b % a.parts;
     b /= a.parts;
@@ -347,7 +352,7 @@ __global__ __launch_bounds__(kKvThreads) void kv_compact(KvArgs a) {
     const uint32_t n = min((uint32_t)max(a.count[i], 0), a.max_keep);
     const int32_t* keep = a.index + (uint64_t)i * a.max_keep;
     const int32_t* row = a.table + (uint64_t)slot * a.max_pages;
-    const uint32_t chunk = part * a.cp + (tid_x() & (a.cp - 1u)), r0 = tid_x() / a.cp, step = kKvThreads / a.cp;
+    const uint32_t chunk = part * a.cp + (tid_x() & (a.cp - 1u)), r0 = tid_x() / a.cp, step = NT / a.cp;
     const uint32_t es = a.f8 ? 1u : 2u, in = a.page_tokens - 1u;
     unsigned char* base = static_cast<unsigned char*>(kv ? a.v : a.k) + (layer * a.layer_stride + head * a.head_stride) * es + 16u * chunk;
     float* sc = kv ? a.v_scale : a.k_scale;
@@ -573,14 +578,16 @@ hipError_t launch_kv_compact(const KvArgs& args, hipStream_t st) {
     hipLaunchKernelGGL(kv_compact_check, dim3(a.n), dim3(kCheckThreads), 0, st, a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    // (few rows' heads: their chunks apart, so that the CUs have more in flight)
-    const uint32_t heads = a.n * a.layers * 2u * a.kv_heads;
+    // (few rows' heads: their chunks apart, in pieces of 128 bytes at least, so that the CUs have more in flight)
+    const bool wide = a.max_keep > kKvThreads;
+    const uint32_t heads = a.n * a.layers * 2u * a.kv_heads, enough = wide ? 512u : 2048u;
     a.parts = 1;
-    while (heads * a.parts < 2048u && a.cp > 4u) {
+    while (heads * a.parts < enough && a.cp > 8u) {
         a.parts *= 2u;
         a.cp /= 2u;
     }
-    hipLaunchKernelGGL(kv_compact, dim3(heads * a.parts), dim3(kKvThreads), 0, st, a);
+    if (wide) hipLaunchKernelGGL(kv_compact<1024>, dim3(heads * a.parts), dim3(1024), 0, st, a);
+    else hipLaunchKernelGGL(kv_compact<kKvThreads>, dim3(heads * a.parts), dim3(kKvThreads), 0, st, a);
     return hipGetLastError();
 }
 

@@ -398,3 +398,16 @@ def test_side_stream_and_graph(s):
             st["start"] += 9
             st["end"] += 9
     assert s.status() == 0
+
+
+@pytest.mark.parametrize("f8", [False, True])
+@pytest.mark.parametrize("layers,heads,dim,page,length,most", [(1, 1, 256, 32, 6000, 5000), (2, 3, 80, 16, 1100, 1024), (1, 2, 128, 64, 900, 257), (1, 2, 128, 16, 900, 256)])
+def test_compact_long(s, layers, heads, dim, page, length, most, f8):
+    """Lists of several rounds of a workgroup's rows, on both sides of what makes it wide, dense and thin."""
+    pages = -(-length // page)
+    c = Pair(s, layers=layers, pages=2 * pages + 2, heads=heads, page=page, dim=dim, seqs=3, max_pages=pages, f8=f8)
+    c.grow([0, 1], [0, 0], [length, length])
+    rng = random.Random(most)
+    keep = [sorted(rng.sample(range(length), most)), sorted(rng.sample(range(length // 2 + most // 2), most))]
+    c.compact([0, 1], [most, most - 3], keep)
+    c.compact([0, 1], [most // 2, most], [sorted(rng.sample(range(most), most // 2)) + [0] * (most - most // 2), list(range(most))])
