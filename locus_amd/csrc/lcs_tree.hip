@@ -9,7 +9,8 @@
 // - A wave takes 32 keys at a time, their keys and values brought to its own part of
 //   LDS by 16-byte DMA loads, so that no register holds data in flight and waves need
 //   no barrier; four waves take 128 consecutive tokens, a step.
-//   Above 64 rows a head two or four waves share a tile, of which each brings its part, with barriers.
+//   Where rows and pairs are many, two or four waves share a tile, of which each brings its
+//   part, with barriers.
 // - Scores are computed transposed, S^T = K Q^T, with Q in registers as the B
 //   operand: a lane then holds eight keys of one row, so that its softmax is the
 //   lane's own, and the weights are already laid out as the B operand of O^T = V^T P^T.
@@ -19,9 +20,10 @@
 //   that most tiles rescale nothing; weights are then up to 2^8, which f32 sums and
 //   bf16 weights hold as well as 1.
 // - The steps of all (sequence, kv head) pairs form one line that is cut into as many
-//   equal pieces as there are workgroups on the card, whatever the lengths: each
-//   workgroup finds its piece from the lengths on the device. A pair that several
-//   workgroups share is joined by a second launch from their partial sums.
+//   equal pieces as there are workgroups on the card, whatever the lengths (and so that
+//   pieces end with a pair, where that costs little): each workgroup finds its piece from
+//   the lengths on the device. A pair that several workgroups share is joined by a
+//   second launch from their partial sums.
 //
 // A weight is rounded to bf16 for the product with the values (2^-8 of itself at most,
 // as the values themselves are); scores, maxima, sums and the normaliser are f32.
@@ -984,8 +986,8 @@ hipError_t launch_rows(const TreeArgs& a, uint32_t cus, hipStream_t st) {
 
 }  // namespace
 
-// Floats of a context's partial results: two results for every workgroup (heads of 256: one
-// workgroup a CU, half as many).
+// Floats of a context's partial results: two of 64 rows for each of two workgroups a CU (of 128 rows
+// or heads of 256: one workgroup a CU).
 uint64_t tree_part_floats() { return 4ull * kTreeSlots * Part<128, 2>::kFloats; }
 static_assert(Part<256, 2>::kFloats <= 2u * Part<128, 2>::kFloats && Part<128, 8>::kFloats <= 4u * Part<128, 2>::kFloats, "the partial results' room");
 
