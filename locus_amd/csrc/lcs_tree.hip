@@ -971,6 +971,9 @@ hipError_t launch(TreeArgs a, uint32_t cus, hipStream_t st) {
 //   whose lengths then matter little (us of one / two a tile, 40 or 64 rows, 8 kv heads: 64
 //   sequences over up to 1300 tokens 73 / 56, 32 over up to 4096 81 / 69, all of 4096 105 / 112;
 //   16 over up to 6000 67 / 60; fewer: 8 over up to 8000 40 / 43, 1 over 100000 87 / 90).
+// - Heads of 256: four a tile of 16 rows each, 64 rows a workgroup, above 32 rows, so that two waves
+//   fit a SIMD (us of one, of 32 rows / four, 8 kv heads: 44 rows, 12 sequences over 800 to 3187
+//   tokens 72 / 47, 256 rows, 2 over up to 4000 49 / 37, 128 rows, 8 over up to 2000 50 / 48; 24 rows 57 / 59).
 // - Not for 8 bits, whose tiles are half as large (256 rows 261 / 276 of two).
 template <int DP, bool F8>
 hipError_t launch_rows(const TreeArgs& a, uint32_t cus, hipStream_t st) {
@@ -981,6 +984,9 @@ hipError_t launch_rows(const TreeArgs& a, uint32_t cus, hipStream_t st) {
         if (rows > (DP == 64 ? 128u : 64u) && (rows - 1u) % 128u >= 64u) return launch<DP, 2, F8, 2, 4, 2>(a, cus, st);
         if (rows > 128u || (rows > 32u && pairs * 2u >= cus)) return launch<DP, 2, F8, 2, 2, 2>(a, cus, st);
     }
+    if constexpr (DP == 256 && !F8) {
+        if (rows > 32u) return launch<DP, 1, F8, 2, 4, 2>(a, cus, st);
+    }
     return launch<DP, 2, F8, ST, 1, 4>(a, cus, st);
 }
 
@@ -989,7 +995,7 @@ hipError_t launch_rows(const TreeArgs& a, uint32_t cus, hipStream_t st) {
 // Floats of a context's partial results: two of 64 rows for each of two workgroups a CU (of 128 rows
 // or heads of 256: one workgroup a CU).
 uint64_t tree_part_floats() { return 4ull * kTreeSlots * Part<128, 2>::kFloats; }
-static_assert(Part<256, 2>::kFloats <= 2u * Part<128, 2>::kFloats && Part<128, 8>::kFloats <= 4u * Part<128, 2>::kFloats, "the partial results' room");
+static_assert(Part<256, 4>::kFloats <= 4u * Part<128, 2>::kFloats && Part<256, 2>::kFloats <= 2u * Part<128, 2>::kFloats && Part<128, 8>::kFloats <= 4u * Part<128, 2>::kFloats, "the partial results' room");
 
 hipError_t launch_tree_attn(const TreeArgs& args, uint32_t cus, hipStream_t st) {
     TreeArgs a = args;

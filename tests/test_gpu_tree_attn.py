@@ -416,3 +416,29 @@ def test_many_pairs_of_uneven_lengths(s, rows, heads, page, mask, dim):
     lengths = [(37 * i * i) % 1500 if i % 5 else i for i in range(17)]
     Case(lengths, rows, heads, 8, dim, page, mask=mask, seed=dim + rows).run(s).check()
     assert s.status() == 0
+
+
+@pytest.mark.parametrize("f8", [False, True])
+@pytest.mark.parametrize("lengths,rows,heads,kv,page,mask,layout", [
+    ([3000, 0, 64, 65, 1], 11, 6, 2, 16, "tree", "token"),        # 33 rows a head
+    ([500, 33], 129, 2, 2, 64, "tree", "head"),                   # new tokens of more than a step
+    ([2000, 700], 65, 4, 1, 32, "any", "head"),                   # 260
+    ([31] * 40, 41, 5, 5, 16, "tree", "head"),
+])
+@pytest.mark.parametrize("dim", [144, 256])
+def test_wide_heads(s, lengths, rows, heads, kv, page, mask, layout, dim, f8):
+    Case(lengths, rows, heads, kv, dim, page, f8, layout, mask, seed=dim + rows).run(s).check()
+    assert s.status() == 0
+
+
+def test_masked_nan_in_wide_heads(s):
+    rows = 70
+    c = Case([90, 0, 333], rows, 2, 1, 256, 16, seed=2)
+    for i in range(3):
+        for j, what in ((2, NAN), (4, INF), (33, -INF), (40, NAN), (64, INF)):
+            c.v_new[i * rows + j, :, j % 5::3] = what
+        c.see[i][:, rows - 1] = False
+        c.k_new[i * rows + rows - 1] = NAN
+        c.v_new[i * rows + rows - 1] = NAN
+    c.mask = torch.cat([words(x) for x in c.see])
+    c.run(s).check()
