@@ -342,11 +342,8 @@ __global__ __launch_bounds__(NT) void kv_compact(KvArgs a) {
     uint32_t b = wg_x();
     const uint32_t part = b % a.parts;
     b /= a.parts;
-    const uint32_t head = b % a.kv_heads;
-    b /= a.kv_heads;
-    const uint32_t kv = b & 1u;
-    b >>= 1;
-    const uint32_t layer = b % a.layers, i = b / a.layers;
+    const uint32_t head = b % a.kv_heads, kv = b / a.kv_heads;
+    const uint32_t layer = __builtin_amdgcn_workgroup_id_y(), i = __builtin_amdgcn_workgroup_id_z();
     const int32_t slot = a.seq[i];
     if (slot == -1 || a.result[i] != 0) return;
     const uint32_t n = min((uint32_t)max(a.count[i], 0), a.max_keep);
@@ -586,8 +583,11 @@ hipError_t launch_kv_compact(const KvArgs& args, hipStream_t st) {
         a.parts *= 2u;
         a.cp /= 2u;
     }
-    if (wide) hipLaunchKernelGGL(kv_compact<1024>, dim3(heads * a.parts), dim3(1024), 0, st, a);
-    else hipLaunchKernelGGL(kv_compact<kKvThreads>, dim3(heads * a.parts), dim3(kKvThreads), 0, st, a);
+    // (a dimension's threads are counted in 32 bits, and past them go missing without an error:
+    // layers and requests have dimensions of their own, and x has 2^21 at most)
+    const dim3 grid(2u * a.kv_heads * a.parts, a.layers, a.n);
+    if (wide) hipLaunchKernelGGL(kv_compact<1024>, grid, dim3(1024), 0, st, a);
+    else hipLaunchKernelGGL(kv_compact<kKvThreads>, grid, dim3(kKvThreads), 0, st, a);
     return hipGetLastError();
 }
 

@@ -1,0 +1,54 @@
+"""The paged cache's row moves past what one dimension of a launch counts: 2^32 threads. Most requests ask for nothing; the first, one in the middle and the
+last do."""
+import pytest
+import torch
+
+from kv_util import Model
+from locus_amd import sampler as S
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def s():
+    x = S.Sampler(device=0, max_rows=64, max_vocab=4096, max_hist=64, max_top=4)
+    x.kv_reserve(64)
+    yield x
+    x.close()
+
+
+def ints(x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+def pool(layers, heads, slots, tokens, seed):
+    """A cache of 16-token pages whose slots hold `tokens` tokens each, and its model."""
+    g = torch.Generator().manual_seed(seed)
+    per = -(-tokens // 16)
+    k, v = (torch.randn(layers, slots * per, heads, 16, 16, generator=g).bfloat16() for _ in range(2))
+    table = torch.arange(slots * per, dtype=torch.int32).view(slots, per)
+    refs = torch.ones(slots * per, dtype=torch.int32)
+    dev = [t.cuda() for t in (k, v, table, refs)]
+    return S.KvCache(*dev), dev, Model(k, v, table, refs)
+
+
+def same(dev, model):
+    for t, w in zip(dev[:2], model.rows):
+        assert torch.equal(t.cpu().view(torch.int16), w.view(torch.int16))
+
+
+@pytest.mark.parametrize("layers,heads,most,threads", [(17, 128, 257, 1024), (65, 128, 12, 256)])
+def test_compact(s, layers, heads, most, threads):
+    n = 1024
+    assert n * layers * 2 * heads * threads > 1 << 32
+    cache, dev, model = pool(layers, heads, 3, 20, layers)
+    seq, count = [-1] * n, [0] * n
+    keep = torch.zeros(n, most, dtype=torch.int32)
+    for i, slot in ((0, 1), (500, 2), (n - 1, 0)):
+        seq[i], count[i] = slot, 11
+        keep[i, :11] = torch.tensor([0, 2, 3, 5, 8, 9, 13, 15, 16, 17, 19])
+    result = ints([9] * n)
+    s.kv_compact_dev(cache, ints(seq), ints(count), keep.cuda(), result)
+    torch.cuda.synchronize()
+    assert result.tolist() == model.compact(seq, count, keep.tolist()) == [0] * n and s.status() == 0
+    same(dev, model)
