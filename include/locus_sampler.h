@@ -379,8 +379,8 @@ typedef struct lcs_tree_verify_out {
  * (1 for a row of zeros, or whose largest |x| is a NaN; 2^-126 at least), x / scale
  * rounded to nearest even. */
 typedef struct lcs_kv_append_batch {
-    uint32_t n_seq;
-    uint32_t rows_per_seq;
+    uint32_t n_seq;            /* up to 1024 */
+    uint32_t rows_per_seq;     /* 1..2^20, and n_seq * n_layers * ceil(rows_per_seq / 4) below 2^32 */
     uint32_t layer, n_layers;  /* the first one, and how many */
     const void* k;             /* layer l (from 0), row r, head h: k + l * layer_stride + r * k_stride + h * head_dim; bf16 */
     const void* v;

@@ -339,7 +339,7 @@ struct KvAppendArgs {
     const void* k;
     const void* v;
     uint64_t new_layer_stride, k_stride, v_stride;
-    uint32_t rows_per_seq, n_layers, blocks;
+    uint32_t rows_per_seq, n_layers;
 };
 
 // attention over the cache and a step's new tokens (lcs_tree.hip)

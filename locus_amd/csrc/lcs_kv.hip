@@ -426,6 +426,7 @@ __global__ __launch_bounds__(NT) void kv_compact(KvArgs a) {
 // the verdict and the pages: 88.9 us; 16 tokens a workgroup, one layer's sequences side
 // by side 90.7. All 16 kept: 39 us by either, 5.2 TB/s.)
 constexpr uint32_t kAppendTokens = 4;
+constexpr uint32_t kAppendBlocks = 2048;   // workgroups of a sequence and layer along x: 2^31 threads with 4096 layers
 
 // x / scale to nearest: RN(1 / scale), a product, and its remainder's share (exact by an fma),
 // which makes the quotient the correctly rounded one. An infinite scale gives 0, and NaN
@@ -456,8 +457,8 @@ __global__ __launch_bounds__(kKvThreads) void kv_append(KvAppendArgs p) {
     constexpr uint32_t U = 4;
     __shared__ int32_t page_s[kAppendTokens], src_s[kAppendTokens];
     const KvArgs& a = p.a;
-    const uint32_t id = wg_x() + __builtin_amdgcn_workgroup_id_y() * p.a.n * p.blocks;   // (n_layers * n * blocks of them: below 2^32)
-    const uint32_t l = id % p.n_layers, wg = id / p.n_layers, i = wg / p.blocks, j0 = wg % p.blocks * kAppendTokens;
+    const uint32_t l = wg_x() % p.n_layers, i = __builtin_amdgcn_workgroup_id_z();
+    const uint32_t j0 = (wg_x() / p.n_layers + __builtin_amdgcn_workgroup_id_y() * kAppendBlocks) * kAppendTokens;
     const int32_t slot = a.seq ? a.seq[i] : (int32_t)i;
     const uint32_t n = a.count ? min((uint32_t)max(a.count[i], 0), p.rows_per_seq) : p.rows_per_seq;
     const int32_t pos0 = a.start[i];
@@ -594,8 +595,9 @@ hipError_t launch_kv_compact(const KvArgs& args, hipStream_t st) {
 hipError_t launch_kv_append(const KvAppendArgs& args, hipStream_t st) {
     KvAppendArgs p = args;
     p.a.cp = pow2_from(p.a.head_dim / 8u);
-    p.blocks = (p.rows_per_seq + kAppendTokens - 1u) / kAppendTokens;
-    const dim3 grid(p.a.n * p.blocks, p.n_layers);
+    // (sequences and what is left of a long one's tokens in dimensions of their own, as kv_compact's)
+    const uint32_t blocks = (p.rows_per_seq + kAppendTokens - 1u) / kAppendTokens;
+    const dim3 grid(p.n_layers * (blocks < kAppendBlocks ? blocks : kAppendBlocks), (blocks + kAppendBlocks - 1u) / kAppendBlocks, p.a.n);
     if (p.a.f8) hipLaunchKernelGGL(kv_append<true>, grid, dim3(kKvThreads), 0, st, p);
     else hipLaunchKernelGGL(kv_append<false>, grid, dim3(kKvThreads), 0, st, p);
     return hipGetLastError();

@@ -106,6 +106,8 @@ inline int check_kv_append(const lcs_kv_cache* c, const lcs_kv_append_batch* b, 
     if (b->k_stride % 8u || b->v_stride % 8u || (b->n_layers > 1 && b->layer_stride % 8u)) {
         return w.no("strides must be multiples of 16 bytes");
     }
+    // (a workgroup for four tokens of a sequence and layer)
+    if ((uint64_t)b->n_seq * ((b->rows_per_seq + 3u) / 4u) * b->n_layers > 0xffffffffull) return w.over("too many rows and layers for a call");
     return LCS_OK;
 }
 

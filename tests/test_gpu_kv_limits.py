@@ -1,5 +1,5 @@
-"""The paged cache's row moves past what one dimension of a launch counts: 2^32 threads. Most requests ask for nothing; the first, one in the middle and the
-last do."""
+"""The paged cache's row moves past what one dimension of a launch counts: 2^32 threads. Most requests
+ask for nothing; the first, one in the middle and the last do."""
 import pytest
 import torch
 
@@ -51,4 +51,29 @@ def test_compact(s, layers, heads, most, threads):
     s.kv_compact_dev(cache, ints(seq), ints(count), keep.cuda(), result)
     torch.cuda.synchronize()
     assert result.tolist() == model.compact(seq, count, keep.tolist()) == [0] * n and s.status() == 0
+    same(dev, model)
+
+
+@pytest.mark.parametrize("layers", [1, 3])
+def test_append(s, layers):
+    n, rows = 1024, 65540
+    assert n * (-(-rows // 4)) * 256 > 1 << 32
+    cache, dev, model = pool(4, 1, 3, 32, 7)
+    g = torch.Generator().manual_seed(8)
+    new = [torch.empty(n * rows, 1, 16, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    seq, pos, count = [-1] * n, [0] * n, [0] * n
+    index = torch.zeros(n, rows, dtype=torch.int32, device="cuda")
+    for i, slot, at, num in ((0, 2, 3, 9), (511, 0, 31, 1), (n - 1, 1, 13, 19)):
+        seq[i], pos[i], count[i] = slot, at, num
+        index[i, :num] = ints(range(rows - num, rows))
+        for t, x in zip(new, model.rows):
+            r = torch.randn(num, 1, 16, generator=g).bfloat16()
+            t[i * rows + rows - num: (i + 1) * rows] = r.cuda()
+            for j in range(num):
+                x[1: 1 + layers, int(model.table[slot, (at + j) // 16]), :, (at + j) % 16] = r[j]
+    # (a layer's rows are another's too: a stride of 0)
+    k, v = (t.expand(layers, *t.shape) for t in new)
+    s.kv_append_dev(cache, k, v, ints(seq), ints(pos), ints(count), rows_per_seq=rows, index=index, layer=1)
+    torch.cuda.synchronize()
+    assert s.status() == 0
     same(dev, model)

@@ -195,3 +195,11 @@ def test_cache_tensors():
                 lambda: S.KvCache(k8, k8, table, refs, k_scale=sc, v_scale=sc[:1])]:
         with pytest.raises(S.SamplerError):
             bad()
+
+
+def test_append_workgroups(lib):
+    """A workgroup for four tokens of a sequence and layer: 2^32 of them are too many."""
+    c = cache(layers=4096, pages=1, kv_heads=1, head_stride=0, page_stride=0, layer_stride=16 * 64)
+    for n, rows, layers, rc in [(1024, 1 << 20, 15, 0), (1024, 1 << 20, 16, -4), (1024, 4097, 4096, -4), (1023, 4096, 4096, 0), (1024, 4092, 4096, 0),
+                                (1024, 1 << 20, 4096, -4), (1, 1 << 20, 4096, 0)]:
+        assert call(lib.append, c, append(n_seq=n, rows_per_seq=rows, n_layers=layers))[0] == rc, (n, rows, layers)
