@@ -451,7 +451,7 @@ hipError_t launch_verify(const VerifyArgs& a, hipStream_t st) {
     return hipGetLastError();
 }
 
-hipError_t launch_tree_verify(const TreeVerifyArgs& a, hipStream_t st) {
+static hipError_t launch_tree_seqs(const TreeVerifyArgs& a, hipStream_t st) {
     if (a.logits) {
         if (a.dtype == LCS_BF16) launch_rows<8>(a, st);
         else launch_rows<4>(a, st);
@@ -462,6 +462,30 @@ hipError_t launch_tree_verify(const TreeVerifyArgs& a, hipStream_t st) {
     if (a.rows_per_seq <= (uint32_t)kWave) hipLaunchKernelGGL(tree_walk<1>, grid, block, 0, st, a);
     else hipLaunchKernelGGL(tree_walk<kTreeMax / kWave>, grid, block, 0, st, a);
     return hipGetLastError();
+}
+
+// (a launch's threads are counted in 32 bits, and past them go missing without an error:
+// 2^22 rows at a time, of 512 threads at most)
+hipError_t launch_tree_verify(const TreeVerifyArgs& all, hipStream_t st) {
+    TreeVerifyArgs a = all;
+    const uint32_t R = a.rows_per_seq, most = (1u << 22) / R;
+    for (uint32_t s0 = 0; s0 < all.n_seq; s0 += most) {
+        const uint64_t r0 = (uint64_t)s0 * R;
+        a.n_seq = all.n_seq - s0 < most ? all.n_seq - s0 : most;
+        if (all.logits) a.logits = static_cast<const char*>(all.logits) + r0 * all.row_stride * (all.dtype == LCS_BF16 ? 2u : 4u);
+        a.tokens = all.tokens + r0;
+        a.parent = all.parent + r0;
+        if (all.length) a.length = all.length + s0;
+        a.argmax_ids = all.argmax_ids + r0;
+        if (all.node_lp) a.node_lp = all.node_lp + r0;
+        a.path = all.path + r0;
+        a.n_path = all.n_path + s0;
+        a.next_id = all.next_id + s0;
+        if (all.new_length) a.new_length = all.new_length + s0;
+        const hipError_t e = launch_tree_seqs(a, st);
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 
 }  // namespace lcs

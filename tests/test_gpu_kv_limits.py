@@ -1,5 +1,6 @@
-"""The paged cache's row moves past what one dimension of a launch counts: 2^32 threads. Most requests
-ask for nothing; the first, one in the middle and the last do."""
+"""The paged cache's row moves and the tree's verdict past what one dimension of a launch
+counts: 2^32 threads. Most of the moves' requests ask for nothing; the first, one in the
+middle and the last do."""
 import pytest
 import torch
 
@@ -77,3 +78,49 @@ def test_append(s, layers):
     torch.cuda.synchronize()
     assert s.status() == 0
     same(dev, model)
+
+
+@pytest.mark.parametrize("n,rows", [((1 << 24) + 5, 1), (5600003, 3)])
+def test_verdict(s, n, rows):
+    """A workgroup of 256 threads a row: every row's argmax, every sequence's path."""
+    assert n * rows * 256 > 1 << 32
+    vocab = 8
+    g = torch.Generator(device="cuda").manual_seed(n)
+    logits = torch.randn(n * rows, vocab, generator=g, device="cuda").bfloat16()
+    logits[:, 5] = -9.0
+    best = torch.randint(0, 2, (n, rows), generator=g, device="cuda", dtype=torch.int32) * 5
+    logits[torch.arange(n * rows, device="cuda"), best.view(-1).long()] = 30.0
+    tokens = torch.randint(0, 2, (n, rows), generator=g, device="cuda", dtype=torch.int32) * 5
+    parent = (torch.arange(rows, device="cuda", dtype=torch.int32) - 1).repeat(n, 1)
+    hit = (tokens[:, 1:] == best[:, :-1]).int().cumprod(1)       # (a chain: the leading nodes that are right)
+    taken = 1 + hit.sum(1, dtype=torch.int32)
+    empty = lambda *sh: torch.full(sh, -7, device="cuda", dtype=torch.int32)   # noqa: E731
+    out = {"argmax_ids": empty(n * rows), "path": empty(n, rows), "n_path": empty(n), "next_id": empty(n), "length": empty(n),
+           "node_lp": torch.full((n * rows,), 7.0, device="cuda")}
+    length = torch.arange(n, device="cuda", dtype=torch.int32)
+    s.tree_verify_dev(tokens.view(-1), parent.reshape(-1), out, rows_per_seq=rows, logits=logits, length=length)
+    torch.cuda.synchronize()
+    at = torch.arange(rows, device="cuda", dtype=torch.int32)
+    assert torch.equal(out["argmax_ids"].view(n, rows), best)
+    assert torch.equal(out["n_path"], taken)
+    assert torch.equal(out["path"], torch.where(at < taken[:, None], at, -1))
+    assert torch.equal(out["next_id"], best.gather(1, (taken - 1)[:, None].long())[:, 0])
+    assert torch.equal(out["length"], length + taken)
+    # (a log-probability is 0 or -20 and less: which one tells the row; the normaliser is held to 1e-5, as lcs_verify's)
+    lp = out["node_lp"].view(n, rows)
+    assert (lp[:, 0] == 0).all()
+    assert ((lp[:, 1:] > -1.0) == (tokens[:, 1:] == best[:, :-1])).all() and (lp <= 1e-5).all()
+
+
+def test_verdict_of_argmaxes(s):
+    """Without logits, a wave a sequence."""
+    n = (1 << 26) + 7
+    assert -(-n // 4) * 256 > 1 << 32
+    best = torch.arange(n, device="cuda", dtype=torch.int32)
+    zero = torch.zeros(n, device="cuda", dtype=torch.int32)
+    out = {"argmax_ids": best.clone(), "path": torch.full((n, 1), -7, device="cuda", dtype=torch.int32),
+           "n_path": torch.full((n,), -7, device="cuda", dtype=torch.int32), "next_id": torch.full((n,), -7, device="cuda", dtype=torch.int32)}
+    s.tree_verify_dev(zero, zero - 1, out, rows_per_seq=1)
+    torch.cuda.synchronize()
+    assert (out["path"] == 0).all() and (out["n_path"] == 1).all()
+    assert torch.equal(out["next_id"], best) and torch.equal(out["argmax_ids"], best)
