@@ -376,8 +376,8 @@ typedef struct lcs_tree_verify_out {
 /* New rows of a cache: token j < count[i] of sequence i goes to position pos[i] + j,
  * from row i * rows_per_seq + (index ? index[i * rows_per_seq + j] : j) of each of
  * n_layers layers. Into e4m3 as lcs_add_rmsnorm's y: a scale of max|x| / 448 per row
- * (1 for a row of zeros, or whose largest |x| is a NaN; 2^-126 at least), x / scale
- * rounded to nearest even. */
+ * (1 for a row of zeros, or one that holds a NaN; 2^-126 at least), x / scale cut to
+ * +-448 and rounded to nearest even, a NaN staying one. */
 typedef struct lcs_kv_append_batch {
     uint32_t n_seq;            /* up to 1024 */
     uint32_t rows_per_seq;     /* 1..2^20, and n_seq * n_layers * ceil(rows_per_seq / 4) below 2^32 */

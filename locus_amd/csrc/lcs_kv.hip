@@ -440,6 +440,12 @@ struct Quotient {
     }
 };
 
+// The low half, a bf16: a number or an infinity cut to +-448 (0x43e0), a NaN as it is.
+__device__ __forceinline__ uint32_t cut448(uint32_t w) {
+    const uint32_t m = w & 0x7fffu;
+    return (w & 0x8000u) | (m > 0x7f80u ? m : min(m, 0x43e0u));
+}
+
 // The largest of cp neighbouring lanes' values (cp a power of two up to 32): pairs, quads, and
 // their mirror images, in which the quads and eights are already alike.
 __device__ __forceinline__ uint32_t row_max(uint32_t v, uint32_t cp) {
@@ -513,6 +519,10 @@ __global__ __launch_bounds__(kKvThreads) void kv_append(KvAppendArgs p) {
 #pragma unroll
                     for (int k = 0; k < 4; ++k) top = max(top, max(x[u][k] & 0x7fffu, x[u][k] >> 16 & 0x7fffu));
                     top = row_max(top, a.cp);
+                    if (top > 0x7f80u) {   // (a NaN in the row, whose scale is 1: what is not one is cut to +-448)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) x[u][k] = cut448(x[u][k]) | cut448(x[u][k] >> 16) << 16;
+                    }
                     const float f = __uint_as_float(top << 16);
                     const float scale = f > 0.0f ? fmaxf(fdiv(f, kE4m3Max), kLeastScale) : 1.0f;   // (a NaN is not above 0)
                     const Quotient by(scale);   // (448 at most, and a rounding)

@@ -10,6 +10,7 @@ from locus_amd import sampler as S
 
 pytestmark = pytest.mark.gpu
 STATUS_PAGES = 8
+NAN, INF = float("nan"), float("inf")
 
 
 @pytest.fixture(scope="module")
@@ -411,3 +412,23 @@ def test_compact_long(s, layers, heads, dim, page, length, most, f8):
     keep = [sorted(rng.sample(range(length), most)), sorted(rng.sample(range(length // 2 + most // 2), most))]
     c.compact([0, 1], [most, most - 3], keep)
     c.compact([0, 1], [most // 2, most], [sorted(rng.sample(range(most), most // 2)) + [0] * (most - most // 2), list(range(most))])
+
+
+def test_append_finite_beside_a_nan(s):
+    """A row that holds a NaN is stored with a scale of 1: what else it holds stays itself up to 448, which bounds the rest."""
+    c = Pair(s, layers=1, heads=2, dim=32, f8=True, pages=8)
+    c.grow([0], [0], [16])
+    row = torch.linspace(-30.0, 30.0, 32)
+    row[:12] = torch.tensor([NAN, 447.0, 448.0, 449.0, 480.0, 500.0, 1e4, 3e38, -500.0, -3e38, INF, -INF])
+    k = torch.stack([row, torch.linspace(-900.0, 900.0, 32)]).bfloat16()[None, None].expand(1, 3, 2, 32).contiguous()
+    k[0, 1, 1, 5] = -NAN                                     # (in one row of the others too)
+    s.kv_append_dev(c.cache, k.cuda(), k.cuda(), c.ints([0]), c.ints([2]), rows_per_seq=3)
+    torch.cuda.synchronize()
+    want, scale = quantise(k[0])
+    assert torch.isfinite(want[0, 0].float()).sum() == 31    # (the oracle's own: the NaN alone is one)
+    page = int(c.table[0, 0])
+    for t, sc in ((c.k, "k_scale"), (c.v, "v_scale")):
+        got = t[0, page, :, 2:5].transpose(0, 1).float().cpu()
+        assert torch.equal(c.scales[sc][0, page, :, 2:5].t().cpu(), scale)
+        assert torch.equal(torch.isnan(got), torch.isnan(want.float()))
+        assert torch.equal(got.nan_to_num(), want.float().nan_to_num())
