@@ -442,3 +442,37 @@ def test_masked_nan_in_wide_heads(s):
         c.v_new[i * rows + rows - 1] = NAN
     c.mask = torch.cat([words(x) for x in c.see])
     c.run(s).check()
+
+
+@pytest.mark.parametrize("f8", [False, True])
+@pytest.mark.parametrize("rows,heads,kv,dim", [(3, 4, 2, 64), (9, 8, 2, 128), (70, 2, 1, 128), (40, 4, 2, 256)])
+def test_nan_and_inf_in_queries(s, rows, heads, kv, dim, f8):
+    """A row whose query holds a NaN, or an infinity that makes a score one, is NaN; the others are as they were."""
+    c = Case([200, 0, 45], rows, heads, kv, dim, 16, f8, seed=dim)
+    c.q[1, 0, 3] = NAN
+    c.q[rows, heads - 1, 0] = NAN
+    c.q[2 * rows + 1, 1, dim - 1] = INF
+    hit = torch.zeros(3 * rows, heads, dtype=torch.bool)
+    for r, h in ((1, 0), (rows, heads - 1), (2 * rows + 1, 1)):
+        hit[r, h] = True
+    c.run(s)
+    o, lse = c.out["o"].cpu(), c.out["lse"].cpu()
+    assert torch.isnan(o[hit]).all() and torch.isnan(lse[hit]).all()
+    # the rest: the formula's (beside those queries' results without the NaN and the infinity)
+    c.q[1, 0, 3] = c.q[rows, heads - 1, 0] = c.q[2 * rows + 1, 1, dim - 1] = 0.0
+    c.run(s)
+    c.out["o"][~hit.cuda()] = o[~hit].cuda()
+    c.out["lse"][~hit.cuda()] = lse[~hit].cuda()
+    c.check()
+
+
+@pytest.mark.parametrize("rows,heads,kv,dim", [(3, 4, 2, 64), (9, 8, 2, 128), (9, 8, 2, 256)])
+def test_nan_codes_in_an_8_bit_context(s, rows, heads, kv, dim):
+    """NaN codes in a key, in a value and in a value's scale: their head's rows, their channel, their head's values."""
+    c = Case([200, 60, 45, 45], rows, heads, kv, dim, 16, True, seed=dim)
+    at = lambda i, t: (c.layer, int(c.table[c.slots[i], t // 16]))   # noqa: E731
+    c.k[at(0, 77)].view(torch.uint8)[1, 77 % 16, 5] = 0xff
+    c.v[at(1, 3)].view(torch.uint8)[0, 3, dim - 1] = 0x7f
+    c.vs[at(2, 44)][1, 44 % 16] = NAN
+    c.run(s).check()
+    assert torch.isnan(c.out["o"].float()).any() and not torch.isnan(c.out["o"][3 * rows:].float()).any()
