@@ -482,16 +482,16 @@ int lcs_kv_reserve(lcs_ctx* ctx, uint32_t new_pages);
 /* The bookkeeping of a paged cache, on the device, for n <= 1024 requests per call. Slots
  * are in device memory, so bad ones are refused there: result[i] is 0, or -1 for a
  * request that changed nothing, with LCS_STATUS_PAGES set. A slot of -1 asks for
- * nothing (result 0). A slot outside [0, seqs) is refused, and one that an earlier
- * request of the call has named. No counterpart call in the reference, which does this on
- * the host (paged_cache.hpp:24-120).
+ * nothing (result 0, but behind a shortage in lcs_kv_grow). A slot outside [0, seqs)
+ * is refused, and one that an earlier request of the call has named. No counterpart
+ * call in the reference, which does this on the host (paged_cache.hpp:24-120).
  *
  * lcs_kv_grow: slot seq[i] gets a page of its own wherever one is missing or shared at
  * its tokens [start[i], end[i]): a missing one a free page, a shared one a copy (all
  * layers) that takes its place, also if all its holders ask in this call. Free pages
  * go to the requests in order, the lowest first; from the first request that there
- * are not enough for, none is served. start > end and ends past the table are
- * refused.
+ * are not enough for, none is served, whatever it asks for: result -1, for a slot of
+ * -1 too. start > end and ends past the table are refused.
  * lcs_kv_fork: slot dst[i], which holds no page, shares slot src[i]'s first tokens[i]
  * tokens. Refused where a page of them is missing, dst holds any, or src is itself
  * some request's dst.

@@ -739,7 +739,8 @@ class Sampler:
     def kv_grow_dev(self, cache, seq, start, end, result, stream=None):
         """Pages of their own for slots seq[i] at tokens [start[i], end[i])
         (lcs_kv_grow): missing ones allocated, shared ones replaced by copies.
-        All (n,) int32; result[i] is 0, or -1 where a request was refused."""
+        All (n,) int32; result[i] is 0, or -1 where a request was refused: from the
+        first that there are not enough pages for on, every one."""
         n, q, s, e, r = self._requests((seq, "seq"), (start, "start"), (end, "end"), (result, "result"))
         rc = _lib.lcs_kv_grow(self.ctx, self._cache(cache), n, q, s, e, r, self._raw_stream(stream))
         if rc != LCS_OK:

@@ -432,3 +432,16 @@ def test_append_finite_beside_a_nan(s):
         assert torch.equal(c.scales[sc][0, page, :, 2:5].t().cpu(), scale)
         assert torch.equal(torch.isnan(got), torch.isnan(want.float()))
         assert torch.equal(got.nan_to_num(), want.float().nan_to_num())
+
+
+def test_padding_behind_a_shortage(s):
+    """Behind a request that there are not enough pages for, every result of lcs_kv_grow is -1, a slot of -1's too; ahead of it
+    and in calls without a shortage that slot's is 0."""
+    c = Pair(s, pages=8)
+    c.grow([-1, 0, -1, 1, -1], [0] * 5, [5, 64, 5, 80, 5])    # 4 + 5 > 8
+    r = c.ints([7] * 5)
+    c.s.kv_grow_dev(c.cache, c.ints([-1, 1, -1, 2, -1]), c.ints([0] * 5), c.ints([0, 80, 9, 0, 0]), r)
+    torch.cuda.synchronize()
+    assert r.tolist() == [0, -1, -1, -1, -1] and s.status() == STATUS_PAGES
+    c.same()
+    c.grow([-1, 1, -1], [0] * 3, [5, 64, 5])
