@@ -19,6 +19,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "lcs_device.hpp"
 #include "lcs_internal.hpp"
 
@@ -332,10 +334,14 @@ __global__ __launch_bounds__(kCheckThreads) void kv_compact_check(KvArgs a) {
 // written. The next round's rows are under way meanwhile, the places of the one after it too
 // (16 contexts of 4000 to 8192 tokens, half kept, 4 layers: 547 us without, 367 so, 356 with
 // stores past the caches). The rounds of a workgroup follow each other, so a long list is
-// walked by 1024 threads; a short one by 256, which start sooner (us of 256 / 1024: the same
-// 350 / 332; 10 contexts of 13000 tokens, one layer, 276 / 192; one of 3000, 6 layers, 64 / 31; 3 of up
-// to 777, 5 layers, 13.2 / 9.3; 5 of 200, a third kept, 13 layers, 9.7 / 20; 10 of 30, 3 layers, 9.9 / 17).
-// 8 rows of a lane are no faster by 256 threads (346; 230 of 10 contexts) and spill by 1024 (550).
+// walked by 1024 threads; a short one by 256, which start sooner (us a call in a graph of
+// 256 / 1024 threads, half of the tokens kept, bf16, 8 heads of 128: the same 352 / 334; 10
+// contexts of 13000, one layer, 190 / 133; one of 3000, 6 layers, 32 / 21; 32 of 1200, 16
+// layers, 523 / 517, of 700 307 / 306, of 520 217 / 236, of 260 102 / 132; 4 of 900, 8 layers,
+// 27 / 26, of 512 16.3 / 16.8, of 260 11 / 13; 5 of 200, a third kept, 13 layers, 12 / 20). The
+// rule goes by the list's room, since the counts are on the device; lists of 257 to
+// 400 rows would be up to a tenth faster by 256.
+// 8 rows of a lane are no faster by 256 threads (346 of the first) and spill by 1024 (550).
 template <int NT>
 __global__ __launch_bounds__(NT) void kv_compact(KvArgs a) {
     constexpr uint32_t U = 4;
@@ -490,61 +496,74 @@ __global__ __launch_bounds__(kKvThreads) void kv_append(KvAppendArgs p) {
     const bool data = chunk < a.head_dim / 8u;
     if (t0 >= per) return;
     const uint32_t layer = a.layer + l;
-    for (uint32_t r = g - t0 * rows; r < rows; r += step) {
-        const bool kv = r >= a.kv_heads;
-        const uint32_t head = kv ? r - a.kv_heads : r;
-        const uint16_t* from = static_cast<const uint16_t*>(kv ? p.v : p.k) + (uint64_t)l * p.new_layer_stride +
-                               (uint64_t)i * p.rows_per_seq * (kv ? p.v_stride : p.k_stride) + head * a.head_dim + 8u * chunk;
-        const uint64_t stride = kv ? p.v_stride : p.k_stride;
-        unsigned char* base = static_cast<unsigned char*>(kv ? a.v : a.k) + place(a, layer, 0, head, 0) + (F8 ? 8u : 16u) * chunk;
-        float* sc = F8 ? (kv ? a.v_scale : a.k_scale) + scale_place(a, layer, 0, head, 0) : nullptr;
-        for (uint32_t t = t0; t < tokens; t += U * per) {
-            u32x4 x[U];
-            int32_t page[U];
+    // A row that holds a NaN has scale 1, and what of it is not one is cut to +-448, which the conversion
+    // would not do. A lane that has met such a row writes its rows again, cut: a branch at each row costs
+    // more than it looks (64 x 16 tokens of 32 layers x 8 heads 48.5 us with it, 46.0 so).
+    uint32_t worst = 0;   // the largest of the rows' |x|, by its bits
+    auto write = [&](auto cut) {
+        constexpr bool CUT = decltype(cut)::value;
+        for (uint32_t r = g - t0 * rows; r < rows; r += step) {
+            const bool kv = r >= a.kv_heads;
+            const uint32_t head = kv ? r - a.kv_heads : r;
+            const uint16_t* from = static_cast<const uint16_t*>(kv ? p.v : p.k) + (uint64_t)l * p.new_layer_stride +
+                                   (uint64_t)i * p.rows_per_seq * (kv ? p.v_stride : p.k_stride) + head * a.head_dim + 8u * chunk;
+            const uint64_t stride = kv ? p.v_stride : p.k_stride;
+            unsigned char* base = static_cast<unsigned char*>(kv ? a.v : a.k) + place(a, layer, 0, head, 0) + (F8 ? 8u : 16u) * chunk;
+            float* sc = F8 ? (kv ? a.v_scale : a.k_scale) + scale_place(a, layer, 0, head, 0) : nullptr;
+            for (uint32_t t = t0; t < tokens; t += U * per) {
+                u32x4 x[U];
+                int32_t page[U];
 #pragma unroll
-            for (uint32_t u = 0; u < U; ++u) {
-                const uint32_t tu = t + u * per;
-                page[u] = tu < tokens ? page_s[tu] : -1;
-                x[u] = u32x4{0, 0, 0, 0};
-                if (page[u] >= 0 && data) x[u] = *reinterpret_cast<const u32x4*>(from + (uint32_t)src_s[tu] * stride);
-            }
+                for (uint32_t u = 0; u < U; ++u) {
+                    const uint32_t tu = t + u * per;
+                    page[u] = tu < tokens ? page_s[tu] : -1;
+                    x[u] = u32x4{0, 0, 0, 0};
+                    if (page[u] >= 0 && data) x[u] = *reinterpret_cast<const u32x4*>(from + (uint32_t)src_s[tu] * stride);
+                }
 #pragma unroll
-            for (uint32_t u = 0; u < U; ++u) {
-                if (t + u * per >= tokens) break;   // (the lanes of a row together)
-                const bool ok = page[u] >= 0;
-                const uint32_t tok = ((uint32_t)pos0 + j0 + t + u * per) & (a.page_tokens - 1u);
-                const uint64_t at = ((uint32_t)page[u] * a.page_stride + tok * a.token_stride) * (F8 ? 1u : 2u);
-                if constexpr (F8) {
-                    uint32_t top = 0;   // the largest |x|, by its bits (a NaN's lie above infinity's)
+                for (uint32_t u = 0; u < U; ++u) {
+                    if (t + u * per >= tokens) break;   // (the lanes of a row together)
+                    const bool ok = page[u] >= 0;
+                    const uint32_t tok = ((uint32_t)pos0 + j0 + t + u * per) & (a.page_tokens - 1u);
+                    const uint64_t at = ((uint32_t)page[u] * a.page_stride + tok * a.token_stride) * (F8 ? 1u : 2u);
+                    if constexpr (F8) {
+                        uint32_t top = 0;   // the largest |x|, by its bits (a NaN's lie above infinity's)
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) top = max(top, max(x[u][k] & 0x7fffu, x[u][k] >> 16 & 0x7fffu));
-                    top = row_max(top, a.cp);
-                    if (top > 0x7f80u) {   // (a NaN in the row, whose scale is 1: what is not one is cut to +-448)
+                        for (int k = 0; k < 4; ++k) top = max(top, max(x[u][k] & 0x7fffu, x[u][k] >> 16 & 0x7fffu));
+                        top = row_max(top, a.cp);
+                        if constexpr (CUT) {
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) x[u][k] = cut448(x[u][k]) | cut448(x[u][k] >> 16) << 16;
-                    }
-                    const float f = __uint_as_float(top << 16);
-                    const float scale = f > 0.0f ? fmaxf(fdiv(f, kE4m3Max), kLeastScale) : 1.0f;   // (a NaN is not above 0)
-                    const Quotient by(scale);   // (448 at most, and a rounding)
-                    uint32_t q[2];
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        float e[4];
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            const uint32_t w = x[u][2 * h + k / 2];
-                            e[k] = by.of(__uint_as_float(k % 2 ? w & 0xffff0000u : w << 16));
+                            for (int k = 0; k < 4; ++k) x[u][k] = top > 0x7f80u ? cut448(x[u][k]) | cut448(x[u][k] >> 16) << 16 : x[u][k];
+                        } else {
+                            worst = max(worst, top);
                         }
-                        const int w = __builtin_amdgcn_cvt_pk_fp8_f32(e[0], e[1], 0, false);
-                        q[h] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(e[2], e[3], w, true);
+                        const float f = __uint_as_float(top << 16);
+                        const float scale = f > 0.0f ? fmaxf(fdiv(f, kE4m3Max), kLeastScale) : 1.0f;   // (a NaN is not above 0)
+                        const Quotient by(scale);   // (448 at most, and a rounding)
+                        uint32_t q[2];
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            float e[4];
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                const uint32_t w = x[u][2 * h + k / 2];
+                                e[k] = by.of(__uint_as_float(k % 2 ? w & 0xffff0000u : w << 16));
+                            }
+                            const int w = __builtin_amdgcn_cvt_pk_fp8_f32(e[0], e[1], 0, false);
+                            q[h] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(e[2], e[3], w, true);
+                        }
+                        if (ok && data) __builtin_nontemporal_store(u32x2{q[0], q[1]}, reinterpret_cast<u32x2*>(base + at));
+                        if (ok && chunk == 0u) sc[((uint64_t)(uint32_t)page[u] * a.kv_heads << a.page_shift) + tok] = scale;
+                    } else {
+                        if (ok && data) __builtin_nontemporal_store(x[u], reinterpret_cast<u32x4*>(base + at));
                     }
-                    if (ok && data) __builtin_nontemporal_store(u32x2{q[0], q[1]}, reinterpret_cast<u32x2*>(base + at));
-                    if (ok && chunk == 0u) sc[((uint64_t)(uint32_t)page[u] * a.kv_heads << a.page_shift) + tok] = scale;
-                } else {
-                    if (ok && data) __builtin_nontemporal_store(x[u], reinterpret_cast<u32x4*>(base + at));
                 }
             }
         }
+    };
+    write(std::false_type{});
+    if constexpr (F8) {
+        if (ballot(worst > 0x7f80u) != 0ull) write(std::true_type{});
     }
 }
 
