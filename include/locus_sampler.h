@@ -316,8 +316,11 @@ typedef struct lcs_kv_cache {
  * only (lcs_kv_append puts the accepted ones there). Query head h reads kv head
  * h / (heads / kv_heads). Scores, statistics and sums are f32; a weight is rounded
  * to bf16 for the product with the values, o once at the end. A row that sees
- * nothing (or scores of -inf only) has o = 0 and lse = -inf. What a row does not see is no part of its
- * result, whatever it holds. */
+ * nothing (or scores of -inf only) has o = 0 and lse = -inf; one that meets a NaN or a
+ * score of +inf is NaN. Scores past 2e38 in size may count as infinite, and an
+ * element's sum, of weights up to 2^8, overflows where the number of tokens times their
+ * largest |v| comes near 1e36. What a row does not see is no part of its result,
+ * whatever it holds. o may not overlap what is read. */
 typedef struct lcs_tree_attn_batch {
     uint32_t n_seq;            /* up to 1024, and n_seq * kv_heads up to 65536 */
     uint32_t rows_per_seq;     /* 1..256 */

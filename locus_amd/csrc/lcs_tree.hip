@@ -192,8 +192,8 @@ __device__ __forceinline__ Seq seq_of(const TreeArgs& a, uint32_t i, bool& bad) 
 __device__ __forceinline__ uint32_t uniform(uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); }
 // The line is cut into a.pieces equal pieces, of `share` steps each. A piece that begins with one
 // pair's end and goes on with another's start pays twice for what a pair costs by itself
-// (about three steps), so pairs are cut by themselves instead, into units of up to kMoreShare
-// steps more than `share`, a piece each, if there are pieces enough (16 trees of 16 nodes over
+// (about three steps), so pairs of up to 64 sequences, one a lane, are cut by themselves instead,
+// into units of up to kMoreShare steps more than `share`, a piece each, if there are pieces enough (16 trees of 16 nodes over
 // 300 to 6000 tokens, 8 kv heads: 64.7 -> 59.5 us; 16 of 48 over 600: 40.3 -> 31.1; 32 single
 // tokens over 4096: 106 -> 99; 7 trees of 13 over up to 1777, 5 heads: 24.3 -> 19.5).
 constexpr uint32_t kMoreShare = 3;

@@ -445,3 +445,28 @@ def test_padding_behind_a_shortage(s):
     assert r.tolist() == [0, -1, -1, -1, -1] and s.status() == STATUS_PAGES
     c.same()
     c.grow([-1, 1, -1], [0] * 3, [5, 64, 5])
+
+
+@pytest.mark.parametrize("f8", [False, True])
+@pytest.mark.parametrize("layers,heads,page,dim", [(1, 1024, 16, 16), (300, 1, 16, 32), (2, 3, 1024, 48)])
+def test_largest_layouts(s, layers, heads, page, dim, f8):
+    """Many heads, many layers, the longest pages: rows appended, copied on write and compacted."""
+    c = Pair(s, layers=layers, heads=heads, page=page, dim=dim, f8=f8, pages=8, max_pages=3)
+    n = page + 7
+    c.grow([0], [0], [n])
+    k, v = (torch.randn(layers, n, heads, dim, generator=torch.Generator().manual_seed(i)).bfloat16() for i in (1, 2))
+    s.kv_append_dev(c.cache, k.cuda(), v.cuda(), c.ints([0]), c.ints([0]), rows_per_seq=n)
+    for t, x in ((0, k), (1, v)):
+        sc = None
+        if f8:
+            x, sc = quantise(x)
+        for j in range(n):
+            pg, off = int(c.model.table[0, j // page]), j % page
+            c.model.rows[t][:, pg, :, off] = x[:, j]
+            if f8:
+                c.model.rows[2 + t][:, pg, :, off] = sc[:, j]
+    torch.cuda.synchronize()
+    c.same()
+    c.fork([0], [1], [n])
+    c.grow([1], [0], [n])
+    c.compact([1], [n // 2], [list(range(0, n // 2 * 2, 2))])

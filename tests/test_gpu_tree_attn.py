@@ -476,3 +476,19 @@ def test_nan_codes_in_an_8_bit_context(s, rows, heads, kv, dim):
     c.vs[at(2, 44)][1, 44 % 16] = NAN
     c.run(s).check()
     assert torch.isnan(c.out["o"].float()).any() and not torch.isnan(c.out["o"][3 * rows:].float()).any()
+
+
+@pytest.mark.parametrize("rows,heads,dim,f8", [(256, 10, 64, True), (256, 9, 256, False), (256, 17, 128, False), (129, 9, 256, True)])
+def test_more_row_tiles_than_a_launch(s, rows, heads, dim, f8):
+    """Rows of one kv head past the 32 tiles that a launch takes."""
+    Case([300, 70], rows, heads, 1, dim, 16, f8, seed=heads, layers=1).run(s).check(only=[0] if dim > 64 else None)
+    assert s.status() == 0
+
+
+@pytest.mark.parametrize("f8", [False, True])
+def test_most_pairs(s, f8):
+    """1024 sequences of 64 kv heads, the most of a call."""
+    rng = random.Random(1)
+    lengths = [rng.choice([0, 1, 15, 16, 40]) for _ in range(1024)]
+    Case(lengths, 1, 64, 64, 16, 16, f8, seed=3, layers=1).run(s).check(only=[0, 1023, *rng.sample(range(1024), 14)])
+    assert s.status() == 0
